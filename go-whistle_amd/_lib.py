@@ -6,12 +6,28 @@ here, loudly; nothing falls back to a CPU path.
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int8, c_int32, c_longlong, c_size_t, c_uint8, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int8, c_int32, c_longlong, c_size_t, c_uint8, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libcqhip.so")
 
 CQ_OK, CQ_ERR_ARG, CQ_ERR_MISUSE, CQ_ERR_DEVICE, CQ_ERR_UNSUPPORTED = 0, 1, 2, 3, 4
+
+
+class KvPaged(Structure):
+    """kv_paged (include/cqhip.h)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("ks", c_void_p), ("vs", c_void_p), ("pages", c_void_p),
+                ("type", c_int), ("kv_heads", c_int), ("qk", c_int), ("vd", c_int), ("page_stride", c_int),
+                ("page_rows", c_int), ("pool_pages", c_int)]
+
+
+class CrossLayout(Structure):
+    """nd_cross_layout (include/cqhip.h)."""
+
+    _fields_ = [(n, c_longlong) for n in ("q_stream", "q_row", "out_stream", "out_row", "k_stream", "k_row", "k_head",
+                                          "v_stream", "v_row", "v_head")]
+
 
 # Every symbol include/cqhip.h declares, with (restype, argtypes).
 SIGNATURES = {
@@ -111,6 +127,18 @@ SIGNATURES = {
     "cq_gemms_tables_dev": (c_int, [c_int, POINTER(c_void_p), POINTER(c_void_p), c_int, c_void_p, c_int,
                                     POINTER(c_void_p), POINTER(c_void_p), c_longlong, c_longlong, c_void_p, c_int,
                                     POINTER(c_void_p), POINTER(c_void_p), c_void_p, c_size_t, c_void_p]),
+    "kv_append_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_longlong, c_longlong, c_void_p, c_longlong,
+                                    c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_longlong,
+                                    c_void_p]),
+    "kv_attend_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int,
+                                    c_void_p, c_int, c_float, c_void_p, c_void_p, c_longlong, c_void_p]),
+    "kv_evict_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_longlong,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "nd_cross_attend_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, POINTER(CrossLayout), c_int, c_int,
+                                    c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float,
+                                    c_void_p]),
+    "nd_logprobs_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
+                                c_void_p, c_int, c_void_p]),
 }
 
 _lib = None

@@ -2265,4 +2265,273 @@ int kv_append_rope_dev(int8_t *q, float *s, const float *x, int batch, int cols,
     return append_impl(q, s, x, batch, cols, width, q_stride, s_stride, pos, cap, cos_t, sin_t, stream);
 }
 
+// ---- caches and memories of any type and length ---------------------------------
+
+// The parts of a paged cache's description that every call checks.
+static int paged_args(const kv_paged *c, int batch, int rows, const char *what, PagedArgs &p) {
+    if (!c) return fail(CQ_ERR_MISUSE, "needle: %s without a cache", what);
+    if (c->type < ND_F32 || c->type > ND_I8) return fail(CQ_ERR_MISUSE, "needle: cache type %d", c->type);
+    if (c->kv_heads <= 0) return fail(CQ_ERR_MISUSE, "needle: a cache of %d heads", c->kv_heads);
+    if (!split_widths_ok(c->qk, c->vd))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: cache heads of %d and %d (multiples of 16 up to 256)", c->qk, c->vd);
+    if (c->page_rows <= 0 || (c->page_rows & (c->page_rows - 1)) != 0 || c->pool_pages <= 0 || c->page_stride < 0 ||
+        static_cast<long long>(c->page_stride) * c->page_rows < rows)
+        return fail(CQ_ERR_MISUSE, "needle: %d pages of %d rows for %d positions (pool %d)", c->page_stride,
+                    c->page_rows, rows, c->pool_pages);
+    if (static_cast<long long>(c->pool_pages) * c->page_rows > 0x7fffffffLL)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: a pool of %d pages of %d rows", c->pool_pages, c->page_rows);
+    if (batch > 0 && (!c->k || !c->v || (rows > 0 && !c->pages) || (c->type == ND_I8 && (!c->ks || !c->vs))))
+        return fail(CQ_ERR_MISUSE, "needle: %s with a nil cache array", what);
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
+        return fail(CQ_ERR_MISUSE, "needle: cache pools that are not aligned to 16 bytes");
+    int shift = 0;
+    while ((1 << shift) < c->page_rows) ++shift;
+    p = PagedArgs{static_cast<unsigned char *>(c->k), static_cast<unsigned char *>(c->v), c->ks, c->vs, c->pages,
+                  c->type, c->kv_heads, c->qk, c->vd, c->page_stride, shift, c->pool_pages};
+    return CQ_OK;
+}
+
+static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_I8 ? 1 : 2; }
+
+int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
+                        long long v_stream, long long v_row, int type, int batch, int t, const int32_t *rows,
+                        const int32_t *pos, int cap, float *acc, long long acc_cap, void *stream) {
+    if (batch < 0 || t < 0 || cap < 0) return fail(CQ_ERR_MISUSE, "needle: append of %d x %d rows (cap %d)", batch, t, cap);
+    PagedAppendArgs a;
+    if (int rc = paged_args(c, batch, cap, "append", a.c)) return rc;
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: rows of type %d", type);
+    if (acc && acc_cap < cap) return fail(CQ_ERR_MISUSE, "needle: %lld weights for %d positions", acc_cap, cap);
+    if (batch == 0 || t == 0 || cap == 0) return CQ_OK;
+    if (!k || !v || !pos) return fail(CQ_ERR_MISUSE, "needle: append with a nil operand");
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: rows that are not aligned to their type");
+    if (static_cast<long long>(batch) * t * c->kv_heads > (0xffffffffLL - 255) / 128)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: append of %d x %d rows of %d heads", batch, t, c->kv_heads);
+    a.x[0] = k;
+    a.x[1] = v;
+    a.stream[0] = k_stream;
+    a.stream[1] = v_stream;
+    a.row[0] = k_row;
+    a.row[1] = v_row;
+    a.type = type;
+    a.batch = batch;
+    a.t = t;
+    a.cap = cap;
+    a.rows = rows;
+    a.pos = pos;
+    a.acc = acc;
+    a.acc_cap = acc_cap;
+    HIP_TRY(launch_paged_append(a, static_cast<hipStream_t>(stream)), "paged append launch");
+    return CQ_OK;
+}
+
+// The parts that a list of up to nk keys is cut into for `lists` workgroups a part: enough for two workgroups a CU,
+// none of fewer than 128 keys (a tile a wavefront).
+static int split_parts(long long lists, int nk) {
+    const long long want = (2LL * device_info().cus + lists - 1) / lists;
+    return static_cast<int>(std::max<long long>(1, std::min<long long>(want, (nk + 127) / 128)));
+}
+
+// The launches of a split attention with the partials' workspace.
+static int run_split_attend(SplitArgs &a, bool weights, hipStream_t stream) {
+    const int group = a.heads / a.c.kv_heads;
+    const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((static_cast<long long>(a.t) * group + 15) / 16);
+    a.splits = split_parts(lists, a.nk_max);
+    const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
+    const long long wblocks = weights ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
+    if (lists * a.splits > grid_limit(256) || (rows + 3) / 4 > grid_limit(256) || wblocks > grid_limit(256))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", a.batch, a.t, a.heads);
+    WsScope ws;
+    a.part = a.part_ml = a.logits = nullptr;
+    if (a.splits > 1 || weights) {
+        const size_t part = align256(static_cast<size_t>(rows) * a.splits * a.c.vd * 4);
+        const size_t ml = align256(static_cast<size_t>(rows) * a.splits * 8);
+        const size_t lg = weights ? static_cast<size_t>(rows) * a.nk_max * 4 : 0;
+        if (int rc = ws_acquire(part + ml + lg, stream, ws.l)) return rc;
+        char *base = static_cast<char *>(ws.l.w->buf);
+        a.part = reinterpret_cast<float *>(base);
+        a.part_ml = reinterpret_cast<float *>(base + part);
+        if (weights) a.logits = reinterpret_cast<float *>(base + part + ml);
+    }
+    HIP_TRY(launch_attend_split(a, stream), "split attention launch");
+    return CQ_OK;
+}
+
+int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, const void *q, long long q_stride,
+                        int type, int batch, int heads, const int32_t *spans, int nk_max, float scale,
+                        const float *acc, float *acc_out, long long acc_cap, void *stream) {
+    if (batch < 0 || nk_max < 0) return fail(CQ_ERR_MISUSE, "needle: attention of %d streams over %d keys", batch, nk_max);
+    SplitArgs a;
+    std::memset(&a, 0, sizeof a);
+    if (int rc = paged_args(c, batch, nk_max, "attention", a.c)) return rc;
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: queries of type %d", type);
+    if (heads <= 0 || heads % c->kv_heads != 0)
+        return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, c->kv_heads);
+    if (!(std::isfinite(scale) && scale != 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (acc_out && acc_cap < nk_max) return fail(CQ_ERR_MISUSE, "needle: %lld weights for %d keys", acc_cap, nk_max);
+    if (heads / c->kv_heads > 1024) return fail(CQ_ERR_UNSUPPORTED, "needle: %d heads a KV head", heads / c->kv_heads);
+    if (batch == 0) return CQ_OK;
+    if (!out || !q || !spans) return fail(CQ_ERR_MISUSE, "needle: attention with a nil operand");
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
+    const int size = value_size(c->type);
+    a.k_head = static_cast<long long>(c->qk) * size;
+    a.v_head = static_cast<long long>(c->vd) * size;
+    a.k_row = a.k_head * c->kv_heads;
+    a.v_row = a.v_head * c->kv_heads;
+    a.spans = spans;
+    a.nk_max = nk_max;
+    a.t = 1;
+    a.heads = heads;
+    a.batch = batch;
+    a.q = q;
+    a.out = out;
+    a.q_stream = q_stride ? q_stride : static_cast<long long>(heads) * c->qk;
+    a.out_stream = out_stride ? out_stride : static_cast<long long>(heads) * c->vd;
+    a.type = type;
+    a.scale_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
+    a.acc = acc;
+    a.acc_out = acc_out;
+    a.acc_cap = acc_cap;
+    return run_split_attend(a, acc_out != nullptr, static_cast<hipStream_t>(stream));
+}
+
+int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
+                       long long acc_cap, float *acc_out, long long acc_out_cap, const int32_t *len, int32_t *len_out,
+                       int32_t *kept, int batch, int nk_max, int keep, int sink, int recent, void *stream) {
+    if (batch < 0 || nk_max < 0 || keep < 0 || sink < 0 || recent < 0 ||
+        static_cast<long long>(sink) + recent > keep)
+        return fail(CQ_ERR_MISUSE, "needle: eviction of %d streams of %d rows to %d (first %d, last %d)", batch, nk_max,
+                    keep, sink, recent);
+    EvictArgs a;
+    if (int rc = paged_args(c, batch, nk_max, "eviction", a.c)) return rc;
+    if (static_cast<long long>(dst_stride) * c->page_rows < keep || acc_cap < nk_max || acc_out_cap < keep)
+        return fail(CQ_ERR_MISUSE, "needle: eviction to %d rows in %d pages of %d, weights %lld to %lld", keep,
+                    dst_stride, c->page_rows, acc_cap, acc_out_cap);
+    if (batch == 0) return CQ_OK;
+    if (!len || !len_out || (nk_max > 0 && !acc) || (keep > 0 && (!dst_pages || !acc_out || !kept)))
+        return fail(CQ_ERR_MISUSE, "needle: eviction with a nil operand");
+    if (acc_out && acc_out == acc) return fail(CQ_ERR_MISUSE, "needle: eviction onto its own weights");
+    const int pieces = (c->qk + c->vd) * value_size(c->type) / 16;
+    if (static_cast<long long>(batch) * c->kv_heads > grid_limit(1024) ||
+        static_cast<double>(batch) * keep * c->kv_heads * pieces > static_cast<double>(grid_limit(256)) * 256)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: eviction of %d streams to %d rows", batch, keep);
+    a.dst_pages = dst_pages;
+    a.dst_stride = dst_stride;
+    a.acc = acc;
+    a.acc_out = acc_out;
+    a.acc_cap = acc_cap;
+    a.acc_out_cap = acc_out_cap;
+    a.len = len;
+    a.len_out = len_out;
+    a.kept = kept;
+    a.batch = batch;
+    a.nk_max = nk_max;
+    a.keep = keep;
+    a.sink = sink;
+    a.recent = recent;
+    HIP_TRY(launch_evict(a, static_cast<hipStream_t>(stream)), "eviction launch");
+    return CQ_OK;
+}
+
+int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
+                        const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
+                        int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,
+                        float scale, void *stream) {
+    if (batch < 0 || t < 0 || memories < 0 || frames < 0)
+        return fail(CQ_ERR_MISUSE, "needle: cross-attention of %d x %d rows to %d memories of %d", batch, t, memories, frames);
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: cross-attention of type %d", type);
+    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0)
+        return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, kv_heads);
+    if (!split_widths_ok(qk, vd))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: cross-attention heads of %d and %d (multiples of 16 up to 256)", qk, vd);
+    if (!(std::isfinite(scale) && scale != 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (batch == 0 || t == 0) return CQ_OK;
+    if (!out || !q || (memories > 0 && frames > 0 && (!k || !v)))
+        return fail(CQ_ERR_MISUSE, "needle: cross-attention with a nil operand");
+    const int size = value_size(type);
+    nd_cross_layout y;
+    if (layout) {
+        y = *layout;
+    } else {
+        y.q_row = static_cast<long long>(heads) * qk;
+        y.out_row = static_cast<long long>(heads) * vd;
+        y.q_stream = y.q_row * t;
+        y.out_stream = y.out_row * t;
+        y.k_head = qk;
+        y.v_head = vd;
+        y.k_row = static_cast<long long>(kv_heads) * qk;
+        y.v_row = static_cast<long long>(kv_heads) * vd;
+        y.k_stream = y.k_row * frames;
+        y.v_stream = y.v_row * frames;
+    }
+    if (((y.k_stream | y.k_row | y.k_head | y.v_stream | y.v_row | y.v_head) * size |
+         static_cast<long long>(reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v))) & 15)
+        return fail(CQ_ERR_MISUSE, "needle: cross-attention memories that are not aligned to 16 bytes");
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % size)
+        return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
+    if (static_cast<long long>(t) * (heads / kv_heads) > 0x7fffffffLL - 64)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: cross-attention of %d rows of %d heads", t, heads);
+    SplitArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.c.k = static_cast<unsigned char *>(const_cast<void *>(k));
+    a.c.v = static_cast<unsigned char *>(const_cast<void *>(v));
+    a.c.type = type;
+    a.c.kv_heads = kv_heads;
+    a.c.qk = qk;
+    a.c.vd = vd;
+    a.k_mem = y.k_stream * size;
+    a.k_row = y.k_row * size;
+    a.k_head = y.k_head * size;
+    a.v_mem = y.v_stream * size;
+    a.v_row = y.v_row * size;
+    a.v_head = y.v_head * size;
+    a.q_len = q_len;
+    a.k_len = k_len;
+    a.index = index;
+    a.memories = memories;
+    a.nk_max = frames;
+    a.t = t;
+    a.heads = heads;
+    a.batch = batch;
+    a.q = q;
+    a.out = out;
+    a.q_stream = y.q_stream;
+    a.q_row = y.q_row;
+    a.out_stream = y.out_stream;
+    a.out_row = y.out_row;
+    a.type = type;
+    a.scale_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
+    return run_split_attend(a, false, static_cast<hipStream_t>(stream));
+}
+
+int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, const void *logits, long long stride,
+                    int type, int rows, int n, const int32_t *tokens, int top, void *stream) {
+    if (rows < 0 || n <= 0 || top < 0 || top > n || stride < 0)
+        return fail(CQ_ERR_MISUSE, "needle: %d log probabilities of %d rows of %d", top, rows, n);
+    if (top > 64) return fail(CQ_ERR_UNSUPPORTED, "needle: %d alternatives (64 at most)", top);
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: logits of type %d", type);
+    if (lp && !tokens) return fail(CQ_ERR_MISUSE, "needle: log probabilities without tokens");
+    if (!top_idx != !top_lp) return fail(CQ_ERR_MISUSE, "needle: alternatives without their indices or values");
+    if (rows == 0 || (!lp && !ent && !top_idx)) return CQ_OK;
+    if (!logits) return fail(CQ_ERR_MISUSE, "needle: log probabilities with a nil operand");
+    if (reinterpret_cast<uintptr_t>(logits) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: logits that are not aligned to their type");
+    LogprobArgs a{lp, ent, top_lp, top_idx, logits, stride, type, rows, n, top_idx ? top : 0, tokens, 1, n, nullptr};
+    const int most = logprob_chunk();
+    a.splits = (n + most - 1) / most;
+    a.chunk = (n + a.splits - 1) / a.splits;
+    if (static_cast<long long>(rows) * a.splits > grid_limit(512))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: log probabilities of %d rows of %d", rows, n);
+    WsScope ws;
+    if (a.splits > 1) {
+        if (int rc = ws_acquire(static_cast<size_t>(rows) * a.splits * (4 + 2 * a.top) * 4,
+                                static_cast<hipStream_t>(stream), ws.l))
+            return rc;
+        a.part = static_cast<float *>(ws.l.w->buf);
+    }
+    HIP_TRY(launch_logprobs(a, static_cast<hipStream_t>(stream)), "log probabilities launch");
+    return CQ_OK;
+}
+
 }  // extern "C"

@@ -469,4 +469,82 @@ hipError_t launch_page_copy(int8_t *q, float *sc, const int32_t *src, const int3
 hipError_t launch_gather_float_rows(float *dst, const float *src, const int32_t *idx, int rows, long long width,
                                     hipStream_t s);
 
+// ---- caches and memories of any type and length (split_kernels.hip, paged_kernels.hip) ----
+
+// A paged cache as kv_paged describes it (pages of 2^shift rows).
+struct PagedArgs {
+    unsigned char *k, *v;
+    float *ks, *vs;
+    const int32_t *pages;
+    int type, kv_heads, qk, vd;
+    int page_stride, shift, pool_pages;
+};
+
+// Rows x[b * stream + i * row] of `type` appended at pos[b] + i (kv_append_paged_dev).
+struct PagedAppendArgs {
+    PagedArgs c;
+    const void *x[2];  // keys, values
+    long long stream[2], row[2];
+    int type, batch, t, cap;
+    const int32_t *rows, *pos;
+    float *acc;
+    long long acc_cap;
+};
+hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s);
+
+// kv_evict_paged_dev: the kept rows of every (stream, key head), then their copies.
+struct EvictArgs {
+    PagedArgs c;
+    const int32_t *dst_pages;
+    int dst_stride;
+    const float *acc;
+    float *acc_out;
+    long long acc_cap, acc_out_cap;
+    const int32_t *len;
+    int32_t *len_out, *kept;
+    int batch, nk_max, keep, sink, recent;
+};
+hipError_t launch_evict(const EvictArgs &a, hipStream_t s);
+
+// Attention of cols = t * (heads / kv_heads) query columns of every (stream,
+// key head) over its keys, in 16-column tiles and `splits` parts of the key
+// list. Keys come from pages (c.pages) or from memories: row j of memory m,
+// head h at byte m * mem + j * row + h * head of c.k / c.v.
+struct SplitArgs {
+    PagedArgs c;
+    long long k_mem, k_row, k_head, v_mem, v_row, v_head;  // bytes
+    const int32_t *spans;                    // paged: the keys' spans
+    const int32_t *q_len, *k_len, *index;    // memories
+    int memories, nk_max, t, heads, batch, splits;
+    const void *q;
+    void *out;
+    long long q_stream, q_row, out_stream, out_row;  // elements
+    int type;
+    float scale_log2;                        // log2(e) / scale
+    // Partials of the splits (splits > 1 or weights asked): per (stream,
+    // head-major column, split) vd sums, and their maximum (of log2 logits) and
+    // sum; the logits [stream][key head][group head][nk_max] for the weights.
+    float *part, *part_ml, *logits;
+    const float *acc;
+    float *acc_out;
+    long long acc_cap;
+};
+bool split_widths_ok(int qk, int vd);
+hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);
+
+// nd_logprobs_dev: `splits` parts of `chunk` logits a row; the parts' results
+// (splits > 1) in part: {m, l, t} and top pairs {value, index bits}.
+struct LogprobArgs {
+    float *lp, *ent, *top_lp;
+    int32_t *top_idx;
+    const void *x;
+    long long stride;
+    int type, rows, n, top;
+    const int32_t *tokens;
+    int splits, chunk;
+    float *part;
+};
+int logprob_chunk();
+hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s);
+
 }  // namespace cqhip

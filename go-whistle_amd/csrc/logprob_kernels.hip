@@ -1,0 +1,228 @@
+// gfx950 log probabilities, entropy and top alternatives of rows of logits
+// (nd_logprobs_dev).
+//
+// A workgroup holds a part of a row in registers: one pass over the logits.
+// With m the part's maximum, l = sum e^(x - m) and t = sum e^(x - m) (x - m):
+// log p(x) = (x - m) - log l, entropy = log l - t / l. The parts of a long
+// row are joined by a second launch: l and t move to the common maximum M by
+// e^(m - M): t' = e^(m - M) (t + (m - M) l).
+#include "cq_internal.hpp"
+#include "cq_device.hpp"
+
+#include <algorithm>
+
+namespace cqhip {
+namespace {
+
+constexpr int kLpThreads = 512;
+constexpr int kLpWaves = kLpThreads / 64;
+constexpr int kVals = 32;  // logits a thread holds
+
+// A logit's place in the order of alternatives: the larger value, then the
+// lower index; a NaN as -inf, -0 as 0. 0 is below every logit.
+__device__ __forceinline__ unsigned long long rank_key(float x, int i) {
+    const uint32_t u = __float_as_uint((x != x ? -INFINITY : x) + 0.0f);
+    const uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+
+__device__ __forceinline__ float logit_at(const void *x, int type, long long i) {
+    if (type == 0) return static_cast<const float *>(x)[i];
+    const uint16_t h = static_cast<const uint16_t *>(x)[i];
+    return type == 1 ? static_cast<float>(__builtin_bit_cast(_Float16, h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
+
+// x - m of a token, and what follows from the row's m, l, t.
+struct RowStats {
+    float m, l, t;
+};
+__device__ __forceinline__ float log_prob(const RowStats &s, float x) {
+    if (s.m == -INFINITY) return s.l != s.l ? s.l : -INFINITY;  // a row of -inf (or NaN) alone
+    return (x - s.m) - logf(s.l);
+}
+__device__ __forceinline__ float entropy(const RowStats &s) {
+    if (s.m == -INFINITY) return s.l != s.l ? s.l : 0.0f;
+    return logf(s.l) - s.t / s.l;
+}
+
+__device__ __forceinline__ void write_row(const LogprobArgs &a, int r, const RowStats &s) {
+    const int tok = a.tokens ? a.tokens[r] : -1;
+    if (a.lp)
+        a.lp[r] = tok < 0 ? 0.0f
+                  : tok >= a.n ? NAN
+                               : log_prob(s, logit_at(a.x, a.type, static_cast<long long>(r) * a.stride + tok));
+    if (a.ent) a.ent[r] = entropy(s);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
+    __shared__ float red[3][kLpWaves];
+    __shared__ unsigned long long best_sh[kLpWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int part = blockIdx.x % a.splits, r = blockIdx.x / a.splits;
+    const int i0 = part * a.chunk, i1 = min(i0 + a.chunk, a.n);
+    const long long base = static_cast<long long>(r) * a.stride;
+
+    float v[kVals];
+    float m = -INFINITY, bad = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) {
+        const int i = i0 + tid + k * kLpThreads;
+        v[k] = i < i1 ? logit_at(a.x, TYPE, base + i) : -INFINITY;
+        m = fmaxf(m, v[k]);
+    }
+    // block maximum
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) m = fmaxf(m, red[0][w]);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) {
+        const float d = v[k] - mu;
+        const float e = __expf(d);
+        l += e;
+        t += e > 0.0f ? e * d : 0.0f;
+        if (v[k] != v[k]) bad = NAN;
+    }
+    l += bad;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        l += __shfl_xor(l, o);
+        t += __shfl_xor(t, o);
+    }
+    if (lane == 0) red[1][wave] = l, red[2][wave] = t;
+    __syncthreads();
+    l = t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) l += red[1][w], t += red[2][w];
+    const RowStats st{m, l, t};
+    float *pt = a.part + (static_cast<long long>(r) * a.splits + part) * (4 + 2 * a.top);
+    if (tid == 0) {
+        if (a.splits == 1) {
+            write_row(a, r, st);
+        } else {
+            pt[0] = m;
+            pt[1] = l;
+            pt[2] = t;
+        }
+    }
+    // The alternatives, one after the other: every thread offers its largest
+    // below the last one chosen.
+    unsigned long long mine = 0, last = ~0ull;
+    for (int q = 0; q < a.top; ++q) {
+        if (q == 0 || mine == last) {
+            mine = 0;
+#pragma unroll
+            for (int k = 0; k < kVals; ++k) {
+                const int i = i0 + tid + k * kLpThreads;
+                const unsigned long long key = rank_key(v[k], i);
+                if (i < i1 && key < last && key > mine) mine = key;
+            }
+        }
+        unsigned long long best = mine;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor(best, o);
+            if (other > best) best = other;
+        }
+        __syncthreads();
+        if (lane == 0) best_sh[wave] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kLpWaves; ++w)
+            if (best_sh[w] > best) best = best_sh[w];
+        last = best;
+        if (tid == 0) {
+            const int i = key_index(best);
+            if (a.splits > 1) {
+                // a part of fewer than `top` logits offers index -1
+                pt[4 + 2 * q] = best ? logit_at(a.x, TYPE, base + i) : -INFINITY;
+                pt[5 + 2 * q] = __int_as_float(best ? i : -1);
+            } else {
+                a.top_idx[static_cast<long long>(r) * a.top + q] = i;
+                a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, TYPE, base + i));
+            }
+        }
+    }
+}
+
+// The parts of a row joined: a wavefront a row.
+__global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
+    const int r = blockIdx.x, lane = threadIdx.x;
+    const int rec = 4 + 2 * a.top;
+    const float *pt = a.part + static_cast<long long>(r) * a.splits * rec;
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, pt[static_cast<long long>(s) * rec]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, t = 0.0f;
+    for (int s = lane; s < a.splits; s += 64) {
+        const float *p = pt + static_cast<long long>(s) * rec;
+        if (p[0] == -INFINITY) {  // nothing above -inf: 0, or NaN
+            l += p[1];
+            continue;
+        }
+        const float d = p[0] - mu, f = __expf(d);
+        l += f * p[1];
+        t += f > 0.0f ? f * (p[2] + d * p[1]) : 0.0f;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        l += __shfl_xor(l, o);
+        t += __shfl_xor(t, o);
+    }
+    const RowStats st{m, l, t};
+    if (lane == 0) write_row(a, r, st);
+    // each part's alternatives are in order: a lane walks the parts s = lane, lane + 64, ...
+    unsigned long long last = ~0ull;
+    for (int q = 0; q < a.top; ++q) {
+        unsigned long long best = 0;
+        for (int s = lane; s < a.splits; s += 64) {
+            const float *p = pt + static_cast<long long>(s) * rec + 4;
+            for (int k = 0; k < a.top; ++k) {
+                const int i = __float_as_int(p[2 * k + 1]);
+                if (i < 0) break;
+                const unsigned long long key = rank_key(p[2 * k], i);
+                if (key < last) {
+                    if (key > best) best = key;
+                    break;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor(best, o);
+            if (other > best) best = other;
+        }
+        last = best;
+        if (lane == 0) {
+            const int i = key_index(best);
+            a.top_idx[static_cast<long long>(r) * a.top + q] = i;
+            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, a.type, static_cast<long long>(r) * a.stride + i));
+        }
+    }
+}
+
+}  // namespace
+
+int logprob_chunk() { return kLpThreads * kVals; }
+
+hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(static_cast<long long>(a.rows) * a.splits));
+    switch (a.type) {
+        case 0: hipLaunchKernelGGL(logprob_kernel<0>, grid, dim3(kLpThreads), 0, s, a); break;
+        case 1: hipLaunchKernelGGL(logprob_kernel<1>, grid, dim3(kLpThreads), 0, s, a); break;
+        default: hipLaunchKernelGGL(logprob_kernel<2>, grid, dim3(kLpThreads), 0, s, a); break;
+    }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
+    hipLaunchKernelGGL(logprob_join_kernel, dim3(a.rows), dim3(64), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace cqhip

@@ -4,7 +4,9 @@ Linear (internal/needle/linear.go) over libcqhip.
 QuantizeRows / Int8Rows.Append (int8.go:116-141) on host arrays or device
 tensors, AttendInt8Spans (int8.go:208-272) on device tensors for one or
 many independent streams, fakeQuant (int8.go:57-75), and Linear with
-WithInt8Input, Apply and ApplyShared on device tensors.
+WithInt8Input, Apply and ApplyShared on device tensors. Caches of any
+type and length (PagedKV), cross-attention to float memories
+(cross_attend_dev) and log probabilities (logprobs_dev) on device tensors.
 """
 
 import ctypes
@@ -12,7 +14,7 @@ from ctypes import POINTER, c_float, c_int8, c_void_p
 
 import numpy as np
 
-from ._lib import CQPanic, check, lib
+from ._lib import CQPanic, CrossLayout, KvPaged, check, lib
 
 
 def QuantizeRows(x, cols, width):
@@ -195,3 +197,232 @@ def ApplyShared(dsts, x, rows, *ls):
         sel = [k for k, l in enumerate(ls) if l.act8 == quant]
         if sel:
             cq.gemms_dev([ls[k].q for k in sel], [dsts[k] for k in sel], xq if quant else x, rows)
+
+
+# ---- caches and memories of any type and length, log probabilities ----------------
+
+
+def _types():
+    import torch
+
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+
+
+_TYPES = None
+
+
+def _type(t, what, cache=False):
+    """ND_F32.. of a tensor's dtype; ND_I8 for caches only."""
+    global _TYPES
+    if _TYPES is None:
+        _TYPES = _types()
+    code = _TYPES.get(t.dtype)
+    if code is None or (code == 3 and not cache):
+        raise CQPanic(f"needle: {what} of {t.dtype}")
+    return code
+
+
+def _want(t, what, shape, dtype=None, dev=None, dense=True):
+    """Refuses a tensor that the call would read or write out of its bounds."""
+    if tuple(t.shape) != tuple(shape):
+        raise CQPanic(f"needle: {what} of shape {tuple(t.shape)}, not {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise CQPanic(f"needle: {what} of {t.dtype}, not {dtype}")
+    if not t.is_cuda or (dev is not None and t.device != dev):
+        raise CQPanic(f"needle: {what} on {t.device}, not {dev or 'a GPU'}")
+    if dense and not t.is_contiguous():
+        raise CQPanic(f"needle: {what} that is not contiguous")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """The device of the tensors current, and its current stream, for one call."""
+
+    def __init__(self, device):
+        import torch
+
+        self.torch, self.device = torch, device
+        self.guard = None
+
+    def __enter__(self):
+        cuda = self.torch.cuda
+        if self.device.index != cuda.current_device():
+            self.guard = cuda.device(self.device)
+            self.guard.__enter__()
+        return cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+class PagedKV:
+    """Paged key and value caches of many streams (kv_paged, cqhip.h): pools k
+    [pages, page_rows, kv_heads, qk] and v [pages, page_rows, kv_heads, vd] of
+    float32, float16, bfloat16 or int8 (with scales ks, vs [pages, page_rows,
+    kv_heads] float32), read through the page table `pages` [streams,
+    pages per stream] int32. The tensors stay the caller's: a changed table
+    entry or a fork's copied table is seen by the next call."""
+
+    def __init__(self, k, v, pages, ks=None, vs=None):
+        import torch
+
+        if k.dim() != 4 or v.dim() != 4 or pages.dim() != 2:
+            raise CQPanic("needle: a paged cache is [pages, page_rows, kv_heads, width] and its table [streams, pages]")
+        _want(k, "keys", k.shape)
+        _want(v, "values", (*k.shape[:3], v.shape[3]), k.dtype, k.device)
+        _want(pages, "page table", pages.shape, torch.int32, k.device)
+        self.type = _type(k, "a cache", cache=True)
+        if (self.type == 3) != (ks is not None) or (ks is None) != (vs is None):
+            raise CQPanic("needle: int8 caches have scales, float ones none")
+        for s, what in ((ks, "key scales"), (vs, "value scales")):
+            if s is not None:
+                _want(s, what, k.shape[:3], torch.float32, k.device)
+        self.k, self.v, self.ks, self.vs, self.pages = k, v, ks, vs, pages
+        self.streams, self.kv_heads, self.qk, self.vd = pages.shape[0], k.shape[2], k.shape[3], v.shape[3]
+        self.device = k.device
+        self._c = KvPaged(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), pages.data_ptr(), self.type, k.shape[2],
+                          k.shape[3], v.shape[3], pages.shape[1], k.shape[1], k.shape[0])
+        self._ref = ctypes.byref(self._c)
+
+    def _acc(self, acc, what, rows):
+        import torch
+
+        _want(acc, what, (self.streams, self.kv_heads, acc.shape[-1]), torch.float32, self.device)
+        if acc.shape[-1] < rows:
+            raise CQPanic(f"needle: {what} of {acc.shape[-1]} rows for {rows}")
+        return acc.shape[-1]
+
+    def append_dev(self, k, v, pos, rows=None, cap=None, acc=None):
+        """Rows k [streams, t, kv_heads, qk], v [streams, t, kv_heads, vd]
+        (float32, float16, bfloat16; any stream and row strides) appended at
+        row pos[b] of stream b, the first rows[b] of them where given; rows
+        at or past cap (all that the table holds) are skipped. acc [streams,
+        kv_heads, >= cap]: their accumulated weights become 0."""
+        import torch
+
+        t = k.shape[1] if k.dim() == 4 else 0
+        _want(k, "key rows", (self.streams, t, self.kv_heads, self.qk), None, self.device, dense=False)
+        _want(v, "value rows", (self.streams, t, self.kv_heads, self.vd), k.dtype, self.device, dense=False)
+        for x, w, what in ((k, self.qk, "key rows"), (v, self.vd, "value rows")):
+            if x.stride(3) != 1 or (x.stride(2) != w and self.kv_heads > 1):
+                raise CQPanic(f"needle: {what} whose heads are not side by side")
+        _want(pos, "positions", (self.streams,), torch.int32, self.device)
+        if rows is not None:
+            _want(rows, "row counts", (self.streams,), torch.int32, self.device)
+        if cap is None:
+            cap = self.pages.shape[1] * self.k.shape[1]
+        acc_cap = self._acc(acc, "weights", cap) if acc is not None else 0
+        with _on(self.device) as st:
+            check(lib().kv_append_paged_dev(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                            v.stride(1), _type(k, "rows"), self.streams, t, _ptr(rows), pos.data_ptr(),
+                                            cap, _ptr(acc), acc_cap, st))
+
+    def attend_dev(self, out, q, spans, nk_max, scale, acc=None, acc_out=None):
+        """Attention of one token a stream: q [streams, heads, qk] and out
+        [streams, heads, vd] of one type (float32, float16, bfloat16), over the
+        rows of spans [streams, 4] int32 in [0, nk_max), logits q.k / scale.
+        acc_out [streams, kv_heads, >= nk_max]: acc (or 0) plus each row's
+        weights; it may be acc."""
+        import torch
+
+        heads = q.shape[1] if q.dim() == 3 else 0
+        _want(q, "queries", (self.streams, heads, self.qk), None, self.device)
+        _want(out, "outputs", (self.streams, heads, self.vd), q.dtype, self.device)
+        _want(spans, "spans", (self.streams, 4), torch.int32, self.device)
+        acc_cap = 0
+        if acc_out is not None:
+            acc_cap = self._acc(acc_out, "weights", nk_max)
+            if acc is not None and self._acc(acc, "weights", nk_max) != acc_cap:
+                raise CQPanic(f"needle: weights of {acc.shape[-1]} rows to {acc_cap}")
+        elif acc is not None:
+            raise CQPanic("needle: weights without an output for them")
+        with _on(self.device) as st:
+            check(lib().kv_attend_paged_dev(self._ref, out.data_ptr(), 0, q.data_ptr(), 0, _type(q, "queries"),
+                                            self.streams, heads, spans.data_ptr(), nk_max, scale, _ptr(acc),
+                                            _ptr(acc_out), acc_cap, st))
+
+    def evict_dev(self, dst_pages, acc, acc_out, length, length_out, kept, nk_max, sink=0, recent=0):
+        """Each stream's first length[b] (<= nk_max) rows cut to keep =
+        kept.shape[2] a key head: the first `sink`, the last `recent`, and the
+        others of the largest acc, in order, written to the rows of dst_pages
+        [streams, pages] of the same pool, which no source row is read from.
+        kept [streams, kv_heads, keep] int32 gets their numbers, acc_out
+        [streams, kv_heads, >= keep] their weights, length_out[b] their count."""
+        import torch
+
+        keep = kept.shape[2] if kept.dim() == 3 else 0
+        _want(kept, "kept rows", (self.streams, self.kv_heads, keep), torch.int32, self.device)
+        _want(dst_pages, "page table", (self.streams, dst_pages.shape[-1]), torch.int32, self.device)
+        _want(length, "lengths", (self.streams,), torch.int32, self.device)
+        _want(length_out, "lengths", (self.streams,), torch.int32, self.device)
+        acc_cap, out_cap = self._acc(acc, "weights", nk_max), self._acc(acc_out, "weights", keep)
+        with _on(self.device) as st:
+            check(lib().kv_evict_paged_dev(self._ref, dst_pages.data_ptr(), dst_pages.shape[1], acc.data_ptr(), acc_cap,
+                                           acc_out.data_ptr(), out_cap, length.data_ptr(), length_out.data_ptr(),
+                                           kept.data_ptr(), self.streams, nk_max, keep, sink, recent, st))
+
+
+def cross_attend_dev(out, q, k, v, scale, q_len=None, k_len=None, index=None):
+    """Cross-attention to encoder states of other lengths: q [streams, t,
+    heads, qk] and out [streams, t, heads, vd] (any stream and row strides)
+    over memories k [memories, frames, kv_heads, qk], v [memories, frames,
+    kv_heads, vd] (any strides but the last), all of one type (float32,
+    float16, bfloat16), logits q.k / scale. q_len [streams]: rows past it are
+    left as they were; k_len [memories]: frames past it are not attended;
+    index [streams]: the memory each stream reads (beams share one)."""
+    import torch
+
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or out.dim() != 4:
+        raise CQPanic("needle: cross-attention of [streams, rows, heads, width]")
+    B, t, heads, qk = q.shape
+    M, frames, kv_heads, _ = k.shape
+    vd, dev = v.shape[3], q.device
+    _want(q, "queries", q.shape, None, None, dense=False)
+    _want(out, "outputs", (B, t, heads, vd), q.dtype, dev, dense=False)
+    _want(k, "keys", (M, frames, kv_heads, qk), q.dtype, dev, dense=False)
+    _want(v, "values", (M, frames, kv_heads, vd), q.dtype, dev, dense=False)
+    for x, w, what in ((q, qk, "queries"), (out, vd, "outputs")):
+        if x.stride(3) != 1 or (x.stride(2) != w and heads > 1):
+            raise CQPanic(f"needle: {what} whose heads are not side by side")
+    if k.stride(3) != 1 or v.stride(3) != 1:
+        raise CQPanic("needle: memories whose values are not side by side")
+    for x, n, what in ((q_len, B, "query lengths"), (k_len, M, "memory lengths"), (index, B, "memory index")):
+        if x is not None:
+            _want(x, what, (n,), torch.int32, dev)
+    y = CrossLayout(q.stride(0), q.stride(1), out.stride(0), out.stride(1), k.stride(0), k.stride(1), k.stride(2),
+                    v.stride(0), v.stride(1), v.stride(2))
+    with _on(dev) as st:
+        check(lib().nd_cross_attend_dev(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _type(q, "queries"),
+                                        ctypes.byref(y), B, t, heads, kv_heads, qk, vd, M, frames, _ptr(q_len),
+                                        _ptr(k_len), _ptr(index), scale, st))
+
+
+def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
+    """From logits [rows, n] (float32, float16, bfloat16; any row stride), in
+    one pass: lp [rows] the log probabilities of tokens [rows] int32 (0 for a
+    negative one, a padded row), ent [rows] the entropies, top [rows, k]
+    int32 and top_lp [rows, k] the k <= 64 likeliest tokens, the lowest first
+    among equals, with their log probabilities."""
+    import torch
+
+    if logits.dim() != 2:
+        raise CQPanic(f"needle: logits of shape {tuple(logits.shape)}, not rows of them")
+    rows, n = logits.shape
+    dev, f32 = logits.device, torch.float32
+    _want(logits, "logits", (rows, n), None, None, dense=False)
+    if n > 1 and logits.stride(1) != 1:
+        raise CQPanic("needle: logits whose rows are not contiguous")
+    k = top.shape[1] if top is not None and top.dim() == 2 else 0
+    for x, shape, dtype, what in ((tokens, (rows,), torch.int32, "tokens"), (lp, (rows,), f32, "log probabilities"),
+                                  (ent, (rows,), f32, "entropies"), (top, (rows, k), torch.int32, "alternatives"),
+                                  (top_lp, (rows, k), f32, "alternatives' log probabilities")):
+        if x is not None:
+            _want(x, what, shape, dtype, dev)
+    with _on(dev) as st:
+        check(lib().nd_logprobs_dev(_ptr(lp), _ptr(ent), _ptr(top) if k else None, _ptr(top_lp) if k else None,
+                                    logits.data_ptr(), logits.stride(0), _type(logits, "logits"), rows, n, _ptr(tokens),
+                                    k, st))

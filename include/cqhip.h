@@ -464,6 +464,122 @@ int nd_gather_rows_dev(float *dst, const float *src, const int32_t *idx, int row
  * (internal/needle/load.go:120-123; internal/decoder/cross.go:240-248). */
 int nd_sigmoid_gate_dev(float *out, float *gate, long long n, void *stream);
 
+/* ---- float and int8 caches of any length, and what a step answers with ---- */
+
+/* Types of the values the calls below read and write. */
+enum {
+    ND_F32 = 0,
+    ND_F16 = 1,
+    ND_BF16 = 2,
+    ND_I8 = 3, /* caches only: codes with one float32 scale a row and head, as QuantizeRow gives them (int8.go:36-55) */
+};
+
+/* Paged key and value caches: pools of pool_pages pages of page_rows rows (a
+ * power of two) of kv_heads keys of qk and values of vd of one type, scales
+ * [row][kv_heads] beside int8 ones (else null). Row j of stream b is row
+ * pages[b*page_stride + j/page_rows]*page_rows + j%page_rows of the pools, as
+ * kv_attend_int8_paged_dev reads them. Device pointers; the pools 16-byte
+ * aligned. qk and vd are multiples of 16 up to 256; pool_pages * page_rows
+ * is below 2^31. */
+typedef struct kv_paged {
+    void *k, *v;
+    float *ks, *vs;
+    const int32_t *pages;
+    int type, kv_heads, qk, vd;
+    int page_stride, page_rows, pool_pages;
+} kv_paged;
+
+/* Rows of keys and values appended to paged caches of any type: Int8Rows.
+ * Append and its float counterpart (internal/needle/int8.go:125-141,
+ * cache.go:88-125) for t rows of each of `batch` streams. Row i < rows[b]
+ * (null: t; counts outside [0, t] append nothing) of stream b goes to row
+ * pos[b] + i of its cache; rows outside [0, cap), and rows in pages outside
+ * the pool, are skipped. k and v hold values of `type` (ND_F32, ND_F16 or
+ * ND_BF16): row i of stream b is kv_heads*qk (kv_heads*vd) values at element
+ * b*k_stream + i*k_row (b*v_stream + i*v_row). Rounded to the cache's type to
+ * the nearest even; int8 rows are quantized per head as QuantizeRow does, bit
+ * for bit. acc non-null ([batch][kv_heads][acc_cap], acc_cap >= cap): the
+ * appended rows' accumulated weights become 0. Rows of one call that land in
+ * the same place race. */
+int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
+                        long long v_stream, long long v_row, int type, int batch, int t, const int32_t *rows,
+                        const int32_t *pos, int cap, float *acc, long long acc_cap, void *stream);
+/* Attention of one new token a stream over its paged cache, the work split
+ * over the cache's length and joined where there are few streams: the float
+ * form of kv_attend_int8_paged_dev (AttendInt8Spans with a float query,
+ * internal/needle/int8.go:208-300) for caches of any type and length. Logits
+ * are q.k / scale; the softmax, its sums and the products' sums are float32.
+ * q and out hold values of `type`: batch streams of heads*qk (heads*vd),
+ * q_stride (out_stride) elements apart (0: dense). Query head h reads key
+ * head h / (heads/kv_heads). spans are [batch][4] as kv_attend_int8_dev
+ * takes them for t = 1: {lo0, hi0, lo1, hi1}, ascending, disjoint and inside
+ * [0, nk_max); others leave the stream's output as it was, and spans with no
+ * key give zeros. A page outside the pool reads page 0.
+ * acc_out non-null ([batch][kv_heads][acc_cap], acc_cap >= nk_max): for
+ * each row j of the spans, acc_out[j] = acc[j] (null: 0) + the sum over the
+ * key head's query heads of their softmax weights; other entries are left
+ * as they were. acc_out may be acc. */
+int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, const void *q, long long q_stride,
+                        int type, int batch, int heads, const int32_t *spans, int nk_max, float scale,
+                        const float *acc, float *acc_out, long long acc_cap, void *stream);
+/* Eviction from paged caches by accumulated attention weight (acc of
+ * kv_attend_paged_dev): of stream b's len[b] rows every key head keeps the
+ * first `sink`, the last `recent`, and of the others those of the largest
+ * weights, `keep` in all (every row where len[b] <= keep); among equal
+ * weights the lowest row; a NaN weight counts as the least. The kept rows
+ * are written in their order to the front of the cache that dst_pages
+ * ([batch][dst_stride] of the same pool, dst_stride * page_rows >= keep)
+ * names, whose pages are none that any stream's rows are read from. The
+ * source pages are only read, so streams that share them after a fork may be
+ * evicted apart. kept ([batch][kv_heads][keep]) gets the kept rows'
+ * numbers, -1 past the last; acc_out ([batch][kv_heads][acc_out_cap],
+ * acc_out_cap >= keep, not acc) their weights; len_out[b] = min(len[b],
+ * keep) (len_out may be len). A stream whose len is outside [0, nk_max] is
+ * left as it was, len_out too. sink + recent <= keep. */
+int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
+                       long long acc_cap, float *acc_out, long long acc_out_cap, const int32_t *len, int32_t *len_out,
+                       int32_t *kept, int batch, int nk_max, int keep, int sink, int recent, void *stream);
+
+/* Where the rows of nd_cross_attend_dev's operands are, in elements: row i
+ * of stream b's queries at b*q_stream + i*q_row (heads side by side, qk
+ * apart), outputs likewise (vd apart); row j of memory m, key head h at
+ * m*k_stream + j*k_row + h*k_head, values likewise. */
+typedef struct nd_cross_layout {
+    long long q_stream, q_row, out_stream, out_row;
+    long long k_stream, k_row, k_head, v_stream, v_row, v_head;
+} nd_cross_layout;
+
+/* Cross-attention to encoder states of other lengths, in floats: the float
+ * form of cross.attend (internal/decoder/cross.go:273-320) for one or many
+ * query rows of many streams. q, k, v and out hold values of `type` (ND_F32,
+ * ND_F16, ND_BF16). Row i < q_len[b] (null: t; clamped to [0, t]) of stream b
+ * attends the first k_len[m] (null: frames; clamped to [0, frames]) of the
+ * `frames` rows of memory m = index[b] (null: b), logits q.k / scale; rows
+ * past q_len, and streams whose index is outside [0, memories), leave their
+ * outputs as they were; an empty memory gives zeros. Query head h reads key
+ * head h / (heads/kv_heads). layout null: dense [batch][t][heads][width] and
+ * [memories][frames][kv_heads][width]. qk and vd are multiples of 16 up to
+ * 256; k, v and their strides are multiples of 16 bytes. ND_F32 products are
+ * float32; with 16-bit types the products take them as they are, sums and
+ * softmax are float32. */
+int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
+                        const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
+                        int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,
+                        float scale, void *stream);
+/* What a step or a teacher-forced hypothesis answers with, from rows of n
+ * logits of `type`, `stride` elements apart, in one pass: lp[r] the log
+ * probability of tokens[r] under the row's softmax (a negative token, a
+ * padded row, gives 0; one past n NaN), ent[r] the softmax's entropy in nats,
+ * and top_idx / top_lp [rows][top] the `top` likeliest tokens, the lowest
+ * index first among equals, with their log probabilities (top <= 64, <= n).
+ * lp, ent and the pair of tops may each be null. The log probabilities of
+ * internal/search's beams (beam.go:501-540) and the alternatives of
+ * greedy's argmax (greedy.go:181-191). Sums are float32. A row of -inf
+ * alone has lp -inf and entropy 0; a NaN or +inf makes the row's values
+ * NaN, a NaN ranking as -inf. */
+int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, const void *logits, long long stride,
+                    int type, int rows, int n, const int32_t *tokens, int top, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
