@@ -2334,9 +2334,17 @@ static int split_parts(long long lists, int nk) {
 
 // The launches of a split attention with the partials' workspace.
 static int run_split_attend(SplitArgs &a, bool weights, hipStream_t stream) {
-    const int group = a.heads / a.c.kv_heads;
-    const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((static_cast<long long>(a.t) * group + 15) / 16);
-    a.splits = split_parts(lists, a.nk_max);
+    const long long cols = static_cast<long long>(a.t) * (a.heads / a.c.kv_heads);
+    const bool many = !a.spans && a.type != ND_F32 && cols > 16;
+    const int cus = device_info().cus;
+    const int wg_cols = many ? cross_workgroup_columns(a, cus) : 16;
+    const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((cols + wg_cols - 1) / wg_cols);
+    // The matrix form's partials cost more than idle CUs as long as the lists
+    // give half of the CUs a workgroup (8 x 448 rows of 8 heads of 48 over 2,
+    // 1500 frames, 224 workgroups: 31.9 us whole, 44.1 in two parts; 2 x 448
+    // rows of 8 heads of 64, 64 workgroups: 20.9 in four, 24.1 in two).
+    a.splits = many ? static_cast<int>(std::max<long long>(1, std::min<long long>(cus / lists, a.nk_max / 256)))
+                    : split_parts(lists, a.nk_max);
     const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
     const long long wblocks = weights ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
     if (lists * a.splits > grid_limit(256) || (rows + 3) / 4 > grid_limit(256) || wblocks > grid_limit(256))
@@ -2353,7 +2361,7 @@ static int run_split_attend(SplitArgs &a, bool weights, hipStream_t stream) {
         a.part_ml = reinterpret_cast<float *>(base + part);
         if (weights) a.logits = reinterpret_cast<float *>(base + part + ml);
     }
-    HIP_TRY(launch_attend_split(a, stream), "split attention launch");
+    HIP_TRY(many ? launch_cross_attend(a, cus, stream) : launch_attend_split(a, stream), "split attention launch");
     return CQ_OK;
 }
 
@@ -2367,7 +2375,7 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: queries of type %d", type);
     if (heads <= 0 || heads % c->kv_heads != 0)
         return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, c->kv_heads);
-    if (!(std::isfinite(scale) && scale != 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (!(std::isfinite(scale) && scale > 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
     if (acc_out && acc_cap < nk_max) return fail(CQ_ERR_MISUSE, "needle: %lld weights for %d keys", acc_cap, nk_max);
     if (heads / c->kv_heads > 1024) return fail(CQ_ERR_UNSUPPORTED, "needle: %d heads a KV head", heads / c->kv_heads);
     if (batch == 0) return CQ_OK;
@@ -2445,7 +2453,7 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
         return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, kv_heads);
     if (!split_widths_ok(qk, vd))
         return fail(CQ_ERR_UNSUPPORTED, "needle: cross-attention heads of %d and %d (multiples of 16 up to 256)", qk, vd);
-    if (!(std::isfinite(scale) && scale != 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (!(std::isfinite(scale) && scale > 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
     if (batch == 0 || t == 0) return CQ_OK;
     if (!out || !q || (memories > 0 && frames > 0 && (!k || !v)))
         return fail(CQ_ERR_MISUSE, "needle: cross-attention with a nil operand");
@@ -2518,9 +2526,10 @@ int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, cons
     if (reinterpret_cast<uintptr_t>(logits) % value_size(type))
         return fail(CQ_ERR_MISUSE, "needle: logits that are not aligned to their type");
     LogprobArgs a{lp, ent, top_lp, top_idx, logits, stride, type, rows, n, top_idx ? top : 0, tokens, 1, n, nullptr};
-    const int most = logprob_chunk();
+    const int most = logprob_chunk(
+        ((reinterpret_cast<uintptr_t>(logits) | static_cast<uintptr_t>(rows > 1 ? stride : 0) * value_size(type)) & 15) == 0);
     a.splits = (n + most - 1) / most;
-    a.chunk = (n + a.splits - 1) / a.splits;
+    a.chunk = ((n + a.splits - 1) / a.splits + 7) / 8 * 8;
     if (static_cast<long long>(rows) * a.splits > grid_limit(512))
         return fail(CQ_ERR_UNSUPPORTED, "needle: log probabilities of %d rows of %d", rows, n);
     WsScope ws;

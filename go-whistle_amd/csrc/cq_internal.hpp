@@ -531,8 +531,14 @@ struct SplitArgs {
 };
 bool split_widths_ok(int qk, int vd);
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);
+// The parts of every output row joined.
+hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s);
+// The same attention of many columns to 16-bit memories of the queries' type
+// (cross_kernels.hip); the columns a workgroup takes.
+int cross_workgroup_columns(const SplitArgs &a, int cus);
+hipError_t launch_cross_attend(const SplitArgs &a, int cus, hipStream_t s);
 
-// nd_logprobs_dev: `splits` parts of `chunk` logits a row; the parts' results
+// nd_logprobs_dev: `splits` parts of `chunk` logits (a multiple of 8) a row; the parts' results
 // (splits > 1) in part: {m, l, t} and top pairs {value, index bits}.
 struct LogprobArgs {
     float *lp, *ent, *top_lp;
@@ -544,7 +550,8 @@ struct LogprobArgs {
     int splits, chunk;
     float *part;
 };
-int logprob_chunk();
+// The logits a part may have, where every row starts on a 16-byte boundary or not.
+int logprob_chunk(bool aligned);
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s);
 
 }  // namespace cqhip

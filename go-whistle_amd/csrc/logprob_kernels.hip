@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kLpThreads = 512;
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kVals = 32;  // logits a thread holds
+constexpr int kLpVals = 32;  // logits a thread holds
 
 // A logit's place in the order of alternatives: the larger value, then the
 // lower index; a NaN as -inf, -0 as 0. 0 is below every logit.
@@ -55,34 +55,95 @@ __device__ __forceinline__ void write_row(const LogprobArgs &a, int r, const Row
     if (a.ent) a.ent[r] = entropy(s);
 }
 
+// A wavefront's lanes' values in falling order: lane i has the i-th largest
+// (a bitonic sort; no NaN).
+__device__ __forceinline__ float sort_lanes(float x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+        for (int h = size >> 1; h > 0; h >>= 1) {
+            const float y = xor_lane(x, h);
+            // the lower lane of a pair keeps the larger value in falling runs
+            const bool larger = ((lane & h) == 0) == ((lane & size) == 0 || size == 64);
+            x = larger ? fmaxf(x, y) : fminf(x, y);
+        }
+    return x;
+}
+
+// A thread's values are pieces of 16 bytes of the row, kLpThreads pieces
+// apart: piece g covers the part's values kPer g - shift and on, shift the
+// distance of the part's first value from the 16-byte boundary before it.
+// Pieces across an end of the part are read value by value.
+//
+// The alternatives: the `top`-th largest of 64 lanes' maxima is a bound that
+// at least `top` values of the part reach, and the largest such bound of the
+// wavefronts leaves few more (about 20 of 16,384 normal values for 10). Those
+// are listed in LDS and ranked by counting. A list of more than kLpList (equal
+// values, more than about 40 alternatives) takes them one after the other.
+constexpr int kLpList = 512;
+
 template <int TYPE>
-__global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
-    __shared__ float red[3][kLpWaves];
-    __shared__ unsigned long long best_sh[kLpWaves];
+__global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
+    constexpr int kPer = TYPE == 0 ? 4 : 8;
+    constexpr int kLpPieces = kLpVals / kPer;
+    __shared__ float red[4][kLpWaves];
+    __shared__ unsigned long long list[kLpList];
+    __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int part = blockIdx.x % a.splits, r = blockIdx.x / a.splits;
-    const int i0 = part * a.chunk, i1 = min(i0 + a.chunk, a.n);
-    const long long base = static_cast<long long>(r) * a.stride;
+    const int i0 = part * a.chunk, count = min(a.chunk, a.n - i0);
+    const long long base = static_cast<long long>(r) * a.stride + i0;
+    const uintptr_t first = reinterpret_cast<uintptr_t>(a.x) + static_cast<uintptr_t>(base) * (16 / kPer);
+    const int shift = static_cast<int>(first & 15) / (16 / kPer);
+    // value e of piece k: place kPer (tid + k kLpThreads) + e - shift of the part
+    auto place = [&](int k) { return kPer * (tid + k * kLpThreads) - shift; };
 
-    float v[kVals];
+    if (tid == 0) listed = 0;
+    float v[kLpVals];
     float m = -INFINITY, bad = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kVals; ++k) {
-        const int i = i0 + tid + k * kLpThreads;
-        v[k] = i < i1 ? logit_at(a.x, TYPE, base + i) : -INFINITY;
-        m = fmaxf(m, v[k]);
-    }
-    // block maximum
+    for (int k = 0; k < kLpPieces; ++k) {
+        const int i = place(k);
+        if (i >= 0 && i + kPer <= count) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(first + static_cast<long long>(i) * (16 / kPer));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (lane == 0) red[0][wave] = m;
+            for (int e = 0; e < kPer; ++e) {
+                if constexpr (TYPE == 0) {
+                    v[k * kPer + e] = __uint_as_float(u[e]);
+                } else if constexpr (TYPE == 1) {
+                    v[k * kPer + e] = static_cast<float>(
+                        __builtin_bit_cast(_Float16, static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)))));
+                } else {
+                    v[k * kPer + e] = __uint_as_float((e & 1) ? (u[e >> 1] & 0xffff0000u) : (u[e >> 1] << 16));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                v[k * kPer + e] = i + e >= 0 && i + e < count ? logit_at(a.x, TYPE, base + i + e) : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kLpVals; ++k) m = fmaxf(m, v[k]);
+    float bound = -INFINITY;
+    if (a.top > 0) {
+        const float sorted = sort_lanes(m);
+        bound = __shfl(sorted, a.top - 1);
+        m = __shfl(sorted, 0);
+    } else {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, xor_lane(m, o));
+    }
+    if (lane == 0) red[0][wave] = m, red[3][wave] = bound;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) m = fmaxf(m, red[0][w]);
+    for (int w = 0; w < kLpWaves; ++w) m = fmaxf(m, red[0][w]), bound = fmaxf(bound, red[3][w]);
     const float mu = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, t = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kVals; ++k) {
+    for (int k = 0; k < kLpVals; ++k) {
         const float d = v[k] - mu;
         const float e = __expf(d);
         l += e;
@@ -90,10 +151,20 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
         if (v[k] != v[k]) bad = NAN;
     }
     l += bad;
+    if (a.top > 0) {
+#pragma unroll
+        for (int k = 0; k < kLpVals; ++k) {
+            const int i = place(k / kPer) + k % kPer;
+            if (!(v[k] < bound) && i >= 0 && i < count) {
+                const int at = atomicAdd(&listed, 1);
+                if (at < kLpList) list[at] = rank_key(v[k], i);
+            }
+        }
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-        l += __shfl_xor(l, o);
-        t += __shfl_xor(t, o);
+        l += xor_lane(l, o);
+        t += xor_lane(t, o);
     }
     if (lane == 0) red[1][wave] = l, red[2][wave] = t;
     __syncthreads();
@@ -111,17 +182,40 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
             pt[2] = t;
         }
     }
-    // The alternatives, one after the other: every thread offers its largest
-    // below the last one chosen.
+    // alternative q: the value of key `best` (0: the part has fewer)
+    auto answer = [&](int q, unsigned long long best) {
+        const int i = i0 + key_index(best);
+        if (a.splits > 1) {
+            pt[4 + 2 * q] = best ? logit_at(a.x, TYPE, base - i0 + i) : -INFINITY;
+            pt[5 + 2 * q] = __int_as_float(best ? i : -1);
+        } else {
+            a.top_idx[static_cast<long long>(r) * a.top + q] = i;
+            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, TYPE, base + i));
+        }
+    };
+    if (a.top == 0) return;
+    const int n = listed;
+    if (n <= kLpList) {
+        if (tid < n) {
+            const unsigned long long mine = list[tid];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += list[j] > mine;
+            if (rank < a.top) answer(rank, mine);
+        } else if (tid < a.top) {
+            answer(tid, 0);
+        }
+        return;
+    }
+    // one after the other: every thread offers its largest below the last one chosen
     unsigned long long mine = 0, last = ~0ull;
     for (int q = 0; q < a.top; ++q) {
         if (q == 0 || mine == last) {
             mine = 0;
 #pragma unroll
-            for (int k = 0; k < kVals; ++k) {
-                const int i = i0 + tid + k * kLpThreads;
+            for (int k = 0; k < kLpVals; ++k) {
+                const int i = place(k / kPer) + k % kPer;
                 const unsigned long long key = rank_key(v[k], i);
-                if (i < i1 && key < last && key > mine) mine = key;
+                if (i >= 0 && i < count && key < last && key > mine) mine = key;
             }
         }
         unsigned long long best = mine;
@@ -131,23 +225,13 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
             if (other > best) best = other;
         }
         __syncthreads();
-        if (lane == 0) best_sh[wave] = best;
+        if (lane == 0) list[wave] = best;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kLpWaves; ++w)
-            if (best_sh[w] > best) best = best_sh[w];
+            if (list[w] > best) best = list[w];
         last = best;
-        if (tid == 0) {
-            const int i = key_index(best);
-            if (a.splits > 1) {
-                // a part of fewer than `top` logits offers index -1
-                pt[4 + 2 * q] = best ? logit_at(a.x, TYPE, base + i) : -INFINITY;
-                pt[5 + 2 * q] = __int_as_float(best ? i : -1);
-            } else {
-                a.top_idx[static_cast<long long>(r) * a.top + q] = i;
-                a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, TYPE, base + i));
-            }
-        }
+        if (tid == 0) answer(q, best);
     }
 }
 
@@ -211,7 +295,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
 
 }  // namespace
 
-int logprob_chunk() { return kLpThreads * kVals; }
+int logprob_chunk(bool aligned) { return kLpThreads * kLpVals - (aligned ? 0 : 8); }  // less a piece where rows start inside one
 
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(static_cast<long long>(a.rows) * a.splits));

@@ -416,6 +416,12 @@ hipError_t launch_split_width(const SplitArgs &a, int col_tiles, unsigned grid, 
 
 bool split_widths_ok(int qk, int vd) { return qk > 0 && vd > 0 && qk % 16 == 0 && vd % 16 == 0 && qk <= 256 && vd <= 256; }
 
+hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {
+    const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
+    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a, rows);
+    return hipGetLastError();
+}
+
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s) {
     const int group = a.heads / a.c.kv_heads;
     const int col_tiles = (a.t * group + kCols - 1) / kCols;
@@ -425,8 +431,7 @@ hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s) {
                    : a.c.type == 2 ? launch_split_width<2>(a, col_tiles, grid, s)
                                    : launch_split_width<3>(a, col_tiles, grid, s);
     if (e != hipSuccess || !a.part) return e;
-    const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
-    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a, rows);
+    if ((e = launch_attend_join(a, s)) != hipSuccess) return e;
     if (a.acc_out) {
         const int blocks = (a.nk_max + 255) / 256;
         hipLaunchKernelGGL(attend_weights_kernel, dim3(static_cast<unsigned>(a.batch) * a.c.kv_heads * blocks),

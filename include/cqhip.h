@@ -508,7 +508,8 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * over the cache's length and joined where there are few streams: the float
  * form of kv_attend_int8_paged_dev (AttendInt8Spans with a float query,
  * internal/needle/int8.go:208-300) for caches of any type and length. Logits
- * are q.k / scale; the softmax, its sums and the products' sums are float32.
+ * are q.k / scale (scale > 0); the softmax, its sums and the products' sums
+ * are float32.
  * q and out hold values of `type`: batch streams of heads*qk (heads*vd),
  * q_stride (out_stride) elements apart (0: dense). Query head h reads key
  * head h / (heads/kv_heads). spans are [batch][4] as kv_attend_int8_dev
@@ -554,14 +555,14 @@ typedef struct nd_cross_layout {
  * query rows of many streams. q, k, v and out hold values of `type` (ND_F32,
  * ND_F16, ND_BF16). Row i < q_len[b] (null: t; clamped to [0, t]) of stream b
  * attends the first k_len[m] (null: frames; clamped to [0, frames]) of the
- * `frames` rows of memory m = index[b] (null: b), logits q.k / scale; rows
+ * `frames` rows of memory m = index[b] (null: b), logits q.k / scale (> 0); rows
  * past q_len, and streams whose index is outside [0, memories), leave their
  * outputs as they were; an empty memory gives zeros. Query head h reads key
  * head h / (heads/kv_heads). layout null: dense [batch][t][heads][width] and
  * [memories][frames][kv_heads][width]. qk and vd are multiples of 16 up to
  * 256; k, v and their strides are multiples of 16 bytes. ND_F32 products are
- * float32; with 16-bit types the products take them as they are, sums and
- * softmax are float32. */
+ * float32; with 16-bit types the products take them as they are and, for many
+ * rows, the softmax weights rounded to the type; sums and softmax are float32. */
 int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
                         const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
                         int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,
