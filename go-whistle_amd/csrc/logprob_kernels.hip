@@ -80,11 +80,12 @@ __device__ __forceinline__ float sort_lanes(float x) {
 // at least `top` values of the part reach, and the largest such bound of the
 // wavefronts leaves few more (about 20 of 16,384 normal values for 10). Those
 // are listed in LDS and ranked by counting. A list of more than kLpList (equal
-// values, more than about 40 alternatives) takes them one after the other.
+// values, more than about 40 alternatives) takes them one after the other,
+// reading the part again: its values' registers are not held for that.
 constexpr int kLpList = 512;
 
 template <int TYPE>
-__global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     constexpr int kPer = TYPE == 0 ? 4 : 8;
     constexpr int kLpPieces = kLpVals / kPer;
     __shared__ float red[4][kLpWaves];
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
 
     if (tid == 0) listed = 0;
     float v[kLpVals];
-    float m = -INFINITY, bad = 0.0f;
+    float m = -INFINITY, most[kLpPieces];
 #pragma unroll
     for (int k = 0; k < kLpPieces; ++k) {
         const int i = place(k);
@@ -126,7 +127,12 @@ __global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
         }
     }
 #pragma unroll
-    for (int k = 0; k < kLpVals; ++k) m = fmaxf(m, v[k]);
+    for (int k = 0; k < kLpPieces; ++k) {
+        most[k] = v[k * kPer];
+#pragma unroll
+        for (int e = 1; e < kPer; ++e) most[k] = fmaxf(most[k], v[k * kPer + e]);
+        m = fmaxf(m, most[k]);
+    }
     float bound = -INFINITY;
     if (a.top > 0) {
         const float sorted = sort_lanes(m);
@@ -146,20 +152,22 @@ __global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
     for (int k = 0; k < kLpVals; ++k) {
         const float d = v[k] - mu;
         const float e = __expf(d);
-        l += e;
-        t += e > 0.0f ? e * d : 0.0f;
-        if (v[k] != v[k]) bad = NAN;
+        l += e;                                // a NaN among the logits is one here
+        t = fmaf(e, fmaxf(d, -0x1p100f), t);  // 0 for -inf
     }
-    l += bad;
     if (a.top > 0) {
 #pragma unroll
-        for (int k = 0; k < kLpVals; ++k) {
-            const int i = place(k / kPer) + k % kPer;
-            if (!(v[k] < bound) && i >= 0 && i < count) {
-                const int at = atomicAdd(&listed, 1);
-                if (at < kLpList) list[at] = rank_key(v[k], i);
+        for (int k = 0; k < kLpPieces; ++k)
+            if (!(most[k] < bound)) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const int i = place(k) + e;
+                    if (!(v[k * kPer + e] < bound) && i >= 0 && i < count) {
+                        const int at = atomicAdd(&listed, 1);
+                        if (at < kLpList) list[at] = rank_key(v[k * kPer + e], i);
+                    }
+                }
             }
-        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -211,11 +219,9 @@ __global__ __launch_bounds__(kLpThreads, 8) void logprob_kernel(LogprobArgs a) {
     for (int q = 0; q < a.top; ++q) {
         if (q == 0 || mine == last) {
             mine = 0;
-#pragma unroll
-            for (int k = 0; k < kLpVals; ++k) {
-                const int i = place(k / kPer) + k % kPer;
-                const unsigned long long key = rank_key(v[k], i);
-                if (i >= 0 && i < count && key < last && key > mine) mine = key;
+            for (int i = tid; i < count; i += kLpThreads) {
+                const unsigned long long key = rank_key(logit_at(a.x, TYPE, base + i), i);
+                if (key < last && key > mine) mine = key;
             }
         }
         unsigned long long best = mine;
