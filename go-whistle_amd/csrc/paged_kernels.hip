@@ -114,49 +114,38 @@ hipError_t launch_append_type(const PagedAppendArgs &a, int vec, hipStream_t s) 
 
 // ---- eviction -------------------------------------------------------------------
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024;  // at most
 
 // A weight's place in the order of weights: larger is kept sooner. Held rows
 // (the first sink, the last recent) come before every weight; -0 is 0; a NaN
 // is the least.
 __device__ __forceinline__ uint32_t weight_key(float w, bool held) {
-    if (held) return 0xffffffffu;
-    if (w != w) return 0;
-    const uint32_t u = __float_as_uint(w + 0.0f);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(w + 0.0f), s = static_cast<uint32_t>(static_cast<int32_t>(u) >> 31);
+    const uint32_t k = u ^ (s | 0x80000000u);
+    return held ? 0xffffffffu : w != w ? 0 : k;
 }
 
-// The sum of v over the workgroup's threads before this one, and over all.
-__device__ __forceinline__ int scan_before(int v, int *sh, int &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();
-    if (lane == 63) sh[wave] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-        if (w < wave) before += sh[w];
-        total += sh[w];
-    }
-    return before + s - v;
+template <int H>
+__device__ __forceinline__ int add_lane(int c) {
+    return c + __builtin_bit_cast(int, xor_lane<H>(__builtin_bit_cast(float, c)));
+}
+__device__ __forceinline__ int wave_sum(int c) {
+    return add_lane<32>(add_lane<16>(add_lane<8>(add_lane<4>(add_lane<2>(add_lane<1>(c))))));
 }
 
-// The kept rows of one (stream, key head): the keep-th largest key by a radix
-// selection of four 8-bit digits (a 256-entry histogram in LDS each), then
-// one ordered pass that writes the rows above it, and the lowest of those
-// equal to it, in row order. Integer counts throughout: the same rows in
-// every run.
+// The kept rows of one (stream, key head). Row k of a thread is row
+// (wavefront * per + k) * 64 + lane, its key in a register (V = 0: read
+// each time, for lists past 32,768). The keep-th largest key is built from its
+// highest bits down: bits stay set if at least `keep` keys reach the value
+// with them (a histogram's atomics would meet in the few exponents that weights
+// have: 30 us for 448 rows), until exactly `keep` do.
+// Then one pass in row order writes the rows above the key, and the lowest of
+// those equal to it. Integer counts throughout: the same rows in every run.
+template <int V>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-    __shared__ int hist[256];
-    __shared__ int scan_sh[kSelThreads / 64];
-    __shared__ int digit_sh, need_sh;
-    const int tid = threadIdx.x;
+    __shared__ int count_sh[32][3];  // a turn's counts over the wavefronts
+    __shared__ int wave_sh[2][kSelThreads / 64];
+    const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6, lane = tid & 63;
     const int h = blockIdx.x % a.c.kv_heads, b = blockIdx.x / a.c.kv_heads;
     const int n = a.len[b];
     if (n < 0 || n > a.nk_max) return;
@@ -164,98 +153,175 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     const float *w = a.acc + bh * a.acc_cap;
     int32_t *kept = a.kept + bh * a.keep;
     float *out = a.acc_out + bh * a.acc_out_cap;
-    const int live = min(n, a.keep);
-    for (int i = live + tid; i < a.keep; i += kSelThreads) kept[i] = -1;
+    for (int i = min(n, a.keep) + tid; i < a.keep; i += threads) kept[i] = -1;
     if (n <= a.keep) {
-        for (int i = tid; i < n; i += kSelThreads) {
+        for (int i = tid; i < n; i += threads) {
             kept[i] = i;
             out[i] = w[i];
         }
         return;
     }
     if (a.keep == 0) return;
-    auto key_of = [&](int j) { return weight_key(w[j], j < a.sink || j >= n - a.recent); };
-    // the keep-th largest key, and how many of the rows that equal it are kept
+    const int per = V ? V : (n + threads - 1) / threads, row0 = wave * per * 64 + lane;  // row k: row0 + 64 k
+    if (tid < 96) (&count_sh[0][0])[tid] = 0;
+    if (threads < 96) (&count_sh[0][0])[min(tid + 64, 95)] = 0;
+    __syncthreads();
+    auto key_at = [&](int j, float x) { return j < n ? weight_key(x, (j < a.sink) | (j >= n - a.recent)) : 0; };
+    float weights[V ? V : 1];
+    uint32_t keys[V ? V : 1];
+    if constexpr (V > 0) {  // all loads in flight before the first is used
+#pragma unroll
+        for (int k = 0; k < V; ++k) weights[k] = w[min(row0 + 64 * k, n - 1)];
+#pragma unroll
+        for (int k = 0; k < V; ++k) keys[k] = key_at(row0 + 64 * k, weights[k]);
+    }
+    auto weight_of = [&](int k) {
+        if constexpr (V > 0)
+            return weights[k];
+        else
+            return w[min(row0 + 64 * k, n - 1)];
+    };
+    auto key_of = [&](int k) {
+        if constexpr (V > 0)
+            return keys[k];
+        else
+            return key_at(row0 + 64 * k, weight_of(k));
+    };
+    // The rows whose key reaches each of three values (above 0): counts of at
+    // most 512 a wavefront, ten bits each, so one sum serves all (V <= 8; else
+    // one value).
+    constexpr int kBits = V > 0 && V <= 8 ? 2 : 1;
+    auto reach = [&](const uint32_t (&at)[3], int turn, int (&total)[3]) {
+        int c = 0;
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                c += keys[k] >= at[0];
+                if constexpr (kBits == 2) c += (keys[k] >= at[1] ? 1 << 10 : 0) + (keys[k] >= at[2] ? 1 << 20 : 0);
+            }
+        } else {
+            for (int k = 0; k < per; ++k) c += key_of(k) >= at[0];
+        }
+        c = wave_sum(c);
+        if (lane < (kBits == 2 ? 3 : 1)) atomicAdd(&count_sh[turn][lane], kBits == 2 ? (c >> (10 * lane)) & 1023 : c);
+        __syncthreads();
+        total[0] = count_sh[turn][0];
+        total[1] = count_sh[turn][1];
+        total[2] = count_sh[turn][2];
+    };
+    // thr: the largest value that at least `keep` keys reach; `above` of them
+    // pass it. Each turn settles kBits bits of it: the least of the values
+    // with them that fewer than `keep` reach stays above it.
     uint32_t thr = 0;
-    int need = a.keep;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += kSelThreads) {
-            const uint32_t k = key_of(j);
-            if (shift == 24 || (k >> (shift + 8)) == (thr >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+    int above = 0;
+    for (int bit = 32 - kBits; bit >= 0; bit -= kBits) {
+        const uint32_t at[3] = {thr | (1u << bit), thr | (2u << bit), thr | (3u << bit)};
+        int c[3];
+        reach(at, bit / kBits, c);
+        uint32_t next = thr;
+        bool done = false;
+#pragma unroll
+        for (int z = 0; z < (kBits == 2 ? 3 : 1); ++z) {
+            if (done || c[z] < a.keep) {
+                if (!done) {
+                    above = c[z];
+                    done = true;
+                }
+                continue;
+            }
+            next = at[z];
+            if (c[z] == a.keep) {  // every key that reaches it, and no other
+                next = at[z] - 1;
+                above = c[z];
+                bit = 0;
+                done = true;
+            }
         }
-        __syncthreads();
-        if (tid == 0) {
-            int left = need, d = 255;
-            while (d > 0 && hist[d] < left) left -= hist[d--];
-            digit_sh = d;
-            need_sh = left;
-        }
-        __syncthreads();
-        thr |= static_cast<uint32_t>(digit_sh) << shift;
-        need = need_sh;
-        __syncthreads();
+        thr = next;
     }
-    // each thread a run of rows
-    const int per = (n + kSelThreads - 1) / kSelThreads;
-    const int r0 = min(tid * per, n), r1 = min(r0 + per, n);
-    int above = 0, equal = 0;
-    for (int j = r0; j < r1; ++j) {
-        const uint32_t k = key_of(j);
-        above += k > thr;
-        equal += k == thr;
+    const int need = a.keep - above;  // of the rows that equal the key, the first
+    int ups = 0, eqs = 0;
+    auto is_equal = [&](int k) { return row0 + 64 * k < n && key_of(k) == thr; };
+#pragma unroll(V ? V : 1)
+    for (int k = 0; k < (V ? V : per); ++k) {
+        ups += __popcll(__ballot(key_of(k) > thr));
+        eqs += __popcll(__ballot(is_equal(k)));
     }
-    int total;
-    int eq = scan_before(equal, scan_sh, total);
-    const int kept_eq = max(0, min(equal, need - eq));
-    int at = scan_before(above + kept_eq, scan_sh, total);
-    for (int j = r0; j < r1; ++j) {
-        const uint32_t k = key_of(j);
-        if (k > thr || (k == thr && eq++ < need)) {
-            kept[at] = j;
-            out[at] = w[j];
-            ++at;
+    if (lane == 0) wave_sh[0][wave] = ups, wave_sh[1][wave] = eqs;
+    __syncthreads();
+    int base = 0, eq_base = 0;  // rows above the key, and equal to it, before this wavefront's row k
+    for (int i = 0; i < wave; ++i) base += wave_sh[0][i], eq_base += wave_sh[1][i];
+    const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll(V ? V : 1)
+    for (int k = 0; k < (V ? V : per); ++k) {
+        const bool up_k = key_of(k) > thr, eq_k = is_equal(k);
+        const unsigned long long up = __ballot(up_k), eq = __ballot(eq_k);
+        const int e = eq_base + __popcll(eq & below);
+        if (up_k || (eq_k && e < need)) {
+            const int at = base + __popcll(up & below) + min(e, need);
+            kept[at] = row0 + 64 * k;
+            out[at] = weight_of(k);
         }
+        base += __popcll(up);
+        eq_base += __popcll(eq);
     }
 }
 
-// The kept rows copied: 16 bytes a thread, pieces of a head's key row, then of
-// its value row; row i of every head of a stream side by side, so a
-// destination row is written whole. The scales of int8 rows ride with the
-// first piece. Also the streams' new lengths.
-__global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a, int kpieces, int pieces, long long total) {
+// The kept rows copied: a thread takes 16 bytes of a head's key row and the
+// same piece of its value row, of two rows half the budget apart (each
+// destination row is written whole by its neighbours): four loads in flight behind one chain of
+// row, page and pool. The scales of int8 rows ride with the first piece. Also
+// the streams' new lengths.
+__global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a, int kpieces, int vpieces, int half_rows,
+                                                         long long total) {
     const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     if (id < a.batch) {
         const int n = a.len[id];
         if (n >= 0 && n <= a.nk_max) a.len_out[id] = min(n, a.keep);
     }
     if (id >= total) return;
-    const int per_row = pieces * a.c.kv_heads;
+    const int pieces = max(kpieces, vpieces), per_row = pieces * a.c.kv_heads;
     const long long bi = id / per_row;
     const int x = static_cast<int>(id - bi * per_row);
-    const int i = static_cast<int>(bi % a.keep), b = static_cast<int>(bi / a.keep);
+    const int h = x / pieces, p = x - h * pieces;
+    const int b = static_cast<int>(bi / half_rows), i0 = static_cast<int>(bi - static_cast<long long>(b) * half_rows);
     const int n = a.len[b];  // or already its new value: in [0, nk_max] both or neither
     if (n < 0 || n > a.nk_max) return;
-    const bool val = x >= kpieces * a.c.kv_heads;  // a row's keys of all heads, then its values
-    const int np = val ? pieces - kpieces : kpieces;
-    const int y = val ? x - kpieces * a.c.kv_heads : x;
-    const int h = y / np, p = y - h * np;
-    const int j = a.kept[(static_cast<long long>(b) * a.c.kv_heads + h) * a.keep + i];
-    if (j < 0) return;
-    int sp = a.c.pages[static_cast<long long>(b) * a.c.page_stride + (j >> a.c.shift)];
-    if (sp < 0 || sp >= a.c.pool_pages) sp = 0;
-    const int dp = a.dst_pages[static_cast<long long>(b) * a.dst_stride + (i >> a.c.shift)];
-    if (dp < 0 || dp >= a.c.pool_pages) return;
     const int mask = (1 << a.c.shift) - 1;
-    const long long from = ((static_cast<long long>(sp) << a.c.shift) + (j & mask)) * a.c.kv_heads + h;
-    const long long to = ((static_cast<long long>(dp) << a.c.shift) + (i & mask)) * a.c.kv_heads + h;
-    uint4 *pool = reinterpret_cast<uint4 *>(val ? a.c.v : a.c.k);
-    pool[to * np + p] = pool[from * np + p];
-    if (a.c.type == 3 && p == 0) {
-        float *s = val ? a.c.vs : a.c.ks;
-        s[to] = s[from];
+    const int32_t *kept = a.kept + (static_cast<long long>(b) * a.c.kv_heads + h) * a.keep;
+    uint4 kx[2], vx[2];
+    float ksc[2], vsc[2];
+    long long to[2];
+    bool ok[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const int i = i0 + z * half_rows;
+        const int j = i < a.keep ? kept[i] : -1;
+        int sp = j >= 0 ? a.c.pages[static_cast<long long>(b) * a.c.page_stride + (j >> a.c.shift)] : 0;
+        const int dp = j >= 0 ? a.dst_pages[static_cast<long long>(b) * a.dst_stride + (i >> a.c.shift)] : -1;
+        if (sp < 0 || sp >= a.c.pool_pages) sp = 0;
+        ok[z] = dp >= 0 && dp < a.c.pool_pages;
+        const long long from = ((static_cast<long long>(sp) << a.c.shift) + (j & mask)) * a.c.kv_heads + h;
+        to[z] = ((static_cast<long long>(dp) << a.c.shift) + (i & mask)) * a.c.kv_heads + h;
+        if (ok[z]) {
+            if (p < kpieces) kx[z] = reinterpret_cast<const uint4 *>(a.c.k)[from * kpieces + p];
+            if (p < vpieces) vx[z] = reinterpret_cast<const uint4 *>(a.c.v)[from * vpieces + p];
+            if (a.c.type == 3 && p == 0) {
+                ksc[z] = a.c.ks[from];
+                vsc[z] = a.c.vs[from];
+            }
+        }
     }
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+        if (ok[z]) {
+            if (p < kpieces) reinterpret_cast<uint4 *>(a.c.k)[to[z] * kpieces + p] = kx[z];
+            if (p < vpieces) reinterpret_cast<uint4 *>(a.c.v)[to[z] * vpieces + p] = vx[z];
+            if (a.c.type == 3 && p == 0) {
+                a.c.ks[to[z]] = ksc[z];
+                a.c.vs[to[z]] = vsc[z];
+            }
+        }
 }
 
 }  // namespace
@@ -274,14 +340,24 @@ hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s) {
 }
 
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(a.batch) * a.c.kv_heads), dim3(kSelThreads), 0, s, a);
+    // a wavefront for each 512 rows, eight rows a thread (32 past 16 wavefronts)
+    const int per = 512;
+    const int threads = std::min(kSelThreads, 64 * std::max(1, (a.nk_max + per - 1) / per));
+    const dim3 grid(static_cast<unsigned>(a.batch) * a.c.kv_heads), block(threads);
+    if (a.nk_max <= 8 * kSelThreads)
+        hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, s, a);
+    else if (a.nk_max <= 32 * kSelThreads)
+        hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int size = a.c.type == 0 ? 4 : a.c.type == 3 ? 1 : 2;
-    const int kpieces = a.c.qk * size / 16, pieces = kpieces + a.c.vd * size / 16;
-    const long long total = static_cast<long long>(a.batch) * a.keep * a.c.kv_heads * pieces;
+    const int kpieces = a.c.qk * size / 16, vpieces = a.c.vd * size / 16, half_rows = (a.keep + 1) / 2;
+    const long long total = static_cast<long long>(a.batch) * half_rows * a.c.kv_heads * std::max(kpieces, vpieces);
     const long long blocks = (std::max<long long>(total, a.batch) + 255) / 256;
-    hipLaunchKernelGGL(evict_copy_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, kpieces, pieces, total);
+    hipLaunchKernelGGL(evict_copy_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, kpieces, vpieces,
+                       half_rows, total);
     return hipGetLastError();
 }
 
