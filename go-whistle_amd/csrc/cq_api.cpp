@@ -2325,41 +2325,49 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
     return CQ_OK;
 }
 
-// The parts that a list of up to nk keys is cut into for `lists` workgroups a part: enough for two workgroups a CU,
-// none of fewer than 128 keys (a tile a wavefront).
-static int split_parts(long long lists, int nk) {
-    const long long want = (2LL * device_info().cus + lists - 1) / lists;
-    return static_cast<int>(std::max<long long>(1, std::min<long long>(want, (nk + 127) / 128)));
-}
-
 // The launches of a split attention with the partials' workspace.
-static int run_split_attend(SplitArgs &a, bool weights, hipStream_t stream) {
+static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     const long long cols = static_cast<long long>(a.t) * (a.heads / a.c.kv_heads);
     const bool many = !a.spans && a.type != ND_F32 && cols > 16;
     const int cus = device_info().cus;
-    const int wg_cols = many ? cross_workgroup_columns(a, cus) : 16;
+    const int wg_cols = many ? cross_workgroup_columns(a, cus) : split_tile_columns(a);
     const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((cols + wg_cols - 1) / wg_cols);
-    // The matrix form's partials cost more than idle CUs as long as the lists
-    // give half of the CUs a workgroup (8 x 448 rows of 8 heads of 48 over 2,
-    // 1500 frames, 224 workgroups: 31.9 us whole, 44.1 in two parts; 2 x 448
-    // rows of 8 heads of 64, 64 workgroups: 20.9 in four, 24.1 in two).
-    a.splits = many ? static_cast<int>(std::max<long long>(1, std::min<long long>(cus / lists, a.nk_max / 256)))
-                    : split_parts(lists, a.nk_max);
+    if (many) {
+        // The matrix form's partials cost more than idle CUs as long as the
+        // lists give half of the CUs a workgroup (8 x 448 rows of 8 heads of 48
+        // over 2, 1500 frames, 224 workgroups: 31.9 us whole, 44.1 in two
+        // parts; 2 x 448 rows of 8 heads of 64, 64 workgroups: 20.9 in four,
+        // 24.1 in two).
+        a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({cus / lists, a.nk_max / 256, 64})));
+    } else {
+        // Eight wavefronts a CU: more to a workgroup first, each with a tile of
+        // keys at least, then parts, each wavefront with 256 keys at least.
+        const long long want = 8LL * cus;
+        const int most = split_max_waves(a);
+        a.waves = 1;
+        while (a.waves < most && lists * a.waves < want && a.waves * 32 < a.nk_max) a.waves *= 2;
+        a.splits = static_cast<int>(std::max<long long>(
+            1, std::min<long long>({want / (lists * a.waves), a.nk_max / (256LL * a.waves), 64})));
+    }
+    const int qsize = value_size(a.type);
+    a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stream * qsize) |
+                static_cast<uintptr_t>(a.q_row * qsize)) & (4 * qsize - 1)) == 0;
+    const bool in_ws = a.acc_out && (a.splits > 1 || !split_weights_in_lds(a, a.waves));
     const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
-    const long long wblocks = weights ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
-    if (lists * a.splits > grid_limit(256) || (rows + 3) / 4 > grid_limit(256) || wblocks > grid_limit(256))
+    const long long wblocks = in_ws ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
+    if (lists * a.splits > grid_limit(1024) || (rows + 3) / 4 > grid_limit(256) || wblocks > grid_limit(256))
         return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", a.batch, a.t, a.heads);
     WsScope ws;
     a.part = a.part_ml = a.logits = nullptr;
-    if (a.splits > 1 || weights) {
+    if (a.splits > 1 || in_ws) {
         const size_t part = align256(static_cast<size_t>(rows) * a.splits * a.c.vd * 4);
         const size_t ml = align256(static_cast<size_t>(rows) * a.splits * 8);
-        const size_t lg = weights ? static_cast<size_t>(rows) * a.nk_max * 4 : 0;
+        const size_t lg = in_ws ? static_cast<size_t>(rows) * a.nk_max * 4 : 0;
         if (int rc = ws_acquire(part + ml + lg, stream, ws.l)) return rc;
         char *base = static_cast<char *>(ws.l.w->buf);
         a.part = reinterpret_cast<float *>(base);
         a.part_ml = reinterpret_cast<float *>(base + part);
-        if (weights) a.logits = reinterpret_cast<float *>(base + part + ml);
+        if (in_ws) a.logits = reinterpret_cast<float *>(base + part + ml);
     }
     HIP_TRY(many ? launch_cross_attend(a, cus, stream) : launch_attend_split(a, stream), "split attention launch");
     return CQ_OK;
@@ -2401,7 +2409,7 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     a.acc = acc;
     a.acc_out = acc_out;
     a.acc_cap = acc_cap;
-    return run_split_attend(a, acc_out != nullptr, static_cast<hipStream_t>(stream));
+    return run_split_attend(a, static_cast<hipStream_t>(stream));
 }
 
 int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
@@ -2510,7 +2518,7 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
     a.out_row = y.out_row;
     a.type = type;
     a.scale_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
-    return run_split_attend(a, false, static_cast<hipStream_t>(stream));
+    return run_split_attend(a, static_cast<hipStream_t>(stream));
 }
 
 int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, const void *logits, long long stride,

@@ -515,21 +515,27 @@ struct SplitArgs {
     long long k_mem, k_row, k_head, v_mem, v_row, v_head;  // bytes
     const int32_t *spans;                    // paged: the keys' spans
     const int32_t *q_len, *k_len, *index;    // memories
-    int memories, nk_max, t, heads, batch, splits;
+    int memories, nk_max, t, heads, batch;
+    int splits;                              // parts of a list, at most 64
+    int waves;                               // wavefronts of a workgroup
     const void *q;
     void *out;
     long long q_stream, q_row, out_stream, out_row;  // elements
-    int type;
+    int type, q_vec;                         // q_vec: the queries' pieces of four are aligned to their size
     float scale_log2;                        // log2(e) / scale
-    // Partials of the splits (splits > 1 or weights asked): per (stream,
-    // head-major column, split) vd sums, and their maximum (of log2 logits) and
-    // sum; the logits [stream][key head][group head][nk_max] for the weights.
+    // Partials of the splits (splits > 1, or weights of a list whose logits
+    // LDS does not hold): per (stream, query row, head, split) vd sums, and
+    // their maximum (of log2 logits) and sum; the logits [stream][key
+    // head][group head][nk_max] for the weights.
     float *part, *part_ml, *logits;
     const float *acc;
     float *acc_out;
     long long acc_cap;
 };
 bool split_widths_ok(int qk, int vd);
+int split_tile_columns(const SplitArgs &a);              // columns a workgroup takes
+int split_max_waves(const SplitArgs &a);                 // wavefronts a workgroup may have
+bool split_weights_in_lds(const SplitArgs &a, int waves);  // a list's logits fit LDS
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);
 // The parts of every output row joined.
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s);

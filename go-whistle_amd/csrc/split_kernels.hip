@@ -5,18 +5,25 @@
 // Per (stream, key head) the query columns are the heads of the group times
 // the query rows. o = sum_j w_j v_j with w = softmax(q.k_j / scale), one pass
 // over the keys with a running maximum m and sum l (in log2 units, p_j =
-// 2^(l_j - m)): a wavefront takes tiles of 16 or 32 keys, four wavefronts
-// share a workgroup's part of the list and are joined in LDS; the parts of
-// one list are joined by a second launch.
+// 2^(l_j - m)): a wavefront takes tiles of 16 to 64 keys, the wavefronts of a
+// workgroup share a part of the list and are joined in LDS; the parts of a
+// list, where there are few lists and many keys, by a second launch. All
+// arithmetic is float32, whatever the types.
 //
-// Both products run on v_mfma_f32_16x16x4_f32 with everything widened to
-// float32, which keeps float32's accuracy for every type and needs no
+// attend_lanes_kernel, one or two columns: lane (r, c) = (lane % 16, lane /
+// 16) reads pieces c, c + 4, ... of 16 bytes of key row r and of value row r.
+// The logit is the four lanes' sum, and a lane keeps the outputs of its
+// pieces for its keys: no exchange of the weights, one sum over r at the end.
+// The vector units do it: a piece of 16 int8 keys costs 32 operations a
+// column there, and 16 matrix instructions whatever the columns.
+//
+// attend_split_kernel, three to 16 columns a tile: both products on
+// v_mfma_f32_16x16x4_f32 with everything widened to float32, without a
 // shuffle:
-//   S = K q^T: A row r (lane % 16) is key r, the contraction index c (lane /
-//     16) a 16-byte piece of the key row, so a lane's global load is its
-//     operand; element e of the piece goes to the e-th MFMA, whose B operand
-//     is the query's same element. S has key 4c + i in register i of lane
-//     (column, c).
+//   S = K q^T: A row r is key r, the contraction index c a 16-byte piece of
+//     the key row, so a lane's global load is its operand; element e of the
+//     piece goes to the e-th MFMA, whose B operand is the query's same
+//     element. S has key 4c + i in register i of lane (column, c).
 //   O = V^T P: the register P_i is the B operand as it lies (contraction
 //     index c is key 4c + i), and A is a lane's piece of value row 4c + i,
 //     elements e of 16 lanes the rows of the e-th MFMA. m and l belong to
@@ -31,8 +38,8 @@ namespace {
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
 constexpr int kCols = 16;
+constexpr size_t kMostLds = 150 * 1024;
 
 // The e-th value of a lane's piece of a row, as float32.
 template <int TYPE>
@@ -115,16 +122,328 @@ __device__ __forceinline__ KeyList key_list(const SplitArgs &a, int b, int mem) 
 
 __device__ __forceinline__ int q_rows(const SplitArgs &a, int b) { return a.q_len ? min(max(a.q_len[b], 0), a.t) : a.t; }
 
-// Keys a part of the list takes: whole tiles of 32 keys a wavefront, equal over the parts.
+// Keys a part of the list takes: whole tiles of 64 keys, equal over the parts.
 __device__ __forceinline__ int part_keys(int n, int splits) {
-    constexpr int unit = 32 * kWaves;
-    const int units = (n + unit - 1) / unit;
-    return (units + splits - 1) / splits * unit;
+    const int units = (n + 63) / 64;
+    return (units + splits - 1) / splits * 64;
+}
+
+// What a workgroup works on.
+struct Place {
+    int sp, ct, h, b, mem, group, cols, j0, j1;
+    KeyList kl;
+    bool ok;
+};
+__device__ __forceinline__ Place place_of(const SplitArgs &a, int col_tiles, int tile_cols) {
+    Place p;
+    int id = blockIdx.x;
+    p.sp = id % a.splits;
+    id /= a.splits;
+    p.ct = id % col_tiles;
+    id /= col_tiles;
+    p.h = id % a.c.kv_heads;
+    p.b = id / a.c.kv_heads;
+    p.group = a.heads / a.c.kv_heads;
+    p.mem = a.index ? a.index[p.b] : p.b;
+    p.kl = key_list(a, p.b, p.mem);
+    p.cols = q_rows(a, p.b) * p.group;
+    p.ok = p.kl.ok && p.ct * tile_cols < p.cols;
+    const int per = part_keys(p.kl.n, a.splits);
+    p.j0 = min(p.sp * per, p.kl.n);
+    p.j1 = min(p.j0 + per, p.kl.n);
+    return p;
+}
+
+// The pool (or memory) row of key j of the list.
+__device__ __forceinline__ int array_row(const SplitArgs &a, const Place &p, int j) {
+    const int row = p.kl.row(j);
+    if (!a.c.pages) return row;
+    int pg = a.c.pages[static_cast<long long>(p.b) * a.c.page_stride + (row >> a.c.shift)];
+    if (pg < 0 || pg >= a.c.pool_pages) pg = 0;
+    return (pg << a.c.shift) + (row & ((1 << a.c.shift) - 1));
+}
+
+// N consecutive query values from element i on, times f.
+template <int N>
+__device__ __forceinline__ void load_query(float *x, const SplitArgs &a, long long i, float f) {
+    if (a.q_vec) {
+        if (a.type == 0) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + i + e);
+                x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+            }
+        } else {
+            uint32_t w[N / 2];
+#pragma unroll
+            for (int e = 0; e < N; e += 4)
+                *reinterpret_cast<uint2 *>(w + e / 2) =
+                    *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.q) + i + e);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = a.type == 1 ? piece_value<1>(w, e) : piece_value<2>(w, e);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = load_value(a.q, a.type, i + e);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] *= f;
+}
+
+// LDS of a workgroup, in floats: per wavefront and column the maximum and the
+// sum, per column the joined maximum and 1 / sum, per wavefront and column the
+// outputs (rows of D + 4), then the logits [column][nk_max] where the weights
+// are asked of a whole list.
+template <int COLS, int D>
+struct Joint {
+    static constexpr int kRow = D + 4;
+    float *ml, *stat, *o, *logits;
+    __device__ Joint(float *smem, int waves)
+        : ml(smem), stat(ml + waves * 2 * COLS), o(stat + 2 * COLS), logits(o + waves * COLS * kRow) {}
+    static constexpr int floats(int waves) { return waves * 2 * COLS + 2 * COLS + waves * COLS * kRow; }
+};
+
+// Joins the wavefronts' columns (o, ml filled, outputs relative to each
+// wavefront's own maximum) and writes them: the outputs, or a part's sums.
+template <int COLS, int D>
+__device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const Joint<COLS, D> &jt) {
+    const int tid = threadIdx.x, threads = blockDim.x, waves = threads >> 6;
+    const int col0 = p.ct * COLS, nc = min(COLS, p.cols - col0);
+    __syncthreads();
+    if (tid < nc) {
+        float mx = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < waves; ++w) mx = fmaxf(mx, jt.ml[(w * 2) * COLS + tid]);
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        for (int w = 0; w < waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(jt.ml[(w * 2) * COLS + tid] - mu);
+            sum += jt.ml[(w * 2 + 1) * COLS + tid] * f;
+            jt.ml[(w * 2) * COLS + tid] = f;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        jt.stat[tid] = mu;
+        jt.stat[COLS + tid] = inv;
+        if (a.part) {
+            const int cn = col0 + tid, head = p.h * p.group + cn % p.group;
+            const long long pi = ((static_cast<long long>(p.b) * a.t + cn / p.group) * a.heads + head) * a.splits + p.sp;
+            a.part_ml[2 * pi] = mx;
+            a.part_ml[2 * pi + 1] = sum;
+        }
+    }
+    __syncthreads();
+    for (int x = tid; x < nc * a.c.vd; x += threads) {
+        const int n = x / a.c.vd, d = x - n * a.c.vd, cn = col0 + n;
+        float v = 0.0f;
+        for (int w = 0; w < waves; ++w) v = fmaf(jt.o[(w * COLS + n) * jt.kRow + d], jt.ml[(w * 2) * COLS + n], v);
+        const int head = p.h * p.group + cn % p.group;
+        if (a.part) {
+            const long long pi = ((static_cast<long long>(p.b) * a.t + cn / p.group) * a.heads + head) * a.splits + p.sp;
+            a.part[pi * a.c.vd + d] = v;
+        } else {
+            store_value(a.out, a.type,
+                        static_cast<long long>(p.b) * a.out_stream + static_cast<long long>(cn / p.group) * a.out_row +
+                            static_cast<long long>(head) * a.c.vd + d,
+                        v * jt.stat[COLS + n]);
+        }
+    }
+    if (a.acc_out && !a.logits) {  // the whole list's weights
+        for (int j = tid; j < p.kl.n; j += threads) {
+            float w = 0.0f;
+            for (int n = 0; n < nc; ++n)
+                w += __builtin_amdgcn_exp2f(jt.logits[n * a.nk_max + j] - jt.stat[n]) * jt.stat[COLS + n];
+            const long long at = (static_cast<long long>(p.b) * a.c.kv_heads + p.h) * a.acc_cap + p.kl.row(j);
+            a.acc_out[at] = (a.acc ? a.acc[at] : 0.0f) + w;
+        }
+    }
+}
+
+// TYPE: the cache's type; D: widths up to D (64, 128, 256); COLS: columns a tile.
+template <int TYPE, int D, int COLS>
+__global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_lanes_kernel(SplitArgs a, int col_tiles) {
+    constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
+    constexpr int kPer = 16 / kSize;         // elements of a piece
+    constexpr int kPieces = D / (4 * kPer);  // pieces of a row a lane reads
+    constexpr int kSub = D * kSize <= 64 ? 4 : D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
+    constexpr int kTile = 16 * kSub;
+    extern __shared__ __align__(16) float smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int r = lane & 15, c = lane >> 4;
+    const Place p = place_of(a, col_tiles, COLS);
+    if (!p.ok) return;
+    const Joint<COLS, D> jt(smem, waves);
+    const int col0 = p.ct * COLS, nc = min(COLS, p.cols - col0);
+
+    float q[COLS][kPieces * kPer], o[COLS][kPieces * kPer], m[COLS], l[COLS];
+#pragma unroll
+    for (int n = 0; n < COLS; ++n) {
+        const int cn = min(col0 + n, p.cols - 1);
+        const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(cn / p.group) * a.q_row +
+                             static_cast<long long>(p.h * p.group + cn % p.group) * a.c.qk;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int d0 = (4 * k + c) * kPer;
+            if (d0 < a.c.qk) {
+                load_query<kPer>(&q[n][k * kPer], a, qo + d0, a.scale_log2);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) q[n][k * kPer + e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kPieces * kPer; ++e) o[n][e] = 0.0f;
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+    }
+    const unsigned char *kp = a.c.k + (a.c.pages ? 0 : static_cast<long long>(p.mem) * a.k_mem) + static_cast<long long>(p.h) * a.k_head;
+    const unsigned char *vp = a.c.v + (a.c.pages ? 0 : static_cast<long long>(p.mem) * a.v_mem) + static_cast<long long>(p.h) * a.v_head;
+    float *lg = a.logits ? a.logits + (static_cast<long long>(p.b) * a.c.kv_heads + p.h) * p.group * a.nk_max : nullptr;
+
+    uint32_t kw[kSub][kPieces][4], vw[kSub][kPieces][4];
+    float ks[kSub], vs[kSub];
+    int rows[kSub];
+    auto rows_of = [&](int j) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) rows[s] = array_row(a, p, min(j + 16 * s + r, p.j1 - 1));
+    };
+    auto load_rows = [&](uint32_t (&w)[kSub][kPieces][4], const unsigned char *base, long long stride, int width) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) {
+            const unsigned char *at = base + static_cast<long long>(rows[s]) * stride;
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const int d0 = (4 * k + c) * kPer;
+                if (d0 < width)
+                    load_words<4>(w[s][k], at + d0 * kSize);
+                else
+                    w[s][k][0] = w[s][k][1] = w[s][k][2] = w[s][k][3] = 0;
+            }
+        }
+    };
+    auto load_scales = [&]() {
+        if constexpr (TYPE == 3) {
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) {
+                ks[s] = a.c.ks[static_cast<long long>(rows[s]) * a.c.kv_heads + p.h];
+                vs[s] = a.c.vs[static_cast<long long>(rows[s]) * a.c.kv_heads + p.h];
+            }
+        }
+    };
+    const int step = waves * kTile;
+    int j = p.j0 + wave * kTile;
+    if (j < p.j1) {
+        rows_of(j);
+        load_rows(kw, kp, a.k_row, a.c.qk);
+        load_rows(vw, vp, a.v_row, a.c.vd);
+        load_scales();
+        if (j + step < p.j1) rows_of(j + step);
+        for (; j < p.j1; j += step) {
+            const bool more = j + step < p.j1;
+            // logits: the four lanes' sums; the keys' registers are then the next tile's
+            float x[COLS][kSub];
+#pragma unroll
+            for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                for (int n = 0; n < COLS; ++n) {
+                    float d = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e) d = fmaf(piece_value<TYPE>(kw[s][k], e), q[n][k * kPer + e], d);
+                    d += xor_lane<16>(d);
+                    d += xor_lane<32>(d);
+                    if constexpr (TYPE == 3) d *= ks[s];
+                    x[n][s] = d;
+                }
+            float vsc[kSub];
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) vsc[s] = TYPE == 3 ? vs[s] : 1.0f;
+            if (more) load_rows(kw, kp, a.k_row, a.c.qk);
+            float w[COLS][kSub];
+#pragma unroll
+            for (int n = 0; n < COLS; ++n) {
+                float mt = m[n];
+#pragma unroll
+                for (int s = 0; s < kSub; ++s) {
+                    const int jj = j + 16 * s + r;
+                    if (jj >= p.j1) {
+                        x[n][s] = -INFINITY;
+                    } else if (a.acc_out && c == 0 && n < nc) {
+                        if (lg)
+                            lg[static_cast<long long>(col0 + n) * a.nk_max + p.kl.row(jj)] = x[n][s];
+                        else
+                            jt.logits[n * a.nk_max + jj] = x[n][s];
+                    }
+                    mt = fmaxf(mt, x[n][s]);
+                }
+                mt = fmaxf(mt, xor_lane<1>(mt));
+                mt = fmaxf(mt, xor_lane<2>(mt));
+                mt = fmaxf(mt, xor_lane<4>(mt));
+                mt = fmaxf(mt, xor_lane<8>(mt));
+                const float mu = mt == -INFINITY ? 0.0f : mt;
+                const float f = __builtin_amdgcn_exp2f(m[n] - mu);
+                m[n] = mt;
+                l[n] *= f;
+#pragma unroll
+                for (int e = 0; e < kPieces * kPer; ++e) o[n][e] *= f;
+#pragma unroll
+                for (int s = 0; s < kSub; ++s) {
+                    const float pw = __builtin_amdgcn_exp2f(x[n][s] - mu);
+                    l[n] += pw;
+                    w[n][s] = pw * vsc[s];
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        const float y = piece_value<TYPE>(vw[s][k], e);
+#pragma unroll
+                        for (int n = 0; n < COLS; ++n) o[n][k * kPer + e] = fmaf(y, w[n][s], o[n][k * kPer + e]);
+                    }
+            if (more) {
+                load_rows(vw, vp, a.v_row, a.c.vd);
+                load_scales();
+                if (j + 2 * step < p.j1) rows_of(j + 2 * step);
+            }
+        }
+    }
+    // the sums over the keys' lanes, then the wavefronts'
+#pragma unroll
+    for (int n = 0; n < COLS; ++n) {
+        float lt = l[n];
+        lt += xor_lane<1>(lt);
+        lt += xor_lane<2>(lt);
+        lt += xor_lane<4>(lt);
+        lt += xor_lane<8>(lt);
+        if (lane == 0) {
+            jt.ml[(wave * 2) * COLS + n] = m[n];
+            jt.ml[(wave * 2 + 1) * COLS + n] = lt;
+        }
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+            for (int e = 0; e < kPer; e += 4) {
+                float4 y;
+                float *ys = &y.x;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    float t = o[n][k * kPer + e + z];
+                    t += xor_lane<1>(t);
+                    t += xor_lane<2>(t);
+                    t += xor_lane<4>(t);
+                    t += xor_lane<8>(t);
+                    ys[z] = t;
+                }
+                if (r == 0) *reinterpret_cast<float4 *>(&jt.o[(wave * COLS + n) * jt.kRow + (4 * k + c) * kPer + e]) = y;
+            }
+    }
+    finish<COLS, D>(a, p, jt);
 }
 
 // TYPE: the cache's type; D: widths up to D (64, 128, 256).
 template <int TYPE, int D>
-__global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, int col_tiles) {
+__global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
     constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
     constexpr int kPer = 16 / kSize;          // elements of a 16-byte piece of a key row
     constexpr int kPieces = D / (4 * kPer);   // pieces of a key row a lane loads
@@ -133,42 +452,29 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
     constexpr int kSub = D * kSize <= 256 ? 2 : 1;  // 16-key steps of a tile
     constexpr int kTile = 16 * kSub;
     extern __shared__ __align__(16) float smem[];
-    float *ml_sh = smem;                      // [waves][2][16]
-    float *o_sh = smem + kWaves * 2 * kCols;  // [waves][16][D + 4]
-    constexpr int kRow = D + 4;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
     const int r = lane & 15, c = lane >> 4;
-    int id = blockIdx.x;
-    const int sp = id % a.splits;
-    id /= a.splits;
-    const int ct = id % col_tiles;
-    id /= col_tiles;
-    const int h = id % a.c.kv_heads, b = id / a.c.kv_heads;
-    const int group = a.heads / a.c.kv_heads;
-    const int mem = a.index ? a.index[b] : b;
-    const KeyList kl = key_list(a, b, mem);
-    if (!kl.ok) return;
-    const int cols = q_rows(a, b) * group;
-    const int col0 = ct * kCols;
-    if (col0 >= cols) return;
-    const int col = col0 + r;  // this lane's column: query row col / group, head col % group of the group
-    const bool col_ok = col < cols;
-    const int per = part_keys(kl.n, a.splits);
-    const int j0 = min(sp * per, kl.n), j1 = min(j0 + per, kl.n);
+    const Place p = place_of(a, col_tiles, kCols);
+    if (!p.ok) return;
+    const Joint<kCols, D> jt(smem, waves);
+    const int col = p.ct * kCols + r;  // this lane's column: query row col / group, head col % group of the group
+    const bool col_ok = col < p.cols;
 
     // The query's pieces, 1/scale and log2(e) folded in.
     float qv[kPieces * kPer];
     {
-        const long long qo = static_cast<long long>(b) * a.q_stream +
-                             static_cast<long long>(col_ok ? col / group : 0) * a.q_row +
-                             static_cast<long long>(h * group + (col_ok ? col % group : 0)) * a.c.qk;
+        const int cn = col_ok ? col : 0;
+        const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(cn / p.group) * a.q_row +
+                             static_cast<long long>(p.h * p.group + cn % p.group) * a.c.qk;
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) {
-            const int d0 = (4 * p + c) * kPer;
+        for (int k = 0; k < kPieces; ++k) {
+            const int d0 = (4 * k + c) * kPer;
+            if (col_ok && d0 < a.c.qk) {
+                load_query<kPer>(&qv[k * kPer], a, qo + d0, a.scale_log2);
+            } else {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                qv[p * kPer + e] = col_ok && d0 < a.c.qk ? load_value(a.q, a.type, qo + d0 + e) * a.scale_log2 : 0.0f;
+                for (int e = 0; e < kPer; ++e) qv[k * kPer + e] = 0.0f;
+            }
         }
     }
 
@@ -177,31 +483,21 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
     for (int e = 0; e < kVals; ++e) o[e] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
 
-    const long long k_base = a.c.pages ? 0 : static_cast<long long>(mem) * a.k_mem;
-    const long long v_base = a.c.pages ? 0 : static_cast<long long>(mem) * a.v_mem;
-    const unsigned char *kp = a.c.k + k_base + static_cast<long long>(h) * a.k_head;
-    const unsigned char *vp = a.c.v + v_base + static_cast<long long>(h) * a.v_head;
+    const unsigned char *kp = a.c.k + (a.c.pages ? 0 : static_cast<long long>(p.mem) * a.k_mem) + static_cast<long long>(p.h) * a.k_head;
+    const unsigned char *vp = a.c.v + (a.c.pages ? 0 : static_cast<long long>(p.mem) * a.v_mem) + static_cast<long long>(p.h) * a.v_head;
     const bool v_ok = r * kVals < a.c.vd;
-    const int last = j1 - 1;
 
-    // The pool (or memory) row of the lane's key of tile j (lanes of a tile;
-    // keys past the part's last read that one's row).
-    auto row_of = [&](int j) {
-        const int row = kl.row(min(j + (lane & (kTile - 1)), last));
-        if (!a.c.pages) return row;
-        int pg = a.c.pages[static_cast<long long>(b) * a.c.page_stride + (row >> a.c.shift)];
-        if (pg < 0 || pg >= a.c.pool_pages) pg = 0;
-        return (pg << a.c.shift) + (row & ((1 << a.c.shift) - 1));
-    };
+    // Row of the lane's key of a tile (its first kTile lanes; keys past the part's last read that one's row).
+    auto row_of = [&](int j) { return array_row(a, p, min(j + (lane & (kTile - 1)), p.j1 - 1)); };
     auto load_keys = [&](uint32_t (&kw)[kSub][kPieces][4], int rows) {
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
-            const unsigned char *p = kp + static_cast<long long>(__shfl(rows, 16 * s + r)) * a.k_row;
+            const unsigned char *at = kp + static_cast<long long>(__shfl(rows, 16 * s + r)) * a.k_row;
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
                 const int d0 = (4 * k + c) * kPer;
                 if (d0 < a.c.qk)
-                    load_words<4>(kw[s][k], p + d0 * kSize);
+                    load_words<4>(kw[s][k], at + d0 * kSize);
                 else
                     kw[s][k][0] = kw[s][k][1] = kw[s][k][2] = kw[s][k][3] = 0;
             }
@@ -209,14 +505,14 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
     };
 
     float *lg = a.logits;
-    if (lg) lg += ((static_cast<long long>(b) * a.c.kv_heads + h) * group + (col_ok ? col : 0)) * a.nk_max;
-    int j = j0 + wave * kTile;
-    constexpr int kStep = kWaves * kTile;
-    if (j < j1) {
+    if (lg) lg += ((static_cast<long long>(p.b) * a.c.kv_heads + p.h) * p.group + (col_ok ? col : 0)) * a.nk_max;
+    const int step = waves * kTile;
+    int j = p.j0 + wave * kTile;
+    if (j < p.j1) {
         int rows = row_of(j);
         uint32_t kw[kSub][kPieces][4];
         load_keys(kw, rows);
-        for (; j < j1; j += kStep) {
+        for (; j < p.j1; j += step) {
             // this tile's values, the next tile's rows
             uint32_t vw[kSub][4][kVWords];
             float ksc[kSub][4], vsc[kSub][4];
@@ -232,12 +528,12 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
                         for (int k = 0; k < kVWords; ++k) vw[s][i][k] = 0;
                     }
                     if constexpr (TYPE == 3) {
-                        ksc[s][i] = a.c.ks[row * a.c.kv_heads + h];
-                        vsc[s][i] = a.c.vs[row * a.c.kv_heads + h];
+                        ksc[s][i] = a.c.ks[row * a.c.kv_heads + p.h];
+                        vsc[s][i] = a.c.vs[row * a.c.kv_heads + p.h];
                     }
                 }
-            const int jn = j + kStep;
-            if (jn < j1) rows = row_of(jn);
+            const int jn = j + step;
+            if (jn < p.j1) rows = row_of(jn);
 
             f32x4 sc[kSub];
 #pragma unroll
@@ -250,7 +546,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
                     for (int s = 0; s < kSub; ++s)
                         sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(kw[s][k], e), qv[k * kPer + e],
                                                                      sc[s], 0, 0, 0);
-            if (jn < j1) load_keys(kw, rows);
+            if (jn < p.j1) load_keys(kw, rows);
 
             float mt = m;
 #pragma unroll
@@ -260,10 +556,13 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
                     const int jj = j + 16 * s + 4 * c + i;
                     float x = sc[s][i];
                     if constexpr (TYPE == 3) x *= ksc[s][i];
-                    if (jj < j1) {
-                        if (lg && col_ok) lg[kl.row(jj)] = x;
-                    } else {
+                    if (jj >= p.j1) {
                         x = -INFINITY;
+                    } else if (a.acc_out && col_ok) {
+                        if (lg)
+                            lg[p.kl.row(jj)] = x;
+                        else
+                            jt.logits[r * a.nk_max + jj] = x;
                     }
                     sc[s][i] = x;
                     mt = fmaxf(mt, x);
@@ -271,7 +570,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
             mt = fmaxf(mt, xor_lane<16>(mt));
             mt = fmaxf(mt, xor_lane<32>(mt));
             const float mu = mt == -INFINITY ? 0.0f : mt;  // no key above -inf so far: every weight 0
-            const float f = exp2f(m - mu);
+            const float f = __builtin_amdgcn_exp2f(m - mu);
             m = mt;
             l *= f;
 #pragma unroll
@@ -280,60 +579,28 @@ __global__ __launch_bounds__(64 * kWaves) void attend_split_kernel(SplitArgs a, 
             for (int s = 0; s < kSub; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float p = exp2f(sc[s][i] - mu);
-                    l += p;
-                    if constexpr (TYPE == 3) p *= vsc[s][i];
+                    float w = __builtin_amdgcn_exp2f(sc[s][i] - mu);
+                    l += w;
+                    if constexpr (TYPE == 3) w *= vsc[s][i];
 #pragma unroll
                     for (int e = 0; e < kVals; ++e)
-                        o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(vw[s][i], e), p, o[e], 0, 0, 0);
+                        o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(vw[s][i], e), w, o[e], 0, 0, 0);
                 }
         }
     }
     l += xor_lane<16>(l);
     l += xor_lane<32>(l);
-
-    // Join the wavefronts.
     if (c == 0) {
-        ml_sh[(wave * 2) * kCols + r] = m;
-        ml_sh[(wave * 2 + 1) * kCols + r] = l;
+        jt.ml[(wave * 2) * kCols + r] = m;
+        jt.ml[(wave * 2 + 1) * kCols + r] = l;
     }
-    __syncthreads();
-    float mt = -INFINITY;
+    if (col_ok) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, ml_sh[(w * 2) * kCols + r]);
-    const float f = exp2f(m - (mt == -INFINITY ? 0.0f : mt));
+        for (int e = 0; e < kVals; ++e)
 #pragma unroll
-    for (int e = 0; e < kVals; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o_sh[(wave * kCols + r) * kRow + kVals * (4 * c + i) + e] = o[e][i] * f;
-    __syncthreads();
-    for (int x = tid; x < kCols * a.c.vd; x += 64 * kWaves) {
-        const int n = x / a.c.vd, d = x - n * a.c.vd, cn = col0 + n;
-        if (cn >= cols) break;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml_sh[(w * 2) * kCols + n]);
-        float sum = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            sum += ml_sh[(w * 2 + 1) * kCols + n] * exp2f(ml_sh[(w * 2) * kCols + n] - (mx == -INFINITY ? 0.0f : mx));
-            v += o_sh[(w * kCols + n) * kRow + d];
-        }
-        const int head = h * group + cn % group;
-        if (a.part) {
-            const long long pi = ((static_cast<long long>(b) * a.t + cn / group) * a.heads + head) * a.splits + sp;
-            a.part[pi * a.c.vd + d] = v;
-            if (d == 0) {
-                a.part_ml[2 * pi] = mx;
-                a.part_ml[2 * pi + 1] = sum;
-            }
-        } else {
-            store_value(a.out, a.type,
-                        static_cast<long long>(b) * a.out_stream + static_cast<long long>(cn / group) * a.out_row +
-                            static_cast<long long>(head) * a.c.vd + d,
-                        sum == 0.0f ? 0.0f : v / sum);
-        }
+            for (int i = 0; i < 4; ++i) jt.o[(wave * kCols + r) * jt.kRow + kVals * (4 * c + i) + e] = o[e][i];
     }
+    finish<kCols, D>(a, p, jt);
 }
 
 // The parts of a list joined: one wavefront an output row (stream, query row, head).
@@ -344,29 +611,36 @@ __global__ __launch_bounds__(256) void attend_join_kernel(SplitArgs a, long long
     const int head = static_cast<int>(id % a.heads);
     const int i = static_cast<int>(id / a.heads % a.t), b = static_cast<int>(id / a.heads / a.t);
     if (!key_list(a, b, a.index ? a.index[b] : b).ok || i >= q_rows(a, b)) return;
+    // lane s has part s's maximum and sum; up to 64 parts
     const float *ml = a.part_ml + 2 * id * a.splits;
-    float m = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[2 * s]);
+    const float2 mine = lane < a.splits ? *reinterpret_cast<const float2 *>(ml + 2 * lane) : make_float2(-INFINITY, 0.0f);
+    float m = mine.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float mu = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int s = lane; s < a.splits; s += 64) l += ml[2 * s + 1] * exp2f(ml[2 * s] - mu);
+    const float f = __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.0f : m));
+    float l = mine.y * f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    const float *p = a.part + id * a.splits * a.c.vd;
-    for (int d = lane; d < a.c.vd; d += 64) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float *part = a.part + id * a.splits * a.c.vd;
+    for (int d = lane; d - lane < a.c.vd; d += 64) {
         float v = 0.0f;
-        for (int s = 0; s < a.splits; ++s) v = fmaf(p[static_cast<long long>(s) * a.c.vd + d], exp2f(ml[2 * s] - mu), v);
-        store_value(a.out, a.type,
-                    static_cast<long long>(b) * a.out_stream + static_cast<long long>(i) * a.out_row +
-                        static_cast<long long>(head) * a.c.vd + d,
-                    l == 0.0f ? 0.0f : v / l);
+#pragma unroll 4
+        for (int s = 0; s < a.splits; ++s) {
+            const float x = d < a.c.vd ? part[s * a.c.vd + d] : 0.0f;
+            v = fmaf(x, __shfl(f, s), v);
+        }
+        if (d < a.c.vd)
+            store_value(a.out, a.type,
+                        static_cast<long long>(b) * a.out_stream + static_cast<long long>(i) * a.out_row +
+                            static_cast<long long>(head) * a.c.vd + d,
+                        v * inv);
     }
 }
 
-// acc_out = acc + the group's softmax weights, a thread a key: key_blocks
-// workgroups of 256 keys for each (stream, key head).
+// acc_out = acc + the group's softmax weights from the logits in the
+// workspace, a thread a key: key_blocks workgroups of 256 keys for each
+// (stream, key head).
 __global__ __launch_bounds__(256) void attend_weights_kernel(SplitArgs a, int key_blocks) {
     extern __shared__ __align__(16) float smem[];  // per group head: maximum, 1 / sum
     const int blk = blockIdx.x % key_blocks, id = blockIdx.x / key_blocks;
@@ -380,7 +654,7 @@ __global__ __launch_bounds__(256) void attend_weights_kernel(SplitArgs a, int ke
         float m = -INFINITY, l = 0.0f;
         for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * s]);
         const float mu = m == -INFINITY ? 0.0f : m;
-        for (int s = 0; s < a.splits; ++s) l += ml[2 * s + 1] * exp2f(ml[2 * s] - mu);
+        for (int s = 0; s < a.splits; ++s) l += ml[2 * s + 1] * __builtin_amdgcn_exp2f(ml[2 * s] - mu);
         smem[2 * g] = mu;
         smem[2 * g + 1] = l == 0.0f ? 0.0f : 1.0f / l;
     }
@@ -389,32 +663,67 @@ __global__ __launch_bounds__(256) void attend_weights_kernel(SplitArgs a, int ke
     const int row = kl.row(j);
     const float *lg = a.logits + (static_cast<long long>(b) * a.c.kv_heads + h) * group * a.nk_max + row;
     float w = 0.0f;
-    for (int g = 0; g < group; ++g) w += exp2f(lg[static_cast<long long>(g) * a.nk_max] - smem[2 * g]) * smem[2 * g + 1];
+    for (int g = 0; g < group; ++g)
+        w += __builtin_amdgcn_exp2f(lg[static_cast<long long>(g) * a.nk_max] - smem[2 * g]) * smem[2 * g + 1];
     const long long at = (static_cast<long long>(b) * a.c.kv_heads + h) * a.acc_cap + row;
     a.acc_out[at] = (a.acc ? a.acc[at] : 0.0f) + w;
 }
 
-template <int TYPE, int D>
-hipError_t launch_split(const SplitArgs &a, int col_tiles, unsigned grid, hipStream_t s) {
-    constexpr size_t lds = sizeof(float) * (kWaves * 2 * kCols + kWaves * kCols * (D + 4));
-    static std::atomic<unsigned long long> attr{0};
+// LDS of a launch, in bytes: the joint of its wavefronts and the logits.
+template <int COLS, int D>
+size_t joint_lds(const SplitArgs &a, int waves) {
+    const size_t lg = a.acc_out && !a.logits ? static_cast<size_t>(a.heads / a.c.kv_heads) * a.nk_max : 0;
+    return sizeof(float) * (Joint<COLS, D>::floats(waves) + lg);
+}
+
+template <class F>
+hipError_t launch_with(F *fn, const SplitArgs &a, int tile_cols, size_t lds, std::atomic<unsigned long long> &attr, hipStream_t s) {
     if (lds > 64 * 1024)
-        if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(&attend_split_kernel<TYPE, D>), lds, attr)) return e;
-    hipLaunchKernelGGL((attend_split_kernel<TYPE, D>), dim3(grid), dim3(64 * kWaves), lds, s, a, col_tiles);
+        if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(fn), kMostLds, attr)) return e;
+    const int cols = a.t * (a.heads / a.c.kv_heads), col_tiles = (cols + tile_cols - 1) / tile_cols;
+    const long long grid = static_cast<long long>(a.batch) * a.c.kv_heads * col_tiles * a.splits;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * a.waves), lds, s, a, col_tiles);
     return hipGetLastError();
 }
 
+template <int TYPE, int D>
+hipError_t launch_split(const SplitArgs &a, hipStream_t s) {
+    static std::atomic<unsigned long long> one{0}, two{0}, many{0};
+    const int tile = split_tile_columns(a);
+    if (tile == 1)
+        return launch_with(&attend_lanes_kernel<TYPE, D, 1>, a, 1, joint_lds<1, D>(a, a.waves), one, s);
+    if (tile == 2)
+        return launch_with(&attend_lanes_kernel<TYPE, D, 2>, a, 2, joint_lds<2, D>(a, a.waves), two, s);
+    return launch_with(&attend_split_kernel<TYPE, D>, a, kCols, joint_lds<kCols, D>(a, a.waves), many, s);
+}
+
 template <int TYPE>
-hipError_t launch_split_width(const SplitArgs &a, int col_tiles, unsigned grid, hipStream_t s) {
+hipError_t launch_split_width(const SplitArgs &a, hipStream_t s) {
     const int w = std::max(a.c.qk, a.c.vd);
-    if (w <= 64) return launch_split<TYPE, 64>(a, col_tiles, grid, s);
-    if (w <= 128) return launch_split<TYPE, 128>(a, col_tiles, grid, s);
-    return launch_split<TYPE, 256>(a, col_tiles, grid, s);
+    if (w <= 64) return launch_split<TYPE, 64>(a, s);
+    if (w <= 128) return launch_split<TYPE, 128>(a, s);
+    return launch_split<TYPE, 256>(a, s);
 }
 
 }  // namespace
 
 bool split_widths_ok(int qk, int vd) { return qk > 0 && vd > 0 && qk % 16 == 0 && vd % 16 == 0 && qk <= 256 && vd <= 256; }
+
+int split_tile_columns(const SplitArgs &a) {
+    const int cols = a.t * (a.heads / a.c.kv_heads);
+    return cols <= 2 ? cols : kCols;
+}
+
+int split_max_waves(const SplitArgs &a) {
+    const int w = std::max(a.c.qk, a.c.vd);
+    return w <= 64 ? 16 : w <= 128 ? 8 : 4;
+}
+
+bool split_weights_in_lds(const SplitArgs &a, int waves) {
+    const int w = std::max(a.c.qk, a.c.vd), d = w <= 64 ? 64 : w <= 128 ? 128 : 256, group = a.heads / a.c.kv_heads;
+    const size_t joint = sizeof(float) * (waves * 2 + 2 + waves * (d + 4)) * split_tile_columns(a);
+    return a.t == 1 && group <= kCols && joint + sizeof(float) * group * static_cast<size_t>(a.nk_max) <= kMostLds / 2;
+}
 
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {
     const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
@@ -423,19 +732,16 @@ hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {
 }
 
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s) {
-    const int group = a.heads / a.c.kv_heads;
-    const int col_tiles = (a.t * group + kCols - 1) / kCols;
-    const unsigned grid = static_cast<unsigned>(static_cast<long long>(a.batch) * a.c.kv_heads * col_tiles * a.splits);
-    hipError_t e = a.c.type == 0   ? launch_split_width<0>(a, col_tiles, grid, s)
-                   : a.c.type == 1 ? launch_split_width<1>(a, col_tiles, grid, s)
-                   : a.c.type == 2 ? launch_split_width<2>(a, col_tiles, grid, s)
-                                   : launch_split_width<3>(a, col_tiles, grid, s);
+    hipError_t e = a.c.type == 0   ? launch_split_width<0>(a, s)
+                   : a.c.type == 1 ? launch_split_width<1>(a, s)
+                   : a.c.type == 2 ? launch_split_width<2>(a, s)
+                                   : launch_split_width<3>(a, s);
     if (e != hipSuccess || !a.part) return e;
     if ((e = launch_attend_join(a, s)) != hipSuccess) return e;
-    if (a.acc_out) {
+    if (a.acc_out && a.logits) {
         const int blocks = (a.nk_max + 255) / 256;
         hipLaunchKernelGGL(attend_weights_kernel, dim3(static_cast<unsigned>(a.batch) * a.c.kv_heads * blocks),
-                           dim3(256), sizeof(float) * 2 * group, s, a, blocks);
+                           dim3(256), sizeof(float) * 2 * (a.heads / a.c.kv_heads), s, a, blocks);
     }
     return hipGetLastError();
 }
