@@ -2327,7 +2327,8 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
 
 // The launches of a split attention with the partials' workspace.
 static int run_split_attend(SplitArgs &a, hipStream_t stream) {
-    const long long cols = static_cast<long long>(a.t) * (a.heads / a.c.kv_heads);
+    a.group = a.heads / a.c.kv_heads;
+    const long long cols = static_cast<long long>(a.t) * a.group;
     const bool many = !a.spans && a.type != ND_F32 && cols > 16;
     const int cus = device_info().cus;
     const int wg_cols = many ? cross_workgroup_columns(a, cus) : split_tile_columns(a);
@@ -2340,14 +2341,17 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
         // 24.1 in two).
         a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({cus / lists, a.nk_max / 256, 64})));
     } else {
-        // Eight wavefronts a CU: more to a workgroup first, each with a tile of
-        // keys at least, then parts, each wavefront with 256 keys at least.
-        const long long want = 8LL * cus;
-        const int most = split_max_waves(a);
-        a.waves = 1;
-        while (a.waves < most && lists * a.waves < want && a.waves * 32 < a.nk_max) a.waves *= 2;
+        // Eight wavefronts a workgroup, four to one as the lists alone give a
+        // CU 32 (256 streams of 448 int8 keys, 8 heads of 64: 32.6 us with four,
+        // 37.2 with eight or one; over 2 key heads of 48, a quarter of the
+        // lists: 16.6 with eight, 18.3 with four); no more than there are
+        // tiles. Parts until a CU has eight wavefronts, each with 64 keys at
+        // least (one stream of 8000 int8 keys: 16 us in 16 parts, 72 in one; of
+        // 448: 8.0 in one, 9.4 in two).
+        a.waves = split_max_waves(a);
+        while (a.waves > 1 && (lists * a.waves > 32LL * cus || (a.waves - 1) * 32 >= a.nk_max)) a.waves /= 2;
         a.splits = static_cast<int>(std::max<long long>(
-            1, std::min<long long>({want / (lists * a.waves), a.nk_max / (256LL * a.waves), 64})));
+            1, std::min<long long>({8LL * cus / (lists * a.waves), a.nk_max / (64LL * a.waves), 64})));
     }
     const int qsize = value_size(a.type);
     a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stream * qsize) |

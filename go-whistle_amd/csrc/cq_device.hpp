@@ -9,6 +9,14 @@
 
 namespace cqhip {
 
+// Workgroup ids go round the 8 XCDs; this order gives each XCD a run of the
+// list, so that neighbours share its L2 (the ids past a multiple of 8 keep
+// their places).
+__device__ __forceinline__ int xcd_run(int id, int total) {
+    const int full = total & ~7;
+    return id < full ? (id & 7) * (full >> 3) + (id >> 3) : id;
+}
+
 // Lane l's value from lane l ^ H of the wavefront, without the LDS
 // crossbar where a DPP move reaches: quad permutes for H = 1, 2, row shifts
 // within 16 lanes for 4, 8 (lane + H below, lane - H above), a ds_swizzle

@@ -516,6 +516,7 @@ struct SplitArgs {
     const int32_t *spans;                    // paged: the keys' spans
     const int32_t *q_len, *k_len, *index;    // memories
     int memories, nk_max, t, heads, batch;
+    int group;                               // heads a key head
     int splits;                              // parts of a list, at most 64
     int waves;                               // wavefronts of a workgroup
     const void *q;

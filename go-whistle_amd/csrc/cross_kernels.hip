@@ -90,13 +90,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, half = lane >> 5;
-    // The workgroups of one (stream, key head) on one XCD, for its L2: ids go
-    // round the 8 XCDs, so each takes a run of the list.
-    int id = blockIdx.x;
-    {
-        const int total = gridDim.x, full = total & ~7;
-        if (id < full) id = (id & 7) * (full >> 3) + (id >> 3);
-    }
+    int id = xcd_run(blockIdx.x, gridDim.x);  // the workgroups of one (stream, key head) on one XCD, for its L2
     const int sp = id % a.splits;
     id /= a.splits;
     const int ct = id % col_tiles;

@@ -136,22 +136,68 @@ struct Place {
 };
 __device__ __forceinline__ Place place_of(const SplitArgs &a, int col_tiles, int tile_cols) {
     Place p;
-    int id = blockIdx.x;
-    p.sp = id % a.splits;
-    id /= a.splits;
-    p.ct = id % col_tiles;
-    id /= col_tiles;
+    // A stream's key heads side by side on one XCD: rows of narrow heads share
+    // cache lines (256 streams of 448 int8 keys, 8 heads of 64, from 8 XCDs
+    // 32.8 us: every line, and the scales' eight times, was read more than once).
+    int id = xcd_run(blockIdx.x, gridDim.x);
+    p.ct = p.sp = 0;
+    if (col_tiles > 1) {
+        p.ct = id % col_tiles;
+        id /= col_tiles;
+    }
     p.h = id % a.c.kv_heads;
-    p.b = id / a.c.kv_heads;
-    p.group = a.heads / a.c.kv_heads;
+    id /= a.c.kv_heads;
+    if (a.splits > 1) {
+        p.sp = id % a.splits;
+        id /= a.splits;
+    }
+    p.b = id;
+    p.group = a.group;
     p.mem = a.index ? a.index[p.b] : p.b;
     p.kl = key_list(a, p.b, p.mem);
     p.cols = q_rows(a, p.b) * p.group;
     p.ok = p.kl.ok && p.ct * tile_cols < p.cols;
-    const int per = part_keys(p.kl.n, a.splits);
-    p.j0 = min(p.sp * per, p.kl.n);
-    p.j1 = min(p.j0 + per, p.kl.n);
+    p.j0 = 0;
+    p.j1 = p.kl.n;
+    if (a.splits > 1) {
+        const int per = part_keys(p.kl.n, a.splits);
+        p.j0 = min(p.sp * per, p.kl.n);
+        p.j1 = min(p.j0 + per, p.kl.n);
+    }
     return p;
+}
+
+// Column cn's query row and head.
+__device__ __forceinline__ void column_of(const SplitArgs &a, const Place &p, int cn, int &row, int &head) {
+    row = a.t == 1 ? 0 : cn / p.group;
+    head = p.h * p.group + cn - row * p.group;
+}
+__device__ __forceinline__ long long query_at(const SplitArgs &a, const Place &p, int cn) {
+    int row, head;
+    column_of(a, p, cn, row, head);
+    return static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(row) * a.q_row +
+           static_cast<long long>(head) * a.c.qk;
+}
+__device__ __forceinline__ long long part_at(const SplitArgs &a, const Place &p, int row, int head) {
+    return ((static_cast<long long>(p.b) * a.t + row) * a.heads + head) * a.splits + p.sp;
+}
+
+// Over the 16 lanes of a row, in all of them.
+template <int N>
+__device__ __forceinline__ float rotated(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += rotated<8>(x);
+    x += rotated<4>(x);
+    x += rotated<2>(x);
+    return x + rotated<1>(x);
+}
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, rotated<8>(x));
+    x = fmaxf(x, rotated<4>(x));
+    x = fmaxf(x, rotated<2>(x));
+    return fmaxf(x, rotated<1>(x));
 }
 
 // The pool (or memory) row of key j of the list.
@@ -223,26 +269,27 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
         jt.stat[tid] = mu;
         jt.stat[COLS + tid] = inv;
         if (a.part) {
-            const int cn = col0 + tid, head = p.h * p.group + cn % p.group;
-            const long long pi = ((static_cast<long long>(p.b) * a.t + cn / p.group) * a.heads + head) * a.splits + p.sp;
+            int row, head;
+            column_of(a, p, col0 + tid, row, head);
+            const long long pi = part_at(a, p, row, head);
             a.part_ml[2 * pi] = mx;
             a.part_ml[2 * pi + 1] = sum;
         }
     }
     __syncthreads();
-    for (int x = tid; x < nc * a.c.vd; x += threads) {
-        const int n = x / a.c.vd, d = x - n * a.c.vd, cn = col0 + n;
-        float v = 0.0f;
-        for (int w = 0; w < waves; ++w) v = fmaf(jt.o[(w * COLS + n) * jt.kRow + d], jt.ml[(w * 2) * COLS + n], v);
-        const int head = p.h * p.group + cn % p.group;
-        if (a.part) {
-            const long long pi = ((static_cast<long long>(p.b) * a.t + cn / p.group) * a.heads + head) * a.splits + p.sp;
-            a.part[pi * a.c.vd + d] = v;
-        } else {
-            store_value(a.out, a.type,
-                        static_cast<long long>(p.b) * a.out_stream + static_cast<long long>(cn / p.group) * a.out_row +
-                            static_cast<long long>(head) * a.c.vd + d,
-                        v * jt.stat[COLS + n]);
+    for (int n = tid >> 6; n < nc; n += waves) {
+        int row, head;
+        column_of(a, p, col0 + n, row, head);
+        for (int d = tid & 63; d < a.c.vd; d += 64) {
+            float v = 0.0f;
+            for (int w = 0; w < waves; ++w) v = fmaf(jt.o[(w * COLS + n) * jt.kRow + d], jt.ml[(w * 2) * COLS + n], v);
+            if (a.part)
+                a.part[part_at(a, p, row, head) * a.c.vd + d] = v;
+            else
+                store_value(a.out, a.type,
+                            static_cast<long long>(p.b) * a.out_stream + static_cast<long long>(row) * a.out_row +
+                                static_cast<long long>(head) * a.c.vd + d,
+                            v * jt.stat[COLS + n]);
         }
     }
     if (a.acc_out && !a.logits) {  // the whole list's weights
@@ -258,11 +305,11 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
 
 // TYPE: the cache's type; D: widths up to D (64, 128, 256); COLS: columns a tile.
 template <int TYPE, int D, int COLS>
-__global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_lanes_kernel(SplitArgs a, int col_tiles) {
+__global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(SplitArgs a, int col_tiles) {
     constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
     constexpr int kPer = 16 / kSize;         // elements of a piece
     constexpr int kPieces = D / (4 * kPer);  // pieces of a row a lane reads
-    constexpr int kSub = D * kSize <= 64 ? 4 : D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
+    constexpr int kSub = D * kSize <= 64 ? 2 : D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
     constexpr int kTile = 16 * kSub;
     extern __shared__ __align__(16) float smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -275,9 +322,7 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
     float q[COLS][kPieces * kPer], o[COLS][kPieces * kPer], m[COLS], l[COLS];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        const int cn = min(col0 + n, p.cols - 1);
-        const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(cn / p.group) * a.q_row +
-                             static_cast<long long>(p.h * p.group + cn % p.group) * a.c.qk;
+        const long long qo = query_at(a, p, min(col0 + n, p.cols - 1));
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
             const int d0 = (4 * k + c) * kPer;
@@ -374,10 +419,7 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
                     }
                     mt = fmaxf(mt, x[n][s]);
                 }
-                mt = fmaxf(mt, xor_lane<1>(mt));
-                mt = fmaxf(mt, xor_lane<2>(mt));
-                mt = fmaxf(mt, xor_lane<4>(mt));
-                mt = fmaxf(mt, xor_lane<8>(mt));
+                mt = row_max(mt);
                 const float mu = mt == -INFINITY ? 0.0f : mt;
                 const float f = __builtin_amdgcn_exp2f(m[n] - mu);
                 m[n] = mt;
@@ -411,11 +453,7 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
     // the sums over the keys' lanes, then the wavefronts'
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        float lt = l[n];
-        lt += xor_lane<1>(lt);
-        lt += xor_lane<2>(lt);
-        lt += xor_lane<4>(lt);
-        lt += xor_lane<8>(lt);
+        const float lt = row_sum(l[n]);
         if (lane == 0) {
             jt.ml[(wave * 2) * COLS + n] = m[n];
             jt.ml[(wave * 2 + 1) * COLS + n] = lt;
@@ -424,17 +462,8 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
         for (int k = 0; k < kPieces; ++k)
 #pragma unroll
             for (int e = 0; e < kPer; e += 4) {
-                float4 y;
-                float *ys = &y.x;
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    float t = o[n][k * kPer + e + z];
-                    t += xor_lane<1>(t);
-                    t += xor_lane<2>(t);
-                    t += xor_lane<4>(t);
-                    t += xor_lane<8>(t);
-                    ys[z] = t;
-                }
+                const float *t = &o[n][k * kPer + e];
+                const float4 y = make_float4(row_sum(t[0]), row_sum(t[1]), row_sum(t[2]), row_sum(t[3]));
                 if (r == 0) *reinterpret_cast<float4 *>(&jt.o[(wave * COLS + n) * jt.kRow + (4 * k + c) * kPer + e]) = y;
             }
     }
@@ -443,7 +472,7 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
 
 // TYPE: the cache's type; D: widths up to D (64, 128, 256).
 template <int TYPE, int D>
-__global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
+__global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
     constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
     constexpr int kPer = 16 / kSize;          // elements of a 16-byte piece of a key row
     constexpr int kPieces = D / (4 * kPer);   // pieces of a key row a lane loads
@@ -463,9 +492,7 @@ __global__ __launch_bounds__(D == 64 ? 1024 : D == 128 ? 512 : 256) void attend_
     // The query's pieces, 1/scale and log2(e) folded in.
     float qv[kPieces * kPer];
     {
-        const int cn = col_ok ? col : 0;
-        const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(cn / p.group) * a.q_row +
-                             static_cast<long long>(p.h * p.group + cn % p.group) * a.c.qk;
+        const long long qo = query_at(a, p, col_ok ? col : 0);
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
             const int d0 = (4 * k + c) * kPer;
@@ -716,7 +743,7 @@ int split_tile_columns(const SplitArgs &a) {
 
 int split_max_waves(const SplitArgs &a) {
     const int w = std::max(a.c.qk, a.c.vd);
-    return w <= 64 ? 16 : w <= 128 ? 8 : 4;
+    return w <= 128 ? 8 : 4;
 }
 
 bool split_weights_in_lds(const SplitArgs &a, int waves) {
