@@ -2329,7 +2329,11 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
 static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     a.group = a.heads / a.c.kv_heads;
     const long long cols = static_cast<long long>(a.t) * a.group;
-    const bool many = !a.spans && a.type != ND_F32 && cols > 16;
+    // 16-bit memories take the matrix form from two columns on (64 streams of
+    // 1500 frames, 8 heads of 128 over 2: 26.9 us against 33.2 at 4 columns,
+    // 27.6 against 35.2 at 16; of one column 82 against 89 at best, 47 against
+    // 39 at worst).
+    const bool many = !a.spans && a.type != ND_F32 && cols > 1;
     const int cus = device_info().cus;
     const int wg_cols = many ? cross_workgroup_columns(a, cus) : split_tile_columns(a);
     const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((cols + wg_cols - 1) / wg_cols);
@@ -2342,14 +2346,14 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
         a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({cus / lists, a.nk_max / 256, 64})));
     } else {
         // Eight wavefronts a workgroup, four to one as the lists alone give a
-        // CU 32 (256 streams of 448 int8 keys, 8 heads of 64: 32.6 us with four,
-        // 37.2 with eight or one; over 2 key heads of 48, a quarter of the
-        // lists: 16.6 with eight, 18.3 with four); no more than there are
+        // CU 16 (256 streams of up to 448 int8 keys, 8 heads of 64: 25.4 us with
+        // two, 27.5 with four, 34.2 with one; over 2 key heads of 48, a quarter
+        // of the lists: 16.6 with eight, 18.3 with four); no more than there are
         // tiles. Parts until a CU has eight wavefronts, each with 64 keys at
         // least (one stream of 8000 int8 keys: 16 us in 16 parts, 72 in one; of
         // 448: 8.0 in one, 9.4 in two).
         a.waves = split_max_waves(a);
-        while (a.waves > 1 && (lists * a.waves > 32LL * cus || (a.waves - 1) * 32 >= a.nk_max)) a.waves /= 2;
+        while (a.waves > 1 && (lists * a.waves > 16LL * cus || (a.waves - 1) * 32 >= a.nk_max)) a.waves /= 2;
         a.splits = static_cast<int>(std::max<long long>(
             1, std::min<long long>({8LL * cus / (lists * a.waves), a.nk_max / (64LL * a.waves), 64})));
     }

@@ -23,7 +23,12 @@
 //   S = K q^T: A row r is key r, the contraction index c a 16-byte piece of
 //     the key row, so a lane's global load is its operand; element e of the
 //     piece goes to the e-th MFMA, whose B operand is the query's same
-//     element. S has key 4c + i in register i of lane (column, c).
+//     element. S has key 4c + i in register i of lane (column, c). 16-bit keys,
+//     and int8 ones widened to bfloat16 (exactly), take v_mfma_f32_16x16x32
+//     instead, eight elements at a time: with the query as it is where it has
+//     the keys' type, else as the exact sum of three bfloat16 parts (24 bits).
+//     The products are exact either way; the eight float32 instructions that
+//     one to three of them replace left the matrix pipe 57% busy at 4.6 TB/s.
 //   O = V^T P: the register P_i is the B operand as it lies (contraction
 //     index c is key 4c + i), and A is a lane's piece of value row 4c + i,
 //     elements e of 16 lanes the rows of the e-th MFMA. m and l belong to
@@ -470,8 +475,27 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
     finish<COLS, D>(a, p, jt);
 }
 
-// TYPE: the cache's type; D: widths up to D (64, 128, 256).
-template <int TYPE, int D>
+// Two floats' upper halves: x in the lower 16 bits, y in the upper.
+__device__ __forceinline__ uint32_t upper_pair(float x, float y) {
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);
+}
+
+template <int TYPE>
+__device__ __forceinline__ f32x4 mfma_16x16x32(const uint32_t *a, const uint32_t *b, f32x4 c) {
+    using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+    const u32x4 x = {a[0], a[1], a[2], a[3]}, y = {b[0], b[1], b[2], b[3]};
+    if constexpr (TYPE == 1) {
+        using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+    } else {
+        using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+    }
+}
+
+// TYPE: the cache's type; D: widths up to D (64, 128, 256); PARTS: 16-bit
+// parts of a query value (0: the products of the logits in float32).
+template <int TYPE, int D, int PARTS>
 __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
     constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
     constexpr int kPer = 16 / kSize;          // elements of a 16-byte piece of a key row
@@ -489,18 +513,44 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
     const int col = p.ct * kCols + r;  // this lane's column: query row col / group, head col % group of the group
     const bool col_ok = col < p.cols;
 
-    // The query's pieces, 1/scale and log2(e) folded in.
-    float qv[kPieces * kPer];
+    // The query's pieces: in float32 with 1/scale and log2(e) folded in, or in
+    // 16-bit parts of eight.
+    constexpr int kEights = PARTS ? kPer / 8 : 1;
+    float qv[PARTS ? 1 : kPieces * kPer];
+    uint32_t qp[PARTS ? PARTS : 1][kPieces][kEights][4];
     {
         const long long qo = query_at(a, p, col_ok ? col : 0);
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
             const int d0 = (4 * k + c) * kPer;
+            float x[kPer];
             if (col_ok && d0 < a.c.qk) {
-                load_query<kPer>(&qv[k * kPer], a, qo + d0, a.scale_log2);
+                load_query<kPer>(x, a, qo + d0, PARTS ? 1.0f : a.scale_log2);
             } else {
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) qv[k * kPer + e] = 0.0f;
+                for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
+            }
+            if constexpr (PARTS == 0) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) qv[k * kPer + e] = x[e];
+            } else if constexpr (TYPE == 1) {  // a float16 query
+#pragma unroll
+                for (int e = 0; e < kPer; e += 2)
+                    qp[0][k][e / 8][e / 2 % 4] =
+                        __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e])) |
+                        static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e + 1]))) << 16;
+            } else {
+#pragma unroll
+                for (int z = 0; z < PARTS; ++z)
+#pragma unroll
+                    for (int e = 0; e < kPer; e += 2) {
+                        qp[z][k][e / 8][e / 2 % 4] = upper_pair(x[e], x[e + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {  // what the part leaves: nothing of an infinity
+                            const float part = __uint_as_float(__float_as_uint(x[e + i]) & 0xffff0000u);
+                            x[e + i] = fabsf(part) < INFINITY ? x[e + i] - part : 0.0f;
+                        }
+                    }
             }
         }
     }
@@ -565,14 +615,32 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
             f32x4 sc[kSub];
 #pragma unroll
             for (int s = 0; s < kSub; ++s) sc[s] = f32x4{0, 0, 0, 0};
+            if constexpr (PARTS == 0) {
 #pragma unroll
-            for (int k = 0; k < kPieces; ++k)
+                for (int k = 0; k < kPieces; ++k)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e)
+                    for (int e = 0; e < kPer; ++e)
 #pragma unroll
-                    for (int s = 0; s < kSub; ++s)
-                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(kw[s][k], e), qv[k * kPer + e],
-                                                                     sc[s], 0, 0, 0);
+                        for (int s = 0; s < kSub; ++s)
+                            sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(kw[s][k], e),
+                                                                         qv[k * kPer + e], sc[s], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+                    for (int e = 0; e < kEights; ++e)
+#pragma unroll
+                        for (int s = 0; s < kSub; ++s) {
+                            uint32_t ka[4];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z)
+                                ka[z] = TYPE == 3 ? upper_pair(piece_value<TYPE>(kw[s][k], 8 * e + 2 * z),
+                                                               piece_value<TYPE>(kw[s][k], 8 * e + 2 * z + 1))
+                                                  : kw[s][k][z];
+#pragma unroll
+                            for (int z = 0; z < PARTS; ++z) sc[s] = mfma_16x16x32<TYPE>(ka, qp[z][k][e], sc[s]);
+                        }
+            }
             if (jn < p.j1) load_keys(kw, rows);
 
             float mt = m;
@@ -582,6 +650,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                 for (int i = 0; i < 4; ++i) {
                     const int jj = j + 16 * s + 4 * c + i;
                     float x = sc[s][i];
+                    if constexpr (PARTS > 0) x *= a.scale_log2;
                     if constexpr (TYPE == 3) x *= ksc[s][i];
                     if (jj >= p.j1) {
                         x = -INFINITY;
@@ -713,15 +782,23 @@ hipError_t launch_with(F *fn, const SplitArgs &a, int tile_cols, size_t lds, std
     return hipGetLastError();
 }
 
+template <int TYPE, int D, int PARTS>
+hipError_t launch_columns(const SplitArgs &a, hipStream_t s) {
+    static std::atomic<unsigned long long> attr{0};
+    return launch_with(&attend_split_kernel<TYPE, D, PARTS>, a, kCols, joint_lds<kCols, D>(a, a.waves), attr, s);
+}
+
 template <int TYPE, int D>
 hipError_t launch_split(const SplitArgs &a, hipStream_t s) {
-    static std::atomic<unsigned long long> one{0}, two{0}, many{0};
+    static std::atomic<unsigned long long> one{0}, two{0};
     const int tile = split_tile_columns(a);
     if (tile == 1)
         return launch_with(&attend_lanes_kernel<TYPE, D, 1>, a, 1, joint_lds<1, D>(a, a.waves), one, s);
     if (tile == 2)
         return launch_with(&attend_lanes_kernel<TYPE, D, 2>, a, 2, joint_lds<2, D>(a, a.waves), two, s);
-    return launch_with(&attend_split_kernel<TYPE, D>, a, kCols, joint_lds<kCols, D>(a, a.waves), many, s);
+    if constexpr (TYPE == 0) return launch_columns<TYPE, D, 0>(a, s);
+    if constexpr (TYPE == 1) return a.type == 1 ? launch_columns<TYPE, D, 1>(a, s) : launch_columns<TYPE, D, 0>(a, s);
+    if constexpr (TYPE >= 2) return a.type == 2 ? launch_columns<TYPE, D, 1>(a, s) : launch_columns<TYPE, D, 3>(a, s);
 }
 
 template <int TYPE>

@@ -202,20 +202,15 @@ def ApplyShared(dsts, x, rows, *ls):
 # ---- caches and memories of any type and length, log probabilities ----------------
 
 
-def _types():
-    import torch
-
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
-
-
-_TYPES = None
+_TYPES = {}
 
 
 def _type(t, what, cache=False):
     """ND_F32.. of a tensor's dtype; ND_I8 for caches only."""
-    global _TYPES
-    if _TYPES is None:
-        _TYPES = _types()
+    if not _TYPES:
+        import torch
+
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3})
     code = _TYPES.get(t.dtype)
     if code is None or (code == 3 and not cache):
         raise CQPanic(f"needle: {what} of {t.dtype}")
@@ -224,7 +219,7 @@ def _type(t, what, cache=False):
 
 def _want(t, what, shape, dtype=None, dev=None, dense=True):
     """Refuses a tensor that the call would read or write out of its bounds."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise CQPanic(f"needle: {what} of shape {tuple(t.shape)}, not {tuple(shape)}")
     if dtype is not None and t.dtype != dtype:
         raise CQPanic(f"needle: {what} of {t.dtype}, not {dtype}")
@@ -238,25 +233,16 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The device of the tensors current, and its current stream, for one call."""
+def _call(fn, device, *args):
+    """fn(*args, the current stream of the tensors' device), with that device current."""
+    import torch
 
-    def __init__(self, device):
-        import torch
-
-        self.torch, self.device = torch, device
-        self.guard = None
-
-    def __enter__(self):
-        cuda = self.torch.cuda
-        if self.device.index != cuda.current_device():
-            self.guard = cuda.device(self.device)
-            self.guard.__enter__()
-        return cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+    index = device.index
+    if index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 class PagedKV:
@@ -316,10 +302,9 @@ class PagedKV:
         if cap is None:
             cap = self.pages.shape[1] * self.k.shape[1]
         acc_cap = self._acc(acc, "weights", cap) if acc is not None else 0
-        with _on(self.device) as st:
-            check(lib().kv_append_paged_dev(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                            v.stride(1), _type(k, "rows"), self.streams, t, _ptr(rows), pos.data_ptr(),
-                                            cap, _ptr(acc), acc_cap, st))
+        _call(lib().kv_append_paged_dev, self.device, self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+              v.stride(0), v.stride(1), _type(k, "rows"), self.streams, t, _ptr(rows), pos.data_ptr(), cap, _ptr(acc),
+              acc_cap)
 
     def attend_dev(self, out, q, spans, nk_max, scale, acc=None, acc_out=None):
         """Attention of one token a stream: q [streams, heads, qk] and out
@@ -340,10 +325,9 @@ class PagedKV:
                 raise CQPanic(f"needle: weights of {acc.shape[-1]} rows to {acc_cap}")
         elif acc is not None:
             raise CQPanic("needle: weights without an output for them")
-        with _on(self.device) as st:
-            check(lib().kv_attend_paged_dev(self._ref, out.data_ptr(), 0, q.data_ptr(), 0, _type(q, "queries"),
-                                            self.streams, heads, spans.data_ptr(), nk_max, scale, _ptr(acc),
-                                            _ptr(acc_out), acc_cap, st))
+        _call(lib().kv_attend_paged_dev, self.device, self._ref, out.data_ptr(), 0, q.data_ptr(), 0,
+              _type(q, "queries"), self.streams, heads, spans.data_ptr(), nk_max, scale, _ptr(acc), _ptr(acc_out),
+              acc_cap)
 
     def evict_dev(self, dst_pages, acc, acc_out, length, length_out, kept, nk_max, sink=0, recent=0):
         """Each stream's first length[b] (<= nk_max) rows cut to keep =
@@ -360,10 +344,9 @@ class PagedKV:
         _want(length, "lengths", (self.streams,), torch.int32, self.device)
         _want(length_out, "lengths", (self.streams,), torch.int32, self.device)
         acc_cap, out_cap = self._acc(acc, "weights", nk_max), self._acc(acc_out, "weights", keep)
-        with _on(self.device) as st:
-            check(lib().kv_evict_paged_dev(self._ref, dst_pages.data_ptr(), dst_pages.shape[1], acc.data_ptr(), acc_cap,
-                                           acc_out.data_ptr(), out_cap, length.data_ptr(), length_out.data_ptr(),
-                                           kept.data_ptr(), self.streams, nk_max, keep, sink, recent, st))
+        _call(lib().kv_evict_paged_dev, self.device, self._ref, dst_pages.data_ptr(), dst_pages.shape[1],
+              acc.data_ptr(), acc_cap, acc_out.data_ptr(), out_cap, length.data_ptr(), length_out.data_ptr(),
+              kept.data_ptr(), self.streams, nk_max, keep, sink, recent)
 
 
 def cross_attend_dev(out, q, k, v, scale, q_len=None, k_len=None, index=None):
@@ -393,12 +376,10 @@ def cross_attend_dev(out, q, k, v, scale, q_len=None, k_len=None, index=None):
     for x, n, what in ((q_len, B, "query lengths"), (k_len, M, "memory lengths"), (index, B, "memory index")):
         if x is not None:
             _want(x, what, (n,), torch.int32, dev)
-    y = CrossLayout(q.stride(0), q.stride(1), out.stride(0), out.stride(1), k.stride(0), k.stride(1), k.stride(2),
-                    v.stride(0), v.stride(1), v.stride(2))
-    with _on(dev) as st:
-        check(lib().nd_cross_attend_dev(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _type(q, "queries"),
-                                        ctypes.byref(y), B, t, heads, kv_heads, qk, vd, M, frames, _ptr(q_len),
-                                        _ptr(k_len), _ptr(index), scale, st))
+    y = CrossLayout(*q.stride()[:2], *out.stride()[:2], *k.stride()[:3], *v.stride()[:3])
+    _call(lib().nd_cross_attend_dev, dev, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+          _type(q, "queries"), ctypes.byref(y), B, t, heads, kv_heads, qk, vd, M, frames, _ptr(q_len), _ptr(k_len),
+          _ptr(index), scale)
 
 
 def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
@@ -422,7 +403,5 @@ def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
                                   (top_lp, (rows, k), f32, "alternatives' log probabilities")):
         if x is not None:
             _want(x, what, shape, dtype, dev)
-    with _on(dev) as st:
-        check(lib().nd_logprobs_dev(_ptr(lp), _ptr(ent), _ptr(top) if k else None, _ptr(top_lp) if k else None,
-                                    logits.data_ptr(), logits.stride(0), _type(logits, "logits"), rows, n, _ptr(tokens),
-                                    k, st))
+    _call(lib().nd_logprobs_dev, dev, _ptr(lp), _ptr(ent), _ptr(top) if k else None, _ptr(top_lp) if k else None,
+          logits.data_ptr(), logits.stride(0), _type(logits, "logits"), rows, n, _ptr(tokens), k)

@@ -515,7 +515,9 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * head h / (heads/kv_heads). spans are [batch][4] as kv_attend_int8_dev
  * takes them for t = 1: {lo0, hi0, lo1, hi1}, ascending, disjoint and inside
  * [0, nk_max); others leave the stream's output as it was, and spans with no
- * key give zeros. A page outside the pool reads page 0.
+ * key give zeros. A page outside the pool reads page 0. Rows outside the spans
+ * may hold anything; an infinity among the keys of a span may make its logit
+ * NaN (a float32 query meets 16-bit keys in three parts, some of them 0).
  * acc_out non-null ([batch][kv_heads][acc_cap], acc_cap >= nk_max): for
  * each row j of the spans, acc_out[j] = acc[j] (null: 0) + the sum over the
  * key head's query heads of their softmax weights; other entries are left
@@ -561,8 +563,9 @@ typedef struct nd_cross_layout {
  * head h / (heads/kv_heads). layout null: dense [batch][t][heads][width] and
  * [memories][frames][kv_heads][width]. qk and vd are multiples of 16 up to
  * 256; k, v and their strides are multiples of 16 bytes. ND_F32 products are
- * float32; with 16-bit types the products take them as they are and, for many
- * rows, the softmax weights rounded to the type; sums and softmax are float32. */
+ * float32; with 16-bit types the products take them as they are and, unless one
+ * query row reads a key head, the softmax weights rounded to the type; sums and
+ * softmax are float32. */
 int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
                         const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
                         int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,
