@@ -11,20 +11,48 @@ namespace {
 
 // ---- append ---------------------------------------------------------------------
 
-// A head's row of width values is one unit: LANES = the power of two of lanes
-// that hold it at four values each, so a wavefront takes 64 / LANES units and
-// an int8 row's bound is a few exchanges within them. Units in (keys or
-// values, stream, row, head) order: a wavefront's loads and stores are
+// Four values of a row, from an array of `type` (vec: its pieces of four are
+// aligned to their size), widened.
+__device__ __forceinline__ void load_four(float *x, const void *p, int type, long long at, bool vec) {
+    if (type == 0) {
+        const float *s = static_cast<const float *>(p) + at;
+        if (vec) {
+            const float4 u = *reinterpret_cast<const float4 *>(s);
+            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = s[e];
+        }
+        return;
+    }
+    const uint16_t *s = static_cast<const uint16_t *>(p) + at;
+    uint32_t w[2];
+    if (vec) {
+        *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(s);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) w[e] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint16_t h = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        x[e] = type == 1 ? static_cast<float>(__builtin_bit_cast(_Float16, h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+    }
+}
+
+// A head's key row and value row of one stream's row are one unit: LANES = the
+// power of two of lanes that hold a row at four values each, so a wavefront
+// takes 64 / LANES units, the way through the page table is paid once for
+// both rows, and an int8 row's bound is a few exchanges within its lanes.
+// Units in (stream, row, head) order: a wavefront's loads and stores are
 // consecutive.
 template <int TYPE, int LANES>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, long long units, int vec) {
-    const long long u = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / LANES;
-    if (u >= 2 * units) return;
-    const int which = u >= units;
-    const long long w = which ? u - units : u;
-    const int h = static_cast<int>(w % a.c.kv_heads);
-    const long long bi = w / a.c.kv_heads;
-    const int i = static_cast<int>(bi % a.t), b = static_cast<int>(bi / a.t);
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, unsigned units, int vec) {
+    const unsigned u = (blockIdx.x * 256u + threadIdx.x) / LANES;
+    if (u >= units) return;
+    const unsigned bi = u / a.c.kv_heads;
+    const int h = static_cast<int>(u - bi * a.c.kv_heads);
+    const int b = static_cast<int>(bi / a.t), i = static_cast<int>(bi - static_cast<unsigned>(b) * a.t);
     if (a.rows) {
         const int n = a.rows[b];
         if (n > a.t || i >= n) return;
@@ -33,74 +61,67 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, lo
     if (p < 0 || p >= a.cap) return;
     const int pg = a.c.pages[static_cast<long long>(b) * a.c.page_stride + (p >> a.c.shift)];
     if (pg < 0 || pg >= a.c.pool_pages) return;
-    const long long row = (static_cast<long long>(pg) << a.c.shift) + (p & ((1 << a.c.shift) - 1));
-    const int width = which ? a.c.vd : a.c.qk;
+    const long long to = ((static_cast<long long>(pg) << a.c.shift) + (p & ((1 << a.c.shift) - 1))) * a.c.kv_heads + h;
     const int lane = threadIdx.x & (LANES - 1), d = 4 * lane;
-    if (a.acc && !which && lane == 0) a.acc[(static_cast<long long>(b) * a.c.kv_heads + h) * a.acc_cap + p] = 0.0f;
-    const long long at = static_cast<long long>(b) * a.stream[which] + static_cast<long long>(i) * a.row[which] +
-                         static_cast<long long>(h) * width + d;
-    const bool live = d < width;
-    float x[4] = {0, 0, 0, 0};
-    if (live) {
-        if (a.type == 0) {
-            const float *s = static_cast<const float *>(a.x[which]) + at;
-            if (vec >> which & 1) {
-                const float4 v = *reinterpret_cast<const float4 *>(s);
-                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-            } else {
+    if (a.acc && lane == 0) a.acc[(static_cast<long long>(b) * a.c.kv_heads + h) * a.acc_cap + p] = 0.0f;
+    const int width[2] = {a.c.qk, a.c.vd};
+    float x[2][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = s[e];
-            }
+    for (int z = 0; z < 2; ++z) {
+        if (d < width[z]) {
+            load_four(x[z], a.x[z], a.type,
+                       static_cast<long long>(b) * a.stream[z] + static_cast<long long>(i) * a.row[z] +
+                           static_cast<long long>(h) * width[z] + d,
+                       vec >> z & 1);
         } else {
-            const uint16_t *s = static_cast<const uint16_t *>(a.x[which]) + at;
-            uint16_t v[4];
-            if (vec >> which & 1) {
-                *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(s);
-            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = s[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[e] = a.type == 1 ? static_cast<float>(__builtin_bit_cast(_Float16, v[e]))
-                                   : __uint_as_float(static_cast<uint32_t>(v[e]) << 16);
+            for (int e = 0; e < 4; ++e) x[z][e] = 0.0f;
         }
     }
-    unsigned char *dst = which ? a.c.v : a.c.k;
-    const long long to = (row * a.c.kv_heads + h) * width + d;
-    if constexpr (TYPE == 3) {
-        // QuantizeRow (int8.go:36-55) over the head's values
-        float m = go_max(go_max(fabsf(x[0]), fabsf(x[1])), go_max(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) m = go_max(m, __shfl_xor(m, o));
-        const float sc = m > 0.0f ? m / 127.0f : 1.0f;
-        if (live) {
-            uint32_t q = 0;
+    for (int z = 0; z < 2; ++z) {
+        unsigned char *dst = z ? a.c.v : a.c.k;
+        const long long at = to * width[z] + d;
+        const bool live = d < width[z];
+        if constexpr (TYPE == 3) {
+            // QuantizeRow (int8.go:36-55) over the head's values
+            float m = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q |= (static_cast<uint32_t>(go_int8_code(rintf(x[e] / sc))) & 255u) << (8 * e);
-            *reinterpret_cast<uint32_t *>(dst + to) = q;
-        }
-        if (lane == 0) (which ? a.c.vs : a.c.ks)[row * a.c.kv_heads + h] = sc;
-    } else if (live) {
-        if constexpr (TYPE == 0) {
-            reinterpret_cast<float4 *>(dst)[to >> 2] = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-            uint16_t v[4];
+            for (int e = 0; e < 4; ++e) m = go_max(m, fabsf(x[z][e]));
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = TYPE == 1 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e]))
-                                 : __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[e]));
-            reinterpret_cast<uint2 *>(dst)[to >> 2] = *reinterpret_cast<uint2 *>(v);
+            for (int o = LANES / 2; o > 0; o >>= 1) m = go_max(m, __shfl_xor(m, o));
+            const float sc = m > 0.0f ? m / 127.0f : 1.0f;
+            if (live) {
+                uint32_t q = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    q |= (static_cast<uint32_t>(go_int8_code(rintf(x[z][e] / sc))) & 255u) << (8 * e);
+                *reinterpret_cast<uint32_t *>(dst + at) = q;
+            }
+            if (lane == 0) (z ? a.c.vs : a.c.ks)[to] = sc;
+        } else if (live) {
+            if constexpr (TYPE == 0) {
+                reinterpret_cast<float4 *>(dst)[at >> 2] = make_float4(x[z][0], x[z][1], x[z][2], x[z][3]);
+            } else {
+                uint32_t w[2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint16_t v = TYPE == 1 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[z][e]))
+                                                 : __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[z][e]));
+                    w[e / 2] = e & 1 ? w[e / 2] | static_cast<uint32_t>(v) << 16 : v;
+                }
+                reinterpret_cast<uint2 *>(dst)[at >> 2] = make_uint2(w[0], w[1]);
+            }
         }
     }
 }
 
 template <int TYPE, int LANES>
 hipError_t launch_append_lanes(const PagedAppendArgs &a, int vec, hipStream_t s) {
-    const long long units = static_cast<long long>(a.batch) * a.t * a.c.kv_heads;
-    const long long blocks = (2 * units * LANES + 255) / 256;
+    const long long units = static_cast<long long>(a.batch) * a.t * a.c.kv_heads;  // below 2^32 / 128
+    const long long blocks = (units * LANES + 255) / 256;
     hipLaunchKernelGGL((paged_append_kernel<TYPE, LANES>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a,
-                       units, vec);
+                       static_cast<unsigned>(units), vec);
     return hipGetLastError();
 }
 
