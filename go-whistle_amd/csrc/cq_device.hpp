@@ -9,12 +9,24 @@
 
 namespace cqhip {
 
-// Workgroup ids go round the 8 XCDs; this order gives each XCD a run of the
-// list, so that neighbours share its L2 (the ids past a multiple of 8 keep
-// their places).
-__device__ __forceinline__ int xcd_run(int id, int total) {
-    const int full = total & ~7;
-    return id < full ? (id & 7) * (full >> 3) + (id >> 3) : id;
+// A launch of `units` groups of `per` workgroups, the workgroups of a group on
+// one XCD, whose L2 they share. Ids go round the 8 XCDs: from kXcdUnits groups
+// on, group u is XCD u % 8's (neighbours in the list, which may be alike in
+// length, on different XCDs; the grid is padded to whole rounds, xcd_grid),
+// fewer groups are cut into 8 runs of workgroups.
+struct XcdPlace {
+    int unit, within;
+    bool ok;
+};
+__device__ __forceinline__ XcdPlace xcd_place(int units, int per) {
+    const int id = blockIdx.x;
+    if (units >= kXcdUnits) {
+        const int s = id >> 3, u = s / per, unit = u * 8 + (id & 7);
+        return {unit, s - u * per, unit < units};
+    }
+    const int full = static_cast<int>(gridDim.x) & ~7;
+    const int x = id < full ? (id & 7) * (full >> 3) + (id >> 3) : id;
+    return {x / per, x % per, true};
 }
 
 // Lane l's value from lane l ^ H of the wavefront, without the LDS

@@ -471,6 +471,12 @@ hipError_t launch_gather_float_rows(float *dst, const float *src, const int32_t 
 
 // ---- caches and memories of any type and length (split_kernels.hip, paged_kernels.hip) ----
 
+// Workgroups of a launch of `units` groups of `per` that xcd_place hands out.
+constexpr int kXcdUnits = 64;
+inline long long xcd_grid(long long units, long long per) {
+    return (units >= kXcdUnits ? (units + 7) / 8 * 8 : units) * per;
+}
+
 // A paged cache as kv_paged describes it (pages of 2^shift rows).
 struct PagedArgs {
     unsigned char *k, *v;

@@ -90,12 +90,10 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, half = lane >> 5;
-    int id = xcd_run(blockIdx.x, gridDim.x);  // the workgroups of one (stream, key head) on one XCD, for its L2
-    const int sp = id % a.splits;
-    id /= a.splits;
-    const int ct = id % col_tiles;
-    id /= col_tiles;
-    const int h = id % a.c.kv_heads, b = id / a.c.kv_heads;
+    const XcdPlace x = xcd_place(a.batch * a.c.kv_heads, col_tiles * a.splits);  // a (stream, key head) on one XCD
+    if (!x.ok) return;
+    const int ct = x.within / a.splits, sp = x.within - ct * a.splits;
+    const int b = x.unit / a.c.kv_heads, h = x.unit - b * a.c.kv_heads;
     const int group = a.heads / a.c.kv_heads;
     const int mem = a.index ? a.index[b] : b;
     if (mem < 0 || mem >= a.memories) return;
@@ -307,7 +305,7 @@ hipError_t launch_cross_full(const SplitArgs &a, int cols, int aligned, hipStrea
     if (lds > 64 * 1024)
         if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(&cross_attend_kernel<TYPE, D, CB, FULL>), lds, attr)) return e;
     const int col_tiles = (cols + kXWaves * 32 * CB - 1) / (kXWaves * 32 * CB);
-    const long long grid = static_cast<long long>(a.batch) * a.c.kv_heads * col_tiles * a.splits;
+    const long long grid = xcd_grid(static_cast<long long>(a.batch) * a.c.kv_heads, static_cast<long long>(col_tiles) * a.splits);
     hipLaunchKernelGGL((cross_attend_kernel<TYPE, D, CB, FULL>), dim3(static_cast<unsigned>(grid)), dim3(64 * kXWaves), lds, s,
                        a, col_tiles, aligned);
     return hipGetLastError();

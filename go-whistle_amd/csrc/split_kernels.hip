@@ -141,22 +141,25 @@ struct Place {
 };
 __device__ __forceinline__ Place place_of(const SplitArgs &a, int col_tiles, int tile_cols) {
     Place p;
-    // A stream's key heads side by side on one XCD: rows of narrow heads share
-    // cache lines (256 streams of 448 int8 keys, 8 heads of 64, from 8 XCDs
-    // 32.8 us: every line, and the scales' eight times, was read more than once).
-    int id = xcd_run(blockIdx.x, gridDim.x);
+    // A part's key heads on one XCD: rows of narrow heads share cache lines
+    // (256 streams of 448 int8 keys, 8 heads of 64, spread over the XCDs 32.8
+    // us: every line, and the scales' eight times, was read more than once).
+    const XcdPlace x = xcd_place(a.batch * a.splits, a.c.kv_heads * col_tiles);
     p.ct = p.sp = 0;
+    p.h = x.within;
     if (col_tiles > 1) {
-        p.ct = id % col_tiles;
-        id /= col_tiles;
+        p.h = x.within / col_tiles;
+        p.ct = x.within - p.h * col_tiles;
     }
-    p.h = id % a.c.kv_heads;
-    id /= a.c.kv_heads;
+    p.b = x.unit;
     if (a.splits > 1) {
-        p.sp = id % a.splits;
-        id /= a.splits;
+        p.b = x.unit / a.splits;
+        p.sp = x.unit - p.b * a.splits;
     }
-    p.b = id;
+    if (!x.ok) {
+        p.ok = false;
+        return p;
+    }
     p.group = a.group;
     p.mem = a.index ? a.index[p.b] : p.b;
     p.kl = key_list(a, p.b, p.mem);
@@ -777,7 +780,7 @@ hipError_t launch_with(F *fn, const SplitArgs &a, int tile_cols, size_t lds, std
     if (lds > 64 * 1024)
         if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(fn), kMostLds, attr)) return e;
     const int cols = a.t * (a.heads / a.c.kv_heads), col_tiles = (cols + tile_cols - 1) / tile_cols;
-    const long long grid = static_cast<long long>(a.batch) * a.c.kv_heads * col_tiles * a.splits;
+    const long long grid = xcd_grid(static_cast<long long>(a.batch) * a.splits, static_cast<long long>(a.c.kv_heads) * col_tiles);
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * a.waves), lds, s, a, col_tiles);
     return hipGetLastError();
 }
