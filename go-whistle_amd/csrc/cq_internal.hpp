@@ -524,7 +524,8 @@ struct SplitArgs {
     int memories, nk_max, t, heads, batch;
     int group;                               // heads a key head
     int splits;                              // parts of a list, at most 64
-    int waves;                               // wavefronts of a workgroup
+    int waves;                               // wavefronts of a workgroup (attend_split)
+    int by_length;                           // streams of long memories first (cross_attend)
     const void *q;
     void *out;
     long long q_stream, q_row, out_stream, out_row;  // elements

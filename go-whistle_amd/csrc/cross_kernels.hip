@@ -77,6 +77,23 @@ __device__ __forceinline__ int v_swizzle(int row) {
     return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
+// The stream with the place-th longest memory (up to 64 streams). A launch of
+// several rounds of workgroups takes the long ones first, so that none
+// begins as the last ones end.
+__device__ __forceinline__ int longest_first(const SplitArgs &a, int place, int lane) {
+    int n = -1;
+    if (lane < a.batch) {
+        const int mem = a.index ? a.index[lane] : lane;
+        n = mem >= 0 && mem < a.memories ? min(max(a.k_len[mem], 0), a.nk_max) : 0;
+    }
+    int rank = 0;
+    for (int j = 0; j < a.batch; ++j) {
+        const int other = __builtin_amdgcn_readlane(n, j);
+        rank += other > n || (other == n && j < lane);
+    }
+    return __ffsll(__ballot(lane < a.batch && rank == place)) - 1;
+}
+
 // D: widths up to D; CB: 32-column blocks a wavefront; FULL: both widths are
 // D (else steps past a width are skipped by branches, which keep the
 // compiler from interleaving the products with the softmax).
@@ -93,7 +110,9 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
     const XcdPlace x = xcd_place(a.batch * a.c.kv_heads, col_tiles * a.splits);  // a (stream, key head) on one XCD
     if (!x.ok) return;
     const int ct = x.within / a.splits, sp = x.within - ct * a.splits;
-    const int b = x.unit / a.c.kv_heads, h = x.unit - b * a.c.kv_heads;
+    int b = x.unit / a.c.kv_heads;
+    const int h = x.unit - b * a.c.kv_heads;
+    if (a.by_length) b = longest_first(a, b, lane);
     const int group = a.heads / a.c.kv_heads;
     const int mem = a.index ? a.index[b] : b;
     if (mem < 0 || mem >= a.memories) return;
@@ -340,8 +359,11 @@ int column_blocks(const SplitArgs &a, int cus) {
 
 int cross_workgroup_columns(const SplitArgs &a, int cus) { return kXWaves * 32 * column_blocks(a, cus); }
 
-hipError_t launch_cross_attend(const SplitArgs &a, int cus, hipStream_t s) {
+hipError_t launch_cross_attend(const SplitArgs &args, int cus, hipStream_t s) {
+    SplitArgs a = args;
     const int cols = a.t * (a.heads / a.c.kv_heads), cb = column_blocks(a, cus);
+    const long long tiles = (cols + kXWaves * 32 * cb - 1) / (kXWaves * 32 * cb);
+    a.by_length = a.k_len && a.batch <= 64 && tiles * a.batch * a.c.kv_heads > 2LL * cus;
     // queries readable in 16-byte pieces, outputs writable in 8-byte ones
     int aligned = 0;
     if (((reinterpret_cast<uintptr_t>(a.q) | (a.q_stream * 2) | (a.q_row * 2)) & 15) == 0) aligned |= 1;

@@ -97,6 +97,16 @@ def test_ragged_shared_and_empty(name, t):
 
 
 @pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("B", [64, 65])
+def test_many_workgroups_of_unequal_memories(name, B):
+    # more workgroups than one round: streams of long memories first (to 64 streams), equal lengths among them
+    lens = [int(x) for x in np.random.default_rng(B).integers(0, 120, 20)]
+    lens[3] = lens[7] = lens[11] = 119
+    index = [(7 * b) % 22 - 1 for b in range(B)]  # one past either end too
+    run(B, name, B, 150, 20, 120, 8, 4, 64, 64, [150 - b for b in range(B)], lens, index, sample=3)
+
+
+@pytest.mark.parametrize("name", FLOATS)
 def test_memories_fewer_than_streams_without_an_index(name):
     run(5, name, 3, 4, 2, 20, 2, 1, 32, 32)
 
