@@ -2329,12 +2329,17 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
 static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     a.group = a.heads / a.c.kv_heads;
     const long long cols = static_cast<long long>(a.t) * a.group;
+    const int cus = device_info().cus;
     // 16-bit memories take the matrix form from two columns on (64 streams of
     // 1500 frames, 8 heads of 128 over 2: 26.9 us against 33.2 at 4 columns,
     // 27.6 against 35.2 at 16; of one column 82 against 89 at best, 47 against
-    // 39 at worst).
-    const bool many = !a.spans && a.type != ND_F32 && cols > 1;
-    const int cus = device_info().cus;
+    // 39 at worst). float32 ones, whose matrix instruction has the rate of the
+    // split form's, once its blocks of 32 columns give three in two CUs one (16 x
+    // 448 rows, 8 heads of 64: 230 us against 342; 4 x 448 of 8 over 2, 448 blocks:
+    // 73 against 93; 1 x 448, 112 blocks: 34 against 28; 16 x 32, a block a
+    // list: 71 against 31).
+    const bool many = !a.spans && (a.type != ND_F32 ? cols > 1
+                                                    : cols > 64 && (cols + 31) / 32 * a.batch * a.c.kv_heads >= 3LL * cus / 2);
     const int wg_cols = many ? cross_workgroup_columns(a, cus) : split_tile_columns(a);
     const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((cols + wg_cols - 1) / wg_cols);
     if (many) {

@@ -317,6 +317,183 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
     }
 }
 
+// The same in float32, for many rows: 32 columns a wavefront on
+// v_mfma_f32_32x32x2_f32. S = K q^T contracts a 16-byte piece of each half's
+// coordinates in four instructions (element e of the halves' pieces in the
+// e-th); O = V^T P takes S's register i as it lies (the half f's key is 8 (i /
+// 4) + 4 f + i % 4) against one value of that key a lane. Tiles of 64 keys (32
+// past heads of 64) through LDS as above; the weights stay float32. The value
+// reads of the two halves, four rows apart, meet in no bank: rows with bit 2
+// set keep their 128-byte halves exchanged.
+template <int D, bool FULL>
+__global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f32_kernel(SplitArgs a, int col_tiles) {
+    constexpr int kKeys = D == 64 ? 64 : 32;   // keys a tile
+    constexpr int kPieces = D / 4;             // 16-byte pieces of a row
+    constexpr int kLoads = kKeys * D / 1024;   // wavefront loads of a tile's keys (values) a wavefront
+    constexpr int kLoadRows = 256 / D;         // rows of a wavefront load
+    constexpr int kBytes = kKeys * D * 4;
+    extern __shared__ __align__(16) unsigned char smem[];  // [2][keys, values]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, half = lane >> 5;
+    const XcdPlace x = xcd_place(a.batch * a.c.kv_heads, col_tiles * a.splits);
+    if (!x.ok) return;
+    const int ct = x.within / a.splits, sp = x.within - ct * a.splits;
+    int b = x.unit / a.c.kv_heads;
+    const int h = x.unit - b * a.c.kv_heads;
+    if (a.by_length) b = longest_first(a, b, lane);
+    const int group = a.group;
+    const int mem = a.index ? a.index[b] : b;
+    if (mem < 0 || mem >= a.memories) return;
+    const int nk = a.k_len ? min(max(a.k_len[mem], 0), a.nk_max) : a.nk_max;
+    const int cols = (a.q_len ? min(max(a.q_len[b], 0), a.t) : a.t) * group;
+    constexpr int kWgCols = kXWaves * 32;
+    if (ct * kWgCols >= cols) return;
+    const int col0 = ct * kWgCols + wave * 32;
+    const bool live = col0 < cols;
+    const int per = ((nk + kKeys - 1) / kKeys + a.splits - 1) / a.splits * kKeys;
+    const int j0 = min(sp * per, nk), j1 = min(j0 + per, nk);
+
+    const unsigned char *kp = a.c.k + static_cast<long long>(mem) * a.k_mem + static_cast<long long>(h) * a.k_head;
+    const unsigned char *vp = a.c.v + static_cast<long long>(mem) * a.v_mem + static_cast<long long>(h) * a.v_head;
+    const int lrow = wave * kLoads * kLoadRows + lane / kPieces, lc = lane % kPieces;
+    auto load_tile = [&](int j, int buf) {
+        lds_bytes *base = (lds_bytes *)smem + buf * 2 * kBytes + wave * kLoads * 1024;
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            const int row = lrow + k * kLoadRows, src = min(j + row, nk - 1);
+            const int ck = (lc ^ (row & 15)) * 16, cv = (lc ^ (((row >> 2) & 1) << 3)) * 16;
+            if (FULL || ck < 4 * a.c.qk)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(kp + src * a.k_row + ck),
+                    (__attribute__((address_space(3))) void *)(base + k * 1024), 16, 0, 0);
+            if (FULL || cv < 4 * a.c.vd)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(vp + src * a.v_row + cv),
+                    (__attribute__((address_space(3))) void *)(base + kBytes + k * 1024), 16, 0, 0);
+        }
+    };
+    if (!FULL) {  // pieces past a row's width stay zero
+        for (int y = tid * 16; y < 4 * kBytes; y += 64 * kXWaves * 16)
+            *reinterpret_cast<uint4 *>(smem + y) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    if (j0 < j1) load_tile(j0, 0);
+
+    // The queries: lane (n, half) holds coordinates 8 s + 4 half + 0..3 of its column.
+    float q[D / 2];
+    {
+        const int col = min(col0 + n, cols - 1);
+        const float *qp = static_cast<const float *>(a.q) + static_cast<long long>(b) * a.q_stream +
+                          static_cast<long long>(col / group) * a.q_row +
+                          static_cast<long long>(h * group + col % group) * a.c.qk;
+#pragma unroll
+        for (int s = 0; s < D / 8; ++s) {
+            const int d = 8 * s + 4 * half;
+            float4 y = make_float4(0, 0, 0, 0);
+            if (FULL || d < a.c.qk) {
+                if (a.q_vec)
+                    y = *reinterpret_cast<const float4 *>(qp + d);
+                else
+                    y = make_float4(qp[d], qp[d + 1], qp[d + 2], qp[d + 3]);
+            }
+            q[4 * s] = y.x * a.scale_log2;
+            q[4 * s + 1] = y.y * a.scale_log2;
+            q[4 * s + 2] = y.z * a.scale_log2;
+            q[4 * s + 3] = y.w * a.scale_log2;
+        }
+    }
+    f32x16 o[D / 32];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < D / 32; ++v)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[v][i] = 0.0f;
+
+    int buf = 0;
+    for (int j = j0; j < j1; j += kKeys, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // this tile is whole, and the other buffer's readers are done
+        if (j + kKeys < j1) load_tile(j + kKeys, buf ^ 1);
+        if (!live) continue;
+        const unsigned char *kt = smem + buf * 2 * kBytes, *vt = kt + kBytes;
+#pragma unroll
+        for (int kb = 0; kb < kKeys / 32; ++kb) {
+            if (j + 32 * kb >= j1) break;
+            f32x16 s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+            const unsigned char *kr = kt + (32 * kb + n) * D * 4;
+#pragma unroll
+            for (int p = 0; p < D / 8; ++p)
+                if (FULL || 8 * p < a.c.qk) {
+                    const float4 ka = *reinterpret_cast<const float4 *>(kr + ((2 * p + half) ^ (n & 15)) * 16);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.x, q[4 * p], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.y, q[4 * p + 1], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.z, q[4 * p + 2], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.w, q[4 * p + 3], s, 0, 0, 0);
+                }
+            if (j + 32 * kb + 32 > j1) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (j + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= j1) s[i] = -INFINITY;
+            }
+            float mt = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+            mt = halves_max(mt);
+            if (__any(mt > m + 8.0f)) {
+                const float mn = fmaxf(m, mt);
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v) o[v] *= f;
+            }
+            const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(s[i] - mu);
+                l += s[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v)
+                    if (FULL || 32 * v < a.c.vd) {
+                        const float va = *reinterpret_cast<const float *>(vt + row * D * 4 + (((32 * v + n) * 4) ^ (half << 7)));
+                        o[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(va, s[i], o[v], 0, 0, 0);
+                    }
+            }
+        }
+    }
+    if (!live) return;
+    const float sum = halves_sum(l);
+    const int col = col0 + n;
+    if (col >= cols) return;
+    const int head = h * group + col % group, row = col / group;
+    const long long pi = ((static_cast<long long>(b) * a.t + row) * a.heads + head) * a.splits + sp;
+    float *dst = a.part ? a.part + pi * a.c.vd
+                        : static_cast<float *>(a.out) + static_cast<long long>(b) * a.out_stream +
+                              static_cast<long long>(row) * a.out_row + static_cast<long long>(head) * a.c.vd;
+    const float f = a.part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int v = 0; v < D / 32; ++v)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * v + 8 * g + 4 * half;
+            if (FULL || d < a.c.vd) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[d + e] = o[v][4 * g + e] * f;
+            }
+        }
+    if (a.part && half == 0) {
+        a.part_ml[2 * pi] = m;
+        a.part_ml[2 * pi + 1] = sum;
+    }
+}
+
 template <int TYPE, int D, int CB, bool FULL>
 hipError_t launch_cross_full(const SplitArgs &a, int cols, int aligned, hipStream_t s) {
     constexpr int lds = 2 * 2 * kXTile * D * 2;
@@ -352,7 +529,25 @@ hipError_t launch_cross_type(const SplitArgs &a, int cols, int cb, int aligned, 
 // of a second wavefront a SIMD.
 int column_blocks(const SplitArgs &a, int cus) {
     const long long cols = static_cast<long long>(a.t) * (a.heads / a.c.kv_heads), wide = kXWaves * 64;
-    return std::max(a.c.qk, a.c.vd) <= 64 && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= cus ? 2 : 1;
+    return a.type != 0 && std::max(a.c.qk, a.c.vd) <= 64 && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= cus ? 2 : 1;
+}
+
+template <int D, bool FULL>
+hipError_t launch_cross_f32_full(const SplitArgs &a, int cols, hipStream_t s) {
+    constexpr int lds = 2 * 2 * (D == 64 ? 64 : 32) * D * 4;
+    static std::atomic<unsigned long long> attr{0};
+    if (lds > 64 * 1024)
+        if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(&cross_attend_f32_kernel<D, FULL>), lds, attr)) return e;
+    const int col_tiles = (cols + kXWaves * 32 - 1) / (kXWaves * 32);
+    const long long grid = xcd_grid(static_cast<long long>(a.batch) * a.c.kv_heads, static_cast<long long>(col_tiles) * a.splits);
+    hipLaunchKernelGGL((cross_attend_f32_kernel<D, FULL>), dim3(static_cast<unsigned>(grid)), dim3(64 * kXWaves), lds, s, a,
+                       col_tiles);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_cross_f32(const SplitArgs &a, int cols, hipStream_t s) {
+    return a.c.qk == D && a.c.vd == D ? launch_cross_f32_full<D, true>(a, cols, s) : launch_cross_f32_full<D, false>(a, cols, s);
 }
 
 }  // namespace
@@ -368,7 +563,12 @@ hipError_t launch_cross_attend(const SplitArgs &args, int cus, hipStream_t s) {
     int aligned = 0;
     if (((reinterpret_cast<uintptr_t>(a.q) | (a.q_stream * 2) | (a.q_row * 2)) & 15) == 0) aligned |= 1;
     if (((reinterpret_cast<uintptr_t>(a.out) | (a.out_stream * 2) | (a.out_row * 2)) & 7) == 0) aligned |= 2;
-    hipError_t e = a.type == 1 ? launch_cross_type<1>(a, cols, cb, aligned, s) : launch_cross_type<2>(a, cols, cb, aligned, s);
+    hipError_t e;
+    const int w = std::max(a.c.qk, a.c.vd);
+    if (a.type == 0)
+        e = w <= 64 ? launch_cross_f32<64>(a, cols, s) : w <= 128 ? launch_cross_f32<128>(a, cols, s) : launch_cross_f32<256>(a, cols, s);
+    else
+        e = a.type == 1 ? launch_cross_type<1>(a, cols, cb, aligned, s) : launch_cross_type<2>(a, cols, cb, aligned, s);
     if (e != hipSuccess || !a.part) return e;
     return launch_attend_join(a, s);
 }

@@ -97,6 +97,15 @@ def test_ragged_shared_and_empty(name, t):
 
 
 @pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("H,Hk,qk,vd,F", [(8, 4, 64, 64, 300), (8, 8, 48, 64, 130), (4, 4, 128, 128, 97),
+                                          (4, 4, 112, 80, 200), (4, 2, 256, 256, 65), (4, 2, 144, 240, 33)])
+def test_many_rows_of_many_streams(name, H, Hk, qk, vd, F):
+    # enough columns for the float32 matrix form at every width, full and narrower than it
+    run(H * qk, name, 40, 130, 40, F, H, Hk, qk, vd, [130 - (b % 7) * 20 for b in range(40)],
+        [F - (m % 5) * (F // 6) for m in range(40)], None, sample=3)
+
+
+@pytest.mark.parametrize("name", FLOATS)
 @pytest.mark.parametrize("B", [64, 65])
 def test_many_workgroups_of_unequal_memories(name, B):
     # more workgroups than one round: streams of long memories first (to 64 streams), equal lengths among them
