@@ -2291,6 +2291,12 @@ static int paged_args(const kv_paged *c, int batch, int rows, const char *what, 
     return CQ_OK;
 }
 
+// log2(e) / scale, the factor of the logits, or 0 where float32 has none.
+static float attention_scale(float scale) {
+    const float f = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
+    return scale > 0.0f && std::isfinite(scale) && std::isfinite(f) ? f : 0.0f;
+}
+
 static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_I8 ? 1 : 2; }
 
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
@@ -2368,7 +2374,7 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     const bool in_ws = a.acc_out && (a.splits > 1 || !split_weights_in_lds(a, a.waves));
     const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
     const long long wblocks = in_ws ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
-    if (lists * a.splits > grid_limit(1024) || (rows + 3) / 4 > grid_limit(256) || wblocks > grid_limit(256))
+    if (lists * a.splits > grid_limit(1024) || 2 * rows > grid_limit(64) || wblocks > grid_limit(256))
         return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", a.batch, a.t, a.heads);
     WsScope ws;
     a.part = a.part_ml = a.logits = nullptr;
@@ -2396,7 +2402,7 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: queries of type %d", type);
     if (heads <= 0 || heads % c->kv_heads != 0)
         return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, c->kv_heads);
-    if (!(std::isfinite(scale) && scale > 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (!attention_scale(scale)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
     if (acc_out && acc_cap < nk_max) return fail(CQ_ERR_MISUSE, "needle: %lld weights for %d keys", acc_cap, nk_max);
     if (heads / c->kv_heads > 1024) return fail(CQ_ERR_UNSUPPORTED, "needle: %d heads a KV head", heads / c->kv_heads);
     if (batch == 0) return CQ_OK;
@@ -2418,7 +2424,7 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     a.q_stream = q_stride ? q_stride : static_cast<long long>(heads) * c->qk;
     a.out_stream = out_stride ? out_stride : static_cast<long long>(heads) * c->vd;
     a.type = type;
-    a.scale_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
+    a.scale_log2 = attention_scale(scale);
     a.acc = acc;
     a.acc_out = acc_out;
     a.acc_cap = acc_cap;
@@ -2474,7 +2480,7 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
         return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, kv_heads);
     if (!split_widths_ok(qk, vd))
         return fail(CQ_ERR_UNSUPPORTED, "needle: cross-attention heads of %d and %d (multiples of 16 up to 256)", qk, vd);
-    if (!(std::isfinite(scale) && scale > 0.0f)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (!attention_scale(scale)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
     if (batch == 0 || t == 0) return CQ_OK;
     if (!out || !q || (memories > 0 && frames > 0 && (!k || !v)))
         return fail(CQ_ERR_MISUSE, "needle: cross-attention with a nil operand");
@@ -2530,7 +2536,7 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
     a.out_stream = y.out_stream;
     a.out_row = y.out_row;
     a.type = type;
-    a.scale_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(scale));
+    a.scale_log2 = attention_scale(scale);
     return run_split_attend(a, static_cast<hipStream_t>(stream));
 }
 
@@ -2539,6 +2545,7 @@ int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, cons
     if (rows < 0 || n <= 0 || top < 0 || top > n || stride < 0)
         return fail(CQ_ERR_MISUSE, "needle: %d log probabilities of %d rows of %d", top, rows, n);
     if (top > 64) return fail(CQ_ERR_UNSUPPORTED, "needle: %d alternatives (64 at most)", top);
+    if (n > 1 << 30) return fail(CQ_ERR_UNSUPPORTED, "needle: rows of %d logits", n);
     if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: logits of type %d", type);
     if (lp && !tokens) return fail(CQ_ERR_MISUSE, "needle: log probabilities without tokens");
     if (!top_idx != !top_lp) return fail(CQ_ERR_MISUSE, "needle: alternatives without their indices or values");

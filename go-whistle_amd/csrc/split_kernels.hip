@@ -702,39 +702,51 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
     finish<kCols, D>(a, p, jt);
 }
 
-// The parts of a list joined: one wavefront an output row (stream, query row, head).
-__global__ __launch_bounds__(256) void attend_join_kernel(SplitArgs a, long long rows) {
-    const int lane = threadIdx.x & 63;
-    const long long id = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (id >= rows) return;
-    const int head = static_cast<int>(id % a.heads);
-    const int i = static_cast<int>(id / a.heads % a.t), b = static_cast<int>(id / a.heads / a.t);
-    if (!key_list(a, b, a.index ? a.index[b] : b).ok || i >= q_rows(a, b)) return;
+// The parts of a list joined: a wavefront 128 values of an output row (stream,
+// query row, head), two a lane. The parts' statistics and values are asked
+// for before the row's spans or length say whether it is written: the three
+// are one wait.
+__global__ __launch_bounds__(64) void attend_join_kernel(SplitArgs a, int blocks) {
+    const int lane = threadIdx.x;
+    const int id = blockIdx.x / blocks, d = (blockIdx.x - id * blocks) * 128 + 2 * lane;
+    const int bi = id / a.heads, head = id - bi * a.heads;
+    const int b = bi / a.t, i = bi - b * a.t;
     // lane s has part s's maximum and sum; up to 64 parts
-    const float *ml = a.part_ml + 2 * id * a.splits;
+    const float *ml = a.part_ml + 2LL * id * a.splits;
     const float2 mine = lane < a.splits ? *reinterpret_cast<const float2 *>(ml + 2 * lane) : make_float2(-INFINITY, 0.0f);
+    const float *part = a.part + static_cast<long long>(id) * a.splits * a.c.vd + min(d, a.c.vd - 2);
+    constexpr int kAhead = 16;
+    float2 x[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) x[s] = *reinterpret_cast<const float2 *>(part + min(s, a.splits - 1) * a.c.vd);
+    if (!key_list(a, b, a.index ? a.index[b] : b).ok || i >= q_rows(a, b)) return;
     float m = mine.x;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, xor_lane(m, o));
     const float f = __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.0f : m));
     float l = mine.y * f;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    for (int o = 32; o > 0; o >>= 1) l += xor_lane(l, o);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float *part = a.part + id * a.splits * a.c.vd;
-    for (int d = lane; d - lane < a.c.vd; d += 64) {
-        float v = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) {
-            const float x = d < a.c.vd ? part[s * a.c.vd + d] : 0.0f;
-            v = fmaf(x, __shfl(f, s), v);
+    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+        if (s < a.splits) {
+            const float fs = __shfl(f, s);
+            v.x = fmaf(x[s].x, fs, v.x);
+            v.y = fmaf(x[s].y, fs, v.y);
         }
-        if (d < a.c.vd)
-            store_value(a.out, a.type,
-                        static_cast<long long>(b) * a.out_stream + static_cast<long long>(i) * a.out_row +
-                            static_cast<long long>(head) * a.c.vd + d,
-                        v * inv);
+    for (int s = kAhead; s < a.splits; ++s) {
+        const float2 y = *reinterpret_cast<const float2 *>(part + s * a.c.vd);
+        const float fs = __shfl(f, s);
+        v.x = fmaf(y.x, fs, v.x);
+        v.y = fmaf(y.y, fs, v.y);
     }
+    if (d >= a.c.vd) return;
+    const long long at = static_cast<long long>(b) * a.out_stream + static_cast<long long>(i) * a.out_row +
+                         static_cast<long long>(head) * a.c.vd + d;
+    store_value(a.out, a.type, at, v.x * inv);
+    store_value(a.out, a.type, at + 1, v.y * inv);
 }
 
 // acc_out = acc + the group's softmax weights from the logits in the
@@ -833,8 +845,9 @@ bool split_weights_in_lds(const SplitArgs &a, int waves) {
 }
 
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {
-    const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
-    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a, rows);
+    const int blocks = (a.c.vd + 127) / 128;
+    const long long grid = static_cast<long long>(a.batch) * a.t * a.heads * blocks;
+    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(grid)), dim3(64), 0, s, a, blocks);
     return hipGetLastError();
 }
 

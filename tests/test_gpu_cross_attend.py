@@ -141,15 +141,15 @@ def test_strides(name, t):
 
 
 @pytest.mark.parametrize("name", FLOATS)
-@pytest.mark.parametrize("t", [1, 80])
-def test_frames_behind_the_last_may_hold_anything(name, t):
+@pytest.mark.parametrize("t,B", [(1, 2), (80, 2), (80, 60)])
+def test_frames_behind_the_last_may_hold_anything(name, t, B):
     import torch
 
     g = gen(19)
     dt = getattr(torch, name)
-    B, F, H, Hk, D = 2, 150, 4, 2, 64
+    F, H, Hk, D = 150, 4, 2, 64
     q, k, v = (torch.randn(*s, generator=g, device="cuda").to(dt) for s in ((B, t, H, D), (B, F, Hk, D), (B, F, Hk, D)))
-    k_len = i32([101, 0])
+    k_len = i32([101, 0] + [150] * (B - 2))
     outs = []
     for fill in (0.0, float("nan"), float("inf")):
         k[0, 101:], v[0, 101:], k[1], v[1] = fill, fill, fill, fill
@@ -162,38 +162,40 @@ def test_frames_behind_the_last_may_hold_anything(name, t):
 
 
 @pytest.mark.parametrize("name", FLOATS)
-@pytest.mark.parametrize("t", [1, 80])
-def test_extreme_logits(name, t):
+@pytest.mark.parametrize("t,B", [(1, 1), (80, 1), (80, 200)])
+def test_extreme_logits(name, t, B):
     import torch
 
     dt = getattr(torch, name)
-    q = torch.zeros(1, t, 1, 64, device="cuda", dtype=dt)
+    q = torch.zeros(B, t, 1, 64, device="cuda", dtype=dt)
     q[..., 0] = 1
-    k = torch.zeros(1, 100, 1, 64, device="cuda", dtype=dt)
-    v = torch.randn(1, 100, 1, 64, generator=gen(3), device="cuda").to(dt)
-    out = torch.empty(1, t, 1, 64, device="cuda", dtype=dt)
+    k = torch.zeros(B, 100, 1, 64, device="cuda", dtype=dt)
+    v = torch.randn(B, 100, 1, 64, generator=gen(3), device="cuda").to(dt)
+    out = torch.empty(B, t, 1, 64, device="cuda", dtype=dt)
     k[..., 0] = -float("inf")
     needle.cross_attend_dev(out, q, k, v, 1.0)
     torch.cuda.synchronize()
     assert (out == 0).all()
     k[..., 0] = -30000
-    k[0, 57, 0, 0] = 30000
+    k[:, 57, 0, 0] = 30000
     needle.cross_attend_dev(out, q, k, v, 1.0)
     torch.cuda.synchronize()
     assert torch.equal(out, v[:, 57:58].expand_as(out))
-    k[0, 99, 0, 0] = float("nan")
+    k[:, 99, 0, 0] = float("nan")
     needle.cross_attend_dev(out, q, k, v, 1.0)
     torch.cuda.synchronize()
     assert torch.isnan(out).all()
 
 
+@pytest.mark.parametrize("name", ["float32", "bfloat16"])
 @pytest.mark.parametrize("t", [2, 200])
-def test_graph_replays(t):
+def test_graph_replays(name, t):
     import torch
 
     g = gen(23)
     B, F, H, D = 2, 700, 4, 64
-    q, k, v = (torch.randn(B, n, H, D, generator=g, device="cuda").bfloat16() for n in (t, F, F))
+    dt = getattr(torch, name)
+    q, k, v = (torch.randn(B, n, H, D, generator=g, device="cuda").to(dt) for n in (t, F, F))
     k_len = i32([F, 333])
     out, other = torch.empty_like(q), torch.empty_like(q)
     needle.cross_attend_dev(other, q, k, v, 8.0, k_len=k_len)
@@ -201,7 +203,7 @@ def test_graph_replays(t):
     with torch.cuda.graph(graph):
         needle.cross_attend_dev(out, q, k, v, 8.0, k_len=k_len)
     for r in range(3):
-        q.copy_(torch.randn(q.shape, generator=g, device="cuda").bfloat16())
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda").to(dt))
         out.zero_()
         graph.replay()
         needle.cross_attend_dev(other, q, k, v, 8.0, k_len=k_len)

@@ -65,7 +65,8 @@ def test_bad_caches(call, edit, err):
     (append, dict(cap=65)), (append, dict(acc=P, acc_cap=63)), (append, dict(k=P + 2)),
     (append, dict(typ=1, v=P + 1)),
     (attend, dict(batch=-1)), (attend, dict(nk=-1)), (attend, dict(nk=65)), (attend, dict(typ=3)),
-    (attend, dict(heads=3)), (attend, dict(heads=0)), (attend, dict(scale=0.0)), (attend, dict(scale=-1.0)), (cross, dict(scale=-1.0)), (attend, dict(scale=float("nan"))),
+    (attend, dict(heads=3)), (attend, dict(heads=0)), (attend, dict(scale=0.0)), (attend, dict(scale=-1.0)), (cross, dict(scale=-1.0)),
+    (attend, dict(scale=1e-40)), (cross, dict(scale=1e-40)), (attend, dict(scale=float("nan"))),
     (attend, dict(scale=float("inf"))), (attend, dict(out=None)), (attend, dict(q=None)), (attend, dict(spans=None)),
     (attend, dict(acc_out=P, acc_cap=63)), (attend, dict(q=P + 2)), (attend, dict(typ=2, out=P + 1)),
     (evict, dict(batch=-1)), (evict, dict(nk=-1)), (evict, dict(keep=-1)), (evict, dict(sink=-1)),
@@ -86,7 +87,7 @@ def test_misuse(call, kw):
 
 
 @pytest.mark.parametrize("call,kw", [
-    (cross, dict(qk=40)), (cross, dict(vd=264)), (logprobs, dict(top=65)),
+    (cross, dict(qk=40)), (cross, dict(vd=264)), (logprobs, dict(top=65)), (logprobs, dict(n=(1 << 30) + 1)),
     (attend, dict(heads=4096)), (append, dict(batch=1 << 20, t=64)),
 ])
 def test_unsupported(call, kw):
