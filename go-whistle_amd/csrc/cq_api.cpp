@@ -2346,7 +2346,8 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     // list: 71 against 31).
     const bool many = !a.spans && (a.type != ND_F32 ? cols > 1
                                                     : cols > 64 && (cols + 31) / 32 * a.batch * a.c.kv_heads >= 3LL * cus / 2);
-    const int wg_cols = many ? cross_workgroup_columns(a, cus) : split_tile_columns(a);
+    a.tile = split_tile_columns(a, cus);
+    const int wg_cols = many ? cross_workgroup_columns(a, cus) : a.tile;
     const long long lists = static_cast<long long>(a.batch) * a.c.kv_heads * ((cols + wg_cols - 1) / wg_cols);
     if (many) {
         // The matrix form's partials cost more than idle CUs as long as the

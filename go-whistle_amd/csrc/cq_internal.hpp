@@ -524,7 +524,7 @@ struct SplitArgs {
     int memories, nk_max, t, heads, batch;
     int group;                               // heads a key head
     int splits;                              // parts of a list, at most 64
-    int waves;                               // wavefronts of a workgroup (attend_split)
+    int tile, waves;                         // columns and wavefronts of a workgroup (attend_split)
     int by_length;                           // streams of long memories first (cross_attend)
     const void *q;
     void *out;
@@ -541,7 +541,7 @@ struct SplitArgs {
     long long acc_cap;
 };
 bool split_widths_ok(int qk, int vd);
-int split_tile_columns(const SplitArgs &a);              // columns a workgroup takes
+int split_tile_columns(const SplitArgs &a, int cus);     // columns a workgroup takes
 int split_max_waves(const SplitArgs &a);                 // wavefronts a workgroup may have
 bool split_weights_in_lds(const SplitArgs &a, int waves);  // a list's logits fit LDS
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);

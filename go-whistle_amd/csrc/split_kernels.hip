@@ -806,7 +806,7 @@ hipError_t launch_columns(const SplitArgs &a, hipStream_t s) {
 template <int TYPE, int D>
 hipError_t launch_split(const SplitArgs &a, hipStream_t s) {
     static std::atomic<unsigned long long> one{0}, two{0};
-    const int tile = split_tile_columns(a);
+    const int tile = a.tile;
     if (tile == 1)
         return launch_with(&attend_lanes_kernel<TYPE, D, 1>, a, 1, joint_lds<1, D>(a, a.waves), one, s);
     if (tile == 2)
@@ -828,9 +828,18 @@ hipError_t launch_split_width(const SplitArgs &a, hipStream_t s) {
 
 bool split_widths_ok(int qk, int vd) { return qk > 0 && vd > 0 && qk % 16 == 0 && vd % 16 == 0 && qk <= 256 && vd <= 256; }
 
-int split_tile_columns(const SplitArgs &a) {
-    const int cols = a.t * (a.heads / a.c.kv_heads);
-    return cols <= 2 ? cols : kCols;
+int split_tile_columns(const SplitArgs &a, int cus) {
+    const long long cols = static_cast<long long>(a.t) * a.group;
+    if (cols <= 2) return static_cast<int>(cols);
+    // Two columns a workgroup on the vector units while every pair gets a CU,
+    // for narrow heads of 16-bit and int8 caches: the keys are read again from
+    // the L2, and a list's products leave one CU's matrix units (one stream of
+    // 200 int8 keys, 8 heads of 48 over 2: 6.9 us against 7.8; of 448 float16
+    // keys, 8 heads over 1: 9.2 against 11.0; float32 9.7 against 9.5, heads of
+    // 128 up to half as long again).
+    const bool narrow = std::max(a.c.qk, a.c.vd) <= 64 && a.c.type != 0;
+    // The weights of a list are summed over its heads by the workgroup that has them all.
+    return narrow && !a.acc_out && (cols + 1) / 2 * a.batch * a.c.kv_heads <= cus ? 2 : kCols;
 }
 
 int split_max_waves(const SplitArgs &a) {
@@ -840,8 +849,8 @@ int split_max_waves(const SplitArgs &a) {
 
 bool split_weights_in_lds(const SplitArgs &a, int waves) {
     const int w = std::max(a.c.qk, a.c.vd), d = w <= 64 ? 64 : w <= 128 ? 128 : 256, group = a.heads / a.c.kv_heads;
-    const size_t joint = sizeof(float) * (waves * 2 + 2 + waves * (d + 4)) * split_tile_columns(a);
-    return a.t == 1 && group <= kCols && joint + sizeof(float) * group * static_cast<size_t>(a.nk_max) <= kMostLds / 2;
+    const size_t joint = sizeof(float) * (waves * 2 + 2 + waves * (d + 4)) * a.tile;
+    return a.t == 1 && group <= a.tile && joint + sizeof(float) * group * static_cast<size_t>(a.nk_max) <= kMostLds / 2;
 }
 
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {

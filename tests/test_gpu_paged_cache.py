@@ -181,6 +181,13 @@ def test_attend_types_and_heads(name, io, H, Hk, qk, vd):
     run_attend(H + qk, name, io, 4, H, Hk, qk, vd, 16, nk, [[0, 0, 0, nk], [0, 0, 0, 0], [0, 3, 40, 70], [2, 3, 3, 4]], True)
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("B,H,Hk", [(1, 6, 2), (1, 10, 2), (2, 16, 1), (90, 3, 1), (140, 4, 1), (300, 4, 1)])
+def test_attend_groups_without_weights(name, B, H, Hk):
+    # odd groups, and as many streams as take two columns a workgroup, or sixteen
+    run_attend(B + H, name, "float32", B, H, Hk, 48, 64, 16, 70, [[0, b % 5, 5, 5 + (7 * b) % 66] for b in range(B)], False)
+
+
 @pytest.mark.parametrize("nk", [1, 2, 15, 16, 17, 31, 32, 33, 64, 65, 127, 128, 129, 257, 1500])
 @pytest.mark.parametrize("name", ["float32", "bfloat16", "i8"])
 def test_attend_lengths(nk, name):
