@@ -831,15 +831,16 @@ bool split_widths_ok(int qk, int vd) { return qk > 0 && vd > 0 && qk % 16 == 0 &
 int split_tile_columns(const SplitArgs &a, int cus) {
     const long long cols = static_cast<long long>(a.t) * a.group;
     if (cols <= 2) return static_cast<int>(cols);
-    // Two columns a workgroup on the vector units while every pair gets a CU,
-    // for narrow heads of 16-bit and int8 caches: the keys are read again from
-    // the L2, and a list's products leave one CU's matrix units (one stream of
-    // 200 int8 keys, 8 heads of 48 over 2: 6.9 us against 7.8; of 448 float16
-    // keys, 8 heads over 1: 9.2 against 11.0; float32 9.7 against 9.5, heads of
-    // 128 up to half as long again).
+    // Two columns a workgroup on the vector units for little work, 512 keys a CU
+    // over the pairs of columns, of narrow heads of 16-bit and int8 caches: the
+    // keys are read again from the L2, but a list's products leave one CU's
+    // matrix units (one stream of 200 int8 keys, 8 heads of 48 over 2: 6.9 us
+    // against 7.8; 32 of 448: 8.6 against 9.8; of 4000: 26.7 against 20.7;
+    // float32 9.7 against 9.5, heads of 128 up to half as long again).
     const bool narrow = std::max(a.c.qk, a.c.vd) <= 64 && a.c.type != 0;
+    const long long pairs = (cols + 1) / 2 * a.batch * a.c.kv_heads;
     // The weights of a list are summed over its heads by the workgroup that has them all.
-    return narrow && !a.acc_out && (cols + 1) / 2 * a.batch * a.c.kv_heads <= cus ? 2 : kCols;
+    return narrow && !a.acc_out && pairs * a.nk_max <= 512LL * cus ? 2 : kCols;
 }
 
 int split_max_waves(const SplitArgs &a) {
