@@ -121,6 +121,38 @@ def test_memories_fewer_than_streams_without_an_index(name):
 
 
 @pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("t", [1, 5, 90])
+def test_no_frames_no_memories_and_the_dense_layout(name, t):
+    import torch
+
+    from go_whistle_amd._lib import check as ok
+    from go_whistle_amd._lib import lib
+
+    g = gen(29)
+    dt = getattr(torch, name)
+    B, F, H, Hk, D = 3, 40, 4, 2, 64
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dt)  # noqa: E731
+    q = mk(B, t, H, D)
+    out = torch.full_like(q, 5.0)
+    needle.cross_attend_dev(out, q, mk(B, 0, Hk, D), mk(B, 0, Hk, D), 8.0)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    out.fill_(5.0)
+    needle.cross_attend_dev(out, q, mk(0, F, Hk, D), mk(0, F, Hk, D), 8.0, index=i32([0, 0, 0]))
+    torch.cuda.synchronize()
+    assert (out == 5).all()
+    needle.cross_attend_dev(out[:0], q[:0], mk(2, F, Hk, D), mk(2, F, Hk, D), 8.0)
+    needle.cross_attend_dev(out[:, :0], q[:, :0], mk(3, F, Hk, D), mk(3, F, Hk, D), 8.0)
+    k, v, want = mk(B, F, Hk, D), mk(B, F, Hk, D), torch.empty_like(q)
+    needle.cross_attend_dev(want, q, k, v, 8.0)
+    ok(lib().nd_cross_attend_dev(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                 FLOATS.index(name), None, B, t, H, Hk, D, D, B, F, None, None, None, 8.0,
+                                 torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("name", FLOATS)
 @pytest.mark.parametrize("t", [1, 100])
 def test_strides(name, t):
     # head-major memories, queries and outputs inside wider rows

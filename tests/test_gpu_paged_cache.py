@@ -422,6 +422,127 @@ def test_evict_choices(weights, nk, keep, sink, recent, R):
     run_evict(nk, "float16", 5, 2, 16, 32, R, nk, keep, sink, recent, [nk, nk + 1, -1, nk // 2, max(0, nk - 1)], weights)
 
 
+def test_evict_of_forked_streams_and_bad_pages():
+    # two streams that share their source pages are cut apart; a source page outside the pool reads page 0, a
+    # destination page outside it is skipped
+    import torch
+
+    g = gen(51)
+    R, nk, keep, Hk, D = 8, 40, 16, 2, 32
+    k, v, ks, vs = make_pool(g, 16, R, Hk, D, D, "i8")
+    pages = i32([[1, 2, 3, 4, 5], [1, 2, 3, 4, 5], [6, -1, 99, 7, 8]])
+    dst = i32([[9, 10], [11, 12], [13, 16]])
+    acc = torch.rand(3, Hk, nk, generator=g, device="cuda")
+    acc_out = torch.zeros(3, Hk, keep, device="cuda")
+    kept = torch.zeros(3, Hk, keep, dtype=torch.int32, device="cuda")
+    n = i32([40, 33, 40])
+    before = [x.clone() for x in (k, v, ks, vs)]
+    needle.PagedKV(k, v, pages, ks, vs).evict_dev(dst, acc, acc_out, n, n, kept, nk, sink=1, recent=2)
+    torch.cuda.synchronize()
+    assert n.tolist() == [16, 16, 16]
+    want = [x.clone() for x in before]
+    for b, length in enumerate((40, 33, 40)):
+        for h in range(Hk):
+            rows = keep_rows(acc[b, h].cpu().numpy(), length, keep, 1, 2)
+            assert kept[b, h].tolist() == rows.tolist()
+            for i, j in enumerate(rows):
+                sp, dp = int(pages[b, j // R]), int(dst[b, i // R])
+                sp = sp if 0 <= sp < 16 else 0
+                if 0 <= dp < 16:
+                    for x, w in zip(before, want):
+                        w[dp, i % R, h] = x[sp, j % R, h]
+    for x, w in zip((k, v, ks, vs), want):
+        assert torch.equal(x, w)
+
+
+def test_c_strides_of_queries_and_outputs():
+    # rows of wider arrays through the C entry, at an odd element
+    import torch
+
+    from go_whistle_amd._lib import check as ok
+    from go_whistle_amd._lib import lib
+
+    g = gen(61)
+    B, H, Hk, D, R, nk = 3, 4, 2, 64, 16, 50
+    for dt, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        k, v, _, _ = make_pool(g, B * 4, R, Hk, D, D, "float16")
+        c = needle.PagedKV(k, v, tables(g, B, 4, B * 4))
+        wide = torch.randn(B, H * D + 9, generator=g, device="cuda").to(dt)
+        out = torch.full((B, H * D + 3), 2.0, device="cuda", dtype=dt)
+        spans = i32([[0, 0, 0, nk], [0, 7, 20, 31], [0, 0, 0, 0]])
+        ok(lib().kv_attend_paged_dev(c._ref, out.data_ptr() + dt.itemsize, H * D + 3, wide.data_ptr() + 5 * dt.itemsize,
+                                     H * D + 9, code, B, H, spans.data_ptr(), nk, 8.0, None, None, 0,
+                                     torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        q, o = wide[:, 5:5 + H * D].reshape(B, H, D), out[:, 1:1 + H * D].reshape(B, H, D)
+        check_attend(k, v, None, None, c.pages, q, spans, nk, 8.0, o, None, None, o, None, R)
+        assert (out[:, 0] == 2).all() and (out[:, 1 + H * D:] == 2).all()
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_no_keys_and_no_streams(name):
+    import torch
+
+    g = gen(71)
+    k, v, ks, vs = make_pool(g, 2, 4, 1, 16, 32, name)
+    q, out = torch.randn(2, 3, 16, device="cuda"), torch.full((2, 3, 32), 4.0, device="cuda")
+    none = needle.PagedKV(k, v, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), ks, vs)
+    acc = torch.zeros(2, 1, 0, device="cuda")
+    none.attend_dev(out, q, torch.zeros(2, 4, dtype=torch.int32, device="cuda"), 0, 4.0, acc_out=acc)
+    none.append_dev(torch.zeros(2, 1, 1, 16, device="cuda"), torch.zeros(2, 1, 1, 32, device="cuda"), i32([0, 0]))
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    empty = needle.PagedKV(k, v, torch.zeros(0, 1, dtype=torch.int32, device="cuda"), ks, vs)
+    e = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    i = lambda *s: e(*s, t=torch.int32)  # noqa: E731
+    empty.attend_dev(e(0, 3, 32), e(0, 3, 16), i(0, 4), 4, 4.0)
+    empty.append_dev(e(0, 1, 1, 16), e(0, 1, 1, 32), i(0))
+    empty.evict_dev(i(0, 1), e(0, 1, 4), e(0, 1, 2), i(0), i(0), i(0, 1, 2), 4)
+
+
+def test_two_graphs_replayed_on_two_streams():
+    # each graph's partials in its own workspace, with eager calls of the same size beside them
+    import torch
+
+    g = gen(81)
+    nk, R, Hk, D = 5000, 16, 1, 64
+    per = -(-nk // R)
+    k, v, _, _ = make_pool(g, per, R, Hk, D, D, "bfloat16")
+    c = needle.PagedKV(k, v, tables(g, 1, per, per))
+    qs = [torch.randn(1, 6, D, generator=g, device="cuda") for _ in range(3)]
+    spans = i32([[0, 0, 0, nk]])
+    acc = torch.rand(1, Hk, nk, generator=g, device="cuda")
+
+    def outs():
+        return torch.zeros(1, 6, D, device="cuda"), torch.zeros(1, Hk, nk, device="cuda")
+
+    want = []
+    for q in qs:
+        o, a = outs()
+        c.attend_dev(o, q, spans, nk, 8.0, acc=acc, acc_out=a)
+        torch.cuda.synchronize()
+        want.append((o, a))
+    got, graphs = [outs() for _ in range(3)], []
+    for z in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.attend_dev(got[z][0], qs[z], spans, nk, 8.0, acc=acc, acc_out=got[z][1])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for r in range(4):
+        for o, a in got:
+            o.zero_(), a.zero_()
+        torch.cuda.synchronize()
+        for z in range(2):
+            with torch.cuda.stream(streams[z]):
+                graphs[z].replay()
+        with torch.cuda.stream(streams[2]):
+            c.attend_dev(got[2][0], qs[2], spans, nk, 8.0, acc=acc, acc_out=got[2][1])
+        torch.cuda.synchronize()
+        for z in range(3):
+            assert torch.equal(got[z][0], want[z][0]) and torch.equal(got[z][1], want[z][1]), (r, z)
+
+
 # ---- a run of them together ----------------------------------------------------------
 
 
