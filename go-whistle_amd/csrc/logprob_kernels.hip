@@ -27,6 +27,12 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int i) {
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
 
+// The logit of a key (a NaN as -inf, -0 as 0).
+__device__ __forceinline__ float key_value(unsigned long long k) {
+    const uint32_t u = static_cast<uint32_t>(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
+
 __device__ __forceinline__ float logit_at(const void *x, int type, long long i) {
     if (type == 0) return static_cast<const float *>(x)[i];
     const uint16_t h = static_cast<const uint16_t *>(x)[i];
@@ -46,12 +52,21 @@ __device__ __forceinline__ float entropy(const RowStats &s) {
     return logf(s.l) - s.t / s.l;
 }
 
-__device__ __forceinline__ void write_row(const LogprobArgs &a, int r, const RowStats &s) {
-    const int tok = a.tokens ? a.tokens[r] : -1;
-    if (a.lp)
-        a.lp[r] = tok < 0 ? 0.0f
-                  : tok >= a.n ? NAN
-                               : log_prob(s, logit_at(a.x, a.type, static_cast<long long>(r) * a.stride + tok));
+// A row's token and its logit, asked for before the row's statistics are known.
+struct Given {
+    int tok;
+    float x;
+};
+__device__ __forceinline__ Given given_of(const LogprobArgs &a, int r) {
+    Given g{-1, 0.0f};
+    if (a.lp) {
+        g.tok = a.tokens[r];
+        if (g.tok >= 0 && g.tok < a.n) g.x = logit_at(a.x, a.type, static_cast<long long>(r) * a.stride + g.tok);
+    }
+    return g;
+}
+__device__ __forceinline__ void write_row(const LogprobArgs &a, int r, const RowStats &s, const Given &g) {
+    if (a.lp) a.lp[r] = g.tok < 0 ? 0.0f : g.tok >= a.n ? NAN : log_prob(s, g.x);
     if (a.ent) a.ent[r] = entropy(s);
 }
 
@@ -100,7 +115,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     // value e of piece k: place kPer (tid + k kLpThreads) + e - shift of the part
     auto place = [&](int k) { return kPer * (tid + k * kLpThreads) - shift; };
 
-    if (tid == 0) listed = 0;
+    Given given{-1, 0.0f};
+    if (tid == 0) {
+        listed = 0;
+        if (a.splits == 1) given = given_of(a, r);
+    }
     float v[kLpVals];
     float m = -INFINITY, most[kLpPieces];
 #pragma unroll
@@ -183,7 +202,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     float *pt = a.part + (static_cast<long long>(r) * a.splits + part) * (4 + 2 * a.top);
     if (tid == 0) {
         if (a.splits == 1) {
-            write_row(a, r, st);
+            write_row(a, r, st, given);
         } else {
             pt[0] = m;
             pt[1] = l;
@@ -194,11 +213,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     auto answer = [&](int q, unsigned long long best) {
         const int i = i0 + key_index(best);
         if (a.splits > 1) {
-            pt[4 + 2 * q] = best ? logit_at(a.x, TYPE, base - i0 + i) : -INFINITY;
+            pt[4 + 2 * q] = key_value(best);
             pt[5 + 2 * q] = __int_as_float(best ? i : -1);
         } else {
             a.top_idx[static_cast<long long>(r) * a.top + q] = i;
-            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, TYPE, base + i));
+            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, key_value(best));
         }
     };
     if (a.top == 0) return;
@@ -246,6 +265,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
     const int r = blockIdx.x, lane = threadIdx.x;
     const int rec = 4 + 2 * a.top;
     const float *pt = a.part + static_cast<long long>(r) * a.splits * rec;
+    const Given given = given_of(a, r);
     float m = -INFINITY;
     for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, pt[static_cast<long long>(s) * rec]);
 #pragma unroll
@@ -268,7 +288,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
         t += __shfl_xor(t, o);
     }
     const RowStats st{m, l, t};
-    if (lane == 0) write_row(a, r, st);
+    if (lane == 0) write_row(a, r, st, given);
     // each part's alternatives are in order: a lane walks the parts s = lane, lane + 64, ...
     unsigned long long last = ~0ull;
     for (int q = 0; q < a.top; ++q) {
@@ -294,7 +314,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
         if (lane == 0) {
             const int i = key_index(best);
             a.top_idx[static_cast<long long>(r) * a.top + q] = i;
-            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, logit_at(a.x, a.type, static_cast<long long>(r) * a.stride + i));
+            a.top_lp[static_cast<long long>(r) * a.top + q] = log_prob(st, key_value(best));
         }
     }
 }
