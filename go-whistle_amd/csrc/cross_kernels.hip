@@ -17,8 +17,10 @@
 // The weights are rounded to the memories' type for the second product (half
 // an ulp of it, the size of the outputs' own rounding); logits, weights
 // before that, their sums and the outputs are float32. The running maximum m
-// is raised only when a column's logits pass it by 2^8: weights stay below
-// 2^8, which float16 holds, and most tiles leave the outputs unscaled.
+// is raised only when a column's logits pass it by 2^8, so most tiles leave
+// the outputs unscaled. float16 weights are 2^(logit - m + 7): up to 2^15,
+// which it holds, and none above 2^-32 of the largest is lost (without the
+// seven, 20,000 frames of weights of 2.9e-8 were).
 //
 // Bank conflicts: row r of a tile keeps its 16-byte pieces in the order c ^
 // f(r): f chosen so that sixteen lanes reading one piece of sixteen key rows,
@@ -41,6 +43,8 @@ using lds_bytes = __attribute__((address_space(3))) unsigned char;
 
 constexpr int kXWaves = 4;
 constexpr int kXTile = 64;
+template <int TYPE>
+constexpr float kLift = TYPE == 1 ? 7.0f : 0.0f;  // log2 of the largest weight, before the lag of the maximum
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c) {
@@ -145,6 +149,15 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
                     (__attribute__((address_space(3))) void *)(base + kBytes + k * 1024), 16, 0, 0);
         }
     };
+    // Values behind the last key: 0, not the last row's, whose infinities times
+    // a weight of 0 are none. A wavefront clears what it loaded.
+    auto clear_tail = [&](int j, int buf) {
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+            if (j + lrow + k * kLoadRows >= j1)
+                *reinterpret_cast<uint4 *>(smem + buf * 2 * kBytes + kBytes + (wave * kLoads + k) * 1024 + lane * 16) =
+                    make_uint4(0, 0, 0, 0);
+    };
     if (!FULL) {  // pieces past a row's width stay zero
         for (int x = tid * 16; x < 4 * kBytes; x += 64 * kXWaves * 16)
             *reinterpret_cast<uint4 *>(smem + x) = make_uint4(0, 0, 0, 0);
@@ -195,6 +208,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
     int buf = 0;
     for (int j = j0; j < j1; j += kXTile, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (j + kXTile > j1) clear_tail(j, buf);
         __syncthreads();  // this tile is whole, and the other buffer's readers are done
         if (j + kXTile < j1) load_tile(j + kXTile, buf ^ 1);
         if (!live) continue;
@@ -244,7 +258,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
                 for (int v = 0; v < D / 32; ++v)
                     if (FULL || 32 * v < a.c.vd) o[cb][v] *= f;
             }
-            const float mu = m[cb] == -INFINITY ? 0.0f : m[cb];
+            const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<TYPE>;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
                             make_float4(o[cb][v][4 * g], o[cb][v][4 * g + 1], o[cb][v][4 * g + 2], o[cb][v][4 * g + 3]);
                 }
             if (half == 0) {
-                a.part_ml[2 * pi] = m[cb];
+                a.part_ml[2 * pi] = m[cb] - kLift<TYPE>;
                 a.part_ml[2 * pi + 1] = sum;
             }
         } else {
@@ -373,6 +387,15 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
                     (__attribute__((address_space(3))) void *)(base + kBytes + k * 1024), 16, 0, 0);
         }
     };
+    // Values behind the last key: 0, not the last row's, whose infinities times
+    // a weight of 0 are none. A wavefront clears what it loaded.
+    auto clear_tail = [&](int j, int buf) {
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+            if (j + lrow + k * kLoadRows >= j1)
+                *reinterpret_cast<uint4 *>(smem + buf * 2 * kBytes + kBytes + (wave * kLoads + k) * 1024 + lane * 16) =
+                    make_uint4(0, 0, 0, 0);
+    };
     if (!FULL) {  // pieces past a row's width stay zero
         for (int y = tid * 16; y < 4 * kBytes; y += 64 * kXWaves * 16)
             *reinterpret_cast<uint4 *>(smem + y) = make_uint4(0, 0, 0, 0);
@@ -413,6 +436,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
     int buf = 0;
     for (int j = j0; j < j1; j += kKeys, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (j + kKeys > j1) clear_tail(j, buf);
         __syncthreads();  // this tile is whole, and the other buffer's readers are done
         if (j + kKeys < j1) load_tile(j + kKeys, buf ^ 1);
         if (!live) continue;

@@ -5,7 +5,7 @@
 // Per (stream, key head) the query columns are the heads of the group times
 // the query rows. o = sum_j w_j v_j with w = softmax(q.k_j / scale), one pass
 // over the keys with a running maximum m and sum l (in log2 units, p_j =
-// 2^(l_j - m)): a wavefront takes tiles of 16 to 64 keys, the wavefronts of a
+// 2^(l_j - m)): a wavefront takes tiles of 16 or 32 keys, the wavefronts of a
 // workgroup share a part of the list and are joined in LDS; the parts of a
 // list, where there are few lists and many keys, by a second launch. All
 // arithmetic is float32, whatever the types.
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
     constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
     constexpr int kPer = 16 / kSize;         // elements of a piece
     constexpr int kPieces = D / (4 * kPer);  // pieces of a row a lane reads
-    constexpr int kSub = D * kSize <= 64 ? 2 : D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
+    constexpr int kSub = D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
     constexpr int kTile = 16 * kSub;
     extern __shared__ __align__(16) float smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -410,6 +410,15 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
 #pragma unroll
             for (int s = 0; s < kSub; ++s) vsc[s] = TYPE == 3 ? vs[s] : 1.0f;
             if (more) load_rows(kw, kp, a.k_row, a.c.qk);
+            // past the last key values of 0, not that key's: a weight of 0 times an infinity
+            if (TYPE != 3 && j + kTile > p.j1) {
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+                    if (j + 16 * s + r >= p.j1) {
+#pragma unroll
+                        for (int k = 0; k < kPieces; ++k) vw[s][k][0] = vw[s][k][1] = vw[s][k][2] = vw[s][k][3] = 0;
+                    }
+            }
             float w[COLS][kSub];
 #pragma unroll
             for (int n = 0; n < COLS; ++n) {
@@ -438,7 +447,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
                 for (int s = 0; s < kSub; ++s) {
                     const float pw = __builtin_amdgcn_exp2f(x[n][s] - mu);
                     l[n] += pw;
-                    w[n][s] = pw * vsc[s];
+                    w[n][s] = TYPE == 3 && j + 16 * s + r >= p.j1 ? 0.0f : pw * vsc[s];
                 }
             }
 #pragma unroll
@@ -645,6 +654,17 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                         }
             }
             if (jn < p.j1) load_keys(kw, rows);
+            // past the last key values of 0, not that key's: a weight of 0 times an infinity
+            if (TYPE != 3 && j + kTile > p.j1) {
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (j + 16 * s + 4 * c + i >= p.j1) {
+#pragma unroll
+                            for (int k = 0; k < kVWords; ++k) vw[s][i][k] = 0;
+                        }
+            }
 
             float mt = m;
 #pragma unroll
@@ -680,7 +700,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                 for (int i = 0; i < 4; ++i) {
                     float w = __builtin_amdgcn_exp2f(sc[s][i] - mu);
                     l += w;
-                    if constexpr (TYPE == 3) w *= vsc[s][i];
+                    if constexpr (TYPE == 3) w = j + 16 * s + 4 * c + i >= p.j1 ? 0.0f : w * vsc[s][i];
 #pragma unroll
                     for (int e = 0; e < kVals; ++e)
                         o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(vw[s][i], e), w, o[e], 0, 0, 0);

@@ -241,3 +241,53 @@ def test_graph_replays(name, t):
         needle.cross_attend_dev(other, q, k, v, 8.0, k_len=k_len)
         torch.cuda.synchronize()
         assert torch.equal(out, other), r
+
+
+@pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("B,t,F", [(1, 1, 5), (2, 1, 300), (2, 3, 77), (2, 40, 33), (2, 80, 150), (60, 80, 150), (1, 90, 65)])
+@pytest.mark.parametrize("D,W", [(64, 64), (48, 64), (128, 80), (256, 256)])
+def test_an_infinite_value_of_the_last_frame(name, B, t, F, D, W):
+    # the last frame's weight is above 0, so its coordinate is the infinity; the others are as without it
+    import torch
+
+    g = gen(31)
+    dt = getattr(torch, name)
+    q, k, v = (torch.randn(*s, generator=g, device="cuda").to(dt) for s in ((B, t, 4, D), (B, F, 2, D), (B, F, 2, W)))
+    outs = []
+    for x in (1.0, float("inf")):
+        v[:, F - 1, :, 7] = x
+        outs.append(torch.empty(B, t, 4, W, device="cuda", dtype=dt))
+        needle.cross_attend_dev(outs[-1], q, k, v, math.sqrt(D))
+    torch.cuda.synchronize()
+    assert (outs[1][..., 7] == float("inf")).all()
+    for o in outs:
+        o[..., 7] = 0
+    assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("B,t", [(1, 2), (16, 400)])
+def test_many_small_weights_beside_a_large_one(name, B, t):
+    # 20,000 frames of weight e^-17.375 = 2.85e-8, below half of float16's
+    # least subnormal, beside one of 1: 5.7e-4 of the sum. The bound of
+    # serve_ref, and where weights are rounded to float16, whose subnormals'
+    # half step 2^-25 is 2^-32 of a largest weight of 2^7, that much of every
+    # |v| = 1: 4.7e-6.
+    import torch
+
+    dt = getattr(torch, name)
+    F = 20001
+    q = torch.ones(B, t, 8, 64, device="cuda", dtype=dt)
+    k = torch.full((1, F, 8, 64), -17.375 / 64, device="cuda", dtype=dt)  # 17.375 / 64 = 139 / 512
+    v = torch.ones(1, F, 8, 64, device="cuda", dtype=dt)
+    k[:, 0] = 0
+    v[:, 0] = 0
+    out = torch.empty_like(q)
+    needle.cross_attend_dev(out, q, k, v, 1.0, index=i32([0] * B))
+    torch.cuda.synchronize()
+    kq, vq = host(k)[0, :, 0], host(v)[0, :, 0]
+    o, bound, _, _ = attend64(host(q)[0, 0, 0], kq, vq, 1.0, dt, None if name == "float32" else dt)
+    err = np.abs(host(out).astype(np.float64) - o)
+    if name == "float16":
+        bound = bound + F * 2.0 ** -32
+    assert (err <= bound).all(), (err / bound).max()

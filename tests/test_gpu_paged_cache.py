@@ -618,3 +618,29 @@ def test_decode_with_a_bounded_cache(name):
             before[b, :, lens[b]] = 0  # the append's
         check_attend(k, v, ks, vs, dst, qq[i], sp, cap, scale, s_out, before, acc2, s_out, before, R)
     assert half_ulp(torch.float32) == 2.0 ** -24
+
+
+@pytest.mark.parametrize("name", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("B,H,Hk", [(1, 2, 2), (2, 16, 1), (140, 4, 1), (3, 3, 1)])
+@pytest.mark.parametrize("nk", [1, 13, 47, 300])
+def test_attend_an_infinite_value_of_the_last_key(name, B, H, Hk, nk):
+    # its weight is above 0, so its coordinate is the infinity; the others are as without it
+    import torch
+
+    g = gen(nk)
+    R, per = 16, -(-nk // 16)
+    for qk, vd in ((48, 64), (128, 128), (256, 144)):
+        k, v, ks, vs = make_pool(g, B * per, R, Hk, qk, vd, name)
+        pages = torch.arange(B * per, device="cuda", dtype=torch.int32).view(B, per)
+        q = torch.randn(B, H, qk, generator=g, device="cuda")
+        spans = i32([[0, nk, nk, nk]] * B)
+        outs = []
+        for x in (1.0, float("inf")):
+            v.view(B, per * R, Hk, vd)[:, nk - 1, :, 5] = x
+            outs.append(torch.empty(B, H, vd, device="cuda"))
+            needle.PagedKV(k, v, pages).attend_dev(outs[-1], q, spans, nk, math.sqrt(qk))
+        torch.cuda.synchronize()
+        assert (outs[1][..., 5] == float("inf")).all()
+        for o in outs:
+            o[..., 5] = 0
+        assert torch.equal(outs[0], outs[1])
