@@ -2297,6 +2297,12 @@ static float attention_scale(float scale) {
     return scale > 0.0f && std::isfinite(scale) && std::isfinite(f) ? f : 0.0f;
 }
 
+// Whether two arrays of floats share memory.
+static bool floats_overlap(const float *x, long long nx, const float *y, long long ny) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return x && y && a < b + static_cast<uintptr_t>(ny) * 4 && b < a + static_cast<uintptr_t>(nx) * 4;
+}
+
 static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_I8 ? 1 : 2; }
 
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
@@ -2410,6 +2416,9 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     if (!out || !q || !spans) return fail(CQ_ERR_MISUSE, "needle: attention with a nil operand");
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % value_size(type))
         return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
+    if (acc != acc_out && floats_overlap(acc, static_cast<long long>(batch) * c->kv_heads * acc_cap, acc_out,
+                                         static_cast<long long>(batch) * c->kv_heads * acc_cap))
+        return fail(CQ_ERR_MISUSE, "needle: attention weights onto a part of themselves");
     const int size = value_size(c->type);
     a.k_head = static_cast<long long>(c->qk) * size;
     a.v_head = static_cast<long long>(c->vd) * size;
@@ -2447,7 +2456,10 @@ int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stri
     if (batch == 0) return CQ_OK;
     if (!len || !len_out || (nk_max > 0 && !acc) || (keep > 0 && (!dst_pages || !acc_out || !kept)))
         return fail(CQ_ERR_MISUSE, "needle: eviction with a nil operand");
-    if (acc_out && acc_out == acc) return fail(CQ_ERR_MISUSE, "needle: eviction onto its own weights");
+    const long long lists = static_cast<long long>(batch) * c->kv_heads;
+    if (floats_overlap(acc, lists * acc_cap, acc_out, lists * acc_out_cap))
+        return fail(CQ_ERR_MISUSE, "needle: eviction onto its own weights");
+    if (keep > 0 && dst_pages == c->pages) return fail(CQ_ERR_MISUSE, "needle: eviction onto its own pages");
     const int pieces = (c->qk + c->vd) * value_size(c->type) / 16;
     if (static_cast<long long>(batch) * c->kv_heads > grid_limit(1024) ||
         static_cast<double>(batch) * keep * c->kv_heads * pieces > static_cast<double>(grid_limit(256)) * 256)
@@ -2501,6 +2513,8 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
         y.k_stream = y.k_row * frames;
         y.v_stream = y.v_row * frames;
     }
+    if ((batch > 1 && y.out_stream == 0) || (t > 1 && y.out_row == 0))
+        return fail(CQ_ERR_MISUSE, "needle: cross-attention outputs of one place");
     if (((y.k_stream | y.k_row | y.k_head | y.v_stream | y.v_row | y.v_head) * size |
          static_cast<long long>(reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v))) & 15)
         return fail(CQ_ERR_MISUSE, "needle: cross-attention memories that are not aligned to 16 bytes");

@@ -333,7 +333,8 @@ class PagedKV:
         """Each stream's first length[b] (<= nk_max) rows cut to keep =
         kept.shape[2] a key head: the first `sink`, the last `recent`, and the
         others of the largest acc, in order, written to the rows of dst_pages
-        [streams, pages] of the same pool, which no source row is read from.
+        [streams, pages] of the same pool, pages that no source row is read
+        from.
         kept [streams, kv_heads, keep] int32 gets their numbers, acc_out
         [streams, kv_heads, >= keep] their weights, length_out[b] their count."""
         import torch

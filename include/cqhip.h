@@ -521,7 +521,8 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * acc_out non-null ([batch][kv_heads][acc_cap], acc_cap >= nk_max): for
  * each row j of the spans, acc_out[j] = acc[j] (null: 0) + the sum over the
  * key head's query heads of their softmax weights; other entries are left
- * as they were. acc_out may be acc. */
+ * as they were. acc_out may be acc; otherwise the two share no memory, and
+ * out and q share none. */
 int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, const void *q, long long q_stride,
                         int type, int batch, int heads, const int32_t *spans, int nk_max, float scale,
                         const float *acc, float *acc_out, long long acc_cap, void *stream);
@@ -532,13 +533,13 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
  * weights the lowest row; a NaN weight counts as the least. The kept rows
  * are written in their order to the front of the cache that dst_pages
  * ([batch][dst_stride] of the same pool, dst_stride * page_rows >= keep)
- * names, whose pages are none that any stream's rows are read from. The
- * source pages are only read, so streams that share them after a fork may be
- * evicted apart. kept ([batch][kv_heads][keep]) gets the kept rows'
+ * names, whose pages are none that any stream's rows are read from (so not
+ * c->pages). The source pages are only read, so streams that share them after a
+ * fork may be evicted apart. kept ([batch][kv_heads][keep]) gets the kept rows'
  * numbers, -1 past the last; acc_out ([batch][kv_heads][acc_out_cap],
- * acc_out_cap >= keep, not acc) their weights; len_out[b] = min(len[b],
- * keep) (len_out may be len). A stream whose len is outside [0, nk_max] is
- * left as it was, len_out too. sink + recent <= keep. */
+ * acc_out_cap >= keep, apart from acc) their weights; len_out[b] = min(len[b],
+ * keep) (len_out may be len). A stream whose len is outside [0, nk_max] is left
+ * as it was, len_out too. sink + recent <= keep. */
 int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
                        long long acc_cap, float *acc_out, long long acc_out_cap, const int32_t *len, int32_t *len_out,
                        int32_t *kept, int batch, int nk_max, int keep, int sink, int recent, void *stream);

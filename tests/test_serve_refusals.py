@@ -122,3 +122,15 @@ def test_wrappers_refuse_host_tensors_and_shapes():
     with pytest.raises(CQPanic):
         needle.cross_attend_dev(q, q[0], q, q, 8.0)
     assert _lib.SIGNATURES["kv_attend_paged_dev"]
+
+
+@pytest.mark.parametrize("call,kw", [
+    (evict, dict(c=cache(pages=3 * P), dst=3 * P)),  # onto the pages that are read
+    (evict, dict(out=P + 1020)), (evict, dict(acc=P + 1020, out=P)),  # weights in part onto themselves
+    (attend, dict(acc=P, acc_out=P + 4, acc_cap=64)), (attend, dict(acc=P + 4, acc_out=P, acc_cap=64)),
+    (cross, dict(layout=CrossLayout(768, 256, 0, 256, 1280, 128, 64, 1280, 128, 64))),  # outputs of one place
+    (cross, dict(layout=CrossLayout(768, 256, 768, 0, 1280, 128, 64, 1280, 128, 64))),
+])
+def test_outputs_that_would_race(call, kw):
+    with pytest.raises(CQPanic, match="onto|one place"):
+        call(**kw)
