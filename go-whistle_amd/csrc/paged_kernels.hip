@@ -136,6 +136,7 @@ hipError_t launch_append_type(const PagedAppendArgs &a, int vec, hipStream_t s) 
 // ---- eviction -------------------------------------------------------------------
 
 constexpr int kSelThreads = 1024;  // at most
+constexpr long long kCopyPieces = 1 << 12;  // a list's pieces of 16 bytes that one workgroup copies
 
 // A weight's place in the order of weights: larger is kept sooner. Held rows
 // (the first sink, the last recent) come before every weight; -0 is 0; a NaN
@@ -154,6 +155,61 @@ __device__ __forceinline__ int wave_sum(int c) {
     return add_lane<32>(add_lane<16>(add_lane<8>(add_lane<4>(add_lane<2>(add_lane<1>(c))))));
 }
 
+using words4 = uint32_t __attribute__((ext_vector_type(4)));
+
+// Where a kept row j of stream b, key head h is, and where row i of its new
+// cache; false where that is in no page. Bad source pages read page 0.
+__device__ __forceinline__ bool kept_place(const EvictArgs &a, int b, int h, int i, int j, long long &from, long long &to) {
+    const int mask = (1 << a.c.shift) - 1;
+    int sp = j >= 0 ? a.c.pages[static_cast<long long>(b) * a.c.page_stride + (j >> a.c.shift)] : 0;
+    const int dp = j >= 0 ? a.dst_pages[static_cast<long long>(b) * a.dst_stride + (i >> a.c.shift)] : -1;
+    if (sp < 0 || sp >= a.c.pool_pages) sp = 0;
+    from = ((static_cast<long long>(sp) << a.c.shift) + (j & mask)) * a.c.kv_heads + h;
+    to = ((static_cast<long long>(dp) << a.c.shift) + (i & mask)) * a.c.kv_heads + h;
+    return dp >= 0 && dp < a.c.pool_pages;
+}
+
+// The copies of one list by the workgroup that chose its rows, kept[i] in
+// LDS: four 16-byte pieces of a key row and a value row a thread at a time.
+__device__ __forceinline__ void copy_kept(const EvictArgs &a, int b, int h, const int *kept, int count, int kpieces,
+                                          int vpieces) {
+    constexpr int kAhead = 4;
+    const int pieces = max(kpieces, vpieces), total = count * pieces, threads = blockDim.x;
+    for (int x0 = threadIdx.x; x0 < total; x0 += kAhead * threads) {
+        words4 kx[kAhead], vx[kAhead];
+        float ksc[kAhead], vsc[kAhead];
+        long long from[kAhead], to[kAhead];
+        int p[kAhead];
+        bool ok[kAhead];
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+            const int x = x0 + z * threads, i = min(x, total - 1) / pieces;
+            p[z] = x - i * pieces;
+            ok[z] = kept_place(a, b, h, i, kept[i], from[z], to[z]) && x < total;
+        }
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z)
+            if (ok[z]) {
+                if (p[z] < kpieces) kx[z] = reinterpret_cast<const words4 *>(a.c.k)[from[z] * kpieces + p[z]];
+                if (p[z] < vpieces) vx[z] = reinterpret_cast<const words4 *>(a.c.v)[from[z] * vpieces + p[z]];
+                if (a.c.type == 3 && p[z] == 0) {
+                    ksc[z] = a.c.ks[from[z]];
+                    vsc[z] = a.c.vs[from[z]];
+                }
+            }
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z)
+            if (ok[z]) {
+                if (p[z] < kpieces) __builtin_nontemporal_store(kx[z], reinterpret_cast<words4 *>(a.c.k) + to[z] * kpieces + p[z]);
+                if (p[z] < vpieces) __builtin_nontemporal_store(vx[z], reinterpret_cast<words4 *>(a.c.v) + to[z] * vpieces + p[z]);
+                if (a.c.type == 3 && p[z] == 0) {
+                    a.c.ks[to[z]] = ksc[z];
+                    a.c.vs[to[z]] = vsc[z];
+                }
+            }
+    }
+}
+
 // The kept rows of one (stream, key head). Row k of a thread is row
 // (wavefront * per + k) * 64 + lane, its key in a register (V = 0: read
 // each time, for lists past 32,768). The keep-th largest key is built from its
@@ -162,14 +218,18 @@ __device__ __forceinline__ int wave_sum(int c) {
 // have: 30 us for 448 rows), until exactly `keep` do.
 // Then one pass in row order writes the rows above the key, and the lowest of
 // those equal to it. Integer counts throughout: the same rows in every run.
-template <int V>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+// COPY: the workgroup also copies them, and a stream's first one writes its
+// new length (which then is not where the others read the old one).
+template <int V, bool COPY>
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, int kpieces, int vpieces) {
+    extern __shared__ int kept_sh[];  // COPY: the kept rows
     __shared__ int count_sh[32][3];  // a turn's counts over the wavefronts
     __shared__ int wave_sh[2][kSelThreads / 64];
     const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6, lane = tid & 63;
     const int h = blockIdx.x % a.c.kv_heads, b = blockIdx.x / a.c.kv_heads;
     const int n = a.len[b];
     if (n < 0 || n > a.nk_max) return;
+    if (COPY && h == 0 && tid == 0) a.len_out[b] = min(n, a.keep);
     const long long bh = static_cast<long long>(b) * a.c.kv_heads + h;
     const float *w = a.acc + bh * a.acc_cap;
     int32_t *kept = a.kept + bh * a.keep;
@@ -179,6 +239,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
         for (int i = tid; i < n; i += threads) {
             kept[i] = i;
             out[i] = w[i];
+            if (COPY) kept_sh[i] = i;
+        }
+        if (COPY) {
+            __syncthreads();
+            copy_kept(a, b, h, kept_sh, n, kpieces, vpieces);
         }
         return;
     }
@@ -281,10 +346,15 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
         if (up_k || (eq_k && e < need)) {
             const int at = base + __popcll(up & below) + min(e, need);
             kept[at] = row0 + 64 * k;
+            if (COPY) kept_sh[at] = row0 + 64 * k;
             out[at] = weight_of(k);
         }
         base += __popcll(up);
         eq_base += __popcll(eq);
+    }
+    if (COPY) {
+        __syncthreads();
+        copy_kept(a, b, h, kept_sh, a.keep, kpieces, vpieces);
     }
 }
 
@@ -311,9 +381,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a, int kpiece
     const int b = static_cast<int>(bi / half_rows), i0 = static_cast<int>(bi - static_cast<long long>(b) * half_rows);
     const int n = a.len[b];  // or already its new value: in [0, nk_max] both or neither
     if (n < 0 || n > a.nk_max) return;
-    const int mask = (1 << a.c.shift) - 1;
     const int32_t *kept = a.kept + (static_cast<long long>(b) * a.c.kv_heads + h) * a.keep;
-    using words4 = uint32_t __attribute__((ext_vector_type(4)));
     words4 kx[2], vx[2];
     float ksc[2], vsc[2];
     long long to[2];
@@ -322,12 +390,8 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a, int kpiece
     for (int z = 0; z < 2; ++z) {
         const int i = i0 + z * half_rows;
         const int j = i < a.keep ? kept[i] : -1;
-        int sp = j >= 0 ? a.c.pages[static_cast<long long>(b) * a.c.page_stride + (j >> a.c.shift)] : 0;
-        const int dp = j >= 0 ? a.dst_pages[static_cast<long long>(b) * a.dst_stride + (i >> a.c.shift)] : -1;
-        if (sp < 0 || sp >= a.c.pool_pages) sp = 0;
-        ok[z] = dp >= 0 && dp < a.c.pool_pages;
-        const long long from = ((static_cast<long long>(sp) << a.c.shift) + (j & mask)) * a.c.kv_heads + h;
-        to[z] = ((static_cast<long long>(dp) << a.c.shift) + (i & mask)) * a.c.kv_heads + h;
+        long long from;
+        ok[z] = kept_place(a, b, h, i, j, from, to[z]);
         if (ok[z]) {
             if (p < kpieces) kx[z] = reinterpret_cast<const words4 *>(a.c.k)[from * kpieces + p];
             if (p < vpieces) vx[z] = reinterpret_cast<const words4 *>(a.c.v)[from * vpieces + p];
@@ -365,20 +429,33 @@ hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s) {
 }
 
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
-    // a wavefront for each 512 rows, eight rows a thread (32 past 16 wavefronts)
-    const int per = 512;
-    const int threads = std::min(kSelThreads, 64 * std::max(1, (a.nk_max + per - 1) / per));
-    const dim3 grid(static_cast<unsigned>(a.batch) * a.c.kv_heads), block(threads);
-    if (a.nk_max <= 8 * kSelThreads)
-        hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, s, a);
-    else if (a.nk_max <= 32 * kSelThreads)
-        hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
     const int size = a.c.type == 0 ? 4 : a.c.type == 3 ? 1 : 2;
     const int kpieces = a.c.qk * size / 16, vpieces = a.c.vd * size / 16, half_rows = (a.keep + 1) / 2;
+    const dim3 grid(static_cast<unsigned>(a.batch) * a.c.kv_heads);
+    const bool apart = a.len_out + a.batch <= a.len || a.len + a.batch <= a.len_out;
+    // One launch for small lists, a row a thread, unless the new lengths lie
+    // over the old ones, which every workgroup of a stream reads (448 rows to
+    // 256 of heads of 48 and 64 float16 values, 3584 pieces: 8 streams of 2 heads
+    // 11.0 -> 10.1 us; 64 of 8 heads of 64, 4096 pieces: 20.3 -> 15.4; 1000 rows,
+    // 8192 pieces: 13.0 -> 12.4; of 2000, 8000 pieces: 13.3 -> 14.6, 32,000: 12.4
+    // -> 21.3).
+    if (apart && a.nk_max <= kSelThreads && static_cast<long long>(a.keep) * (kpieces + vpieces) <= kCopyPieces) {
+        const dim3 block(64 * std::max(1, (a.nk_max + 63) / 64));
+        hipLaunchKernelGGL((evict_select_kernel<1, true>), grid, block, sizeof(int) * std::min(a.keep, a.nk_max), s, a, kpieces,
+                           vpieces);
+        return hipGetLastError();
+    }
+    // a wavefront for each 512 rows, eight rows a thread (32 past 16 wavefronts)
+    const int per = 512;
+    const dim3 block(std::min(kSelThreads, 64 * std::max(1, (a.nk_max + per - 1) / per)));
+    if (a.nk_max <= 8 * kSelThreads)
+        hipLaunchKernelGGL((evict_select_kernel<8, false>), grid, block, 0, s, a, 0, 0);
+    else if (a.nk_max <= 32 * kSelThreads)
+        hipLaunchKernelGGL((evict_select_kernel<32, false>), grid, block, 0, s, a, 0, 0);
+    else
+        hipLaunchKernelGGL((evict_select_kernel<0, false>), grid, block, 0, s, a, 0, 0);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     const long long total = static_cast<long long>(a.batch) * half_rows * a.c.kv_heads * std::max(kpieces, vpieces);
     const long long blocks = (std::max<long long>(total, a.batch) + 255) / 256;
     hipLaunchKernelGGL(evict_copy_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, kpieces, vpieces,

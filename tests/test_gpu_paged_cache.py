@@ -644,3 +644,35 @@ def test_attend_an_infinite_value_of_the_last_key(name, B, H, Hk, nk):
         for o in outs:
             o[..., 5] = 0
         assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("nk,keep", [(1, 3), (64, 70), (63, 1), (65, 64), (1023, 100), (1024, 102), (1024, 103), (447, 0)])
+def test_evict_small_lists_in_one_launch(name, nk, keep):
+    # heads of 64 and 96: float32 rows of 40 pieces, 102 of them at most in one launch
+    sink = min(2, keep)
+    run_evict(nk, name, 3, 2, 64, 96, 16, nk, keep, sink, min(7, keep - sink), [nk, nk // 2, nk + 1], random_weights)
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_evict_over_the_old_lengths_is_the_same(name):
+    import torch
+
+    g = gen(61)
+    B, Hk, D, R, nk, keep = 33, 3, 64, 16, 200, 60
+    k, v, ks, vs = make_pool(g, B * 17, R, Hk, D, D, name)
+    perm = torch.randperm(B * 17, generator=g, device="cuda").int()
+    pages, dst = perm[:B * 13].view(B, 13).contiguous(), perm[B * 13:].view(B, 4).contiguous()
+    acc = random_weights(g, (B, Hk, nk))
+    lens = torch.randint(-1, nk + 2, (B,), generator=g, device="cuda").int()
+    got = []
+    for over in (False, True):
+        pools = [x.clone() if x is not None else None for x in (k, v, ks, vs)]
+        n = lens.clone()
+        n_out = n if over else lens.clone()
+        kept, out = torch.full((B, Hk, keep), 5, dtype=torch.int32, device="cuda"), torch.zeros(B, Hk, keep, device="cuda")
+        c = needle.PagedKV(pools[0], pools[1], pages, pools[2], pools[3])
+        c.evict_dev(dst, acc, out, n, n_out, kept, nk, sink=1, recent=5)
+        torch.cuda.synchronize()
+        got.append([x for x in (*pools, n_out, kept, out) if x is not None])
+    assert all(torch.equal(x, y) for x, y in zip(*got))
