@@ -2568,11 +2568,10 @@ int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, cons
     if (!logits) return fail(CQ_ERR_MISUSE, "needle: log probabilities with a nil operand");
     if (reinterpret_cast<uintptr_t>(logits) % value_size(type))
         return fail(CQ_ERR_MISUSE, "needle: logits that are not aligned to their type");
-    LogprobArgs a{lp, ent, top_lp, top_idx, logits, stride, type, rows, n, top_idx ? top : 0, tokens, 1, n, nullptr};
-    const int most = logprob_chunk(
-        ((reinterpret_cast<uintptr_t>(logits) | static_cast<uintptr_t>(rows > 1 ? stride : 0) * value_size(type)) & 15) == 0);
-    a.splits = (n + most - 1) / most;
-    a.chunk = ((n + a.splits - 1) / a.splits + 7) / 8 * 8;
+    LogprobArgs a{lp, ent, top_lp, top_idx, logits, stride, type, rows, n, top_idx ? top : 0, tokens, 1, n, 0, nullptr};
+    const bool aligned =
+        ((reinterpret_cast<uintptr_t>(logits) | static_cast<uintptr_t>(rows > 1 ? stride : 0) * value_size(type)) & 15) == 0;
+    logprob_parts(a, aligned);
     if (static_cast<long long>(rows) * a.splits > grid_limit(512))
         return fail(CQ_ERR_UNSUPPORTED, "needle: log probabilities of %d rows of %d", rows, n);
     WsScope ws;

@@ -561,11 +561,11 @@ struct LogprobArgs {
     long long stride;
     int type, rows, n, top;
     const int32_t *tokens;
-    int splits, chunk;
+    int splits, chunk, waves;
     float *part;
 };
-// The logits a part may have, where every row starts on a 16-byte boundary or not.
-int logprob_chunk(bool aligned);
+// Sets splits, chunk and waves; aligned: every row starts on a 16-byte boundary.
+void logprob_parts(LogprobArgs &a, bool aligned);
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s);
 
 }  // namespace cqhip

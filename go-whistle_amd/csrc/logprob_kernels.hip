@@ -14,9 +14,6 @@
 namespace cqhip {
 namespace {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kLpVals = 32;  // logits a thread holds
 
 // A logit's place in the order of alternatives: the larger value, then the
 // lower index; a NaN as -inf, -0 as 0. 0 is below every logit.
@@ -86,7 +83,7 @@ __device__ __forceinline__ float sort_lanes(float x) {
     return x;
 }
 
-// A thread's values are pieces of 16 bytes of the row, kLpThreads pieces
+// A thread's values are pieces of 16 bytes of the row, kThreads pieces
 // apart: piece g covers the part's values kPer g - shift and on, shift the
 // distance of the part's first value from the 16-byte boundary before it.
 // Pieces across an end of the part are read value by value.
@@ -99,11 +96,12 @@ __device__ __forceinline__ float sort_lanes(float x) {
 // reading the part again: its values' registers are not held for that.
 constexpr int kLpList = 512;
 
-template <int TYPE>
-__global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
+template <int TYPE, int WAVES, int VALS>
+__global__ __launch_bounds__(64 * WAVES) void logprob_kernel(LogprobArgs a) {
+    constexpr int kThreads = 64 * WAVES;
     constexpr int kPer = TYPE == 0 ? 4 : 8;
-    constexpr int kLpPieces = kLpVals / kPer;
-    __shared__ float red[4][kLpWaves];
+    constexpr int kLpPieces = VALS / kPer;
+    __shared__ float red[4][WAVES];
     __shared__ unsigned long long list[kLpList];
     __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -112,15 +110,15 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     const long long base = static_cast<long long>(r) * a.stride + i0;
     const uintptr_t first = reinterpret_cast<uintptr_t>(a.x) + static_cast<uintptr_t>(base) * (16 / kPer);
     const int shift = static_cast<int>(first & 15) / (16 / kPer);
-    // value e of piece k: place kPer (tid + k kLpThreads) + e - shift of the part
-    auto place = [&](int k) { return kPer * (tid + k * kLpThreads) - shift; };
+    // value e of piece k: place kPer (tid + k kThreads) + e - shift of the part
+    auto place = [&](int k) { return kPer * (tid + k * kThreads) - shift; };
 
     Given given{-1, 0.0f};
     if (tid == 0) {
         listed = 0;
         if (a.splits == 1) given = given_of(a, r);
     }
-    float v[kLpVals];
+    float v[VALS];
     float m = -INFINITY, most[kLpPieces];
 #pragma unroll
     for (int k = 0; k < kLpPieces; ++k) {
@@ -164,11 +162,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     if (lane == 0) red[0][wave] = m, red[3][wave] = bound;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) m = fmaxf(m, red[0][w]), bound = fmaxf(bound, red[3][w]);
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[0][w]), bound = fmaxf(bound, red[3][w]);
     const float mu = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, t = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kLpVals; ++k) {
+    for (int k = 0; k < VALS; ++k) {
         const float d = v[k] - mu;
         const float e = __expf(d);
         l += e;                                // a NaN among the logits is one here
@@ -197,7 +195,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     __syncthreads();
     l = t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) l += red[1][w], t += red[2][w];
+    for (int w = 0; w < WAVES; ++w) l += red[1][w], t += red[2][w];
     const RowStats st{m, l, t};
     float *pt = a.part + (static_cast<long long>(r) * a.splits + part) * (4 + 2 * a.top);
     if (tid == 0) {
@@ -223,14 +221,13 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     if (a.top == 0) return;
     const int n = listed;
     if (n <= kLpList) {
-        if (tid < n) {
-            const unsigned long long mine = list[tid];
+        for (int x = tid; x < n; x += kThreads) {
+            const unsigned long long mine = list[x];
             int rank = 0;
             for (int j = 0; j < n; ++j) rank += list[j] > mine;
             if (rank < a.top) answer(rank, mine);
-        } else if (tid < a.top) {
-            answer(tid, 0);
         }
+        for (int x = n + tid; x < a.top; x += kThreads) answer(x, 0);
         return;
     }
     // one after the other: every thread offers its largest below the last one chosen
@@ -238,7 +235,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
     for (int q = 0; q < a.top; ++q) {
         if (q == 0 || mine == last) {
             mine = 0;
-            for (int i = tid; i < count; i += kLpThreads) {
+            for (int i = tid; i < count; i += kThreads) {
                 const unsigned long long key = rank_key(logit_at(a.x, TYPE, base + i), i);
                 if (key < last && key > mine) mine = key;
             }
@@ -253,7 +250,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a) {
         if (lane == 0) list[wave] = best;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kLpWaves; ++w)
+        for (int w = 0; w < WAVES; ++w)
             if (list[w] > best) best = list[w];
         last = best;
         if (tid == 0) answer(q, best);
@@ -319,18 +316,52 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LogprobArgs a) {
     }
 }
 
+template <int WAVES, int VALS = 32>
+hipError_t launch_rows(const LogprobArgs &a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(static_cast<long long>(a.rows) * a.splits)), block(64 * WAVES);
+    switch (a.type) {
+        case 0: hipLaunchKernelGGL((logprob_kernel<0, WAVES, VALS>), grid, block, 0, s, a); break;
+        case 1: hipLaunchKernelGGL((logprob_kernel<1, WAVES, VALS>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((logprob_kernel<2, WAVES, VALS>), grid, block, 0, s, a); break;
+    }
+    return hipGetLastError();
+}
+
+// Workgroups of `waves` wavefronts of 32 logits a thread; past eight, eight of 64.
+hipError_t launch_parts(const LogprobArgs &a, int waves, hipStream_t s) {
+    switch (waves) {
+        case 1: return launch_rows<1>(a, s);
+        case 2: return launch_rows<2>(a, s);
+        case 3: return launch_rows<3>(a, s);
+        case 4: return launch_rows<4>(a, s);
+        case 5: return launch_rows<5>(a, s);
+        case 6: return launch_rows<6>(a, s);
+        case 7: return launch_rows<7>(a, s);
+        case 8: return launch_rows<8>(a, s);
+        default: return launch_rows<8, 64>(a, s);
+    }
+}
+
 }  // namespace
 
-int logprob_chunk(bool aligned) { return kLpThreads * kLpVals - (aligned ? 0 : 8); }  // less a piece where rows start inside one
+// The fewest wavefronts that hold a row, 32 logits a thread: what a wavefront
+// does once (the sort, the sums' exchanges) is then done least (7168 rows,
+// five alternatives, float32: 2048 logits 16 us in one, 31 in four, 64 in
+// eight; one row of 2048: 4.8, 5.5, 6.0). Up to twice eight's, 64 a thread
+// rather than two parts (one row of 32,768 float32 logits 6.5 us against
+// 12.1, 2000 rows 45 against 53; but 16 against 22 for the 7168 rows of 2048 and
+// 82 against 88 for those of 16,384). Then parts of eight's at most.
+void logprob_parts(LogprobArgs &a, bool aligned) {
+    const int wave = 64 * 32, slack = aligned ? 0 : 8;  // a piece where rows start inside one
+    const int most = 8 * wave - slack;
+    a.splits = a.n <= 16 * wave - slack ? 1 : (a.n + most - 1) / most;
+    a.chunk = ((a.n + a.splits - 1) / a.splits + 7) / 8 * 8;
+    a.waves = (std::min(a.chunk, a.n) + slack + wave - 1) / wave;
+}
 
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(static_cast<long long>(a.rows) * a.splits));
-    switch (a.type) {
-        case 0: hipLaunchKernelGGL(logprob_kernel<0>, grid, dim3(kLpThreads), 0, s, a); break;
-        case 1: hipLaunchKernelGGL(logprob_kernel<1>, grid, dim3(kLpThreads), 0, s, a); break;
-        default: hipLaunchKernelGGL(logprob_kernel<2>, grid, dim3(kLpThreads), 0, s, a); break;
-    }
-    if (hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
+    const hipError_t e = launch_parts(a, a.waves, s);
+    if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(logprob_join_kernel, dim3(a.rows), dim3(64), 0, s, a);
     return hipGetLastError();
 }
