@@ -134,7 +134,7 @@ SIGNATURES = {
                                     c_void_p, c_int, c_float, c_void_p, c_void_p, c_longlong, c_void_p]),
     "kv_evict_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_longlong,
                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
-    "nd_cross_attend_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, POINTER(CrossLayout), c_int, c_int,
+    "nd_cross_attend_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
                                     c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float,
                                     c_void_p]),
     "nd_logprobs_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,

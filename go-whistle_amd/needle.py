@@ -10,11 +10,12 @@ type and length (PagedKV), cross-attention to float memories
 """
 
 import ctypes
+import struct
 from ctypes import POINTER, c_float, c_int8, c_void_p
 
 import numpy as np
 
-from ._lib import CQPanic, CrossLayout, KvPaged, check, lib
+from ._lib import CQPanic, KvPaged, check, lib
 
 
 def QuantizeRows(x, cols, width):
@@ -202,47 +203,62 @@ def ApplyShared(dsts, x, rows, *ls):
 # ---- caches and memories of any type and length, log probabilities ----------------
 
 
+# A small call's kernel takes 4 to 8 us, so the checks here are kept to 2 to 4:
+# one attribute of a tensor costs 50 to 200 ns.
 _TYPES = {}
+_torch = _i32 = _f32 = None
+_layout = struct.Struct("10q").pack  # nd_cross_layout
 
 
 def _type(t, what, cache=False):
     """ND_F32.. of a tensor's dtype; ND_I8 for caches only."""
-    if not _TYPES:
+    global _torch, _i32, _f32
+    if _torch is None:
         import torch
 
         _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3})
+        _torch, _i32, _f32 = torch, torch.int32, torch.float32
     code = _TYPES.get(t.dtype)
     if code is None or (code == 3 and not cache):
         raise CQPanic(f"needle: {what} of {t.dtype}")
     return code
 
 
-def _want(t, what, shape, dtype=None, dev=None, dense=True):
+def _index(t, what):
+    """The index of the GPU a tensor is on."""
+    index = t.get_device()
+    if index < 0:
+        raise CQPanic(f"needle: {what} on {t.device}, not a GPU")
+    return index
+
+
+def _want(t, what, shape, dtype, index, dense=True):
     """Refuses a tensor that the call would read or write out of its bounds."""
+    if t.dtype is dtype and t.get_device() == index and t.shape == shape and (not dense or t.is_contiguous()):
+        return
     if t.shape != shape:
         raise CQPanic(f"needle: {what} of shape {tuple(t.shape)}, not {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype != dtype:
         raise CQPanic(f"needle: {what} of {t.dtype}, not {dtype}")
-    if not t.is_cuda or (dev is not None and t.device != dev):
-        raise CQPanic(f"needle: {what} on {t.device}, not {dev or 'a GPU'}")
-    if dense and not t.is_contiguous():
-        raise CQPanic(f"needle: {what} that is not contiguous")
+    if t.get_device() != index:
+        raise CQPanic(f"needle: {what} on {t.device}, not cuda:{index}")
+    raise CQPanic(f"needle: {what} that is not contiguous")
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(fn, device, *args):
-    """fn(*args, the current stream of the tensors' device), with that device current."""
-    import torch
-
-    index = device.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+def _call(fn, index, *args):
+    """fn(*args, the current stream of that GPU), with it current."""
+    c = _torch._C
+    if index == c._cuda_getDevice():
+        rc = fn(*args, c._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        with _torch.cuda.device(index):
+            rc = fn(*args, c._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 class PagedKV:
@@ -254,33 +270,30 @@ class PagedKV:
     entry or a fork's copied table is seen by the next call."""
 
     def __init__(self, k, v, pages, ks=None, vs=None):
-        import torch
-
         if k.dim() != 4 or v.dim() != 4 or pages.dim() != 2:
             raise CQPanic("needle: a paged cache is [pages, page_rows, kv_heads, width] and its table [streams, pages]")
-        _want(k, "keys", k.shape)
-        _want(v, "values", (*k.shape[:3], v.shape[3]), k.dtype, k.device)
-        _want(pages, "page table", pages.shape, torch.int32, k.device)
-        self.type = _type(k, "a cache", cache=True)
+        self.type, self.index = _type(k, "a cache", cache=True), _index(k, "keys")
+        _want(k, "keys", k.shape, k.dtype, self.index)
+        _want(v, "values", (*k.shape[:3], v.shape[3]), k.dtype, self.index)
+        _want(pages, "page table", pages.shape, _i32, self.index)
         if (self.type == 3) != (ks is not None) or (ks is None) != (vs is None):
             raise CQPanic("needle: int8 caches have scales, float ones none")
         for s, what in ((ks, "key scales"), (vs, "value scales")):
             if s is not None:
-                _want(s, what, k.shape[:3], torch.float32, k.device)
+                _want(s, what, k.shape[:3], _f32, self.index)
         self.k, self.v, self.ks, self.vs, self.pages = k, v, ks, vs, pages
         self.streams, self.kv_heads, self.qk, self.vd = pages.shape[0], k.shape[2], k.shape[3], v.shape[3]
-        self.device = k.device
+        self.device, self.cap = k.device, pages.shape[1] * k.shape[1]
         self._c = KvPaged(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), pages.data_ptr(), self.type, k.shape[2],
                           k.shape[3], v.shape[3], pages.shape[1], k.shape[1], k.shape[0])
         self._ref = ctypes.byref(self._c)
 
     def _acc(self, acc, what, rows):
-        import torch
-
-        _want(acc, what, (self.streams, self.kv_heads, acc.shape[-1]), torch.float32, self.device)
-        if acc.shape[-1] < rows:
-            raise CQPanic(f"needle: {what} of {acc.shape[-1]} rows for {rows}")
-        return acc.shape[-1]
+        cap = acc.shape[-1]
+        _want(acc, what, (self.streams, self.kv_heads, cap), _f32, self.index)
+        if cap < rows:
+            raise CQPanic(f"needle: {what} of {cap} rows for {rows}")
+        return cap
 
     def append_dev(self, k, v, pos, rows=None, cap=None, acc=None):
         """Rows k [streams, t, kv_heads, qk], v [streams, t, kv_heads, vd]
@@ -288,23 +301,22 @@ class PagedKV:
         row pos[b] of stream b, the first rows[b] of them where given; rows
         at or past cap (all that the table holds) are skipped. acc [streams,
         kv_heads, >= cap]: their accumulated weights become 0."""
-        import torch
-
-        t = k.shape[1] if k.dim() == 4 else 0
-        _want(k, "key rows", (self.streams, t, self.kv_heads, self.qk), None, self.device, dense=False)
-        _want(v, "value rows", (self.streams, t, self.kv_heads, self.vd), k.dtype, self.device, dense=False)
-        for x, w, what in ((k, self.qk, "key rows"), (v, self.vd, "value rows")):
-            if x.stride(3) != 1 or (x.stride(2) != w and self.kv_heads > 1):
+        shape, code = k.shape, _type(k, "rows")
+        t = shape[1] if len(shape) == 4 else 0
+        _want(k, "key rows", (self.streams, t, self.kv_heads, self.qk), k.dtype, self.index, dense=False)
+        _want(v, "value rows", (self.streams, t, self.kv_heads, self.vd), k.dtype, self.index, dense=False)
+        ks, vs = k.stride(), v.stride()
+        for x, w, what in ((ks, self.qk, "key rows"), (vs, self.vd, "value rows")):
+            if x[3] != 1 or (x[2] != w and self.kv_heads > 1):
                 raise CQPanic(f"needle: {what} whose heads are not side by side")
-        _want(pos, "positions", (self.streams,), torch.int32, self.device)
+        _want(pos, "positions", (self.streams,), _i32, self.index)
         if rows is not None:
-            _want(rows, "row counts", (self.streams,), torch.int32, self.device)
+            _want(rows, "row counts", (self.streams,), _i32, self.index)
         if cap is None:
-            cap = self.pages.shape[1] * self.k.shape[1]
+            cap = self.cap
         acc_cap = self._acc(acc, "weights", cap) if acc is not None else 0
-        _call(lib().kv_append_paged_dev, self.device, self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-              v.stride(0), v.stride(1), _type(k, "rows"), self.streams, t, _ptr(rows), pos.data_ptr(), cap, _ptr(acc),
-              acc_cap)
+        _call(lib().kv_append_paged_dev, self.index, self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              code, self.streams, t, _ptr(rows), pos.data_ptr(), cap, _ptr(acc), acc_cap)
 
     def attend_dev(self, out, q, spans, nk_max, scale, acc=None, acc_out=None):
         """Attention of one token a stream: q [streams, heads, qk] and out
@@ -312,12 +324,11 @@ class PagedKV:
         rows of spans [streams, 4] int32 in [0, nk_max), logits q.k / scale.
         acc_out [streams, kv_heads, >= nk_max]: acc (or 0) plus each row's
         weights; it may be acc."""
-        import torch
-
-        heads = q.shape[1] if q.dim() == 3 else 0
-        _want(q, "queries", (self.streams, heads, self.qk), None, self.device)
-        _want(out, "outputs", (self.streams, heads, self.vd), q.dtype, self.device)
-        _want(spans, "spans", (self.streams, 4), torch.int32, self.device)
+        shape, code = q.shape, _type(q, "queries")
+        heads = shape[1] if len(shape) == 3 else 0
+        _want(q, "queries", (self.streams, heads, self.qk), q.dtype, self.index)
+        _want(out, "outputs", (self.streams, heads, self.vd), q.dtype, self.index)
+        _want(spans, "spans", (self.streams, 4), _i32, self.index)
         acc_cap = 0
         if acc_out is not None:
             acc_cap = self._acc(acc_out, "weights", nk_max)
@@ -325,9 +336,8 @@ class PagedKV:
                 raise CQPanic(f"needle: weights of {acc.shape[-1]} rows to {acc_cap}")
         elif acc is not None:
             raise CQPanic("needle: weights without an output for them")
-        _call(lib().kv_attend_paged_dev, self.device, self._ref, out.data_ptr(), 0, q.data_ptr(), 0,
-              _type(q, "queries"), self.streams, heads, spans.data_ptr(), nk_max, scale, _ptr(acc), _ptr(acc_out),
-              acc_cap)
+        _call(lib().kv_attend_paged_dev, self.index, self._ref, out.data_ptr(), 0, q.data_ptr(), 0, code, self.streams,
+              heads, spans.data_ptr(), nk_max, scale, _ptr(acc), _ptr(acc_out), acc_cap)
 
     def evict_dev(self, dst_pages, acc, acc_out, length, length_out, kept, nk_max, sink=0, recent=0):
         """Each stream's first length[b] (<= nk_max) rows cut to keep =
@@ -337,15 +347,14 @@ class PagedKV:
         from.
         kept [streams, kv_heads, keep] int32 gets their numbers, acc_out
         [streams, kv_heads, >= keep] their weights, length_out[b] their count."""
-        import torch
-
-        keep = kept.shape[2] if kept.dim() == 3 else 0
-        _want(kept, "kept rows", (self.streams, self.kv_heads, keep), torch.int32, self.device)
-        _want(dst_pages, "page table", (self.streams, dst_pages.shape[-1]), torch.int32, self.device)
-        _want(length, "lengths", (self.streams,), torch.int32, self.device)
-        _want(length_out, "lengths", (self.streams,), torch.int32, self.device)
+        shape, width = kept.shape, dst_pages.shape[-1]
+        keep = shape[2] if len(shape) == 3 else 0
+        _want(kept, "kept rows", (self.streams, self.kv_heads, keep), _i32, self.index)
+        _want(dst_pages, "page table", (self.streams, width), _i32, self.index)
+        _want(length, "lengths", (self.streams,), _i32, self.index)
+        _want(length_out, "lengths", (self.streams,), _i32, self.index)
         acc_cap, out_cap = self._acc(acc, "weights", nk_max), self._acc(acc_out, "weights", keep)
-        _call(lib().kv_evict_paged_dev, self.device, self._ref, dst_pages.data_ptr(), dst_pages.shape[1],
+        _call(lib().kv_evict_paged_dev, self.index, self._ref, dst_pages.data_ptr(), width,
               acc.data_ptr(), acc_cap, acc_out.data_ptr(), out_cap, length.data_ptr(), length_out.data_ptr(),
               kept.data_ptr(), self.streams, nk_max, keep, sink, recent)
 
@@ -358,29 +367,29 @@ def cross_attend_dev(out, q, k, v, scale, q_len=None, k_len=None, index=None):
     float16, bfloat16), logits q.k / scale. q_len [streams]: rows past it are
     left as they were; k_len [memories]: frames past it are not attended;
     index [streams]: the memory each stream reads (beams share one)."""
-    import torch
-
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or out.dim() != 4:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise CQPanic("needle: cross-attention of [streams, rows, heads, width]")
-    B, t, heads, qk = q.shape
-    M, frames, kv_heads, _ = k.shape
-    vd, dev = v.shape[3], q.device
-    _want(q, "queries", q.shape, None, None, dense=False)
-    _want(out, "outputs", (B, t, heads, vd), q.dtype, dev, dense=False)
-    _want(k, "keys", (M, frames, kv_heads, qk), q.dtype, dev, dense=False)
-    _want(v, "values", (M, frames, kv_heads, vd), q.dtype, dev, dense=False)
-    for x, w, what in ((q, qk, "queries"), (out, vd, "outputs")):
-        if x.stride(3) != 1 or (x.stride(2) != w and heads > 1):
-            raise CQPanic(f"needle: {what} whose heads are not side by side")
-    if k.stride(3) != 1 or v.stride(3) != 1:
+    B, t, heads, qk = qs
+    M, frames, kv_heads, _ = ks
+    vd, code, dtype, dev = vs[3], _type(q, "queries"), q.dtype, _index(q, "queries")
+    _want(out, "outputs", (B, t, heads, vd), dtype, dev, False)
+    _want(k, "keys", (M, frames, kv_heads, qk), dtype, dev, False)
+    _want(v, "values", (M, frames, kv_heads, vd), dtype, dev, False)
+    qs, ys, ks, vs = q.stride(), out.stride(), k.stride(), v.stride()
+    if qs[3] != 1 or ys[3] != 1 or (heads > 1 and (qs[2] != qk or ys[2] != vd)):
+        raise CQPanic("needle: queries or outputs whose heads are not side by side")
+    if ks[3] != 1 or vs[3] != 1:
         raise CQPanic("needle: memories whose values are not side by side")
-    for x, n, what in ((q_len, B, "query lengths"), (k_len, M, "memory lengths"), (index, B, "memory index")):
-        if x is not None:
-            _want(x, what, (n,), torch.int32, dev)
-    y = CrossLayout(*q.stride()[:2], *out.stride()[:2], *k.stride()[:3], *v.stride()[:3])
-    _call(lib().nd_cross_attend_dev, dev, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-          _type(q, "queries"), ctypes.byref(y), B, t, heads, kv_heads, qk, vd, M, frames, _ptr(q_len), _ptr(k_len),
-          _ptr(index), scale)
+    if q_len is not None:
+        _want(q_len, "query lengths", (B,), _i32, dev)
+    if k_len is not None:
+        _want(k_len, "memory lengths", (M,), _i32, dev)
+    if index is not None:
+        _want(index, "memory index", (B,), _i32, dev)
+    _call(lib().nd_cross_attend_dev, dev, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), code,
+          _layout(qs[0], qs[1], ys[0], ys[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), B, t, heads, kv_heads, qk, vd, M,
+          frames, _ptr(q_len), _ptr(k_len), _ptr(index), scale)
 
 
 def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
@@ -389,20 +398,23 @@ def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
     negative one, a padded row), ent [rows] the entropies, top [rows, k]
     int32 and top_lp [rows, k] the k <= 64 likeliest tokens, the lowest first
     among equals, with their log probabilities."""
-    import torch
-
-    if logits.dim() != 2:
-        raise CQPanic(f"needle: logits of shape {tuple(logits.shape)}, not rows of them")
-    rows, n = logits.shape
-    dev, f32 = logits.device, torch.float32
-    _want(logits, "logits", (rows, n), None, None, dense=False)
-    if n > 1 and logits.stride(1) != 1:
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2:
+        raise CQPanic(f"needle: logits of shape {tuple(shape)}, not rows of them")
+    rows, n = shape
+    code, dev = _type(logits, "logits"), _index(logits, "logits")
+    if n > 1 and stride[1] != 1:
         raise CQPanic("needle: logits whose rows are not contiguous")
     k = top.shape[1] if top is not None and top.dim() == 2 else 0
-    for x, shape, dtype, what in ((tokens, (rows,), torch.int32, "tokens"), (lp, (rows,), f32, "log probabilities"),
-                                  (ent, (rows,), f32, "entropies"), (top, (rows, k), torch.int32, "alternatives"),
-                                  (top_lp, (rows, k), f32, "alternatives' log probabilities")):
-        if x is not None:
-            _want(x, what, shape, dtype, dev)
+    if tokens is not None:
+        _want(tokens, "tokens", (rows,), _i32, dev)
+    if lp is not None:
+        _want(lp, "log probabilities", (rows,), _f32, dev)
+    if ent is not None:
+        _want(ent, "entropies", (rows,), _f32, dev)
+    if top is not None:
+        _want(top, "alternatives", (rows, k), _i32, dev)
+    if top_lp is not None:
+        _want(top_lp, "alternatives' log probabilities", (rows, k), _f32, dev)
     _call(lib().nd_logprobs_dev, dev, _ptr(lp), _ptr(ent), _ptr(top) if k else None, _ptr(top_lp) if k else None,
-          logits.data_ptr(), logits.stride(0), _type(logits, "logits"), rows, n, _ptr(tokens), k)
+          logits.data_ptr(), stride[0], code, rows, n, _ptr(tokens), k)
