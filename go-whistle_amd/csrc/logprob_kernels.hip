@@ -92,7 +92,7 @@ __device__ __forceinline__ float sort_lanes(float x) {
 // at least `top` values of the part reach, and the largest such bound of the
 // wavefronts leaves few more (about 20 of 16,384 normal values for 10). Those
 // are listed in LDS and ranked by counting. A list of more than kLpList (equal
-// values, more than about 40 alternatives) takes them one after the other,
+// values, or more than about 40 alternatives of a long row) takes them one after the other,
 // reading the part again: its values' registers are not held for that.
 constexpr int kLpList = 512;
 

@@ -360,8 +360,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
 
 // The kept rows copied: a thread takes 16 bytes of a head's key row and the
 // same piece of its value row, of two rows half the budget apart (each
-// destination row is written whole by its neighbours): four loads in flight behind one chain of
-// row, page and pool. The stores go past the L2 to memory at once, not at the
+// destination row is written whole by its neighbours): four loads in flight
+// behind one chain of row, page and pool. The stores go past the L2 to memory at once, not at the
 // launch's end, when the L2s give up their dirty lines (270 MB 53.5 -> 42 us,
 // 0.8 MB 8.6 -> 3.3 us; the appends and the attention's narrower stores gain
 // nothing by it or lose). The scales of int8 rows ride with the first piece.

@@ -7,10 +7,11 @@
 // over the keys with a running maximum m and sum l (in log2 units, p_j =
 // 2^(l_j - m)): a wavefront takes tiles of 16 or 32 keys, the wavefronts of a
 // workgroup share a part of the list and are joined in LDS; the parts of a
-// list, where there are few lists and many keys, by a second launch. All
-// arithmetic is float32, whatever the types.
+// list, where there are few lists and many keys, by a second launch. Sums and
+// softmax are float32, whatever the types, and the products exact in it.
 //
-// attend_lanes_kernel, one or two columns: lane (r, c) = (lane % 16, lane /
+// attend_lanes_kernel, one or two columns (of more, two a workgroup where a
+// call has little work: split_tile_columns): lane (r, c) = (lane % 16, lane /
 // 16) reads pieces c, c + 4, ... of 16 bytes of key row r and of value row r.
 // The logit is the four lanes' sum, and a lane keeps the outputs of its
 // pieces for its keys: no exchange of the weights, one sum over r at the end.
