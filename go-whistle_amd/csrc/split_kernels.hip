@@ -7,8 +7,8 @@
 // over the keys with a running maximum m and sum l (in log2 units, p_j =
 // 2^(l_j - m)): a wavefront takes tiles of 16 or 32 keys, the wavefronts of a
 // workgroup share a part of the list and are joined in LDS; the parts of a
-// list, where there are few lists and many keys, by a second launch. Sums and
-// softmax are float32, whatever the types, and the products exact in it.
+// list, where there are few lists and many keys, by a second launch. Weights,
+// softmax and sums are float32, whatever the types.
 //
 // attend_lanes_kernel, one or two columns (of more, two a workgroup where a
 // call has little work: split_tile_columns): lane (r, c) = (lane % 16, lane /
