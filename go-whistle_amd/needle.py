@@ -217,7 +217,7 @@ def _type(t, what, cache=False):
         import torch
 
         _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3})
-        _torch, _i32, _f32 = torch, torch.int32, torch.float32
+        _i32, _f32, _torch = torch.int32, torch.float32, torch  # _torch last: other threads look at it
     code = _TYPES.get(t.dtype)
     if code is None or (code == 3 and not cache):
         raise CQPanic(f"needle: {what} of {t.dtype}")
@@ -289,7 +289,7 @@ class PagedKV:
         self._ref = ctypes.byref(self._c)
 
     def _acc(self, acc, what, rows):
-        cap = acc.shape[-1]
+        cap = acc.shape[-1] if acc.dim() else 0
         _want(acc, what, (self.streams, self.kv_heads, cap), _f32, self.index)
         if cap < rows:
             raise CQPanic(f"needle: {what} of {cap} rows for {rows}")
@@ -347,7 +347,7 @@ class PagedKV:
         from.
         kept [streams, kv_heads, keep] int32 gets their numbers, acc_out
         [streams, kv_heads, >= keep] their weights, length_out[b] their count."""
-        shape, width = kept.shape, dst_pages.shape[-1]
+        shape, width = kept.shape, dst_pages.shape[-1] if dst_pages.dim() else 0
         keep = shape[2] if len(shape) == 3 else 0
         _want(kept, "kept rows", (self.streams, self.kv_heads, keep), _i32, self.index)
         _want(dst_pages, "page table", (self.streams, width), _i32, self.index)

@@ -203,3 +203,29 @@ def test_graph_replays():
         graph.replay()
         want = run(x, tok, 8)
         assert all(torch.equal(a, b) for a, b in zip((lp, ent, top, tl), want))
+
+
+@pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("n", [2040, 2041, 2048, 2049, 4097, 6145, 8185, 10241, 12289, 14337, 32760, 32761, 32768, 32769])
+def test_wavefronts_of_a_row(name, n):
+    # sizes either side of what one more wavefront holds, in rows that start on a 16-byte boundary and in others
+    import torch
+
+    g = gen(n)
+    wide = (3 * torch.randn(4, n + 8 - n % 8 + 8, generator=g, device="cuda")).to(getattr(torch, name))
+    tok = torch.tensor([n - 1, 0, n // 3, 7], dtype=torch.int32, device="cuda")
+    check(wide[:, :n], tok, 3)
+    check(wide[:, 1:n + 1], tok, 33)
+    check(wide.view(-1)[7:7 + n].view(1, n), tok[:1], 64)
+
+
+@pytest.mark.parametrize("name", FLOATS)
+@pytest.mark.parametrize("n,top", [(600, 64), (2000, 7), (3000, 64), (20000, 5)])
+def test_equal_logits_of_short_rows(name, n, top):
+    # more of them than are ranked at once
+    import torch
+
+    x = torch.full((3, n), -2.5, device="cuda", dtype=getattr(torch, name))
+    x[1, n // 2:] = 1.0
+    x[2, n - 1] = 4.0
+    check(x, torch.tensor([0, n - 1, n], dtype=torch.int32, device="cuda"), top)
