@@ -14,13 +14,18 @@
 //     them: the half f's eight are 4 f + {0..3} and 8 + 4 f + {0..3}, so the
 //     weights are S's registers rounded in place and A's two halves are
 //     transposing LDS reads (four keys by sixteen values each).
-// The weights are rounded to the memories' type for the second product (half
-// an ulp of it, the size of the outputs' own rounding); logits, weights
-// before that, their sums and the outputs are float32. The running maximum m
-// is raised only when a column's logits pass it by 2^8, so most tiles leave
-// the outputs unscaled. float16 weights are 2^(logit - m + 7): up to 2^15,
-// which it holds, and none above 2^-32 of the largest is lost (without the
-// seven, 20,000 frames of weights of 2.9e-8 were).
+// The second product takes a weight in two parts of the memories' type, their
+// sum off by 2^-16 of it in bfloat16 (a truncation, then the nearest to what
+// that leaves) and 2^-22 in float16 (the nearest, twice). One part is off by
+// 2^-9 and 2^-12, and the outputs' error against 64 bits was then 1.4 times
+// that of their own rounding. The second costs its products, half as many
+// again, and three vector operations a weight: 64 x 448 rows to 1500 frames,
+// 8 heads of 64, 118 -> 156 us; 32 x 448 of 128 119 -> 145; 2 x 448 of 64
+// 20.0 -> 21.7; 5 rows to 375 frames 9.0 -> 10.5. Logits, weights, their sums
+// and the outputs are float32. The running maximum m is raised only when a
+// column's logits pass it by 2^8, so most tiles leave the outputs unscaled.
+// float16 weights are 2^(logit - m + 7): up to 2^15, which it holds, and none
+// loses more than 2^-32 of the largest.
 //
 // Bank conflicts: row r of a tile keeps its 16-byte pieces in the order c ^
 // f(r): f chosen so that sixteen lanes reading one piece of sixteen key rows,
@@ -30,6 +35,7 @@
 #include "cq_device.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cqhip {
 namespace {
@@ -39,6 +45,9 @@ using s16x4 = short __attribute__((ext_vector_type(4)));
 using s16x8 = short __attribute__((ext_vector_type(8)));
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using lds_bytes = __attribute__((address_space(3))) unsigned char;
 
 constexpr int kXWaves = 4;
@@ -60,6 +69,37 @@ __device__ __forceinline__ short round16(float x) {
         return __builtin_bit_cast(short, static_cast<_Float16>(x));
     else
         return __builtin_bit_cast(short, static_cast<__bf16>(x));
+}
+
+// The first and the second parts of two weights.
+template <int TYPE>
+__device__ __forceinline__ uint32_t first_parts(float x, float y) {
+    if constexpr (TYPE == 1)
+        return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+    else  // the upper halves
+        return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t second_parts(float x, float y, uint32_t parts) {
+    if constexpr (TYPE == 1) {  // x - part by a dot with (-1, 0): one instruction
+        const f16x2 p = __builtin_bit_cast(f16x2, parts);
+        const f16x2 lower = {static_cast<_Float16>(-1.0f), static_cast<_Float16>(0.0f)};
+        const f16x2 upper = {static_cast<_Float16>(0.0f), static_cast<_Float16>(-1.0f)};
+        return first_parts<1>(__builtin_amdgcn_fdot2(p, lower, x, false), __builtin_amdgcn_fdot2(p, upper, y, false));
+    } else {
+        const bf16x2 p = {static_cast<__bf16>(x - __uint_as_float(__float_as_uint(x) & 0xffff0000u)),
+                          static_cast<__bf16>(y - __uint_as_float(__float_as_uint(y) & 0xffff0000u))};
+        return __builtin_bit_cast(uint32_t, p);
+    }
+}
+
+// Four pairs of 16-bit values, with 0 in place of infinities and NaNs.
+template <int TYPE>
+__device__ __forceinline__ s16x8 finite16(s16x8 x) {
+    constexpr short kExponent = TYPE == 1 ? 0x7c00 : 0x7f80;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (x[e] & kExponent) == kExponent ? 0 : x[e];
+    return x;
 }
 
 // The larger of the two halves' values, in both.
@@ -101,13 +141,14 @@ __device__ __forceinline__ int longest_first(const SplitArgs &a, int place, int 
 // D: widths up to D; CB: 32-column blocks a wavefront; FULL: both widths are
 // D (else steps past a width are skipped by branches, which keep the
 // compiler from interleaving the products with the softmax).
+constexpr int kXFlags = 4 * kXWaves;  // bytes behind the tiles: an int a wavefront
 template <int TYPE, int D, int CB, bool FULL>
 __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_kernel(SplitArgs a, int col_tiles, int aligned) {
     constexpr int kPieces = D / 8;              // 16-byte pieces of a row
     constexpr int kLoads = D / 32;              // wavefront loads of a tile's keys (values) a wavefront
     constexpr int kLoadRows = 512 / D;          // rows of a wavefront load
     constexpr int kBytes = kXTile * D * 2;      // a tile's keys (values)
-    extern __shared__ __align__(16) unsigned char smem[];  // [2][keys, values]
+    extern __shared__ __align__(16) unsigned char smem[];  // [2][keys, values], flags
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, half = lane >> 5;
@@ -163,7 +204,6 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
             *reinterpret_cast<uint4 *>(smem + x) = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
-    if (j0 < j1) load_tile(j0, 0);
 
     // The queries: lane (n, half) holds coordinates 16 s + 8 half + 0..7 of its columns.
     s16x8 q[CB][D / 16];
@@ -191,98 +231,134 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 
     f32x16 o[CB][D / 32];
     float m[CB], l[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        m[cb] = -INFINITY;
-        l[cb] = 0.0f;
-#pragma unroll
-        for (int v = 0; v < D / 32; ++v)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[cb][v][i] = 0.0f;
-    }
     // LDS addresses: the keys' row n of a block, the values' row (lane % 16) / 4 and piece of a transposing read.
     const int kaddr = n * D * 2, kswz = k_swizzle<D>(n);
     const int ti = lane & 15, trow = 4 * half + (ti >> 2);
     const int vaddr = trow * D * 2 + 8 * (ti & 1), vpiece = 2 * ((lane >> 4) & 1) + ((ti & 3) >> 1), vswz = v_swizzle<D>(trow);
 
-    int buf = 0;
-    for (int j = j0; j < j1; j += kXTile, buf ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (j + kXTile > j1) clear_tail(j, buf);
-        __syncthreads();  // this tile is whole, and the other buffer's readers are done
-        if (j + kXTile < j1) load_tile(j + kXTile, buf ^ 1);
-        if (!live) continue;
-        const unsigned char *kt = smem + buf * 2 * kBytes, *vt = kt + kBytes;
-        f32x16 s[CB][2];
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[cb][kb][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-            if (FULL || 16 * ks < a.c.qk) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const s16x8 ka = *reinterpret_cast<const s16x8 *>(kt + kb * 32 * D * 2 + kaddr + ((2 * ks + half) ^ kswz) * 16);
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16<TYPE>(ka, q[cb][ks], s[cb][kb]);
-                }
-            }
-        if (j + kXTile > j1) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (j + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= j1) {
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][kb][i] = -INFINITY;
-                    }
-        }
-        s16x8 p[CB][4];
+    // finite: the second parts, which may be 0 or below it, meet no infinite value.
+    auto attend = [&](auto finite_values) {
+        constexpr bool finite = decltype(finite_values)::value;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
-            float mt = s[cb][0][0];
+            m[cb] = -INFINITY;
+            l[cb] = 0.0f;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[cb][0][i]);
+            for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[cb][1][i]);
-            mt = halves_max(mt) * a.scale_log2;
-            if (__any(mt > m[cb] + 8.0f)) {
-                const float mn = fmaxf(m[cb], mt);
-                const float f = m[cb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
-                m[cb] = mn;
-                l[cb] *= f;
+                for (int i = 0; i < 16; ++i) o[cb][v][i] = 0.0f;
+        }
+        if (j0 < j1) load_tile(j0, 0);
+        int buf = 0;
+        for (int j = j0; j < j1; j += kXTile, buf ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (j + kXTile > j1) clear_tail(j, buf);
+            __syncthreads();  // this tile is whole, and the other buffer's readers are done
+            if (j + kXTile < j1) load_tile(j + kXTile, buf ^ 1);
+            if (!live) continue;
+            const unsigned char *kt = smem + buf * 2 * kBytes, *vt = kt + kBytes;
+            f32x16 s[CB][2];
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[cb][kb][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+                if (FULL || 16 * ks < a.c.qk) {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+                        const s16x8 ka = *reinterpret_cast<const s16x8 *>(kt + kb * 32 * D * 2 + kaddr + ((2 * ks + half) ^ kswz) * 16);
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16<TYPE>(ka, q[cb][ks], s[cb][kb]);
+                    }
+                }
+            if (j + kXTile > j1) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (j + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3) >= j1) {
+#pragma unroll
+                            for (int cb = 0; cb < CB; ++cb) s[cb][kb][i] = -INFINITY;
+                        }
+            }
+            u32x4 p[CB][4], rest[CB][4];
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                float mt = s[cb][0][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[cb][0][i]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[cb][1][i]);
+                mt = halves_max(mt) * a.scale_log2;
+                if (__any(mt > m[cb] + 8.0f)) {
+                    const float mn = fmaxf(m[cb], mt);
+                    const float f = m[cb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
+                    m[cb] = mn;
+                    l[cb] *= f;
+#pragma unroll
+                    for (int v = 0; v < D / 32; ++v)
+                        if (FULL || 32 * v < a.c.vd) o[cb][v] *= f;
+                }
+                const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<TYPE>;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], a.scale_log2, -mu));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i + 1], a.scale_log2, -mu));
+                        l[cb] += x;
+                        l[cb] += y;
+                        const uint32_t parts = first_parts<TYPE>(x, y);
+                        p[cb][2 * kb + (i >> 3)][(i & 7) >> 1] = parts;
+                        rest[cb][2 * kb + (i >> 3)][(i & 7) >> 1] = second_parts<TYPE>(x, y, parts);
+                    }
+            }
+            // all first parts of 16 keys, then all second ones: no product waits for the one before it
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                s16x8 va[D / 32];
 #pragma unroll
                 for (int v = 0; v < D / 32; ++v)
-                    if (FULL || 32 * v < a.c.vd) o[cb][v] *= f;
+                    if (FULL || 32 * v < a.c.vd) {
+                        const unsigned char *at = vt + 16 * st * D * 2 + vaddr + ((4 * v + vpiece) ^ vswz) * 16;
+                        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+                        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4 *)(at + 8 * D * 2));
+                        va[v] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb)
+                            o[cb][v] = mfma16<TYPE>(va[v], __builtin_bit_cast(s16x8, p[cb][st]), o[cb][v]);
+                    }
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v)
+                    if (FULL || 32 * v < a.c.vd) {
+                        if (finite) va[v] = finite16<TYPE>(va[v]);
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb)
+                            o[cb][v] = mfma16<TYPE>(va[v], __builtin_bit_cast(s16x8, rest[cb][st]), o[cb][v]);
+                    }
             }
-            const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<TYPE>;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], a.scale_log2, -mu));
-                    l[cb] += w;
-                    p[cb][2 * kb + (i >> 3)][i & 7] = round16<TYPE>(w);
-                }
         }
+    };
+    attend(std::false_type{});
+    // A NaN: an infinite value may be behind it, which the first parts alone
+    // make infinite. All over again for the workgroup, whose wavefronts share the tiles.
+    bool nan = false;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int v = 0; v < D / 32; ++v)
-            if (FULL || 32 * v < a.c.vd) {
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    const unsigned char *at = vt + 16 * st * D * 2 + vaddr + ((4 * v + vpiece) ^ vswz) * 16;
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4 *)(at + 8 * D * 2));
-                    const s16x8 va = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) o[cb][v] = mfma16<TYPE>(va, p[cb][st], o[cb][v]);
-                }
-            }
-    }
+            for (int i = 0; i < 16; ++i) nan |= o[cb][v][i] != o[cb][v][i];
+    const bool wave_nan = live && __any(nan);
+    int *flags = reinterpret_cast<int *>(smem + 4 * kBytes);
+    if (lane == 0) flags[wave] = wave_nan;
+    __syncthreads();  // also: the tiles' readers are done
+    const int4 any = *reinterpret_cast<const int4 *>(flags);
+    if (any.x | any.y | any.z | any.w) attend(std::true_type{});
     if (!live) return;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
@@ -520,7 +596,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
 
 template <int TYPE, int D, int CB, bool FULL>
 hipError_t launch_cross_full(const SplitArgs &a, int cols, int aligned, hipStream_t s) {
-    constexpr int lds = 2 * 2 * kXTile * D * 2;
+    constexpr int lds = 2 * 2 * kXTile * D * 2 + kXFlags;
     static std::atomic<unsigned long long> attr{0};
     if (lds > 64 * 1024)
         if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(&cross_attend_kernel<TYPE, D, CB, FULL>), lds, attr)) return e;
