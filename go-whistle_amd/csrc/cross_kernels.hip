@@ -141,6 +141,12 @@ __device__ __forceinline__ int longest_first(const SplitArgs &a, int place, int 
 // D: widths up to D; CB: 32-column blocks a wavefront; FULL: both widths are
 // D (else steps past a width are skipped by branches, which keep the
 // compiler from interleaving the products with the softmax).
+// The exponents s scale - m are rounded once (fmaf), so the largest is off 0 by
+// the rounding of m = max(s) scale, at most half an ulp: the same factor in
+// every weight of a column and their sum, and below 2^(1/32) as long as |m| is
+// below 2^20. From there on, where it could leave float16 (from 2^28) or
+// float32 (2^31), s scale is rounded first, as m is.
+constexpr float kFar = 0x1p20f;
 constexpr int kXFlags = 4 * kXWaves;  // bytes behind the tiles: an int a wavefront
 template <int TYPE, int D, int CB, bool FULL>
 __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_kernel(SplitArgs a, int col_tiles, int aligned) {
@@ -293,7 +299,8 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[cb][1][i]);
                 mt = halves_max(mt) * a.scale_log2;
-                if (__any(mt > m[cb] + 8.0f)) {
+                float scale = a.scale_log2;
+                if (__any(mt > m[cb] + 8.0f || fabsf(m[cb]) >= kFar)) {
                     const float mn = fmaxf(m[cb], mt);
                     const float f = m[cb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
                     m[cb] = mn;
@@ -301,14 +308,21 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 #pragma unroll
                     for (int v = 0; v < D / 32; ++v)
                         if (FULL || 32 * v < a.c.vd) o[cb][v] *= f;
+                    const bool far = fabsf(mn) >= kFar;
+                    if (__any(far)) {
+                        const float first = far ? scale : 1.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[cb][0][i] *= first, s[cb][1][i] *= first;
+                        scale = far ? 1.0f : scale;
+                    }
                 }
                 const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<TYPE>;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], a.scale_log2, -mu));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i + 1], a.scale_log2, -mu));
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], scale, -mu));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i + 1], scale, -mu));
                         l[cb] += x;
                         l[cb] += y;
                         const uint32_t parts = first_parts<TYPE>(x, y);

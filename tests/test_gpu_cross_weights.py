@@ -97,3 +97,51 @@ def test_a_row_of_nan_leaves_the_others_as_they_are(name, qk, vd):
     outs[0][1, 77, 0] = outs[1][1, 77, 0] = 0
     o = outs[0].float()
     assert (outs[1].float() - o).abs().max() <= 2 * half_ulp(dt) * o.abs().max()
+
+
+@pytest.mark.parametrize("name", ["float32"] + HALVES)
+@pytest.mark.parametrize("scale", [1.0, 8.0, math.sqrt(48)])
+@pytest.mark.parametrize("B,t,F", [(1, 1, 100), (2, 2, 100), (2, 2, 700), (2, 80, 100), (70, 33, 65), (2, 400, 70)])
+def test_far_logits(name, scale, B, t, F):
+    # dots past 2^28 (float16: 64 products of 30000 and about as much, exact in
+    # float32) or about +-1e30: the frame of the largest logit is the answer,
+    # of two equal ones their mean, also from far below 0
+    import torch
+
+    dt, D = getattr(torch, name), 64
+    q = torch.full((B, t, 1, D), 30000.0 if name == "float16" else 1e15, device="cuda", dtype=dt)
+    v = torch.randn(B, F, 1, D, generator=gen(F), device="cuda").to(dt)
+    base = torch.arange(F, device="cuda").view(1, F, 1, 1).expand(B, F, 1, D)
+    for low, step, high in ((20000.0, 16.0, 30000.0), (-30000.0, 16.0, -16.0), (-30000.0, 0.0, 0.0)):
+        k = (low + step * (base * 7 % 11)) * (1.0 if name == "float16" else 1e9)
+        k[:, F // 2] = high * (1.0 if name == "float16" else 1e9)
+        k = k.to(dt)
+        out = torch.full((B, t, 1, D), 5.0, device="cuda", dtype=dt)
+        needle.cross_attend_dev(out, q, k, v, scale)
+        torch.cuda.synchronize()
+        assert torch.equal(out, v[:, F // 2:F // 2 + 1].expand_as(out)), low
+        k[:, F - 1] = k[:, F // 2]
+        needle.cross_attend_dev(out, q, k, v, scale)
+        torch.cuda.synchronize()
+        want = ((v[:, F // 2].double() + v[:, F - 1].double()) / 2).to(dt)
+        assert torch.equal(out, want.unsqueeze(1).expand_as(out)), low
+
+
+@pytest.mark.parametrize("name", ["float32"] + HALVES)
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 19, 2.0 ** 20, 2.0 ** 21, 2.0 ** 24, 2.0 ** 27])
+def test_outputs_stay_between_the_values(name, size):
+    # logits of each size, of rows side by side in a wavefront that differ in it
+    import torch
+
+    g, dt, B, t, F, D = gen(3), getattr(torch, name), 4, 130, 200, 64
+    q, k, v = (torch.randn(B, n, 2, D, generator=g, device="cuda").to(dt) for n in (t, F, F))
+    q[:, ::3] *= 2.0 ** 12
+    q[:, 1::3] = 0
+    out = torch.empty_like(q)
+    needle.cross_attend_dev(out, q, k, v, 2.0 ** 15 / size)
+    torch.cuda.synchronize()
+    lo, hi = v.float().amin(1, keepdim=True), v.float().amax(1, keepdim=True)
+    slack = 2 * half_ulp(dt) * v.float().abs().max()
+    assert (out.float() >= lo - slack).all() and (out.float() <= hi + slack).all()
+    mean = v.double().mean(1, keepdim=True)
+    assert (out[:, 1::3].double() - mean).abs().max() <= 2 * half_ulp(dt) * mean.abs().max() + F * 2.0 ** -24
