@@ -38,6 +38,7 @@
 #include "cq_device.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cqhip {
 namespace {
@@ -246,16 +247,24 @@ __device__ __forceinline__ void load_query(float *x, const SplitArgs &a, long lo
 }
 
 // LDS of a workgroup, in floats: per wavefront and column the maximum and the
-// sum, per column the joined maximum and 1 / sum, per wavefront and column the
-// outputs (rows of D + 4), then the logits [column][nk_max] where the weights
-// are asked of a whole list.
+// sum, per column the joined maximum and 1 / sum, then from a 16-byte boundary
+// per wavefront and column the outputs (rows of D + 4), then the logits
+// [column][nk_max] where the weights are asked of a whole list.
 template <int COLS, int D>
 struct Joint {
     static constexpr int kRow = D + 4;
     float *ml, *stat, *o, *logits;
+    static constexpr int stats(int waves) { return (waves * 2 * COLS + 2 * COLS + 3) / 4 * 4; }
+    static constexpr int floats(int waves) { return stats(waves) + waves * COLS * kRow; }
+    static constexpr bool aligned() {  // the outputs' rows, stored as float4, for every number of wavefronts
+        for (int w = 1; w <= 8; ++w)
+            if (stats(w) % 4 != 0) return false;
+        return kRow % 4 == 0;
+    }
     __device__ Joint(float *smem, int waves)
-        : ml(smem), stat(ml + waves * 2 * COLS), o(stat + 2 * COLS), logits(o + waves * COLS * kRow) {}
-    static constexpr int floats(int waves) { return waves * 2 * COLS + 2 * COLS + waves * COLS * kRow; }
+        : ml(smem), stat(ml + waves * 2 * COLS), o(smem + stats(waves)), logits(smem + floats(waves)) {
+        static_assert(aligned(), "outputs off their 16-byte boundary");
+    }
 };
 
 // Joins the wavefronts' columns (o, ml filled, outputs relative to each
@@ -870,9 +879,15 @@ int split_max_waves(const SplitArgs &a) {
 }
 
 bool split_weights_in_lds(const SplitArgs &a, int waves) {
-    const int w = std::max(a.c.qk, a.c.vd), d = w <= 64 ? 64 : w <= 128 ? 128 : 256, group = a.heads / a.c.kv_heads;
-    const size_t joint = sizeof(float) * (waves * 2 + 2 + waves * (d + 4)) * a.tile;
-    return a.t == 1 && group <= a.tile && joint + sizeof(float) * group * static_cast<size_t>(a.nk_max) <= kMostLds / 2;
+    const int w = std::max(a.c.qk, a.c.vd), group = a.heads / a.c.kv_heads;
+    const auto joint = [&](auto d) {
+        constexpr int kD = decltype(d)::value;
+        return a.tile == 1 ? Joint<1, kD>::floats(waves) : a.tile == 2 ? Joint<2, kD>::floats(waves) : Joint<kCols, kD>::floats(waves);
+    };
+    const int floats = w <= 64    ? joint(std::integral_constant<int, 64>{})
+                       : w <= 128 ? joint(std::integral_constant<int, 128>{})
+                                  : joint(std::integral_constant<int, 256>{});
+    return a.t == 1 && group <= a.tile && sizeof(float) * (floats + group * static_cast<size_t>(a.nk_max)) <= kMostLds / 2;
 }
 
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s) {
