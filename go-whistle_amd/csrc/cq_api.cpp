@@ -2378,7 +2378,7 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     const int qsize = value_size(a.type);
     a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stream * qsize) |
                 static_cast<uintptr_t>(a.q_row * qsize)) & (4 * qsize - 1)) == 0;
-    const bool in_ws = a.acc_out && (a.splits > 1 || !split_weights_in_lds(a, a.waves));
+    const bool in_ws = a.acc_out && a.nk_max > 0 && (a.splits > 1 || !split_weights_in_lds(a, a.waves));  // of 0 keys: no launch for them
     const long long rows = static_cast<long long>(a.batch) * a.t * a.heads;
     const long long wblocks = in_ws ? static_cast<long long>(a.batch) * a.c.kv_heads * ((a.nk_max + 255LL) / 256) : 0;
     if (lists * a.splits > grid_limit(1024) || 2 * rows > grid_limit(64) || wblocks > grid_limit(256))
