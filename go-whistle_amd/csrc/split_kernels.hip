@@ -663,6 +663,33 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                             for (int z = 0; z < PARTS; ++z) sc[s] = mfma_16x16x32<TYPE>(ka, qp[z][k][e], sc[s]);
                         }
             }
+            // An infinite key times a part of 0 is NaN: such logits again, in float32.
+            if constexpr (PARTS == 3 && TYPE != 3) {
+                bool nan = false;
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) nan |= sc[s][i] != sc[s][i];
+                if (__any(nan)) {
+                    f32x4 y[kSub];
+#pragma unroll
+                    for (int s = 0; s < kSub; ++s) y[s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e) {
+                            const float q = (piece_value<2>(qp[0][k][e / 8], e & 7) + piece_value<2>(qp[1][k][e / 8], e & 7)) +
+                                            piece_value<2>(qp[2][k][e / 8], e & 7);
+#pragma unroll
+                            for (int s = 0; s < kSub; ++s)
+                                y[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(kw[s][k], e), q, y[s], 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[s][i] = sc[s][i] != sc[s][i] ? y[s][i] : sc[s][i];
+                }
+            }
             if (jn < p.j1) load_keys(kw, rows);
             // past the last key values of 0, not that key's: a weight of 0 times an infinity
             if (TYPE != 3 && j + kTile > p.j1) {

@@ -516,8 +516,7 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * takes them for t = 1: {lo0, hi0, lo1, hi1}, ascending, disjoint and inside
  * [0, nk_max); others leave the stream's output as it was, and spans with no
  * key give zeros. A page outside the pool reads page 0. Rows outside the spans
- * may hold anything; an infinity among the keys of a span may make its logit
- * NaN (a float32 query meets 16-bit keys in three parts, some of them 0).
+ * may hold anything.
  * acc_out non-null ([batch][kv_heads][acc_cap], acc_cap >= nk_max): for
  * each row j of the spans, acc_out[j] = acc[j] (null: 0) + the sum over the
  * key head's query heads of their softmax weights; other entries are left

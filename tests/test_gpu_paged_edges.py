@@ -36,3 +36,35 @@ def test_no_keys_with_weights(group, name):
     c.attend_dev(out, q, torch.zeros(2, 4, dtype=torch.int32, device="cuda"), 0, 8.0, acc_out=acc)
     torch.cuda.synchronize()
     assert (out == 0).all() and (acc == 7).all()
+
+
+FORMS = [(1, 1, 1), (2, 2, 1), (300, 1, 1), (1, 6, 2), (3, 16, 1), (64, 16, 2), (2, 20, 1), (140, 4, 1)]
+
+
+@pytest.mark.parametrize("name", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("io", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("B,H,Hk", FORMS)
+@pytest.mark.parametrize("nk", [20, 500])
+def test_infinite_keys_have_the_logits_of_float32(name, io, B, H, Hk, nk):
+    # -inf where the query's coordinate is negative: a weight of 0, as the
+    # type's largest value gives, whatever the form the sizes choose. Queries
+    # whose coordinate takes one, two and three bfloat16 parts.
+    import torch
+
+    g, R, per = gen(nk + B), 16, -(-nk // 16)
+    for qk, vd in ((48, 64), (128, 128), (256, 144)):
+        k, v, _, _ = make_pool(g, B * per, R, Hk, qk, vd, name)
+        pages = torch.arange(B * per, device="cuda", dtype=torch.int32).view(B, per)
+        q = torch.randn(B, H, qk, generator=g, device="cuda")
+        q[..., 3] = torch.tensor([-1.0, -1.0 - 2.0 ** -9, -1.0 - 2.0 ** -20], device="cuda")[torch.arange(H, device="cuda") % 3]
+        q = q.to(getattr(torch, io))
+        spans, outs = i32([[0, nk, nk, nk]] * B), []
+        for x in (torch.finfo(k.dtype).max, float("inf")):
+            k.view(B, per * R, Hk, qk)[:, [0, nk // 2, nk - 1], :, 3] = x
+            outs.append(torch.empty(B, H, vd, device="cuda", dtype=q.dtype))
+            acc = torch.empty(B, Hk, nk, device="cuda")
+            needle.PagedKV(k, v, pages).attend_dev(outs[-1], q, spans, nk, 2.0, acc_out=acc)
+            outs.append(acc)
+        torch.cuda.synchronize()
+        assert torch.isfinite(outs[0]).all() and (outs[1][..., nk // 2] == 0).all()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
