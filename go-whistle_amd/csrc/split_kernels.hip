@@ -563,6 +563,8 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                         static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e + 1]))) << 16;
             } else {
 #pragma unroll
+                for (int e = 0; e < kPer; ++e) x[e] = __builtin_canonicalizef(x[e]);  // a NaN's mark in the upper half
+#pragma unroll
                 for (int z = 0; z < PARTS; ++z)
 #pragma unroll
                     for (int e = 0; e < kPer; e += 2) {

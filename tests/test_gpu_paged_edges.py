@@ -68,3 +68,26 @@ def test_infinite_keys_have_the_logits_of_float32(name, io, B, H, Hk, nk):
         torch.cuda.synchronize()
         assert torch.isfinite(outs[0]).all() and (outs[1][..., nk // 2] == 0).all()
         assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+
+
+@pytest.mark.parametrize("name", ["float32", "float16", "bfloat16", "i8"])
+@pytest.mark.parametrize("B,H,Hk", FORMS)
+@pytest.mark.parametrize("bits", [0x7f800001, 0x7fc00000, 0xff80ffff - (1 << 32), 0x7fffffff])
+def test_a_nan_in_a_query(name, B, H, Hk, bits):
+    # whatever its bits, its head is NaN and the others are as without it
+    import torch
+
+    g, nk, R = gen(B), 40, 16
+    k, v, ks, vs = make_pool(g, 3 * B, R, Hk, 80, 64, name)
+    k[..., 17] = -1  # a query of infinity there would find no key above -inf
+    c = needle.PagedKV(k, v, torch.arange(3 * B, device="cuda", dtype=torch.int32).view(B, 3), ks, vs)
+    q, outs = torch.randn(B, H, 80, generator=g, device="cuda"), []
+    for i in range(2):
+        if i:
+            q.view(torch.int32)[B - 1, H - 1, 17] = bits
+        outs.append(torch.empty(B, H, 64, device="cuda"))
+        c.attend_dev(outs[-1], q, i32([[0, nk, nk, nk]] * B), nk, 8.0)
+    torch.cuda.synchronize()
+    assert torch.isnan(outs[1][B - 1, H - 1]).all()
+    outs[0][B - 1, H - 1] = outs[1][B - 1, H - 1] = 0
+    assert torch.equal(outs[0], outs[1])
