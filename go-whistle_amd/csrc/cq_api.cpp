@@ -14,10 +14,12 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <memory>
 #include <mutex>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/cqhip.h"
@@ -2303,6 +2305,26 @@ static bool floats_overlap(const float *x, long long nx, const float *y, long lo
     return x && y && a < b + static_cast<uintptr_t>(ny) * 4 && b < a + static_cast<uintptr_t>(nx) * 4;
 }
 
+// Whether rows of `width` values at i*s0 + j*s1 (i < n0, j < n1) share no element.
+static bool rows_apart(long long width, long long n0, long long s0, long long n1, long long s1) {
+    s0 = std::llabs(s0);  // the differences take both signs
+    s1 = std::llabs(s1);
+    if (s0 < s1) {
+        std::swap(s0, s1);
+        std::swap(n0, n1);
+    }
+    if ((n0 > 1 && s0 < width) || (n1 > 1 && s1 < width)) return false;
+    if (n0 <= 1 || n1 <= 1) return true;
+    // |i s0 - j s1| < width for some i, j: rows of one dimension inside the other's
+    const __int128 reach = static_cast<__int128>(n1 - 1) * s1 + width;
+    for (__int128 i = 1; i < n0 && i * s0 < reach; ++i) {
+        const __int128 j = i * s0 / s1;  // the nearest below; the next one above
+        if (i * s0 - j * s1 < width) return false;
+        if (j + 1 < n1 && (j + 1) * s1 - i * s0 < width) return false;
+    }
+    return true;
+}
+
 static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_I8 ? 1 : 2; }
 
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
@@ -2416,6 +2438,9 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     if (!out || !q || !spans) return fail(CQ_ERR_MISUSE, "needle: attention with a nil operand");
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % value_size(type))
         return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
+    if (out_stride && !rows_apart(static_cast<long long>(heads) * c->vd, batch, out_stride, 1, 0))
+        return fail(CQ_ERR_MISUSE, "needle: attention outputs of one place (%lld values, %lld apart)",
+                    static_cast<long long>(heads) * c->vd, out_stride);
     if (acc != acc_out && floats_overlap(acc, static_cast<long long>(batch) * c->kv_heads * acc_cap, acc_out,
                                          static_cast<long long>(batch) * c->kv_heads * acc_cap))
         return fail(CQ_ERR_MISUSE, "needle: attention weights onto a part of themselves");
@@ -2513,8 +2538,14 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
         y.k_stream = y.k_row * frames;
         y.v_stream = y.v_row * frames;
     }
-    if ((batch > 1 && y.out_stream == 0) || (t > 1 && y.out_row == 0))
-        return fail(CQ_ERR_MISUSE, "needle: cross-attention outputs of one place");
+    if (2.0 * batch * t * heads > static_cast<double>(grid_limit(64)))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: cross-attention of %d streams of %d rows of %d heads", batch, t, heads);
+    // Of q_len[b] rows the host knows only that they are rows.
+    const long long width = static_cast<long long>(heads) * vd;
+    if (q_len ? !rows_apart(width, batch, y.out_stream, 1, 0) || !rows_apart(width, t, y.out_row, 1, 0)
+              : !rows_apart(width, batch, y.out_stream, t, y.out_row))
+        return fail(CQ_ERR_MISUSE, "needle: cross-attention outputs of one place (%lld values, rows %lld apart, streams %lld)",
+                    width, y.out_row, y.out_stream);
     if (((y.k_stream | y.k_row | y.k_head | y.v_stream | y.v_row | y.v_head) * size |
          static_cast<long long>(reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v))) & 15)
         return fail(CQ_ERR_MISUSE, "needle: cross-attention memories that are not aligned to 16 bytes");

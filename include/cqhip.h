@@ -511,7 +511,7 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * are q.k / scale (scale > 0); the softmax, its sums and the products' sums
  * are float32.
  * q and out hold values of `type`: batch streams of heads*qk (heads*vd),
- * q_stride (out_stride) elements apart (0: dense). Query head h reads key
+ * q_stride (out_stride, at least heads*vd) elements apart (0: dense). Query head h reads key
  * head h / (heads/kv_heads). spans are [batch][4] as kv_attend_int8_dev
  * takes them for t = 1: {lo0, hi0, lo1, hi1}, ascending, disjoint and inside
  * [0, nk_max); others leave the stream's output as it was, and spans with no
@@ -546,7 +546,8 @@ int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stri
 /* Where the rows of nd_cross_attend_dev's operands are, in elements: row i
  * of stream b's queries at b*q_stream + i*q_row (heads side by side, qk
  * apart), outputs likewise (vd apart); row j of memory m, key head h at
- * m*k_stream + j*k_row + h*k_head, values likewise. */
+ * m*k_stream + j*k_row + h*k_head, values likewise. The output rows that are
+ * written share no element. */
 typedef struct nd_cross_layout {
     long long q_stream, q_row, out_stream, out_row;
     long long k_stream, k_row, k_head, v_stream, v_row, v_head;

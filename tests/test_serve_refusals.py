@@ -134,3 +134,61 @@ def test_wrappers_refuse_host_tensors_and_shapes():
 def test_outputs_that_would_race(call, kw):
     with pytest.raises(CQPanic, match="onto|one place"):
         call(**kw)
+
+
+def layout(out_stream, out_row):
+    return CrossLayout(768, 256, out_stream, out_row, 1280, 128, 64, 1280, 128, 64)
+
+
+def spread(batch, t, out_stream, out_row, width=256):
+    """Whether batch x t rows of `width` elements share none, by counting."""
+    seen = set()
+    for b in range(batch):
+        for i in range(t):
+            at = b * out_stream + i * out_row
+            row = set(range(at, at + width))
+            if seen & row:
+                return False
+            seen |= row
+    return True
+
+
+@pytest.mark.parametrize("batch,t", [(1, 1), (1, 3), (2, 1), (2, 3), (3, 2), (4, 5)])
+def test_cross_attention_outputs_lie_apart(batch, t):
+    # heads * vd = 256; rows that lie apart get as far as the next check, of the memories' alignment
+    for out_stream in (0, 1, 255, 256, 257, 300, 511, 512, 600, 767, 768, 1000, 1024, 1279, 1280, 1536, -256, -700, 1 << 40):
+        for out_row in (0, 1, 255, 256, 257, 400, 512, 513, 768, 1024, 1300, -256, -512, 1 << 41):
+            y = layout(out_stream, out_row)
+            if spread(batch, t, out_stream, out_row):
+                with pytest.raises(CQPanic, match="aligned to 16 bytes"):
+                    cross(batch=batch, t=t, layout=y, k=P + 2)
+            else:
+                with pytest.raises(CQPanic, match="one place"):
+                    cross(batch=batch, t=t, layout=y)
+
+
+def test_outputs_of_ragged_rows_may_be_packed():
+    # rows of 256: with lengths only the first rows of two streams, and two rows of one, are known to be written
+    for out_stream, out_row, ok in ((300, 256, True), (256, 600, True), (255, 256, False), (0, 256, False), (768, 255, False)):
+        y = layout(out_stream, out_row)
+        with pytest.raises(CQPanic, match="aligned to 16 bytes" if ok else "one place"):
+            check(lib().nd_cross_attend_dev(P, P, P + 2, P, 1, ctypes.byref(y), 3, 3, 4, 2, 64, 64, 2, 10, P, None, None,
+                                            8.0, None))
+
+
+def test_attention_outputs_lie_apart():
+    def strided(stride, batch=2):
+        check(lib().kv_attend_paged_dev(cache(), P, stride, P, 0, 0, batch, 4, P, 64, 8.0, P, P + 4, 64, None))
+
+    for stride in (1, 64, 255, -255):  # 4 heads of 64
+        with pytest.raises(CQPanic, match="one place"):
+            strided(stride)
+    for stride, batch in ((0, 2), (256, 2), (257, 2), (-256, 2), (1, 1)):
+        with pytest.raises(CQPanic, match="onto"):  # the next check
+            strided(stride, batch)
+
+
+@pytest.mark.parametrize("batch,t", [((1 << 31) - 1, (1 << 31) - 1), (1 << 20, 1 << 10)])
+def test_more_outputs_than_a_launch(batch, t):
+    with pytest.raises(CQDeviceError):
+        cross(batch=batch, t=t, layout=layout(257, 258))
