@@ -2299,8 +2299,8 @@ static float attention_scale(float scale) {
     return scale > 0.0f && std::isfinite(scale) && std::isfinite(f) ? f : 0.0f;
 }
 
-// Whether two arrays of floats share memory.
-static bool floats_overlap(const float *x, long long nx, const float *y, long long ny) {
+// Whether two arrays of four-byte values share memory.
+static bool words_overlap(const void *x, long long nx, const void *y, long long ny) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
     return x && y && a < b + static_cast<uintptr_t>(ny) * 4 && b < a + static_cast<uintptr_t>(nx) * 4;
 }
@@ -2441,7 +2441,7 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
     if (out_stride && !rows_apart(static_cast<long long>(heads) * c->vd, batch, out_stride, 1, 0))
         return fail(CQ_ERR_MISUSE, "needle: attention outputs of one place (%lld values, %lld apart)",
                     static_cast<long long>(heads) * c->vd, out_stride);
-    if (acc != acc_out && floats_overlap(acc, static_cast<long long>(batch) * c->kv_heads * acc_cap, acc_out,
+    if (acc != acc_out && words_overlap(acc, static_cast<long long>(batch) * c->kv_heads * acc_cap, acc_out,
                                          static_cast<long long>(batch) * c->kv_heads * acc_cap))
         return fail(CQ_ERR_MISUSE, "needle: attention weights onto a part of themselves");
     const int size = value_size(c->type);
@@ -2482,8 +2482,10 @@ int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stri
     if (!len || !len_out || (nk_max > 0 && !acc) || (keep > 0 && (!dst_pages || !acc_out || !kept)))
         return fail(CQ_ERR_MISUSE, "needle: eviction with a nil operand");
     const long long lists = static_cast<long long>(batch) * c->kv_heads;
-    if (floats_overlap(acc, lists * acc_cap, acc_out, lists * acc_out_cap))
+    if (words_overlap(acc, lists * acc_cap, acc_out, lists * acc_out_cap))
         return fail(CQ_ERR_MISUSE, "needle: eviction onto its own weights");
+    if (len_out != len && words_overlap(len, batch, len_out, batch))
+        return fail(CQ_ERR_MISUSE, "needle: eviction lengths onto a part of themselves");
     if (keep > 0 && dst_pages == c->pages) return fail(CQ_ERR_MISUSE, "needle: eviction onto its own pages");
     const int pieces = (c->qk + c->vd) * value_size(c->type) / 16;
     if (static_cast<long long>(batch) * c->kv_heads > grid_limit(1024) ||

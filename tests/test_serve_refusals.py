@@ -192,3 +192,13 @@ def test_attention_outputs_lie_apart():
 def test_more_outputs_than_a_launch(batch, t):
     with pytest.raises(CQDeviceError):
         cross(batch=batch, t=t, layout=layout(257, 258))
+
+
+@pytest.mark.parametrize("shift", [-4, 4])
+def test_lengths_in_part_onto_themselves(shift):
+    # a copy would read one stream's new length as another's old one
+    with pytest.raises(CQPanic, match="onto a part"):
+        evict(out=64 * P, ln=4 * P, ln_out=4 * P + shift)
+    for ln_out in (4 * P, 4 * P + 2 * shift):  # the next check
+        with pytest.raises(CQPanic, match="own pages"):
+            evict(c=cache(pages=3 * P), dst=3 * P, out=64 * P, ln=4 * P, ln_out=ln_out)
