@@ -245,6 +245,15 @@ def _want(t, what, shape, dtype, index, dense=True):
     raise CQPanic(f"needle: {what} that is not contiguous")
 
 
+_INT = 0x7FFFFFFF  # the calls' sizes are C ints, which ctypes cuts to 32 bits
+
+
+def _sizes(what, *sizes):
+    for n in sizes:
+        if not 0 <= n <= _INT:
+            raise CQPanic(f"needle: {what} of {n}")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -283,7 +292,8 @@ class PagedKV:
                 _want(s, what, k.shape[:3], _f32, self.index)
         self.k, self.v, self.ks, self.vs, self.pages = k, v, ks, vs, pages
         self.streams, self.kv_heads, self.qk, self.vd = pages.shape[0], k.shape[2], k.shape[3], v.shape[3]
-        self.device, self.cap = k.device, pages.shape[1] * k.shape[1]
+        _sizes("a paged cache", *pages.shape, *k.shape, v.shape[3])
+        self.device, self.cap = k.device, min(pages.shape[1] * k.shape[1], _INT)
         self._c = KvPaged(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), pages.data_ptr(), self.type, k.shape[2],
                           k.shape[3], v.shape[3], pages.shape[1], k.shape[1], k.shape[0])
         self._ref = ctypes.byref(self._c)
@@ -314,6 +324,8 @@ class PagedKV:
             _want(rows, "row counts", (self.streams,), _i32, self.index)
         if cap is None:
             cap = self.cap
+        if t > _INT or not 0 <= cap <= _INT:
+            _sizes("append", t, cap)
         acc_cap = self._acc(acc, "weights", cap) if acc is not None else 0
         _call(lib().kv_append_paged_dev, self.index, self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
               code, self.streams, t, _ptr(rows), pos.data_ptr(), cap, _ptr(acc), acc_cap)
@@ -329,6 +341,8 @@ class PagedKV:
         _want(q, "queries", (self.streams, heads, self.qk), q.dtype, self.index)
         _want(out, "outputs", (self.streams, heads, self.vd), q.dtype, self.index)
         _want(spans, "spans", (self.streams, 4), _i32, self.index)
+        if not 0 <= nk_max <= _INT:
+            _sizes("attention over keys", nk_max)
         acc_cap = 0
         if acc_out is not None:
             acc_cap = self._acc(acc_out, "weights", nk_max)
@@ -353,6 +367,7 @@ class PagedKV:
         _want(dst_pages, "page table", (self.streams, width), _i32, self.index)
         _want(length, "lengths", (self.streams,), _i32, self.index)
         _want(length_out, "lengths", (self.streams,), _i32, self.index)
+        _sizes("eviction", nk_max, keep, width, sink, recent)
         acc_cap, out_cap = self._acc(acc, "weights", nk_max), self._acc(acc_out, "weights", keep)
         _call(lib().kv_evict_paged_dev, self.index, self._ref, dst_pages.data_ptr(), width,
               acc.data_ptr(), acc_cap, acc_out.data_ptr(), out_cap, length.data_ptr(), length_out.data_ptr(),
@@ -373,6 +388,8 @@ def cross_attend_dev(out, q, k, v, scale, q_len=None, k_len=None, index=None):
     B, t, heads, qk = qs
     M, frames, kv_heads, _ = ks
     vd, code, dtype, dev = vs[3], _type(q, "queries"), q.dtype, _index(q, "queries")
+    if max(B, t, M, frames) > _INT:
+        _sizes("cross-attention", B, t, M, frames)
     _want(out, "outputs", (B, t, heads, vd), dtype, dev, False)
     _want(k, "keys", (M, frames, kv_heads, qk), dtype, dev, False)
     _want(v, "values", (M, frames, kv_heads, vd), dtype, dev, False)
@@ -402,6 +419,8 @@ def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
     if len(shape) != 2:
         raise CQPanic(f"needle: logits of shape {tuple(shape)}, not rows of them")
     rows, n = shape
+    if rows > _INT or n > _INT:
+        _sizes("logits", rows, n)
     code, dev = _type(logits, "logits"), _index(logits, "logits")
     if n > 1 and stride[1] != 1:
         raise CQPanic("needle: logits whose rows are not contiguous")

@@ -91,3 +91,50 @@ def test_a_nan_in_a_query(name, B, H, Hk, bits):
     assert torch.isnan(outs[1][B - 1, H - 1]).all()
     outs[0][B - 1, H - 1] = outs[1][B - 1, H - 1] = 0
     assert torch.equal(outs[0], outs[1])
+
+
+def test_a_table_of_more_rows_than_an_int():
+    # 2^20 entries of pages of 4096 rows: by default all of them may be appended to
+    import torch
+
+    k, v, _, _ = make_pool(gen(5), 3, 4096, 1, 16, 16, "float16")
+    k.zero_(), v.zero_()
+    pages = torch.zeros(1, 1 << 20, dtype=torch.int32, device="cuda")
+    pages[0, 1], pages[0, (1 << 19) - 1] = 2, 1
+    c = needle.PagedKV(k, v, pages)
+    one = torch.ones(1, 1, 1, 16, device="cuda")
+    c.append_dev(one, one, i32([4099]))
+    c.append_dev(2 * one, 2 * one, i32([(1 << 31) - 2]))
+    torch.cuda.synchronize()
+    assert (k[2, 3] == 1).all() and (v[1, 4094] == 2).all() and k.count_nonzero() == 32 and v.count_nonzero() == 32
+
+
+def test_sizes_past_an_int_are_refused():
+    import torch
+
+    from go_whistle_amd._lib import CQPanic
+
+    far = 1 << 32
+    k, v, _, _ = make_pool(gen(6), 4, 16, 2, 64, 64, "float32")
+    c = needle.PagedKV(k, v, i32([[0, 1]]))
+    q, spans, out = torch.ones(1, 2, 64, device="cuda"), i32([[0, 0, 0, 3]]), torch.full((1, 2, 64), 3.0, device="cuda")
+    for nk in (far + 5, far, -far + 5, 1 << 31):
+        with pytest.raises(CQPanic):
+            c.attend_dev(out, q, spans, nk, 8.0)
+        with pytest.raises(CQPanic):
+            c.append_dev(q.view(1, 1, 2, 64), q.view(1, 1, 2, 64), i32([0]), cap=nk)
+    acc, kept = torch.zeros(1, 2, 32, device="cuda"), torch.full((1, 2, 8), 7, dtype=torch.int32, device="cuda")
+    for more in (dict(sink=far), dict(recent=far + 1), dict(nk_max=far + 3), dict(sink=-far)):
+        with pytest.raises(CQPanic):
+            c.evict_dev(i32([[2, 3]]), acc, acc.clone(), i32([20]), i32([0]), kept, **{"nk_max": 20, **more})
+    rows = torch.ones(1, 1, 2, 64, device="cuda")
+    many = rows.expand(1, far + 3, 2, 64)
+    with pytest.raises(CQPanic):
+        needle.cross_attend_dev(out.view(1, 1, 2, 64), rows, many, many, 8.0)
+    with pytest.raises(CQPanic):
+        needle.cross_attend_dev(many, many, rows, rows, 8.0)
+    ent = torch.full((1,), 3.0, device="cuda")
+    with pytest.raises(CQPanic):
+        needle.logprobs_dev(torch.empty(1, far + 8, dtype=torch.float16, device="cuda"), ent=ent)
+    torch.cuda.synchronize()
+    assert (out == 3).all() and (ent == 3).all() and (kept == 7).all()
