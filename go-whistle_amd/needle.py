@@ -276,7 +276,8 @@ class PagedKV:
     float32, float16, bfloat16 or int8 (with scales ks, vs [pages, page_rows,
     kv_heads] float32), read through the page table `pages` [streams,
     pages per stream] int32. The tensors stay the caller's: a changed table
-    entry or a fork's copied table is seen by the next call."""
+    entry or a fork's copied table is seen by the next call. Another tensor
+    takes another PagedKV."""
 
     def __init__(self, k, v, pages, ks=None, vs=None):
         if k.dim() != 4 or v.dim() != 4 or pages.dim() != 2:
@@ -290,13 +291,16 @@ class PagedKV:
         for s, what in ((ks, "key scales"), (vs, "value scales")):
             if s is not None:
                 _want(s, what, k.shape[:3], _f32, self.index)
-        self.k, self.v, self.ks, self.vs, self.pages = k, v, ks, vs, pages
+        self._tensors = k, v, ks, vs, pages
         self.streams, self.kv_heads, self.qk, self.vd = pages.shape[0], k.shape[2], k.shape[3], v.shape[3]
         _sizes("a paged cache", *pages.shape, *k.shape, v.shape[3])
         self.device, self.cap = k.device, min(pages.shape[1] * k.shape[1], _INT)
         self._c = KvPaged(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), pages.data_ptr(), self.type, k.shape[2],
                           k.shape[3], v.shape[3], pages.shape[1], k.shape[1], k.shape[0])
         self._ref = ctypes.byref(self._c)
+
+    # Read-only: the calls go by the addresses that _c took.
+    k, v, ks, vs, pages = (property(lambda self, i=i: self._tensors[i]) for i in range(5))
 
     def _acc(self, acc, what, rows):
         cap = acc.shape[-1] if acc.dim() else 0

@@ -297,3 +297,25 @@ def test_log_probabilities_past_32_bits(name, n):
     assert (outs[0][0].double() - want.gather(1, tokens.long().view(3, 1)).view(3)).abs().max() <= slack
     assert (outs[0][3].double() - want.gather(1, best)).abs().max() <= slack
     assert (outs[0][1].double() + (want.exp() * want).sum(-1)).abs().max() <= 16 * slack
+
+
+def test_the_tensors_of_a_cache_stay():
+    # the calls hold their addresses: another table or pool is another PagedKV, not an attribute
+    import torch
+
+    k, v, ks, vs = make_pool(gen(8), 4, 16, 2, 64, 64, "i8")
+    c = needle.PagedKV(k, v, i32([[0, 1]]), ks, vs)
+    assert c.k is k and c.v is v and c.ks is ks and c.vs is vs
+    for name in ("k", "v", "ks", "vs", "pages"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, torch.zeros_like(getattr(c, name)))
+    q, outs = torch.randn(1, 2, 64, generator=gen(9), device="cuda"), []
+    for change in (None, lambda: c.pages.copy_(i32([[3, 2]]))):  # an entry that changes is seen
+        if change:
+            change()
+        outs.append(torch.empty_like(q))
+        c.attend_dev(outs[-1], q, i32([[0, 0, 0, 20]]), 20, 8.0)
+    other = torch.empty_like(q)
+    needle.PagedKV(k, v, i32([[3, 2]]), ks, vs).attend_dev(other, q, i32([[0, 0, 0, 20]]), 20, 8.0)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], other) and not torch.equal(outs[0], other)
