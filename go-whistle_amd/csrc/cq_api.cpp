@@ -2364,15 +2364,26 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     a.group = a.heads / a.c.kv_heads;
     const long long cols = static_cast<long long>(a.t) * a.group;
     const int cus = device_info().cus;
-    // 16-bit memories take the matrix form from two columns on (64 streams of
-    // 1500 frames, 8 heads of 128 over 2: 26.9 us against 33.2 at 4 columns,
-    // 27.6 against 35.2 at 16; of one column 82 against 89 at best, 47 against
-    // 39 at worst). float32 ones, whose matrix instruction has the rate of the
+    // 16-bit memories take the matrix form from two columns on (heads of 128, 8
+    // over 2, of 64 streams of 1500 frames: 28.1 us against 27.7 of the split
+    // form at 4 columns, 30.4 against 35.4 at 32, 33.5 against 64 at 64; of
+    // one stream 13.6 against 21.3; one column 82 against 89 at best, 47 against
+    // 39 at worst), but not up to 16 columns of heads of 64 and less where its
+    // workgroups would take lists of 256 frames and more whole: the second parts
+    // of the weights, which the split form does not need, are then its time
+    // (heads of 64, 4 columns of 8 key heads: 32 streams of 1500 frames 45.1 us
+    // against 23.8, 64 streams 47.1 against 43.6, 128 of 375 31.3 against 26.3,
+    // one of 375 10.6 against 9.4; 16 columns of 32 streams 45.1 against 24.6;
+    // of 200 frames 8.5 against 8.7, of 60 5.3 against 7.0; where the matrix
+    // form splits the lists, one of 1500 11.7 against 14.7).
+    // float32 ones, whose matrix instruction has the rate of the
     // split form's, once its blocks of 32 columns give three in two CUs one (16 x
     // 448 rows, 8 heads of 64: 230 us against 342; 4 x 448 of 8 over 2, 448 blocks:
     // 73 against 93; 1 x 448, 112 blocks: 34 against 28; 16 x 32, a block a
     // list: 71 against 31).
-    const bool many = !a.spans && (a.type != ND_F32 ? cols > 1
+    const bool lists_fill = 2LL * a.batch * a.c.kv_heads >= cus;
+    const bool few = std::max(a.c.qk, a.c.vd) <= 64 && a.nk_max >= 256 && (lists_fill ? cols <= 16 : cols <= 8 && a.nk_max < 512);
+    const bool many = !a.spans && (a.type != ND_F32 ? cols > 1 && !few
                                                     : cols > 64 && (cols + 31) / 32 * a.batch * a.c.kv_heads >= 3LL * cus / 2);
     a.tile = split_tile_columns(a, cus);
     const int wg_cols = many ? cross_workgroup_columns(a, cus) : a.tile;

@@ -145,3 +145,39 @@ def test_outputs_stay_between_the_values(name, size):
     assert (out.float() >= lo - slack).all() and (out.float() <= hi + slack).all()
     mean = v.double().mean(1, keepdim=True)
     assert (out[:, 1::3].double() - mean).abs().max() <= 2 * half_ulp(dt) * mean.abs().max() + F * 2.0 ** -24
+
+
+@pytest.mark.parametrize("name", HALVES)
+@pytest.mark.parametrize("B,t,H,Hk,qk,vd,F", [(1, 8, 4, 4, 64, 64, 256), (2, 1, 8, 1, 48, 64, 300), (3, 4, 4, 2, 16, 16, 511),
+                                              (40, 3, 4, 4, 64, 48, 290), (70, 16, 2, 2, 32, 64, 257), (70, 2, 16, 2, 64, 64, 700),
+                                              (33, 5, 12, 4, 64, 64, 1030)])
+def test_few_rows_of_narrow_heads(name, B, t, H, Hk, qk, vd, F):
+    # lists taken whole by the split form: its weights are float32. Ragged rows
+    # and memories, shared and missing ones, rows inside wider ones.
+    import torch
+
+    g, dt = gen(B + F), getattr(torch, name)
+    M = max(1, B // 2)
+    q = torch.randn(B, t, H * qk + 8, generator=g, device="cuda").to(dt)[..., 5:5 + H * qk].unflatten(2, (H, qk))
+    k, v = (torch.randn(M, Hk, F, w, generator=g, device="cuda").to(dt).transpose(1, 2) for w in (qk, vd))
+    wide = torch.full((B, t, H * vd + 3), 7.0, device="cuda", dtype=dt)
+    out = wide[..., 1:1 + H * vd].unflatten(2, (H, vd))
+    q_len = [(b * 5) % (t + 2) - (b == 4) for b in range(B)]
+    q_len[0] = t
+    k_len = [F - (m * 37) % (F + 1) for m in range(M)]
+    index = [(b * 3) % (M + (B > 8)) for b in range(B)]
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    needle.cross_attend_dev(out, q, k, v, math.sqrt(qk), q_len=dev(q_len), k_len=dev(k_len), index=dev(index))
+    torch.cuda.synchronize()
+    assert (wide[..., 0] == 7).all() and (wide[..., 1 + H * vd:] == 7).all()
+    ho, hq, hk, hv = (host(x).astype(np.float64) for x in (out, q, k, v))
+    pick = np.random.default_rng(t)
+    for b in range(B):
+        n, m = min(max(q_len[b], 0), t), index[b]
+        n = n if m < M else 0
+        assert (ho[b, n:] == 7).all(), b
+        for i in {0, n - 1} if n else ():
+            for h in pick.integers(0, H, 3).tolist():
+                o, bound, _, _ = attend64(hq[b, i, h], hk[m, :k_len[m], h // (H // Hk)], hv[m, :k_len[m], h // (H // Hk)],
+                                          math.sqrt(qk), dt)
+                assert (np.abs(ho[b, i, h] - o) <= bound).all(), (b, i, h)
