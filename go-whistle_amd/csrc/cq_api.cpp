@@ -2391,9 +2391,9 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     if (many) {
         // The matrix form's partials cost more than idle CUs as long as the
         // lists give half of the CUs a workgroup (8 x 448 rows of 8 heads of 48
-        // over 2, 1500 frames, 224 workgroups: 31.9 us whole, 44.1 in two
-        // parts; 2 x 448 rows of 8 heads of 64, 64 workgroups: 20.9 in four,
-        // 24.1 in two).
+        // and 64 over 2, 1500 frames, 224 workgroups: 37.7 us whole, 50.6 in two
+        // parts; 2 x 448 rows of 8 heads of 64, 64 workgroups: 21.5 in four,
+        // 25.7 in two, 31.1 whole).
         a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({cus / lists, a.nk_max / 256, 64})));
     } else {
         // Eight wavefronts a workgroup, four to one as the lists alone give a

@@ -547,7 +547,7 @@ bool split_weights_in_lds(const SplitArgs &a, int waves);  // a list's logits fi
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);
 // The parts of every output row joined.
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s);
-// The same attention of many columns to 16-bit memories of the queries' type
+// The same attention of many columns to memories of the queries' type
 // (cross_kernels.hip); the columns a workgroup takes.
 int cross_workgroup_columns(const SplitArgs &a, int cus);
 hipError_t launch_cross_attend(const SplitArgs &a, int cus, hipStream_t s);

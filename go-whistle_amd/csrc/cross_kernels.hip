@@ -1,5 +1,5 @@
-// gfx950 cross-attention of many query rows to 16-bit memories
-// (nd_cross_attend_dev).
+// gfx950 cross-attention of many query rows (nd_cross_attend_dev): 16-bit
+// memories (cross_attend_kernel), and float32 ones (cross_attend_f32_kernel).
 //
 // Per (stream, key head) the query columns are the group's heads times the
 // query rows, a wavefront holding 32 or 64 of them. Keys and values pass
@@ -123,7 +123,8 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 // The stream with the place-th longest memory (up to 64 streams). A launch of
 // several rounds of workgroups takes the long ones first, so that none
-// begins as the last ones end.
+// begins as the last ones end (40 ragged streams, 16 heads of 128 over 4: 109 ->
+// 103 us).
 __device__ __forceinline__ int longest_first(const SplitArgs &a, int place, int lane) {
     int n = -1;
     if (lane < a.batch) {
@@ -636,11 +637,11 @@ hipError_t launch_cross_type(const SplitArgs &a, int cols, int cb, int aligned, 
 }
 
 // 64 columns a wavefront for heads of up to 64 once they still give every CU
-// a workgroup: half the LDS reads an operation (64 x 448 rows to 1500 frames
-// of 8 heads of 64: 143 against 155 us; 2 x 448 rows, 32 workgroups of 64
-// columns a wavefront or 64 of 32: 24.0 against 20.9). Heads of 128 lose by
-// it (290 against 230 us for 40 x 333 rows): 64 columns take the registers
-// of a second wavefront a SIMD.
+// a workgroup: half the LDS reads an operation (448 rows to 1500 frames, 8
+// heads of 64: 64 streams 156 us against 162 with 32 columns, 32 streams 80
+// against 86, 16, just a workgroup a CU, 49 against 47; 2 streams, 32 workgroups
+// of 64 columns a wavefront or 64 of 32: 25.5 against 21.7). Heads of 128 keep
+// 32: 64 columns take the registers of a second wavefront a SIMD.
 int column_blocks(const SplitArgs &a, int cus) {
     const long long cols = static_cast<long long>(a.t) * (a.heads / a.c.kv_heads), wide = kXWaves * 64;
     return a.type != 0 && std::max(a.c.qk, a.c.vd) <= 64 && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= cus ? 2 : 1;

@@ -216,6 +216,11 @@ __device__ __forceinline__ void copy_kept(const EvictArgs &a, int b, int h, cons
 // highest bits down: bits stay set if at least `keep` keys reach the value
 // with them (a histogram's atomics would meet in the few exponents that weights
 // have: 30 us for 448 rows), until exactly `keep` do.
+// Two bits a turn as long as three counts of a wavefront fit one word (eight
+// rows a thread, 8192 rows), then one. To keep 2048 rows of 128 bfloat16 values,
+// one list and 32 of them, both launches: of 8192 rows 17.9 and 20.6 us, of
+// 20,000 26.7 and 37.3, of 32,768 31.8 and 39.4; of 65,000, whose keys are read
+// again each turn, 155 and 300.
 // Then one pass in row order writes the rows above the key, and the lowest of
 // those equal to it. Integer counts throughout: the same rows in every run.
 // COPY: the workgroup also copies them, and a stream's first one writes its
@@ -362,9 +367,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a, 
 // same piece of its value row, of two rows half the budget apart (each
 // destination row is written whole by its neighbours): four loads in flight
 // behind one chain of row, page and pool. The stores go past the L2 to memory at once, not at the
-// launch's end, when the L2s give up their dirty lines (270 MB 53.5 -> 42 us,
-// 0.8 MB 8.6 -> 3.3 us; the appends and the attention's narrower stores gain
-// nothing by it or lose). The scales of int8 rows ride with the first piece.
+// launch's end, when the L2s give up their dirty lines (16 streams of up to 8192
+// rows to 2048, 8 heads of 128, 237 MB read and written: both launches 57.7 ->
+// 52.2 us, this one 44 to 46, 5.2 TB/s, under the profiler; the appends and the
+// attention's narrower stores gain nothing by it or lose). The scales of int8
+// rows ride with the first piece.
 // Also the streams' new lengths.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a, int kpieces, int vpieces, int half_rows,
                                                          long long total) {
@@ -436,7 +443,7 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     // One launch for small lists, a row a thread, unless the new lengths lie
     // over the old ones, which every workgroup of a stream reads (448 rows to
     // 256 of heads of 48 and 64 float16 values, 3584 pieces: 8 streams of 2 heads
-    // 11.0 -> 10.1 us; 64 of 8 heads of 64, 4096 pieces: 20.3 -> 15.4; 1000 rows,
+    // 12.9 -> 11.5 us; 8 of 8 heads of 64, 4096 pieces: 11.5 -> 10.0; 64 of them: 20.3 -> 15.4; 1000 rows,
     // 8192 pieces: 13.0 -> 12.4; of 2000, 8000 pieces: 13.3 -> 14.6, 32,000: 12.4
     // -> 21.3).
     if (apart && a.nk_max <= kSelThreads && static_cast<long long>(a.keep) * (kpieces + vpieces) <= kCopyPieces) {

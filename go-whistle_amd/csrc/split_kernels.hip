@@ -29,7 +29,9 @@
 //     instead, eight elements at a time: with the query as it is where it has
 //     the keys' type, else as the exact sum of three bfloat16 parts (24 bits).
 //     The products are exact either way; the eight float32 instructions that
-//     one to three of them replace left the matrix pipe 57% busy at 4.6 TB/s.
+//     one to three of them replace kept the matrix pipe 57% busy (4 streams of
+//     65,000 bfloat16 keys 220 -> 212 us). An infinite key times a part of 0 is
+//     NaN: logits that are, are computed again in float32.
 //   O = V^T P: the register P_i is the B operand as it lies (contraction
 //     index c is key 4c + i), and A is a lane's piece of value row 4c + i,
 //     elements e of 16 lanes the rows of the e-th MFMA. m and l belong to

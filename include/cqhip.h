@@ -538,7 +538,9 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
  * numbers, -1 past the last; acc_out ([batch][kv_heads][acc_out_cap],
  * acc_out_cap >= keep, apart from acc) their weights; len_out[b] = min(len[b],
  * keep) (len_out may be len, or lies apart from it). A stream whose len is
- * outside [0, nk_max] is left as it was, len_out too. sink + recent <= keep. */
+ * outside [0, nk_max] is left as it was, len_out too. A source page outside the
+ * pool reads page 0, and rows of a destination page outside it are not
+ * written. sink + recent <= keep. */
 int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
                        long long acc_cap, float *acc_out, long long acc_out_cap, const int32_t *len, int32_t *len_out,
                        int32_t *kept, int batch, int nk_max, int keep, int sink, int recent, void *stream);
