@@ -2559,7 +2559,10 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
               : !rows_apart(width, batch, y.out_stream, t, y.out_row))
         return fail(CQ_ERR_MISUSE, "needle: cross-attention outputs of one place (%lld values, rows %lld apart, streams %lld)",
                     width, y.out_row, y.out_stream);
-    if (((y.k_stream | y.k_row | y.k_head | y.v_stream | y.v_row | y.v_head) * size |
+    // strides of one row, frame or head are never taken
+    const long long strides = (memories > 1 ? y.k_stream | y.v_stream : 0) | (frames > 1 ? y.k_row | y.v_row : 0) |
+                              (kv_heads > 1 ? y.k_head | y.v_head : 0);
+    if ((strides * size |
          static_cast<long long>(reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v))) & 15)
         return fail(CQ_ERR_MISUSE, "needle: cross-attention memories that are not aligned to 16 bytes");
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % size)

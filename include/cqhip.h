@@ -565,10 +565,10 @@ typedef struct nd_cross_layout {
  * outputs as they were; an empty memory gives zeros. Query head h reads key
  * head h / (heads/kv_heads). layout null: dense [batch][t][heads][width] and
  * [memories][frames][kv_heads][width]. qk and vd are multiples of 16 up to
- * 256; k, v and their strides are multiples of 16 bytes. ND_F32 products are
- * float32; with 16-bit types the products take them as they are, and the softmax
- * weights are float32 or, for many rows, two parts of the type (16 bits in
- * bfloat16, 22 in float16); sums and softmax are float32. */
+ * 256; k, v and their strides (of dimensions past 1) are multiples of 16 bytes.
+ * ND_F32 products are float32; with 16-bit types the products take them as they
+ * are, and the softmax weights are float32 or, for many rows, two parts of the
+ * type (16 bits in bfloat16, 22 in float16); sums and softmax are float32. */
 int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
                         const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
                         int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,

@@ -55,12 +55,12 @@ def test_weights_hold_more_than_their_type(name, H, Hk, qk, vd, t, F):
 
 @pytest.mark.parametrize("name", ["float32"] + HALVES)
 @pytest.mark.parametrize("qk,vd", [(64, 64), (48, 64), (128, 80), (256, 256)])
-@pytest.mark.parametrize("B,t", [(1, 1), (2, 2), (2, 140), (70, 33)])
-def test_infinite_values_of_equal_weights(name, qk, vd, B, t):
+@pytest.mark.parametrize("B,t,F", [(1, 1, 100), (2, 2, 100), (2, 140, 100), (70, 33, 100), (2, 2, 300), (70, 3, 300), (1, 9, 3000)])
+def test_infinite_values_of_equal_weights(name, qk, vd, B, t, F):
     # weights of exactly 1 before the sum: one part holds them, the second is 0
     import torch
 
-    g, dt, F, H = gen(qk + t), getattr(torch, name), 100, 2
+    g, dt, H = gen(qk + t), getattr(torch, name), 2
     q = torch.zeros(B, t, H, qk, device="cuda", dtype=dt)
     k, v = (torch.randn(B, F, H, w, generator=g, device="cuda").to(dt) for w in (qk, vd))
     v[:, 3, :, 5], v[:, 77, :, 9] = float("inf"), -float("inf")

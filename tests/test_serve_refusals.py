@@ -202,3 +202,15 @@ def test_lengths_in_part_onto_themselves(shift):
     for ln_out in (4 * P, 4 * P + 2 * shift):  # the next check
         with pytest.raises(CQPanic, match="own pages"):
             evict(c=cache(pages=3 * P), dst=3 * P, out=64 * P, ln=4 * P, ln_out=ln_out)
+
+
+@pytest.mark.parametrize("name", ["k_stream", "v_stream", "k_row", "v_row", "k_head", "v_head"])
+def test_strides_of_single_memories_frames_and_heads(name):
+    # a stride that leads nowhere may be anything, as torch's strides of dimensions of 1 are
+    y = CrossLayout(256, 256, 256, 256, 1280, 128, 64, 1280, 128, 64)
+    setattr(y, name, 63)
+    single = {"stream": dict(memories=1), "row": dict(frames=1), "head": dict(kv_heads=1)}[name.split("_")[1]]
+    with pytest.raises(CQPanic, match="aligned to their type"):  # the next check
+        cross(layout=y, batch=1, t=1, q=P + 1, **single)
+    with pytest.raises(CQPanic, match="aligned to 16 bytes"):
+        cross(layout=y, batch=1, t=1, q=P + 1)
