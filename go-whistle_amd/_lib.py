@@ -6,7 +6,7 @@ here, loudly; nothing falls back to a CPU path.
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int8, c_int32, c_longlong, c_size_t, c_uint8, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int8, c_int32, c_longlong, c_size_t, c_uint8, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libcqhip.so")
@@ -27,6 +27,13 @@ class CrossLayout(Structure):
 
     _fields_ = [(n, c_longlong) for n in ("q_stream", "q_row", "out_stream", "out_row", "k_stream", "k_row", "k_head",
                                           "v_stream", "v_row", "v_head")]
+
+
+class HeadsLayout(Structure):
+    """nd_heads_layout (include/cqhip.h)."""
+
+    _fields_ = [(n, c_longlong) for n in ("q_stream", "q_row", "k_stream", "k_row", "q_out_stream", "q_out_row",
+                                          "k_out_stream", "k_out_row")]
 
 
 # Every symbol include/cqhip.h declares, with (restype, argtypes).
@@ -137,6 +144,17 @@ SIGNATURES = {
     "nd_cross_attend_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
                                     c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float,
                                     c_void_p]),
+    "kv_read_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong,
+                                  c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "kv_attend_rows_paged_dev": (c_int, [POINTER(KvPaged), c_void_p, c_longlong, c_longlong, c_void_p, c_longlong,
+                                         c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                                         c_int, c_float, c_void_p]),
+    "nd_qk_norm_rope_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
+                                    c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                    c_void_p]),
+    "nd_verify_drafts_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p,
+                                     c_longlong, c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_double, c_void_p]),
     "nd_logprobs_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
                                 c_void_p, c_int, c_void_p]),
 }

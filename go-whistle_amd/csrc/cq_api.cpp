@@ -2272,7 +2272,8 @@ int kv_append_rope_dev(int8_t *q, float *s, const float *x, int batch, int cols,
 // The parts of a paged cache's description that every call checks.
 static int paged_args(const kv_paged *c, int batch, int rows, const char *what, PagedArgs &p) {
     if (!c) return fail(CQ_ERR_MISUSE, "needle: %s without a cache", what);
-    if (c->type < ND_F32 || c->type > ND_I8) return fail(CQ_ERR_MISUSE, "needle: cache type %d", c->type);
+    const bool by_page = c->type == ND_I8_PAGES || c->type == ND_E4M3_PAGES;
+    if (!by_page && (c->type < ND_F32 || c->type > ND_I8)) return fail(CQ_ERR_MISUSE, "needle: cache type %d", c->type);
     if (c->kv_heads <= 0) return fail(CQ_ERR_MISUSE, "needle: a cache of %d heads", c->kv_heads);
     if (!split_widths_ok(c->qk, c->vd))
         return fail(CQ_ERR_UNSUPPORTED, "needle: cache heads of %d and %d (multiples of 16 up to 256)", c->qk, c->vd);
@@ -2282,14 +2283,15 @@ static int paged_args(const kv_paged *c, int batch, int rows, const char *what, 
                     c->page_rows, rows, c->pool_pages);
     if (static_cast<long long>(c->pool_pages) * c->page_rows > 0x7fffffffLL)
         return fail(CQ_ERR_UNSUPPORTED, "needle: a pool of %d pages of %d rows", c->pool_pages, c->page_rows);
-    if (batch > 0 && (!c->k || !c->v || (rows > 0 && !c->pages) || (c->type == ND_I8 && (!c->ks || !c->vs))))
+    if (batch > 0 && (!c->k || !c->v || (rows > 0 && !c->pages) || ((c->type == ND_I8 || by_page) && (!c->ks || !c->vs))))
         return fail(CQ_ERR_MISUSE, "needle: %s with a nil cache array", what);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
         return fail(CQ_ERR_MISUSE, "needle: cache pools that are not aligned to 16 bytes");
     int shift = 0;
     while ((1 << shift) < c->page_rows) ++shift;
     p = PagedArgs{static_cast<unsigned char *>(c->k), static_cast<unsigned char *>(c->v), c->ks, c->vs, c->pages,
-                  c->type, c->kv_heads, c->qk, c->vd, c->page_stride, shift, c->pool_pages};
+                  c->type == ND_E4M3_PAGES ? 4 : by_page ? 3 : c->type, c->kv_heads, c->qk, c->vd, c->page_stride, shift,
+                  c->pool_pages, by_page ? shift : 0};
     return CQ_OK;
 }
 
@@ -2325,7 +2327,7 @@ static bool rows_apart(long long width, long long n0, long long s0, long long n1
     return true;
 }
 
-static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_I8 ? 1 : 2; }
+static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_F16 || type == ND_BF16 ? 2 : 1; }
 
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
                         long long v_stream, long long v_row, int type, int batch, int t, const int32_t *rows,
@@ -2355,7 +2357,121 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
     a.pos = pos;
     a.acc = acc;
     a.acc_cap = acc_cap;
+    if (c->type == ND_I8_PAGES || c->type == ND_E4M3_PAGES) {
+        const long long each = (static_cast<long long>(t) + c->page_rows - 2) / c->page_rows + 1;  // pages of a stream
+        if (2.0 * batch * c->kv_heads * each > static_cast<double>(grid_limit(512)))
+            return fail(CQ_ERR_UNSUPPORTED, "needle: append of %d x %d rows of %d heads", batch, t, c->kv_heads);
+        HIP_TRY(launch_page8_append(a, static_cast<hipStream_t>(stream)), "paged append launch");
+        return CQ_OK;
+    }
     HIP_TRY(launch_paged_append(a, static_cast<hipStream_t>(stream)), "paged append launch");
+    return CQ_OK;
+}
+
+int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long k_row, void *v, long long v_stream,
+                      long long v_row, int type, int batch, int t, const int32_t *rows, const int32_t *pos,
+                      void *stream) {
+    if (batch < 0 || t < 0) return fail(CQ_ERR_MISUSE, "needle: %d x %d rows read back", batch, t);
+    PagedReadArgs a;
+    if (int rc = paged_args(c, batch, 0, "a read", a.c)) return rc;
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: rows of type %d", type);
+    if (batch == 0 || t == 0 || c->page_stride == 0) return CQ_OK;
+    if (!k || !v || !pos || !c->pages) return fail(CQ_ERR_MISUSE, "needle: a read with a nil operand");
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: rows that are not aligned to their type");
+    const long long widths[2] = {static_cast<long long>(c->kv_heads) * c->qk, static_cast<long long>(c->kv_heads) * c->vd};
+    const long long streams[2] = {k_stream, v_stream}, rs[2] = {k_row, v_row};
+    for (int z = 0; z < 2; ++z)  // of rows[b] rows the host knows only that they are rows
+        if (rows ? !rows_apart(widths[z], batch, streams[z], 1, 0) || !rows_apart(widths[z], t, rs[z], 1, 0)
+                 : !rows_apart(widths[z], batch, streams[z], t, rs[z]))
+            return fail(CQ_ERR_MISUSE, "needle: rows read to one place (%lld values, rows %lld apart, streams %lld)",
+                        widths[z], rs[z], streams[z]);
+    if (static_cast<double>(batch) * t * c->kv_heads > (0xffffffffLL - 255) / 128)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: a read of %d x %d rows of %d heads", batch, t, c->kv_heads);
+    a.y[0] = k;
+    a.y[1] = v;
+    a.stream[0] = k_stream;
+    a.stream[1] = v_stream;
+    a.row[0] = k_row;
+    a.row[1] = v_row;
+    a.type = type;
+    a.batch = batch;
+    a.t = t;
+    a.rows = rows;
+    a.pos = pos;
+    HIP_TRY(launch_paged_read(a, static_cast<hipStream_t>(stream)), "paged read launch");
+    return CQ_OK;
+}
+
+int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream, long long out_row, const void *q,
+                             long long q_stream, long long q_row, int type, int batch, int t, int heads,
+                             const int32_t *rows, const int32_t *pos, int nk_max, int window, int sink, float scale,
+                             void *stream) {
+    if (batch < 0 || t < 0 || nk_max < 0 || window < 0 || sink < 0)
+        return fail(CQ_ERR_MISUSE, "needle: attention of %d x %d rows over %d keys (window %d, first %d)", batch, t, nk_max,
+                    window, sink);
+    RowsArgs a;
+    std::memset(&a, 0, sizeof a);
+    if (int rc = paged_args(c, batch, nk_max, "attention", a.c)) return rc;
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: queries of type %d", type);
+    if (heads <= 0 || heads % c->kv_heads != 0)
+        return fail(CQ_ERR_MISUSE, "needle: %d heads over %d KV heads", heads, c->kv_heads);
+    if (!attention_scale(scale)) return fail(CQ_ERR_MISUSE, "needle: attention scale %g", scale);
+    if (batch == 0 || t == 0 || nk_max == 0) return CQ_OK;
+    if (!out || !q || !pos) return fail(CQ_ERR_MISUSE, "needle: attention with a nil operand");
+    if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
+    a.q_row = q_row || q_stream ? q_row : static_cast<long long>(heads) * c->qk;
+    a.q_stream = q_row || q_stream ? q_stream : a.q_row * t;
+    const bool dense = !out_row && !out_stream;
+    const long long width = static_cast<long long>(heads) * c->vd;
+    a.out_row = dense ? width : out_row;
+    a.out_stream = dense ? width * t : out_stream;
+    // Of rows[b] rows the host knows only that they are rows.
+    if (rows ? !rows_apart(width, batch, a.out_stream, 1, 0) || !rows_apart(width, t, a.out_row, 1, 0)
+             : !rows_apart(width, batch, a.out_stream, t, a.out_row))
+        return fail(CQ_ERR_MISUSE, "needle: attention outputs of one place (%lld values, rows %lld apart, streams %lld)", width,
+                    a.out_row, a.out_stream);
+    a.group = heads / c->kv_heads;
+    if (static_cast<double>(t) * a.group > 1 << 30 || nk_max > 0x7fffffff - 256 ||
+        2.0 * batch * t * heads > static_cast<double>(grid_limit(64)))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads over %d keys", batch, t, heads,
+                    nk_max);
+    const int size = value_size(c->type), cus = device_info().cus;
+    a.k_head = static_cast<long long>(c->qk) * size;
+    a.v_head = static_cast<long long>(c->vd) * size;
+    a.k_row = a.k_head * c->kv_heads;
+    a.v_row = a.v_head * c->kv_heads;
+    a.q = q;
+    a.out = out;
+    a.rows = rows;
+    a.pos = pos;
+    a.type = type;
+    a.batch = batch;
+    a.t = t;
+    a.heads = heads;
+    a.nk_max = nk_max;
+    a.window = window;
+    a.sink = window ? sink : 0;
+    a.scale_log2 = attention_scale(scale);
+    const int wg_cols = rows_workgroup_columns(a, cus);
+    const long long cols = static_cast<long long>(t) * a.group, tiles = (cols + wg_cols - 1) / wg_cols;
+    const long long lists = static_cast<long long>(batch) * c->kv_heads * tiles;
+    // the keys a workgroup walks, at most
+    const long long keys = window ? std::min<long long>(nk_max, static_cast<long long>(window) + a.sink + wg_cols / a.group + 128)
+                                  : nk_max;
+    a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({2LL * cus / lists, keys / 256, 64})));
+    if (static_cast<double>(lists + 8 * tiles) * a.splits > static_cast<double>(grid_limit(256)))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", batch, t, heads);
+    WsScope ws;
+    if (a.splits > 1) {
+        const size_t out_rows = static_cast<size_t>(batch) * t * heads;
+        const size_t part = align256(out_rows * a.splits * c->vd * 4);
+        if (int rc = ws_acquire(part + align256(out_rows * a.splits * 8), static_cast<hipStream_t>(stream), ws.l)) return rc;
+        a.part = static_cast<float *>(ws.l.w->buf);
+        a.part_ml = reinterpret_cast<float *>(static_cast<char *>(ws.l.w->buf) + part);
+    }
+    HIP_TRY(launch_attend_rows(a, cus, static_cast<hipStream_t>(stream)), "attention launch");
     return CQ_OK;
 }
 
@@ -2486,6 +2602,8 @@ int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stri
                     keep, sink, recent);
     EvictArgs a;
     if (int rc = paged_args(c, batch, nk_max, "eviction", a.c)) return rc;
+    if (c->type == ND_I8_PAGES || c->type == ND_E4M3_PAGES)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: eviction from a cache with a scale a page");
     if (static_cast<long long>(dst_stride) * c->page_rows < keep || acc_cap < nk_max || acc_out_cap < keep)
         return fail(CQ_ERR_MISUSE, "needle: eviction to %d rows in %d pages of %d, weights %lld to %lld", keep,
                     dst_stride, c->page_rows, acc_cap, acc_out_cap);
@@ -2629,6 +2747,133 @@ int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, cons
         a.part = static_cast<float *>(ws.l.w->buf);
     }
     HIP_TRY(launch_logprobs(a, static_cast<hipStream_t>(stream)), "log probabilities launch");
+    return CQ_OK;
+}
+
+// Whether two arrays of rows of nx and ny values, batch x t of them, share an
+// element, as far as the host can tell apart arrays that lie inside each
+// other's reach: rows at the same strides that fit between each other.
+static bool rows_meet(const void *x, long long nx, long long xs, long long xr, const void *y, long long ny, long long ys,
+                      long long yr, int batch, int t, int size) {
+    const auto reach = [&](const void *p, long long n, long long s, long long r, __int128 &lo, __int128 &hi) {
+        const __int128 a = static_cast<__int128>(batch - 1) * s, b = static_cast<__int128>(t - 1) * r;
+        lo = reinterpret_cast<uintptr_t>(p) + size * (std::min<__int128>(a, 0) + std::min<__int128>(b, 0));
+        hi = reinterpret_cast<uintptr_t>(p) + size * (std::max<__int128>(a, 0) + std::max<__int128>(b, 0) + n);
+    };
+    __int128 x0, x1, y0, y1;
+    reach(x, nx, xs, xr, x0, x1);
+    reach(y, ny, ys, yr, y0, y1);
+    if (x1 <= y0 || y1 <= x0) return false;
+    // multiples of one stride: apart if they are modulo it
+    const long long r = t > 1 ? xr : xs;
+    if ((t > 1 && xr != yr) || (batch > 1 && xs != ys) || r <= 0 || (t > 1 && batch > 1 && xs % r != 0)) return true;
+    const __int128 d = static_cast<__int128>(reinterpret_cast<uintptr_t>(y)) - static_cast<__int128>(reinterpret_cast<uintptr_t>(x));
+    const __int128 m = (d % (r * size) + r * size) % (r * size);
+    return m < static_cast<__int128>(nx) * size || m + static_cast<__int128>(ny) * size > static_cast<__int128>(r) * size;
+}
+
+int nd_qk_norm_rope_dev(void *q_out, void *k_out, const void *q, const void *k, int type, const nd_heads_layout *layout,
+                        int batch, int t, int heads, int kv_heads, int width, const float *q_gain, const float *k_gain,
+                        const float *cos_t, const float *sin_t, int positions, const int32_t *pos, const int32_t *rows,
+                        void *stream) {
+    if (batch < 0 || t < 0 || heads < 0 || kv_heads < 0 || positions < 0)
+        return fail(CQ_ERR_MISUSE, "needle: norms of %d x %d rows of %d and %d heads", batch, t, heads, kv_heads);
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: heads of type %d", type);
+    if (width <= 0 || width % 16 != 0 || width > 256)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: norms of heads of %d (multiples of 16 up to 256)", width);
+    if (!cos_t != !sin_t) return fail(CQ_ERR_MISUSE, "needle: RoPE with one of its tables");
+    if (batch == 0 || t == 0 || heads + static_cast<long long>(kv_heads) == 0) return CQ_OK;
+    if ((heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)))
+        return fail(CQ_ERR_MISUSE, "needle: norms with a nil operand");
+    const int size = value_size(type);
+    if ((reinterpret_cast<uintptr_t>(heads ? q : nullptr) | reinterpret_cast<uintptr_t>(heads ? q_out : nullptr) |
+         reinterpret_cast<uintptr_t>(kv_heads ? k : nullptr) | reinterpret_cast<uintptr_t>(kv_heads ? k_out : nullptr)) %
+        size)
+        return fail(CQ_ERR_MISUSE, "needle: heads that are not aligned to their type");
+    const long long qw = static_cast<long long>(heads) * width, kw = static_cast<long long>(kv_heads) * width;
+    nd_heads_layout y = {qw * t, qw, kw * t, kw, qw * t, qw, kw * t, kw};
+    if (layout) y = *layout;
+    NormRopeArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.x[0] = q;
+    a.x[1] = k;
+    a.y[0] = q_out;
+    a.y[1] = k_out;
+    a.x_stream[0] = y.q_stream, a.x_row[0] = y.q_row;
+    a.x_stream[1] = y.k_stream, a.x_row[1] = y.k_row;
+    a.y_stream[0] = y.q_out_stream, a.y_row[0] = y.q_out_row;
+    a.y_stream[1] = y.k_out_stream, a.y_row[1] = y.k_out_row;
+    a.heads[0] = heads;
+    a.heads[1] = kv_heads;
+    const long long w[2] = {qw, kw};
+    for (int z = 0; z < 2; ++z) {
+        if (!a.heads[z]) continue;
+        if (rows ? !rows_apart(w[z], batch, a.y_stream[z], 1, 0) || !rows_apart(w[z], t, a.y_row[z], 1, 0)
+                 : !rows_apart(w[z], batch, a.y_stream[z], t, a.y_row[z]))
+            return fail(CQ_ERR_MISUSE, "needle: normed heads of one place (%lld values, rows %lld apart, streams %lld)", w[z],
+                        a.y_row[z], a.y_stream[z]);
+        for (int o = 0; o < 2; ++o) {  // against both inputs, and the other output
+            if (!a.heads[o]) continue;
+            const bool in_place = o == z && a.x[o] == a.y[z] && (t == 1 || a.x_row[o] == a.y_row[z]) &&
+                                  (batch == 1 || a.x_stream[o] == a.y_stream[z]);
+            if ((!in_place && rows_meet(a.y[z], w[z], a.y_stream[z], a.y_row[z], a.x[o], w[o], a.x_stream[o], a.x_row[o], batch, t, size)) ||
+                (o > z && rows_meet(a.y[z], w[z], a.y_stream[z], a.y_row[z], a.y[o], w[o], a.y_stream[o], a.y_row[o], batch, t, size)))
+                return fail(CQ_ERR_MISUSE, "needle: normed heads onto a part of others");
+        }
+    }
+    if (cos_t && !pos) return fail(CQ_ERR_MISUSE, "needle: RoPE without positions (nil)");
+    if (static_cast<double>(batch) * t * (static_cast<double>(heads) + kv_heads) > (0xffffffffLL - 255) / 32)
+        return fail(CQ_ERR_UNSUPPORTED, "needle: norms of %d x %d rows of %d and %d heads", batch, t, heads, kv_heads);
+    a.gain[0] = q_gain;
+    a.gain[1] = k_gain;
+    a.cos_t = cos_t;
+    a.sin_t = sin_t;
+    a.positions = positions;
+    a.pos = pos;
+    a.rows = rows;
+    a.type = type;
+    a.batch = batch;
+    a.t = t;
+    a.width = width;
+    HIP_TRY(launch_norm_rope(a, static_cast<hipStream_t>(stream)), "norm launch");
+    return CQ_OK;
+}
+
+int nd_verify_drafts_dev(int32_t *accepted, int32_t *tokens, float *lp, const void *target, long long target_stream,
+                         long long target_row, const void *draft, long long draft_stream, long long draft_row, int type,
+                         int batch, int t, int n, const int32_t *drafts, const int32_t *drafted, const float *u,
+                         const float *u_next, double temperature, void *stream) {
+    if (batch < 0 || t < 0 || n <= 0) return fail(CQ_ERR_MISUSE, "needle: %d x %d drafts of %d tokens", batch, t, n);
+    if (type < ND_F32 || type > ND_BF16) return fail(CQ_ERR_MISUSE, "needle: logits of type %d", type);
+    if (!(temperature >= 0.0) || !std::isfinite(temperature) || (temperature > 0.0 && !std::isfinite(1.0 / temperature)))
+        return fail(CQ_ERR_MISUSE, "needle: drafts at temperature %g", temperature);
+    if (t > 1 << 20 || n > 1 << 30) return fail(CQ_ERR_UNSUPPORTED, "needle: %d drafts of %d tokens", t, n);
+    if (batch == 0) return CQ_OK;
+    if (!accepted || !tokens || !target || (t > 0 && (!drafts || (temperature > 0.0 && !u))) || (temperature > 0.0 && !u_next))
+        return fail(CQ_ERR_MISUSE, "needle: drafts with a nil operand");
+    if (temperature == 0.0 || t == 0) draft = nullptr;
+    if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) % value_size(type))
+        return fail(CQ_ERR_MISUSE, "needle: logits that are not aligned to their type");
+    const long long outs = static_cast<long long>(batch) * (t + 1), ins = static_cast<long long>(batch) * t;
+    const struct { const void *p; long long n; } in[] = {{drafts, ins}, {drafted, batch}, {u, ins}, {u_next, batch}},
+                                                 out[] = {{accepted, batch}, {tokens, outs}, {lp, outs}};
+    for (int i = 0; i < 3; ++i) {
+        for (const auto &x : in)
+            if (words_overlap(out[i].p, out[i].n, x.p, x.n))
+                return fail(CQ_ERR_MISUSE, "needle: verified tokens onto their inputs");
+        for (int j = 0; j < i; ++j)
+            if (words_overlap(out[i].p, out[i].n, out[j].p, out[j].n))
+                return fail(CQ_ERR_MISUSE, "needle: verified tokens onto their inputs");
+    }
+    VerifyArgs a{accepted, tokens, lp, target, draft, target_stream, target_row, draft_stream, draft_row, type, batch, t, n,
+                 drafts, drafted, u, u_next, temperature > 0.0 ? 1.0 / temperature : 0.0, 1, n, nullptr};
+    const size_t bytes = verify_parts(a, device_info().cus);
+    if ((2.0 * t + 1) * batch * a.splits > static_cast<double>(grid_limit(1024)))
+        return fail(CQ_ERR_UNSUPPORTED, "needle: %d x %d drafts of %d tokens", batch, t, n);
+    WsScope ws;
+    if (int rc = ws_acquire(bytes, static_cast<hipStream_t>(stream), ws.l)) return rc;
+    a.part = static_cast<double *>(ws.l.w->buf);
+    HIP_TRY(launch_verify(a, static_cast<hipStream_t>(stream)), "verification launch");
     return CQ_OK;
 }
 

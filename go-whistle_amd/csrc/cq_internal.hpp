@@ -477,13 +477,16 @@ inline long long xcd_grid(long long units, long long per) {
     return (units >= kXcdUnits ? (units + 7) / 8 * 8 : units) * per;
 }
 
-// A paged cache as kv_paged describes it (pages of 2^shift rows).
+// A paged cache as kv_paged describes it (pages of 2^shift rows): float32,
+// float16, bfloat16, int8 or e4m3 (0 to 4). The scales of 8-bit row r of the
+// pool, head h are at (r >> sshift) * kv_heads + h.
 struct PagedArgs {
     unsigned char *k, *v;
     float *ks, *vs;
     const int32_t *pages;
     int type, kv_heads, qk, vd;
     int page_stride, shift, pool_pages;
+    int sshift;  // 0: a scale a row; shift: a scale a page
 };
 
 // Rows x[b * stream + i * row] of `type` appended at pos[b] + i (kv_append_paged_dev).
@@ -497,6 +500,18 @@ struct PagedAppendArgs {
     long long acc_cap;
 };
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s);
+// The same into 8-bit caches with a scale a page (page8_kernels.hip).
+hipError_t launch_page8_append(const PagedAppendArgs &a, hipStream_t s);
+
+// Rows pos[b] + i of the caches as values y[b * stream + i * row] of `type` (kv_read_paged_dev).
+struct PagedReadArgs {
+    PagedArgs c;
+    void *y[2];  // keys, values
+    long long stream[2], row[2];
+    int type, batch, t;
+    const int32_t *rows, *pos;
+};
+hipError_t launch_paged_read(const PagedReadArgs &a, hipStream_t s);
 
 // kv_evict_paged_dev: the kept rows of every (stream, key head), then their copies.
 struct EvictArgs {
@@ -551,6 +566,60 @@ hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s);
 // (cross_kernels.hip); the columns a workgroup takes.
 int cross_workgroup_columns(const SplitArgs &a, int cus);
 hipError_t launch_cross_attend(const SplitArgs &a, int cus, hipStream_t s);
+
+// kv_attend_rows_paged_dev (rows_kernels.hip): causal attention of `rows[b]`
+// rows of every stream, at positions pos[b] + i, in `splits` parts of their keys.
+struct RowsArgs {
+    PagedArgs c;
+    long long k_row, v_row, k_head, v_head;  // bytes
+    const void *q;
+    void *out;
+    long long q_stream, q_row, out_stream, out_row;  // elements
+    const int32_t *rows, *pos;
+    int type, batch, t, heads, group, nk_max;
+    int window, sink;     // window 0: none
+    int splits;
+    int aligned;          // bit 0: queries readable in 16-byte pieces, bit 1: outputs writable in 8-byte ones
+    float scale_log2;     // log2(e) / scale
+    // Per (stream, row, head, part) vd sums, their maximum and their sum of weights.
+    float *part, *part_ml;
+};
+// The columns (rows times heads of a group) a workgroup takes.
+int rows_workgroup_columns(const RowsArgs &a, int cus);
+hipError_t launch_attend_rows(const RowsArgs &a, int cus, hipStream_t s);
+hipError_t launch_attend_rows_f32(const RowsArgs &a, hipStream_t s);  // in float32, without the join (rows_f32_kernels.hip)
+
+// nd_qk_norm_rope_dev (norm_kernels.hip): queries and keys [0], [1].
+struct NormRopeArgs {
+    const void *x[2];
+    void *y[2];
+    long long x_stream[2], x_row[2], y_stream[2], y_row[2];  // elements
+    int heads[2];
+    const float *gain[2];  // null: no norm
+    const float *cos_t, *sin_t;
+    int positions;
+    const int32_t *pos, *rows;
+    int type, batch, t, width;
+};
+hipError_t launch_norm_rope(const NormRopeArgs &a, hipStream_t s);
+
+// nd_verify_drafts_dev (verify_kernels.hip): rows of n logits in `splits`
+// parts of `chunk`; the parts' results in part.
+struct VerifyArgs {
+    int32_t *accepted, *tokens;
+    float *lp;
+    const void *target, *draft;
+    long long target_stream, target_row, draft_stream, draft_row;
+    int type, batch, t, n;
+    const int32_t *drafts, *drafted;
+    const float *u, *u_next;
+    double inv_temp;  // 0: greedy
+    int splits, chunk;
+    double *part;
+};
+// Sets splits and chunk; the bytes of part.
+size_t verify_parts(VerifyArgs &a, int cus);
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 
 // nd_logprobs_dev: `splits` parts of `chunk` logits (a multiple of 8) a row; the parts' results
 // (splits > 1) in part: {m, l, t} and top pairs {value, index bits}.

@@ -1,0 +1,328 @@
+// gfx950 kernels of 8-bit paged caches with one scale a page and key head
+// (the append of kv_append_paged_dev), and the read-back of paged caches of
+// any type (kv_read_paged_dev).
+//
+// The values of a (page, head) are scale * code, scale the largest |x| that
+// the page has held since it was begun over 127 (int8) or 448 (e4m3), codes the
+// nearest to x / scale. Rows that raise the scale of a begun page have the
+// codes of the rows before them rounded anew under the new one.
+#include "cq_internal.hpp"
+#include "cq_device.hpp"
+
+#include <algorithm>
+
+namespace cqhip {
+namespace {
+
+constexpr int kHold = 8;  // steps of a unit's new rows kept in registers
+
+template <int TYPE>
+constexpr float kMost = TYPE == 3 ? 127.0f : 448.0f;
+
+// Four values of a row, from an array of `type` (vec: its pieces of four are
+// aligned to their size), widened.
+__device__ __forceinline__ void load_row4(float *x, const void *p, int type, long long at, bool vec) {
+    if (type == 0) {
+        const float *s = static_cast<const float *>(p) + at;
+        if (vec) {
+            const float4 u = *reinterpret_cast<const float4 *>(s);
+            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = s[e];
+        }
+        return;
+    }
+    const uint16_t *s = static_cast<const uint16_t *>(p) + at;
+    uint32_t w[2];
+    if (vec) {
+        *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(s);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) w[e] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint16_t h = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        x[e] = type == 1 ? static_cast<float>(__builtin_bit_cast(_Float16, h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+    }
+}
+
+// The codes of four values; NaN is 0 in int8 and NaN in e4m3.
+template <int TYPE>
+__device__ __forceinline__ uint32_t four_codes(const float *x, float sc) {
+    const float div = sc > 0.0f ? sc : 1.0f;
+    uint32_t q = 0;
+    if constexpr (TYPE == 3) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float r = rintf(x[e] / div);
+            q |= (static_cast<uint32_t>(r != r ? 0 : static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f))) & 255u) << (8 * e);
+        }
+    } else {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float r = x[e] / div;
+            y[e] = r != r ? r : fminf(fmaxf(r, -448.0f), 448.0f);
+        }
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        q = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true));
+    }
+    return q;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void four_values(float *x, uint32_t w) {
+    if constexpr (TYPE == 3) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int32_t>(w << (24 - 8 * e)) >> 24);
+    } else {
+        const int v = static_cast<int>(w);
+        x[0] = __builtin_amdgcn_cvt_f32_fp8(v, 0);
+        x[1] = __builtin_amdgcn_cvt_f32_fp8(v, 1);
+        x[2] = __builtin_amdgcn_cvt_f32_fp8(v, 2);
+        x[3] = __builtin_amdgcn_cvt_f32_fp8(v, 3);
+    }
+}
+
+// The unit of work is the keys or the values of one head in one page that a
+// stream's rows reach, a workgroup of one to eight wavefronts: LANES lanes
+// hold a row at four values each. The page's new rows are read once (kept in
+// registers up to kHold steps, behind those read again) for their bound, then
+// written; the rows before them only where the bound raises the scale.
+template <int TYPE, int LANES>
+__global__ __launch_bounds__(512) void page8_append_kernel(PagedAppendArgs a, int pages_each, unsigned units, int vec) {
+    __shared__ float wave_max[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    unsigned u = blockIdx.x;
+    const int z = static_cast<int>(u & 1);
+    u >>= 1;
+    const int h = static_cast<int>(u % a.c.kv_heads);
+    u /= a.c.kv_heads;
+    const int pi = static_cast<int>(u % pages_each), b = static_cast<int>(u / pages_each);
+    const int n = a.rows ? a.rows[b] : a.t;
+    const long long p0 = a.pos[b];
+    if (n <= 0 || n > a.t) return;
+    // the stream's rows that the cache takes: [lo, hi)
+    const long long lo = max(p0, 0LL), hi = min(p0 + n, static_cast<long long>(a.cap));
+    const long long page = (lo >> a.c.shift) + pi, first = page << a.c.shift;
+    const long long from = max(lo, first), to = min(hi, first + (1LL << a.c.shift));
+    if (from >= to) return;
+    const int pg = a.c.pages[static_cast<long long>(b) * a.c.page_stride + page];
+    if (pg < 0 || pg >= a.c.pool_pages) return;
+    const int width = z ? a.c.vd : a.c.qk, d = 4 * (tid & (LANES - 1));
+    const bool live = d < width;
+    const int per = static_cast<int>(blockDim.x) / LANES, r0 = tid / LANES;  // rows a step, this thread's first
+    const int count = static_cast<int>(to - from), held = static_cast<int>(from - first);
+    const long long src = static_cast<long long>(b) * a.stream[z] + (from - p0) * a.row[z] + static_cast<long long>(h) * width + d;
+    const bool v4 = vec >> z & 1;
+    float *scales = z ? a.c.vs : a.c.ks;
+    const long long sat = static_cast<long long>(pg) * a.c.kv_heads + h;
+    const float had = held > 0 ? scales[sat] : 0.0f;
+
+    float x[kHold][4], m = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kHold; ++s) {
+        const int r = r0 + s * per;
+        if (r < count && live) {
+            load_row4(x[s], a.x[z], a.type, src + r * a.row[z], v4);
+        } else {
+            x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.0f;
+        }
+    }
+    // the bound: of the finite values
+    auto bound = [&](const float *y) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(y[e]) < INFINITY ? fabsf(y[e]) : 0.0f);
+    };
+#pragma unroll
+    for (int s = 0; s < kHold; ++s) bound(x[s]);
+    for (int r = r0 + kHold * per; r < count; r += per)
+        if (live) {
+            float y[4];
+            load_row4(y, a.x[z], a.type, src + r * a.row[z], v4);
+            bound(y);
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, xor_lane(m, o));
+    if (waves > 1) {
+        if (lane == 0) wave_max[wave] = m;
+        __syncthreads();
+        for (int w = 0; w < waves; ++w) m = fmaxf(m, wave_max[w]);
+    }
+    const float sc = fmaxf(had, m / kMost<TYPE>);
+
+    unsigned char *pool = z ? a.c.v : a.c.k;
+    const long long row_bytes = static_cast<long long>(a.c.kv_heads) * width;
+    unsigned char *at = pool + (static_cast<long long>(pg) << a.c.shift) * row_bytes + static_cast<long long>(h) * width + d;
+    auto put = [&](int r, const float *y) {
+        *reinterpret_cast<uint32_t *>(at + (held + r) * row_bytes) = four_codes<TYPE>(y, sc);
+    };
+#pragma unroll
+    for (int s = 0; s < kHold; ++s) {
+        const int r = r0 + s * per;
+        if (r < count && live) put(r, x[s]);
+    }
+    for (int r = r0 + kHold * per; r < count; r += per)
+        if (live) {
+            float y[4];
+            load_row4(y, a.x[z], a.type, src + r * a.row[z], v4);
+            put(r, y);
+        }
+    if (sc != had && live)  // (a scale that was not a number included)
+        for (int r = r0; r < held; r += per) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(at + r * row_bytes);
+            float y[4];
+            four_values<TYPE>(y, *w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] *= had;
+            *w = four_codes<TYPE>(y, sc);
+        }
+    if (tid == 0) scales[sat] = sc;
+    if (a.acc && z == 0)
+        for (int r = tid; r < count; r += blockDim.x)
+            a.acc[(static_cast<long long>(b) * a.c.kv_heads + h) * a.acc_cap + from + r] = 0.0f;
+}
+
+template <int TYPE, int LANES>
+hipError_t launch_append(const PagedAppendArgs &a, int vec, hipStream_t s) {
+    const int rows = 1 << a.c.shift, most = std::min(rows, a.t);
+    const int pages_each = static_cast<int>((static_cast<long long>(a.t) + rows - 2) / rows + 1);
+    const long long units = 2LL * a.batch * a.c.kv_heads * pages_each;
+    // wavefronts until eight steps take a page's new rows
+    int waves = 1;
+    while (waves < 8 && most * LANES > 64 * waves * kHold) waves *= 2;
+    hipLaunchKernelGGL((page8_append_kernel<TYPE, LANES>), dim3(static_cast<unsigned>(units)), dim3(64 * waves), 0, s, a,
+                       pages_each, static_cast<unsigned>(units), vec);
+    return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t launch_append_type(const PagedAppendArgs &a, int vec, hipStream_t s) {
+    const int w = std::max(a.c.qk, a.c.vd);
+    if (w <= 64) return launch_append<TYPE, 16>(a, vec, s);
+    if (w <= 128) return launch_append<TYPE, 32>(a, vec, s);
+    return launch_append<TYPE, 64>(a, vec, s);
+}
+
+// ---- read back --------------------------------------------------------------------
+
+// Eight values from element i on to an array of `type` (vec: its 16-byte pieces are aligned).
+__device__ __forceinline__ void store_row8(void *p, int type, long long i, const float *x, bool vec) {
+    if (type == 0) {
+        float *y = static_cast<float *>(p) + i;
+        if (vec) {
+            reinterpret_cast<float4 *>(y)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4 *>(y)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+        }
+        return;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint16_t v = type == 1 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e]))
+                                     : __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[e]));
+        w[e / 2] = e & 1 ? w[e / 2] | static_cast<uint32_t>(v) << 16 : v;
+    }
+    uint16_t *y = static_cast<uint16_t *>(p) + i;
+    if (vec) {
+        *reinterpret_cast<uint4 *>(y) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+// As the append of rows: a head's key row and value row are one unit of LANES
+// lanes at eight values each, units in (stream, row, head) order.
+template <int TYPE, int LANES>
+__global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs a, unsigned units, int vec) {
+    const unsigned u = (blockIdx.x * 256u + threadIdx.x) / LANES;
+    if (u >= units) return;
+    const unsigned bi = u / a.c.kv_heads;
+    const int h = static_cast<int>(u - bi * a.c.kv_heads);
+    const int b = static_cast<int>(bi / a.t), i = static_cast<int>(bi - static_cast<unsigned>(b) * a.t);
+    if (a.rows) {
+        const int n = a.rows[b];
+        if (n > a.t || i >= n) return;
+    }
+    const long long p = static_cast<long long>(a.pos[b]) + i, page = p >> a.c.shift;
+    if (p < 0 || page >= a.c.page_stride) return;
+    const int pg = a.c.pages[static_cast<long long>(b) * a.c.page_stride + page];
+    if (pg < 0 || pg >= a.c.pool_pages) return;
+    const long long row = (static_cast<long long>(pg) << a.c.shift) + (p & ((1 << a.c.shift) - 1));
+    const int d = 8 * (threadIdx.x & (LANES - 1));
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const int width = z ? a.c.vd : a.c.qk;
+        if (d >= width) continue;
+        const long long from = (row * a.c.kv_heads + h) * width + d;
+        const unsigned char *pool = z ? a.c.v : a.c.k;
+        float x[8];
+        if constexpr (TYPE == 0) {
+            load_row4(x, pool, 0, from, true);
+            load_row4(x + 4, pool, 0, from + 4, true);
+        } else if constexpr (TYPE <= 2) {
+            load_row4(x, pool, TYPE, from, true);
+            load_row4(x + 4, pool, TYPE, from + 4, true);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2 *>(pool + from);
+            four_values<TYPE>(x, w.x);
+            four_values<TYPE>(x + 4, w.y);
+            const float sc = (z ? a.c.vs : a.c.ks)[(row >> a.c.sshift) * a.c.kv_heads + h];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= sc;
+        }
+        store_row8(a.y[z], a.type,
+                   static_cast<long long>(b) * a.stream[z] + static_cast<long long>(i) * a.row[z] +
+                       static_cast<long long>(h) * width + d,
+                   x, vec >> z & 1);
+    }
+}
+
+template <int TYPE, int LANES>
+hipError_t launch_read(const PagedReadArgs &a, int vec, hipStream_t s) {
+    const long long units = static_cast<long long>(a.batch) * a.t * a.c.kv_heads;
+    const long long blocks = (units * LANES + 255) / 256;
+    hipLaunchKernelGGL((paged_read_kernel<TYPE, LANES>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a,
+                       static_cast<unsigned>(units), vec);
+    return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t launch_read_type(const PagedReadArgs &a, int vec, hipStream_t s) {
+    const int w = std::max(a.c.qk, a.c.vd);
+    if (w <= 64) return launch_read<TYPE, 8>(a, vec, s);
+    if (w <= 128) return launch_read<TYPE, 16>(a, vec, s);
+    return launch_read<TYPE, 32>(a, vec, s);
+}
+
+}  // namespace
+
+hipError_t launch_page8_append(const PagedAppendArgs &a, hipStream_t s) {
+    int vec = 0;  // the rows' four-value pieces are aligned to their size
+    const int size = a.type == 0 ? 4 : 2;
+    for (int k = 0; k < 2; ++k)
+        if ((reinterpret_cast<uintptr_t>(a.x[k]) | (a.stream[k] * size) | (a.row[k] * size)) % (4 * size) == 0) vec |= 1 << k;
+    return a.c.type == 3 ? launch_append_type<3>(a, vec, s) : launch_append_type<4>(a, vec, s);
+}
+
+hipError_t launch_paged_read(const PagedReadArgs &a, hipStream_t s) {
+    int vec = 0;  // the rows' 16-byte pieces are aligned
+    const int size = a.type == 0 ? 4 : 2;
+    for (int k = 0; k < 2; ++k)
+        if ((reinterpret_cast<uintptr_t>(a.y[k]) | (a.stream[k] * size) | (a.row[k] * size)) % 16 == 0) vec |= 1 << k;
+    switch (a.c.type) {
+        case 0: return launch_read_type<0>(a, vec, s);
+        case 1: return launch_read_type<1>(a, vec, s);
+        case 2: return launch_read_type<2>(a, vec, s);
+        case 3: return launch_read_type<3>(a, vec, s);
+        default: return launch_read_type<4>(a, vec, s);
+    }
+}
+
+}  // namespace cqhip

@@ -60,9 +60,29 @@ __device__ __forceinline__ float piece_value(const uint32_t *w, int e) {
         return static_cast<float>(__builtin_bit_cast(_Float16, h));
     } else if constexpr (TYPE == 2) {
         return __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
-    } else {
+    } else if constexpr (TYPE == 3) {
         return static_cast<float>(static_cast<int32_t>(w[e >> 2] << (24 - 8 * (e & 3))) >> 24);
+    } else {
+        const int x = static_cast<int>(w[e >> 2]);
+        switch (e & 3) {  // the byte is an immediate
+            case 0: return __builtin_amdgcn_cvt_f32_fp8(x, 0);
+            case 1: return __builtin_amdgcn_cvt_f32_fp8(x, 1);
+            case 2: return __builtin_amdgcn_cvt_f32_fp8(x, 2);
+            default: return __builtin_amdgcn_cvt_f32_fp8(x, 3);
+        }
     }
+}
+
+// The cache types: float32, float16, bfloat16, then codes of 8 bits with
+// scales (int8, e4m3). Only int8 values are always finite.
+template <int TYPE>
+constexpr bool kScaled = TYPE >= 3;
+template <int TYPE>
+constexpr int kValueSize = TYPE == 0 ? 4 : kScaled<TYPE> ? 1 : 2;
+
+// Where the scales of an 8-bit row are.
+__device__ __forceinline__ long long scale_at(const SplitArgs &a, long long row, int h) {
+    return (row >> a.c.sshift) * a.c.kv_heads + h;
 }
 
 template <int WORDS>
@@ -326,7 +346,7 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
 // TYPE: the cache's type; D: widths up to D (64, 128, 256); COLS: columns a tile.
 template <int TYPE, int D, int COLS>
 __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(SplitArgs a, int col_tiles) {
-    constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
+    constexpr int kSize = kValueSize<TYPE>;
     constexpr int kPer = 16 / kSize;         // elements of a piece
     constexpr int kPieces = D / (4 * kPer);  // pieces of a row a lane reads
     constexpr int kSub = D * kSize <= 128 ? 2 : 1;  // 16-key steps of a tile
@@ -384,11 +404,11 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
         }
     };
     auto load_scales = [&]() {
-        if constexpr (TYPE == 3) {
+        if constexpr (kScaled<TYPE>) {
 #pragma unroll
             for (int s = 0; s < kSub; ++s) {
-                ks[s] = a.c.ks[static_cast<long long>(rows[s]) * a.c.kv_heads + p.h];
-                vs[s] = a.c.vs[static_cast<long long>(rows[s]) * a.c.kv_heads + p.h];
+                ks[s] = a.c.ks[scale_at(a, rows[s], p.h)];
+                vs[s] = a.c.vs[scale_at(a, rows[s], p.h)];
             }
         }
     };
@@ -415,12 +435,12 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
                         for (int e = 0; e < kPer; ++e) d = fmaf(piece_value<TYPE>(kw[s][k], e), q[n][k * kPer + e], d);
                     d += xor_lane<16>(d);
                     d += xor_lane<32>(d);
-                    if constexpr (TYPE == 3) d *= ks[s];
+                    if constexpr (kScaled<TYPE>) d *= ks[s];
                     x[n][s] = d;
                 }
             float vsc[kSub];
 #pragma unroll
-            for (int s = 0; s < kSub; ++s) vsc[s] = TYPE == 3 ? vs[s] : 1.0f;
+            for (int s = 0; s < kSub; ++s) vsc[s] = kScaled<TYPE> ? vs[s] : 1.0f;
             if (more) load_rows(kw, kp, a.k_row, a.c.qk);
             // past the last key values of 0, not that key's: a weight of 0 times an infinity
             if (TYPE != 3 && j + kTile > p.j1) {
@@ -459,7 +479,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
                 for (int s = 0; s < kSub; ++s) {
                     const float pw = __builtin_amdgcn_exp2f(x[n][s] - mu);
                     l[n] += pw;
-                    w[n][s] = TYPE == 3 && j + 16 * s + r >= p.j1 ? 0.0f : pw * vsc[s];
+                    w[n][s] = kScaled<TYPE> && j + 16 * s + r >= p.j1 ? 0.0f : pw * vsc[s];
                 }
             }
 #pragma unroll
@@ -521,7 +541,7 @@ __device__ __forceinline__ f32x4 mfma_16x16x32(const uint32_t *a, const uint32_t
 // parts of a query value (0: the products of the logits in float32).
 template <int TYPE, int D, int PARTS>
 __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
-    constexpr int kSize = TYPE == 0 ? 4 : TYPE == 3 ? 1 : 2;
+    constexpr int kSize = kValueSize<TYPE>;
     constexpr int kPer = 16 / kSize;          // elements of a 16-byte piece of a key row
     constexpr int kPieces = D / (4 * kPer);   // pieces of a key row a lane loads
     constexpr int kVals = D / 16;             // elements of a lane's piece of a value row
@@ -630,9 +650,9 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
 #pragma unroll
                         for (int k = 0; k < kVWords; ++k) vw[s][i][k] = 0;
                     }
-                    if constexpr (TYPE == 3) {
-                        ksc[s][i] = a.c.ks[row * a.c.kv_heads + p.h];
-                        vsc[s][i] = a.c.vs[row * a.c.kv_heads + p.h];
+                    if constexpr (kScaled<TYPE>) {
+                        ksc[s][i] = a.c.ks[scale_at(a, row, p.h)];
+                        vsc[s][i] = a.c.vs[scale_at(a, row, p.h)];
                     }
                 }
             const int jn = j + step;
@@ -660,7 +680,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                             uint32_t ka[4];
 #pragma unroll
                             for (int z = 0; z < 4; ++z)
-                                ka[z] = TYPE == 3 ? upper_pair(piece_value<TYPE>(kw[s][k], 8 * e + 2 * z),
+                                ka[z] = kScaled<TYPE> ? upper_pair(piece_value<TYPE>(kw[s][k], 8 * e + 2 * z),
                                                                piece_value<TYPE>(kw[s][k], 8 * e + 2 * z + 1))
                                                   : kw[s][k][z];
 #pragma unroll
@@ -668,7 +688,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                         }
             }
             // An infinite key times a part of 0 is NaN: such logits again, in float32.
-            if constexpr (PARTS == 3 && TYPE != 3) {
+            if constexpr (PARTS == 3 && !kScaled<TYPE>) {
                 bool nan = false;
 #pragma unroll
                 for (int s = 0; s < kSub; ++s)
@@ -715,7 +735,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                     const int jj = j + 16 * s + 4 * c + i;
                     float x = sc[s][i];
                     if constexpr (PARTS > 0) x *= a.scale_log2;
-                    if constexpr (TYPE == 3) x *= ksc[s][i];
+                    if constexpr (kScaled<TYPE>) x *= ksc[s][i];
                     if (jj >= p.j1) {
                         x = -INFINITY;
                     } else if (a.acc_out && col_ok) {
@@ -741,7 +761,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                 for (int i = 0; i < 4; ++i) {
                     float w = __builtin_amdgcn_exp2f(sc[s][i] - mu);
                     l += w;
-                    if constexpr (TYPE == 3) w = j + 16 * s + 4 * c + i >= p.j1 ? 0.0f : w * vsc[s][i];
+                    if constexpr (kScaled<TYPE>) w = j + 16 * s + 4 * c + i >= p.j1 ? 0.0f : w * vsc[s][i];
 #pragma unroll
                     for (int e = 0; e < kVals; ++e)
                         o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(vw[s][i], e), w, o[e], 0, 0, 0);
@@ -932,7 +952,8 @@ hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s) {
     hipError_t e = a.c.type == 0   ? launch_split_width<0>(a, s)
                    : a.c.type == 1 ? launch_split_width<1>(a, s)
                    : a.c.type == 2 ? launch_split_width<2>(a, s)
-                                   : launch_split_width<3>(a, s);
+                   : a.c.type == 3 ? launch_split_width<3>(a, s)
+                                   : launch_split_width<4>(a, s);
     if (e != hipSuccess || !a.part) return e;
     if ((e = launch_attend_join(a, s)) != hipSuccess) return e;
     if (a.acc_out && a.logits) {

@@ -6,7 +6,9 @@ tensors, AttendInt8Spans (int8.go:208-272) on device tensors for one or
 many independent streams, fakeQuant (int8.go:57-75), and Linear with
 WithInt8Input, Apply and ApplyShared on device tensors. Caches of any
 type and length (PagedKV), cross-attention to float memories
-(cross_attend_dev) and log probabilities (logprobs_dev) on device tensors.
+(cross_attend_dev), the query and key heads' norms with their rotation
+(qk_norm_rope_dev), log probabilities (logprobs_dev) and the verification of
+drafted tokens (verify_drafts_dev) on device tensors.
 """
 
 import ctypes
@@ -208,18 +210,19 @@ def ApplyShared(dsts, x, rows, *ls):
 _TYPES = {}
 _torch = _i32 = _f32 = None
 _layout = struct.Struct("10q").pack  # nd_cross_layout
+_heads_layout = struct.Struct("8q").pack  # nd_heads_layout
 
 
 def _type(t, what, cache=False):
-    """ND_F32.. of a tensor's dtype; ND_I8 for caches only."""
+    """ND_F32.. of a tensor's dtype; ND_I8 and ND_E4M3_PAGES for caches only."""
     global _torch, _i32, _f32
     if _torch is None:
         import torch
 
-        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3})
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3, torch.float8_e4m3fn: 6})
         _i32, _f32, _torch = torch.int32, torch.float32, torch  # _torch last: other threads look at it
     code = _TYPES.get(t.dtype)
-    if code is None or (code == 3 and not cache):
+    if code is None or (code >= 3 and not cache):
         raise CQPanic(f"needle: {what} of {t.dtype}")
     return code
 
@@ -274,10 +277,11 @@ class PagedKV:
     """Paged key and value caches of many streams (kv_paged, cqhip.h): pools k
     [pages, page_rows, kv_heads, qk] and v [pages, page_rows, kv_heads, vd] of
     float32, float16, bfloat16 or int8 (with scales ks, vs [pages, page_rows,
-    kv_heads] float32), read through the page table `pages` [streams,
-    pages per stream] int32. The tensors stay the caller's: a changed table
-    entry or a fork's copied table is seen by the next call. Another tensor
-    takes another PagedKV."""
+    kv_heads] float32), or of int8 or float8_e4m3fn with one scale a page and
+    head (ks, vs [pages, kv_heads] float32), read through the page table `pages`
+    [streams, pages per stream] int32. The tensors stay the caller's: a changed
+    table entry or a fork's copied table is seen by the next call. Another
+    tensor takes another PagedKV."""
 
     def __init__(self, k, v, pages, ks=None, vs=None):
         if k.dim() != 4 or v.dim() != 4 or pages.dim() != 2:
@@ -286,11 +290,13 @@ class PagedKV:
         _want(k, "keys", k.shape, k.dtype, self.index)
         _want(v, "values", (*k.shape[:3], v.shape[3]), k.dtype, self.index)
         _want(pages, "page table", pages.shape, _i32, self.index)
-        if (self.type == 3) != (ks is not None) or (ks is None) != (vs is None):
-            raise CQPanic("needle: int8 caches have scales, float ones none")
+        if (self.type >= 3) != (ks is not None) or (ks is None) != (vs is None):
+            raise CQPanic("needle: 8-bit caches have scales, float ones none")
+        if ks is not None and self.type == 3 and ks.dim() == 2:
+            self.type = 5  # a scale a page
         for s, what in ((ks, "key scales"), (vs, "value scales")):
             if s is not None:
-                _want(s, what, k.shape[:3], _f32, self.index)
+                _want(s, what, k.shape[:3] if self.type == 3 else (k.shape[0], k.shape[2]), _f32, self.index)
         self._tensors = k, v, ks, vs, pages
         self.streams, self.kv_heads, self.qk, self.vd = pages.shape[0], k.shape[2], k.shape[3], v.shape[3]
         _sizes("a paged cache", *pages.shape, *k.shape, v.shape[3])
@@ -314,7 +320,9 @@ class PagedKV:
         (float32, float16, bfloat16; any stream and row strides) appended at
         row pos[b] of stream b, the first rows[b] of them where given; rows
         at or past cap (all that the table holds) are skipped. acc [streams,
-        kv_heads, >= cap]: their accumulated weights become 0."""
+        kv_heads, >= cap]: their accumulated weights become 0. With a scale a
+        page, a page's scale rises with the rows appended to it, and its codes
+        are rounded anew (kv_append_paged_dev, cqhip.h)."""
         shape, code = k.shape, _type(k, "rows")
         t = shape[1] if len(shape) == 4 else 0
         _want(k, "key rows", (self.streams, t, self.kv_heads, self.qk), k.dtype, self.index, dense=False)
@@ -333,6 +341,52 @@ class PagedKV:
         acc_cap = self._acc(acc, "weights", cap) if acc is not None else 0
         _call(lib().kv_append_paged_dev, self.index, self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
               code, self.streams, t, _ptr(rows), pos.data_ptr(), cap, _ptr(acc), acc_cap)
+
+    def read_dev(self, k, v, pos, rows=None):
+        """Rows pos[b] + i of stream b's cache as values into k [streams, t,
+        kv_heads, qk] and v [streams, t, kv_heads, vd] (float32, float16,
+        bfloat16; any stream and row strides), the first rows[b] of them where
+        given; rows that the cache does not hold are left as they were."""
+        shape, code = k.shape, _type(k, "rows")
+        t = shape[1] if len(shape) == 4 else 0
+        _want(k, "key rows", (self.streams, t, self.kv_heads, self.qk), k.dtype, self.index, dense=False)
+        _want(v, "value rows", (self.streams, t, self.kv_heads, self.vd), k.dtype, self.index, dense=False)
+        ks, vs = k.stride(), v.stride()
+        for x, w, what in ((ks, self.qk, "key rows"), (vs, self.vd, "value rows")):
+            if x[3] != 1 or (x[2] != w and self.kv_heads > 1):
+                raise CQPanic(f"needle: {what} whose heads are not side by side")
+        _want(pos, "positions", (self.streams,), _i32, self.index)
+        if rows is not None:
+            _want(rows, "row counts", (self.streams,), _i32, self.index)
+        if t > _INT:
+            _sizes("a read", t)
+        _call(lib().kv_read_paged_dev, self.index, self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              code, self.streams, t, _ptr(rows), pos.data_ptr())
+
+    def attend_rows_dev(self, out, q, pos, scale, rows=None, nk_max=None, window=0, sink=0):
+        """Causal attention of many rows a stream: row i of q [streams, t,
+        heads, qk] and out [streams, t, heads, vd] (one type of float32, float16,
+        bfloat16; any stream and row strides) at position pos[b] + i attends the
+        cache's rows up to its own, with window > 0 only the last `window` of
+        them and the first `sink`; logits q.k / scale. rows [streams]: rows past
+        it are left as they were. nk_max (all that the table holds): streams
+        whose rows pass it are left as they were."""
+        shape, code = q.shape, _type(q, "queries")
+        t, heads = (shape[1], shape[2]) if len(shape) == 4 else (0, 0)
+        _want(q, "queries", (self.streams, t, heads, self.qk), q.dtype, self.index, dense=False)
+        _want(out, "outputs", (self.streams, t, heads, self.vd), q.dtype, self.index, dense=False)
+        qs, ys = q.stride(), out.stride()
+        if qs[3] != 1 or ys[3] != 1 or (heads > 1 and (qs[2] != self.qk or ys[2] != self.vd)):
+            raise CQPanic("needle: queries or outputs whose heads are not side by side")
+        _want(pos, "positions", (self.streams,), _i32, self.index)
+        if rows is not None:
+            _want(rows, "row counts", (self.streams,), _i32, self.index)
+        if nk_max is None:
+            nk_max = self.cap
+        if t > _INT or not 0 <= nk_max <= _INT or not 0 <= window <= _INT or not 0 <= sink <= _INT:
+            _sizes("attention", t, nk_max, window, sink)
+        _call(lib().kv_attend_rows_paged_dev, self.index, self._ref, out.data_ptr(), ys[0], ys[1], q.data_ptr(), qs[0],
+              qs[1], code, self.streams, t, heads, _ptr(rows), pos.data_ptr(), nk_max, window, sink, scale)
 
     def attend_dev(self, out, q, spans, nk_max, scale, acc=None, acc_out=None):
         """Attention of one token a stream: q [streams, heads, qk] and out
@@ -441,3 +495,91 @@ def logprobs_dev(logits, tokens=None, lp=None, ent=None, top=None, top_lp=None):
         _want(top_lp, "alternatives' log probabilities", (rows, k), _f32, dev)
     _call(lib().nd_logprobs_dev, dev, _ptr(lp), _ptr(ent), _ptr(top) if k else None, _ptr(top_lp) if k else None,
           logits.data_ptr(), stride[0], code, rows, n, _ptr(tokens), k)
+
+
+def qk_norm_rope_dev(q_out, k_out, q, k, q_gain=None, k_gain=None, rope=None, pos=None, rows=None):
+    """The norms of the query heads q [streams, t, heads, width] and the key
+    heads k [streams, t, kv_heads, width] (one type of float32, float16,
+    bfloat16; any stream and row strides) and their rotation in one pass, to
+    q_out and k_out, which may be q and k: ZCRMSNorm a head with q_gain, k_gain
+    [width] float32 (None: none), then RoPE by row pos[b] + i of rope = (cos, sin),
+    tables [positions, width / 2] float32 (None: none). rows [streams]: rows past
+    it are left as they were. q and q_out, or k and k_out, may be None."""
+    some = q if q is not None else k
+    if some is None or (q is None) != (q_out is None) or (k is None) != (k_out is None):
+        raise CQPanic("needle: norms without heads or without an output for them")
+    if some.dim() != 4:
+        raise CQPanic("needle: norms of [streams, rows, heads, width]")
+    B, t, _, width = some.shape
+    code, dtype, dev = _type(some, "heads"), some.dtype, _index(some, "heads")
+    heads, strides = [0, 0], [0] * 8
+    for z, (x, y, what) in enumerate(((q, q_out, "queries"), (k, k_out, "keys"))):
+        if x is None:
+            continue
+        n = heads[z] = x.shape[2] if x.dim() == 4 else 0
+        _want(x, what, (B, t, n, width), dtype, dev, False)
+        _want(y, f"normed {what}", (B, t, n, width), dtype, dev, False)
+        xs, ys = x.stride(), y.stride()
+        if xs[3] != 1 or ys[3] != 1 or (n > 1 and (xs[2] != width or ys[2] != width)):
+            raise CQPanic(f"needle: {what} whose heads are not side by side")
+        strides[2 * z], strides[2 * z + 1], strides[4 + 2 * z], strides[5 + 2 * z] = xs[0], xs[1], ys[0], ys[1]
+    for gain, what in ((q_gain, "query gains"), (k_gain, "key gains")):
+        if gain is not None:
+            _want(gain, what, (width,), _f32, dev)
+    cos, sin, positions = None, None, 0
+    if rope is not None:
+        cos, sin = rope
+        positions = cos.shape[0] if cos.dim() == 2 else 0
+        _want(cos, "cosines", (positions, width // 2), _f32, dev)
+        _want(sin, "sines", (positions, width // 2), _f32, dev)
+        if pos is None:
+            raise CQPanic("needle: RoPE without positions")
+        _want(pos, "positions", (B,), _i32, dev)
+    if rows is not None:
+        _want(rows, "row counts", (B,), _i32, dev)
+    if max(B, t, *heads, width, positions) > _INT:
+        _sizes("norms", B, t, *heads, width, positions)
+    _call(lib().nd_qk_norm_rope_dev, dev, _ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), code, _heads_layout(*strides), B, t,
+          heads[0], heads[1], width, _ptr(q_gain), _ptr(k_gain), _ptr(cos), _ptr(sin), positions,
+          _ptr(pos) if rope is not None else None, _ptr(rows))
+
+
+def verify_drafts_dev(accepted, tokens, target, drafts, draft=None, u=None, u_next=None, drafted=None, temperature=1.0,
+                      lp=None):
+    """Drafted tokens drafts [streams, t] int32 (the first drafted[b] of them
+    where given) verified against the target's logits target [streams, t + 1, n]
+    (float32, float16, bfloat16; any stream and row strides) from the random
+    numbers u [streams, t] and u_next [streams] float32 in [0, 1); draft
+    [streams, t, n]: the logits that they were drawn from (None: each was chosen
+    for sure). accepted [streams] int32 gets the count of those kept, tokens
+    [streams, t + 1] int32 them, the next token, and -1 behind, lp [streams,
+    t + 1] float32 their log probabilities. temperature 0 is greedy, and takes
+    no random numbers (nd_verify_drafts_dev, cqhip.h)."""
+    shape = target.shape
+    if len(shape) != 3 or drafts.dim() != 2:
+        raise CQPanic("needle: drafts [streams, t] against logits [streams, t + 1, n]")
+    B, t, n = drafts.shape[0], drafts.shape[1], shape[2]
+    code, dtype, dev = _type(target, "logits"), target.dtype, _index(target, "logits")
+    _want(target, "logits", (B, t + 1, n), dtype, dev, False)
+    _want(drafts, "drafts", (B, t), _i32, dev)
+    _want(accepted, "accepted counts", (B,), _i32, dev)
+    _want(tokens, "tokens", (B, t + 1), _i32, dev)
+    ts, ds = target.stride(), (0, 0, 1)
+    if draft is not None:
+        _want(draft, "the draft's logits", (B, t, n), dtype, dev, False)
+        ds = draft.stride()
+    if n > 1 and (ts[2] != 1 or ds[2] != 1):
+        raise CQPanic("needle: logits whose rows are not contiguous")
+    if u is not None:
+        _want(u, "random numbers", (B, t), _f32, dev)
+    if u_next is not None:
+        _want(u_next, "random numbers", (B,), _f32, dev)
+    if drafted is not None:
+        _want(drafted, "draft counts", (B,), _i32, dev)
+    if lp is not None:
+        _want(lp, "log probabilities", (B, t + 1), _f32, dev)
+    if max(B, t, n) > _INT:
+        _sizes("drafts", B, t, n)
+    _call(lib().nd_verify_drafts_dev, dev, accepted.data_ptr(), tokens.data_ptr(), _ptr(lp), target.data_ptr(), ts[0],
+          ts[1], _ptr(draft), ds[0], ds[1], code, B, t, n, drafts.data_ptr(), _ptr(drafted), _ptr(u), _ptr(u_next),
+          temperature)

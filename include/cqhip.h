@@ -472,11 +472,17 @@ enum {
     ND_F16 = 1,
     ND_BF16 = 2,
     ND_I8 = 3, /* caches only: codes with one float32 scale a row and head, as QuantizeRow gives them (int8.go:36-55) */
+    /* caches only: codes with one float32 scale a page and head, the largest
+     * |x| that the page has held over 127 (int8) or 448 (e4m3, the OCP 8-bit
+     * float without infinities) */
+    ND_I8_PAGES = 5,
+    ND_E4M3_PAGES = 6,
 };
 
 /* Paged key and value caches: pools of pool_pages pages of page_rows rows (a
  * power of two) of kv_heads keys of qk and values of vd of one type, scales
- * [row][kv_heads] beside int8 ones (else null). Row j of stream b is row
+ * [row][kv_heads] beside ND_I8 ones, [page][kv_heads] beside ND_I8_PAGES and
+ * ND_E4M3_PAGES (else null). Row j of stream b is row
  * pages[b*page_stride + j/page_rows]*page_rows + j%page_rows of the pools, as
  * kv_attend_int8_paged_dev reads them. Device pointers; the pools 16-byte
  * aligned. qk and vd are multiples of 16 up to 256; pool_pages * page_rows
@@ -500,7 +506,18 @@ typedef struct kv_paged {
  * the nearest even; int8 rows are quantized per head as QuantizeRow does, bit
  * for bit. acc non-null ([batch][kv_heads][acc_cap], acc_cap >= cap): the
  * appended rows' accumulated weights become 0. Rows of one call that land in
- * the same place race. */
+ * the same place race.
+ * Caches with a scale a page: the page of the first appended row keeps its
+ * rows before it and, for them, a scale that does not fall; rows that raise it
+ * have those rows' codes rounded anew, from their float32 values, under the new
+ * one. A page that the appended rows begin, and every page behind, takes its
+ * scale from them alone; rows behind the last appended one stand for nothing. Codes
+ * are the nearest (ties to the even one) to float32(x / scale). The scale goes
+ * by the finite values: infinities are held as the largest code of their sign,
+ * NaN as 0 (int8) or NaN (e4m3); a page of zeros has the scale 0. Streams of one
+ * call that append into one page race, also in different rows of it: a shared
+ * page is copied first (kv_page_copy_dev with rows of a page's head each:
+ * page_rows 1, cols page_rows * kv_heads * width, width page_rows * width). */
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
                         long long v_stream, long long v_row, int type, int batch, int t, const int32_t *rows,
                         const int32_t *pos, int cap, float *acc, long long acc_cap, void *stream);
@@ -540,10 +557,43 @@ int kv_attend_paged_dev(const kv_paged *c, void *out, long long out_stride, cons
  * keep) (len_out may be len, or lies apart from it). A stream whose len is
  * outside [0, nk_max] is left as it was, len_out too. A source page outside the
  * pool reads page 0, and rows of a destination page outside it are not
- * written. sink + recent <= keep. */
+ * written. sink + recent <= keep. Caches with a scale a page, whose rows cannot
+ * move without their page, are not taken (CQ_ERR_UNSUPPORTED). */
 int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stride, const float *acc,
                        long long acc_cap, float *acc_out, long long acc_out_cap, const int32_t *len, int32_t *len_out,
                        int32_t *kept, int batch, int nk_max, int keep, int sink, int recent, void *stream);
+
+/* Rows of paged caches of any type read back: row pos[b] + i of stream b's
+ * cache, i < rows[b] (null: t; counts outside [0, t] read nothing), as values of
+ * `type` (ND_F32, ND_F16 or ND_BF16; codes times their scale in float32, then
+ * rounded to the nearest even) to element b*k_stream + i*k_row of k and b*v_stream +
+ * i*v_row of v, kv_heads*qk and kv_heads*vd values each. Rows that the table does
+ * not hold (below 0, at or past page_stride * page_rows), and rows in pages
+ * outside the pool, are left as they were in the outputs. */
+int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long k_row, void *v, long long v_stream,
+                      long long v_row, int type, int batch, int t, const int32_t *rows, const int32_t *pos,
+                      void *stream);
+/* Causal attention of many rows a stream over its paged cache of any type: the
+ * prompt's rows after their append, and drafted tokens'. Row i < rows[b] (null:
+ * t) of stream b is at position p = pos[b] + i and attends the cache's rows j
+ * <= p, of which with window > 0 only j > p - window and j < sink (the last
+ * `window` rows, its own among them, and the first `sink`); logits q.k / scale (>
+ * 0). Streams whose count is outside [1, t], or whose rows are not inside [0,
+ * nk_max), and rows past the count leave their outputs as they were. q and out
+ * hold values of `type` (ND_F32, ND_F16, ND_BF16): row i of stream b is
+ * heads*qk values at element b*q_stream + i*q_row (heads*vd at b*out_stream +
+ * i*out_row; a stream and row stride of 0: dense [batch][t][heads][width]).
+ * Query head h reads key head h / (heads/kv_heads). A page outside the pool
+ * reads page 0. Cache rows that no row attends may hold anything. The written
+ * output rows share no element, and none with q.
+ * 16-bit queries over caches of their type, and over codes, take 16-bit
+ * products: the operands as they are (codes exactly), the softmax weights in
+ * two parts (22 bits with float16 caches, 16 else). Everything else is
+ * float32; sums and softmax are float32 throughout. */
+int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream, long long out_row, const void *q,
+                             long long q_stream, long long q_row, int type, int batch, int t, int heads,
+                             const int32_t *rows, const int32_t *pos, int nk_max, int window, int sink, float scale,
+                             void *stream);
 
 /* Where the rows of nd_cross_attend_dev's operands are, in elements: row i
  * of stream b's queries at b*q_stream + i*q_row (heads side by side, qk
@@ -586,6 +636,60 @@ int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, 
  * NaN, a NaN ranking as -inf. */
 int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, const void *logits, long long stride,
                     int type, int rows, int n, const int32_t *tokens, int top, void *stream);
+/* Where the rows of nd_qk_norm_rope_dev's operands are, in elements: row i of
+ * stream b's queries at b*q_stream + i*q_row (heads side by side, `width`
+ * apart), keys, and the outputs of both likewise. */
+typedef struct nd_heads_layout {
+    long long q_stream, q_row, k_stream, k_row;
+    long long q_out_stream, q_out_row, k_out_stream, k_out_row;
+} nd_heads_layout;
+
+/* The norms of the query and key heads and their rotation in one pass
+ * (normRotate, internal/needle/attention.go:298-330; Rope.apply,
+ * rope.go:69-81), for rows of any count: row i < rows[b] (null: t; counts
+ * outside [0, t] are none) of stream b has `heads` query and kv_heads key heads
+ * of `width` values of `type` (ND_F32, ND_F16, ND_BF16). Each head is
+ * ZCRMSNorm'ed (norm.go:53-109) with q_gain or k_gain (float32 [width]; null: no
+ * norm of those), then rotated by row pos[b] + i of the (positions x width/2)
+ * float32 tables (cos_t null: no rotation, and pos may be null; positions outside the
+ * tables: that row is not rotated), and rounded once, to q_out and k_out. Rows past
+ * the count are left as they were. ND_F32 arithmetic is ZCRMSNorm's and
+ * Rope.apply's but for the order of the float64 squares' sum; 16-bit types
+ * compute in float32. The outputs may be the inputs in place (same pointer and
+ * strides); else they share no element with an input. Written rows share none.
+ * heads or kv_heads may be 0. width is a multiple of 16 up to 256. layout null:
+ * dense [batch][t][heads][width]. */
+int nd_qk_norm_rope_dev(void *q_out, void *k_out, const void *q, const void *k, int type, const nd_heads_layout *layout,
+                        int batch, int t, int heads, int kv_heads, int width, const float *q_gain, const float *k_gain,
+                        const float *cos_t, const float *sin_t, int positions, const int32_t *pos, const int32_t *rows,
+                        void *stream);
+/* Drafted tokens verified against the target's probabilities, from given random
+ * numbers. target holds t + 1 rows of n logits of `type` (ND_F32, ND_F16,
+ * ND_BF16) a stream, row i at element b*target_stream + i*target_row: what the
+ * target gives before drafts[b][i] (i < drafted[b]; null: t; clamped to [0, t]), row
+ * drafted[b] behind the last. draft: the t rows of logits that the drafts were
+ * drawn from (null: each was chosen for sure). With p = softmax(target /
+ * temperature) and q = softmax(draft / temperature) of a row (q = 1 for the
+ * draft without them), draft d of row i is kept while u[b][i] * q(d) < p(d). At
+ * the first that is not, the stream's next token is the least j at which the
+ * running sum of max(p - q, 0) passes u_next[b] times its total (without draft: p
+ * without d), behind the last draft that of p; where rounding leaves none, or
+ * u_next is 1 or more, the last j of any weight; where the whole residual is 0
+ * or not a number, p is sampled. temperature 0 is greedy: a draft is kept if it
+ * is the first of its row's largest logits, the next token is that, and u, u_next
+ * and draft are not read. accepted[b] is the number of drafts kept; tokens
+ * ([batch][t + 1]) the kept drafts, the next token, then -1; lp (null or
+ * [batch][t + 1]) their log probabilities under softmax(target / temperature),
+ * of temperature 1 where it is 0, then 0. A draft outside [0, n) is not kept.
+ * A target row that holds NaN or +inf, or -inf alone, keeps nothing, and its
+ * next token is -1 with the log probability 0; a draft row of that kind keeps
+ * nothing. Exponentials and sums are float64. The outputs lie apart from the
+ * inputs. What internal/search's steps of one token (beam.go:501-540) take
+ * one by one. */
+int nd_verify_drafts_dev(int32_t *accepted, int32_t *tokens, float *lp, const void *target, long long target_stream,
+                         long long target_row, const void *draft, long long draft_stream, long long draft_row, int type,
+                         int batch, int t, int n, const int32_t *drafts, const int32_t *drafted, const float *u,
+                         const float *u_next, double temperature, void *stream);
 
 #ifdef __cplusplus
 }
