@@ -2290,7 +2290,7 @@ static int paged_args(const kv_paged *c, int batch, int rows, const char *what, 
     int shift = 0;
     while ((1 << shift) < c->page_rows) ++shift;
     p = PagedArgs{static_cast<unsigned char *>(c->k), static_cast<unsigned char *>(c->v), c->ks, c->vs, c->pages,
-                  c->type == ND_E4M3_PAGES ? 4 : by_page ? 3 : c->type, c->kv_heads, c->qk, c->vd, c->page_stride, shift,
+                  c->type == ND_E4M3_PAGES ? 4 : by_page ? 5 : c->type, c->kv_heads, c->qk, c->vd, c->page_stride, shift,
                   c->pool_pages, by_page ? shift : 0};
     return CQ_OK;
 }
@@ -2403,6 +2403,31 @@ int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long 
     return CQ_OK;
 }
 
+static int run_split_attend(SplitArgs &a, hipStream_t stream);
+
+// Whether attention of many rows takes the split form, in tiles of up to 32
+// columns straight from the caches, with float32 weights, or the tiles of
+// rows_kernels.hip in LDS. Measured on MI355X, us a call from a graph, split form
+// against tiles:
+// - float32 queries over 16-bit caches and codes, and 16-bit queries over the other
+//   16-bit type: the split form, whose products are 16-bit parts where the tiles
+//   would be float32's (8 streams, 8 heads of 64 over 2, 2000 bfloat16 keys: 512
+//   columns 44 against 68, 2048 112 against 207).
+// - float32 caches: the tiles once they give two blocks of 32 columns a CU (16
+//   streams, 8 heads of 64, 500 keys: 512 columns 207 against 154; 4 streams, 16
+//   heads of 128 over 4, 3000 keys: 1024 columns 287 against 263, 512 167 against 207).
+// - codes: up to 32 columns (32 streams, 32 heads of 128 over 8, 4000 e4m3 keys: 16
+//   columns 66 against 92, 32 85 against 92, 48 125 against 104).
+// - 16-bit caches of the queries' type: up to 16 columns of few lists (one such
+//   stream, 16,000 bfloat16 keys: 16 columns 29 against 38, 32 36 against 38; 32
+//   streams of 4000: 119 against 105).
+static bool rows_split_form(const RowsArgs &a, int cus) {
+    const long long cols = static_cast<long long>(a.t) * a.group, lists = static_cast<long long>(a.batch) * a.c.kv_heads;
+    if (a.c.type == 0) return (cols + 31) / 32 * lists < 2LL * cus;
+    if (a.c.type >= 3) return a.type == 0 || cols <= 32;
+    return a.c.type != a.type || (cols <= 16 && lists <= 64);
+}
+
 int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream, long long out_row, const void *q,
                              long long q_stream, long long q_row, int type, int batch, int t, int heads,
                              const int32_t *rows, const int32_t *pos, int nk_max, int window, int sink, float scale,
@@ -2454,13 +2479,35 @@ int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream,
     a.window = window;
     a.sink = window ? sink : 0;
     a.scale_log2 = attention_scale(scale);
+    if (rows_split_form(a, cus)) {
+        SplitArgs p;
+        std::memset(&p, 0, sizeof p);
+        p.c = a.c;
+        p.k_row = a.k_row, p.v_row = a.v_row, p.k_head = a.k_head, p.v_head = a.v_head;
+        p.q_len = rows;
+        p.pos = pos;
+        p.window = a.window;
+        p.sink = a.sink;
+        p.nk_max = nk_max;
+        p.t = t;
+        p.heads = heads;
+        p.batch = batch;
+        p.q = q;
+        p.out = out;
+        p.q_stream = a.q_stream, p.q_row = a.q_row, p.out_stream = a.out_stream, p.out_row = a.out_row;
+        p.type = type;
+        p.scale_log2 = a.scale_log2;
+        return run_split_attend(p, static_cast<hipStream_t>(stream));
+    }
     const int wg_cols = rows_workgroup_columns(a, cus);
     const long long cols = static_cast<long long>(t) * a.group, tiles = (cols + wg_cols - 1) / wg_cols;
     const long long lists = static_cast<long long>(batch) * c->kv_heads * tiles;
     // the keys a workgroup walks, at most
     const long long keys = window ? std::min<long long>(nk_max, static_cast<long long>(window) + a.sink + wg_cols / a.group + 128)
                                   : nk_max;
-    a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({2LL * cus / lists, keys / 256, 64})));
+    // Two workgroups a CU, where a part keeps 256 keys (1024 where the parts of
+    // many columns have to be written and joined).
+    a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({2LL * cus / lists, keys / (tiles == 1 ? 256 : 1024), 64})));
     if (static_cast<double>(lists + 8 * tiles) * a.splits > static_cast<double>(grid_limit(256)))
         return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", batch, t, heads);
     WsScope ws;
@@ -2499,7 +2546,9 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
     // list: 71 against 31).
     const bool lists_fill = 2LL * a.batch * a.c.kv_heads >= cus;
     const bool few = std::max(a.c.qk, a.c.vd) <= 64 && a.nk_max >= 256 && (lists_fill ? cols <= 16 : cols <= 8 && a.nk_max < 512);
-    const bool many = !a.spans && (a.type != ND_F32 ? cols > 1 && !few
+    // keys of a list, at most (rows of a tile see one window)
+    const long long nk = a.pos && a.window ? std::min<long long>(a.nk_max, static_cast<long long>(a.window) + a.sink + 16) : a.nk_max;
+    const bool many = !a.spans && !a.pos && (a.type != ND_F32 ? cols > 1 && !few
                                                     : cols > 64 && (cols + 31) / 32 * a.batch * a.c.kv_heads >= 3LL * cus / 2);
     a.tile = split_tile_columns(a, cus);
     const int wg_cols = many ? cross_workgroup_columns(a, cus) : a.tile;
@@ -2520,9 +2569,19 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
         // least (one stream of 8000 int8 keys: 16 us in 16 parts, 72 in one; of
         // 448: 8.0 in one, 9.4 in two).
         a.waves = split_max_waves(a);
-        while (a.waves > 1 && (lists * a.waves > 16LL * cus || (a.waves - 1) * 32 >= a.nk_max)) a.waves /= 2;
+        while (a.waves > 1 && (lists * a.waves > 16LL * cus || (a.waves - 1) * 32 >= nk)) a.waves /= 2;
         a.splits = static_cast<int>(std::max<long long>(
-            1, std::min<long long>({8LL * cus / (lists * a.waves), a.nk_max / (64LL * a.waves), 64})));
+            1, std::min<long long>({8LL * cus / (lists * a.waves), nk / (64LL * a.waves), 64})));
+    }
+    if (!many && a.pos && a.t > 1 && 2 * lists >= cus) {
+        // Rows of many lists, whose streams differ in length: smaller workgroups
+        // and more parts (5 rows of 32 streams of up to 8000 e4m3 keys, 32 heads of
+        // 128 over 8, 256 lists: 100 us with four wavefronts and three parts, 108
+        // with eight and one, 105 with two and six).
+        a.waves = std::min(a.waves, 4);
+        const int fit = a.tile > 16 || std::max(a.c.qk, a.c.vd) > 64 && a.c.type < 3 ? 8 : 12;  // wavefronts a CU holds
+        a.splits = static_cast<int>(
+            std::max<long long>(1, std::min<long long>({1LL * fit * cus / (lists * a.waves), nk / (64LL * a.waves), 64})));
     }
     const int qsize = value_size(a.type);
     a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stream * qsize) |

@@ -478,8 +478,9 @@ inline long long xcd_grid(long long units, long long per) {
 }
 
 // A paged cache as kv_paged describes it (pages of 2^shift rows): float32,
-// float16, bfloat16, int8 or e4m3 (0 to 4). The scales of 8-bit row r of the
-// pool, head h are at (r >> sshift) * kv_heads + h.
+// float16, bfloat16, int8 with a scale a row, e4m3 and int8 with a scale a page
+// (0 to 5). The scales of 8-bit row r of the pool, head h are at (r >> sshift) *
+// kv_heads + h.
 struct PagedArgs {
     unsigned char *k, *v;
     float *ks, *vs;
@@ -536,6 +537,10 @@ struct SplitArgs {
     long long k_mem, k_row, k_head, v_mem, v_row, v_head;  // bytes
     const int32_t *spans;                    // paged: the keys' spans
     const int32_t *q_len, *k_len, *index;    // memories
+    // Causal rows (pos non-null): row i of stream b is at pos[b] + i and sees the
+    // keys up to it, of a window (> 0) the last `window` and the first `sink`.
+    const int32_t *pos;
+    int window, sink;
     int memories, nk_max, t, heads, batch;
     int group;                               // heads a key head
     int splits;                              // parts of a list, at most 64
@@ -560,6 +565,7 @@ int split_tile_columns(const SplitArgs &a, int cus);     // columns a workgroup 
 int split_max_waves(const SplitArgs &a);                 // wavefronts a workgroup may have
 bool split_weights_in_lds(const SplitArgs &a, int waves);  // a list's logits fit LDS
 hipError_t launch_attend_split(const SplitArgs &a, hipStream_t s);
+hipError_t launch_attend_parts(const SplitArgs &a, hipStream_t s);  // of more than two columns (parts_kernels.hip), without the join
 // The parts of every output row joined.
 hipError_t launch_attend_join(const SplitArgs &a, hipStream_t s);
 // The same attention of many columns to memories of the queries' type
@@ -587,7 +593,7 @@ struct RowsArgs {
 // The columns (rows times heads of a group) a workgroup takes.
 int rows_workgroup_columns(const RowsArgs &a, int cus);
 hipError_t launch_attend_rows(const RowsArgs &a, int cus, hipStream_t s);
-hipError_t launch_attend_rows_f32(const RowsArgs &a, hipStream_t s);  // in float32, without the join (rows_f32_kernels.hip)
+hipError_t launch_attend_rows_f32(const RowsArgs &a, hipStream_t s);  // float32 caches, without the join (rows_f32_kernels.hip)
 
 // nd_qk_norm_rope_dev (norm_kernels.hip): queries and keys [0], [1].
 struct NormRopeArgs {

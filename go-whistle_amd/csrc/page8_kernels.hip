@@ -308,7 +308,7 @@ hipError_t launch_page8_append(const PagedAppendArgs &a, hipStream_t s) {
     const int size = a.type == 0 ? 4 : 2;
     for (int k = 0; k < 2; ++k)
         if ((reinterpret_cast<uintptr_t>(a.x[k]) | (a.stream[k] * size) | (a.row[k] * size)) % (4 * size) == 0) vec |= 1 << k;
-    return a.c.type == 3 ? launch_append_type<3>(a, vec, s) : launch_append_type<4>(a, vec, s);
+    return a.c.type == 4 ? launch_append_type<4>(a, vec, s) : launch_append_type<3>(a, vec, s);
 }
 
 hipError_t launch_paged_read(const PagedReadArgs &a, hipStream_t s) {
@@ -320,8 +320,8 @@ hipError_t launch_paged_read(const PagedReadArgs &a, hipStream_t s) {
         case 0: return launch_read_type<0>(a, vec, s);
         case 1: return launch_read_type<1>(a, vec, s);
         case 2: return launch_read_type<2>(a, vec, s);
-        case 3: return launch_read_type<3>(a, vec, s);
-        default: return launch_read_type<4>(a, vec, s);
+        case 4: return launch_read_type<4>(a, vec, s);
+        default: return launch_read_type<3>(a, vec, s);  // int8 with scales a row or a page
     }
 }
 

@@ -23,8 +23,17 @@ template <int KEYS>
 __device__ __forceinline__ RowsPlace rows_place(const RowsArgs &a, int col_tiles, int wg_cols) {
     RowsPlace p;
     p.ok = false;
-    const XcdPlace x = xcd_place(a.batch * a.c.kv_heads, col_tiles * a.splits);  // a (stream, key head) on one XCD
-    if (!x.ok) return p;
+    // A (stream, key head) on one XCD; but streams of unequal counts, where there
+    // are few, over all of them: tile by tile, each turn of the units one place on.
+    const int units = a.batch * a.c.kv_heads;
+    XcdPlace x;
+    if (a.rows && units < kXcdUnits) {
+        x.within = static_cast<int>(blockIdx.x) / units;
+        x.unit = (static_cast<int>(blockIdx.x) - x.within * units + x.within) % units;
+    } else {
+        x = xcd_place(units, col_tiles * a.splits);
+        if (!x.ok) return p;
+    }
     const int ct = x.within / a.splits;
     p.sp = x.within - ct * a.splits;
     p.ct = col_tiles - 1 - ct;  // the last rows, which see most keys, first
@@ -89,7 +98,7 @@ __device__ __forceinline__ void store_any(void *p, int type, long long i, float 
 // Value d of a cache row's head, without its scale.
 __device__ __forceinline__ float cache_value(const unsigned char *row, int type, int d) {
     if (type <= 2) return load_any(row, type, d);
-    return type == 3 ? static_cast<float>(static_cast<int8_t>(row[d])) : __builtin_amdgcn_cvt_f32_fp8(row[d], 0);
+    return type == 4 ? __builtin_amdgcn_cvt_f32_fp8(row[d], 0) : static_cast<float>(static_cast<int8_t>(row[d]));
 }
 
 // Columns c of `mask` (first column col0) again, key by key, by one wavefront:

@@ -1,5 +1,5 @@
-// gfx950 causal attention of many rows over paged caches in float32: what
-// rows_kernels.hip, which describes both, does not take on 16-bit products.
+// gfx950 causal attention of many rows over paged float32 caches
+// (rows_kernels.hip describes the tiles, the masks and the columns computed again).
 #include "rows_device.hpp"
 
 #include <algorithm>
@@ -7,17 +7,14 @@
 namespace cqhip {
 namespace {
 
-// Everything in float32: 32 columns a wavefront on v_mfma_f32_32x32x2_f32, the
-// products of cross_attend_f32_kernel. Cache values of any type are widened
-// (codes times their scales) on their way into LDS.
-template <int CT, int D, bool FULL>
+// 32 columns a wavefront on v_mfma_f32_32x32x2_f32, the products of
+// cross_attend_f32_kernel.
+template <int D, bool FULL>
 __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f32_kernel(RowsArgs a, int col_tiles) {
     constexpr int kKeys = D == 64 ? 64 : 32;   // keys a tile
     constexpr int kBytes = kKeys * D * 4;
-    constexpr int kSize = CT == 0 ? 4 : CT <= 2 ? 2 : 1;
-    constexpr int kPer = 16 / kSize;           // values of a 16-byte piece of a cache row
-    constexpr int kRowPieces = D / kPer;
-    constexpr int kStage = (kKeys * kRowPieces + 255) / 256;  // pieces a thread stages
+    constexpr int kRowPieces = D / 4;             // 16-byte pieces of a row
+    constexpr int kStage = kKeys * kRowPieces / 256;  // pieces a thread stages
     extern __shared__ __align__(16) unsigned char smem[];  // [2][keys, values]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -33,48 +30,25 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
     const unsigned char *vp = a.c.v + static_cast<long long>(p.h) * a.v_head;
 
     auto rows_of = [&](int i) { return pool_row(a, p.b, min(tile_key<kKeys>(p, i) + (lane & (kKeys - 1)), p.end - 1)); };
-    uint4 kst[kStage], vst[kStage];
-    float kss[kStage], vss[kStage];
+    float4 kst[kStage], vst[kStage];
     auto fetch = [&](int rows) {
 #pragma unroll
         for (int k = 0; k < kStage; ++k) {
             const int piece = tid + 256 * k, row = piece / kRowPieces, c = piece % kRowPieces;
-            const long long src = __shfl(rows, row & (kKeys - 1));
-            const bool in = row < kKeys;
-            kst[k] = in && (FULL || c * kPer < a.c.qk) ? *reinterpret_cast<const uint4 *>(kp + src * a.k_row + c * 16) : make_uint4(0, 0, 0, 0);
-            vst[k] = in && (FULL || c * kPer < a.c.vd) ? *reinterpret_cast<const uint4 *>(vp + src * a.v_row + c * 16) : make_uint4(0, 0, 0, 0);
-            if constexpr (CT >= 3) {
-                const long long sat = (src >> a.c.sshift) * a.c.kv_heads + p.h;
-                kss[k] = a.c.ks[sat];
-                vss[k] = a.c.vs[sat];
-            }
+            const long long src = __shfl(rows, row);
+            kst[k] = FULL || 4 * c < a.c.qk ? *reinterpret_cast<const float4 *>(kp + src * a.k_row + c * 16) : make_float4(0, 0, 0, 0);
+            vst[k] = FULL || 4 * c < a.c.vd ? *reinterpret_cast<const float4 *>(vp + src * a.v_row + c * 16) : make_float4(0, 0, 0, 0);
         }
-    };
-    auto widen = [&](const uint4 &v, int e, float sc) {  // value e of a piece
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        if constexpr (CT == 0) return __uint_as_float(w[e]);
-        if constexpr (CT == 1 || CT == 2) return half_value(static_cast<uint16_t>(w[(e >> 1) & 3] >> (16 * (e & 1))), CT);
-        if constexpr (CT == 3) return static_cast<float>(static_cast<int32_t>(w[(e >> 2) & 3] << (24 - 8 * (e & 3))) >> 24) * sc;
-        const int x = static_cast<int>(w[(e >> 2) & 3] >> (8 * (e & 3)));
-        return __builtin_amdgcn_cvt_f32_fp8(x, 0) * sc;
     };
     auto store = [&](int j, int buf) {
         unsigned char *kt = smem + buf * 2 * kBytes, *vt = kt + kBytes;
 #pragma unroll
         for (int k = 0; k < kStage; ++k) {
             const int piece = tid + 256 * k, row = piece / kRowPieces, c = piece % kRowPieces;
-            if (row >= kKeys) continue;
-            const bool dead = j + row >= p.end;  // values behind the last key: 0
-#pragma unroll
-            for (int e = 0; e < kPer; e += 4) {
-                const int c4 = c * (kPer / 4) + e / 4;  // 16-byte piece of the float32 row
-                *reinterpret_cast<float4 *>(kt + row * D * 4 + ((c4 ^ (row & 15)) * 16)) =
-                    make_float4(widen(kst[k], e, kss[k]), widen(kst[k], e + 1, kss[k]), widen(kst[k], e + 2, kss[k]), widen(kst[k], e + 3, kss[k]));
-                *reinterpret_cast<float4 *>(vt + row * D * 4 + ((c4 ^ (((row >> 2) & 1) << 3)) * 16)) =
-                    dead ? make_float4(0, 0, 0, 0)
-                         : make_float4(widen(vst[k], e, vss[k]), widen(vst[k], e + 1, vss[k]), widen(vst[k], e + 2, vss[k]),
-                                       widen(vst[k], e + 3, vss[k]));
-            }
+            *reinterpret_cast<float4 *>(kt + row * D * 4 + ((c ^ (row & 15)) * 16)) = kst[k];
+            // values behind the last key: 0
+            *reinterpret_cast<float4 *>(vt + row * D * 4 + ((c ^ (((row >> 2) & 1) << 3)) * 16)) =
+                j + row >= p.end ? make_float4(0, 0, 0, 0) : vst[k];
         }
     };
 
@@ -209,30 +183,19 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
     if (bad) repair_columns<kKeys>(a, p, col0, static_cast<unsigned>(bad) | static_cast<unsigned>(bad >> 32));
 }
 
-template <int CT, int D>
-hipError_t launch_f32_full(const RowsArgs &a, hipStream_t s) {
+template <int D>
+hipError_t launch_f32(const RowsArgs &a, hipStream_t s) {
     static std::atomic<unsigned long long> full{0}, part{0};
     constexpr int lds = 4 * (D == 64 ? 64 : 32) * D * 4;
-    return a.c.qk == D && a.c.vd == D ? launch_with(&rows_attend_f32_kernel<CT, D, true>, a, kRWaves * 32, lds, full, s)
-                                      : launch_with(&rows_attend_f32_kernel<CT, D, false>, a, kRWaves * 32, lds, part, s);
-}
-
-template <int CT>
-hipError_t launch_f32_width(const RowsArgs &a, hipStream_t s) {
-    const int w = std::max(a.c.qk, a.c.vd);
-    return w <= 64 ? launch_f32_full<CT, 64>(a, s) : w <= 128 ? launch_f32_full<CT, 128>(a, s) : launch_f32_full<CT, 256>(a, s);
+    return a.c.qk == D && a.c.vd == D ? launch_with(&rows_attend_f32_kernel<D, true>, a, kRWaves * 32, lds, full, s)
+                                      : launch_with(&rows_attend_f32_kernel<D, false>, a, kRWaves * 32, lds, part, s);
 }
 
 }  // namespace
 
 hipError_t launch_attend_rows_f32(const RowsArgs &a, hipStream_t s) {
-    switch (a.c.type) {
-        case 0: return launch_f32_width<0>(a, s);
-        case 1: return launch_f32_width<1>(a, s);
-        case 2: return launch_f32_width<2>(a, s);
-        case 3: return launch_f32_width<3>(a, s);
-        default: return launch_f32_width<4>(a, s);
-    }
+    const int w = std::max(a.c.qk, a.c.vd);
+    return w <= 64 ? launch_f32<64>(a, s) : w <= 128 ? launch_f32<128>(a, s) : launch_f32<256>(a, s);
 }
 
 }  // namespace cqhip

@@ -27,6 +27,7 @@
 #include "rows_device.hpp"
 
 #include <algorithm>
+#include <cstring>
 
 namespace cqhip {
 namespace {
@@ -53,7 +54,9 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w, int pair) {
 // both widths are D (else steps past a width are skipped by branches, which
 // keep the compiler from interleaving the products with the softmax).
 constexpr float kRowsFar = 0x1p20f;  // from a maximum of it on, logits are rounded before it is subtracted, as it was
-template <int QT, int CT, int D, int CB, bool FULL>
+// KS: 1, or 2 where few columns would leave wavefronts idle: wavefronts 0 and 1
+// take the first 32 keys of a tile, 2 and 3 the others, joined at the end.
+template <int QT, int CT, int D, int CB, int KS, bool FULL>
 __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_kernel(RowsArgs a, int col_tiles) {
     constexpr bool kCodes = CT >= 3;
     constexpr int VT = kCodes ? 2 : QT;          // the values' type in LDS
@@ -66,10 +69,12 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, half = lane >> 5;
-    constexpr int kWgCols = kRWaves * 32 * CB;
+    constexpr int kWgCols = kRWaves / KS * 32 * CB;
+    constexpr int kBlocks = 2 / KS;              // blocks of 32 keys of a tile a wavefront takes
     const RowsPlace p = rows_place<kRTile>(a, col_tiles, kWgCols);
     if (!p.ok) return;
-    const int col0 = p.ct * kWgCols + wave * 32 * CB;
+    const int col_wave = wave % (kRWaves / KS), block0 = wave / (kRWaves / KS);
+    const int col0 = p.ct * kWgCols + col_wave * 32 * CB;
     const bool live = col0 < p.cols;
     // the wavefront's rows' positions, its columns' own
     const int first = p.pos + min(col0, p.cols - 1) / a.group, last = p.pos + (min(col0 + 32 * CB, p.cols) - 1) / a.group;
@@ -218,29 +223,30 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
                 load_tile(rows, buf ^ 1);
             if (i + 2 < p.i1) rows = rows_of(i + 2);
         }
-        if (live && !none_sees(a, first, last, j, j + kRTile - 1)) {
-            const unsigned char *kt = smem + buf * 2 * kBytes, *vt = kt + kBytes;
-            f32x16 s[CB][2];
+        const int jw = j + 32 * block0;  // the wavefront's keys of the tile
+        if (live && !none_sees(a, first, last, jw, jw + 32 * kBlocks - 1)) {
+            const unsigned char *kt = smem + buf * 2 * kBytes + block0 * 32 * D * 2, *vt = kt + kBytes;
+            f32x16 s[CB][kBlocks];
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[cb][kb][e] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
                 if (FULL || 16 * ks < a.c.qk) {
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
+                    for (int kb = 0; kb < kBlocks; ++kb) {
                         const s16x8 ka = *reinterpret_cast<const s16x8 *>(kt + kb * 32 * D * 2 + kaddr + ((2 * ks + half) ^ kswz) * 16);
 #pragma unroll
                         for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16<QT>(ka, q[cb][ks], s[cb][kb]);
                     }
                 }
             if constexpr (kCodes) {
-                const float *ks = scales + 2 * buf * kRTile + 4 * half;
+                const float *ks = scales + 2 * buf * kRTile + 32 * block0 + 4 * half;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const float4 x = *reinterpret_cast<const float4 *>(ks + 32 * kb + 8 * g);
@@ -253,24 +259,26 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
                         }
                     }
             }
-            if (!all_see(a, first, last, j, j + kRTile - 1)) {
+            if (!all_see(a, first, last, jw, jw + 32 * kBlocks - 1)) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int key = j + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
+                        const int key = jw + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
 #pragma unroll
                         for (int cb = 0; cb < CB; ++cb) s[cb][kb][e] = sees(a, at[cb], key) ? s[cb][kb][e] : -INFINITY;
                     }
             }
-            u32x4 w[CB][4], rest[CB][4];
+            u32x4 w[CB][2 * kBlocks], rest[CB][2 * kBlocks];
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 float mt = s[cb][0][0];
 #pragma unroll
                 for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[cb][0][e]);
+                if constexpr (kBlocks == 2) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[cb][1][e]);
+                    for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[cb][1][e]);
+                }
                 mt = halves_max(mt) * a.scale_log2;
                 float scale = a.scale_log2;
                 if (__any(mt > m[cb] + 8.0f || fabsf(m[cb]) >= kRowsFar)) {
@@ -285,14 +293,14 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
                     if (__any(far)) {
                         const float one = far ? scale : 1.0f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s[cb][0][e] *= one, s[cb][1][e] *= one;
+                        for (int kb = 0; kb < kBlocks; ++kb) s[cb][kb] *= one;
                         scale = far ? 1.0f : scale;
                     }
                 }
                 const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<VT>;
-                const float *vs = scales + (2 * buf + 1) * kRTile + 4 * half;
+                const float *vs = scales + (2 * buf + 1) * kRTile + 32 * block0 + 4 * half;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][e], scale, -mu));
@@ -311,7 +319,7 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
             }
             // all first parts of 16 keys, then all second ones: no product waits for the one before it
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
+            for (int st = 0; st < 2 * kBlocks; ++st) {
                 s16x8 va[D / 32];
 #pragma unroll
                 for (int v = 0; v < D / 32; ++v)
@@ -336,6 +344,36 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
         }
         if constexpr (kCodes)
             if (more) store_codes(tile_key<kRTile>(p, i + 1), buf ^ 1);
+    }
+    if constexpr (KS == 2) {
+        // the other half's outputs, maximum and sum, from LDS: registers side by side
+        constexpr int kRegs = D / 2 + 2;
+        float *join = reinterpret_cast<float *>(smem) + col_wave * CB * kRegs * 64 + lane;
+        __syncthreads();  // the tiles' readers are done
+        if (block0 == 1) {
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) join[(cb * kRegs + 16 * v + e) * 64] = o[cb][v][e];
+                join[(cb * kRegs + D / 2) * 64] = m[cb];
+                join[(cb * kRegs + D / 2 + 1) * 64] = l[cb];
+            }
+        }
+        __syncthreads();
+        if (block0 == 1) return;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            const float m1 = join[(cb * kRegs + D / 2) * 64], mn = fmaxf(m[cb], m1), mu = mn == -INFINITY ? 0.0f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(m[cb] - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+            m[cb] = mn;
+            l[cb] = l[cb] * f0 + join[(cb * kRegs + D / 2 + 1) * 64] * f1;
+#pragma unroll
+            for (int v = 0; v < D / 32; ++v)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[cb][v][e] = o[cb][v][e] * f0 + join[(cb * kRegs + 16 * v + e) * 64] * f1;
+        }
     }
     if (!live) return;
 #pragma unroll
@@ -393,72 +431,53 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
     }
 }
 
-// The parts of every output row joined: a wavefront 128 values, two a lane.
-__global__ __launch_bounds__(64) void rows_join_kernel(RowsArgs a, int blocks) {
-    const int lane = threadIdx.x;
-    const int id = blockIdx.x / blocks, d = (blockIdx.x - id * blocks) * 128 + 2 * lane;
-    const int bi = id / a.heads, head = id - bi * a.heads, b = bi / a.t, i = bi - b * a.t;
-    const int n = a.rows ? a.rows[b] : a.t, pos = a.pos[b];
-    if (n <= 0 || n > a.t || i >= n || pos < 0 || pos > a.nk_max - n) return;
-    const float *ml = a.part_ml + 2LL * id * a.splits;
-    const float2 mine = lane < a.splits ? *reinterpret_cast<const float2 *>(ml + 2 * lane) : make_float2(-INFINITY, 0.0f);
-    float m = mine.x;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, xor_lane(m, o));
-    const float f = __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.0f : m));
-    float l = mine.y * f;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l += xor_lane(l, o);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (d >= a.c.vd) return;
-    const float *part = a.part + static_cast<long long>(id) * a.splits * a.c.vd + d;
-    float2 v = make_float2(0.0f, 0.0f);
-    for (int s = 0; s < a.splits; ++s) {
-        const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-        const float2 y = *reinterpret_cast<const float2 *>(part + static_cast<long long>(s) * a.c.vd);
-        if (fs == 0.0f) continue;  // a part that none of the row's keys are in
-        v.x = fmaf(y.x, fs, v.x);
-        v.y = fmaf(y.y, fs, v.y);
-    }
-    const long long to = static_cast<long long>(b) * a.out_stream + static_cast<long long>(i) * a.out_row +
-                         static_cast<long long>(head) * a.c.vd + d;
-    store_any(a.out, a.type, to, v.x * inv);
-    store_any(a.out, a.type, to + 1, v.y * inv);
-}
-
-template <int QT, int CT, int D, int CB, bool FULL>
+template <int QT, int CT, int D, int CB, int KS, bool FULL>
 hipError_t launch_16(const RowsArgs &a, hipStream_t s) {
     static std::atomic<unsigned long long> attr{0};
     constexpr int lds = 4 * kRTile * D * 2 + (CT >= 3 ? 4 * kRTile * 4 : 0);
-    return launch_with(&rows_attend_kernel<QT, CT, D, CB, FULL>, a, kRWaves * 32 * CB, lds, attr, s);
+    static_assert(KS == 1 || kRWaves / KS * CB * (D / 2 + 2) * 64 * 4 <= lds, "the join's registers past the tiles");
+    return launch_with(&rows_attend_kernel<QT, CT, D, CB, KS, FULL>, a, kRWaves / KS * 32 * CB, lds, attr, s);
 }
 
-template <int QT, int CT, int D, int CB>
+template <int QT, int CT, int D, int CB, int KS>
 hipError_t launch_16_full(const RowsArgs &a, hipStream_t s) {
-    return a.c.qk == D && a.c.vd == D ? launch_16<QT, CT, D, CB, true>(a, s) : launch_16<QT, CT, D, CB, false>(a, s);
+    return a.c.qk == D && a.c.vd == D ? launch_16<QT, CT, D, CB, KS, true>(a, s) : launch_16<QT, CT, D, CB, KS, false>(a, s);
 }
+
+// What the columns of a launch ask for: 32-column blocks a wavefront, halves of the keys.
+struct RowsShape {
+    int cb, ks;
+};
 
 template <int QT, int CT>
-hipError_t launch_16_width(const RowsArgs &a, int cb, hipStream_t s) {
+hipError_t launch_16_width(const RowsArgs &a, RowsShape x, hipStream_t s) {
     const int w = std::max(a.c.qk, a.c.vd);
-    if (w <= 64) return cb == 2 ? launch_16_full<QT, CT, 64, 2>(a, s) : launch_16_full<QT, CT, 64, 1>(a, s);
-    if (w <= 128) return launch_16_full<QT, CT, 128, 1>(a, s);
-    return launch_16_full<QT, CT, 256, 1>(a, s);
+    if (w <= 64)
+        return x.ks == 2   ? launch_16_full<QT, CT, 64, 1, 2>(a, s)
+               : x.cb == 2 ? launch_16_full<QT, CT, 64, 2, 1>(a, s)
+                           : launch_16_full<QT, CT, 64, 1, 1>(a, s);
+    if (w <= 128) return x.ks == 2 ? launch_16_full<QT, CT, 128, 1, 2>(a, s) : launch_16_full<QT, CT, 128, 1, 1>(a, s);
+    return x.ks == 2 ? launch_16_full<QT, CT, 256, 1, 2>(a, s) : launch_16_full<QT, CT, 256, 1, 1>(a, s);
 }
 
 // 16-bit products: queries of 16 bits over a cache of their type or of codes.
 bool rows_16(const RowsArgs &a) { return a.type != 0 && (a.c.type == a.type || a.c.type >= 3); }
 
 // 64 columns a wavefront for heads of up to 64 once they still give every CU a
-// workgroup: half the LDS reads an operation.
-int column_blocks(const RowsArgs &a, int cus) {
+// workgroup: half the LDS reads an operation. The keys in halves where 64 columns are all.
+RowsShape rows_shape(const RowsArgs &a, int cus) {
+    if (!rows_16(a)) return {1, 1};
     const long long cols = static_cast<long long>(a.t) * a.group, wide = kRWaves * 64;
-    return rows_16(a) && std::max(a.c.qk, a.c.vd) <= 64 && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= cus ? 2 : 1;
+    if (cols <= kRWaves / 2 * 32) return {1, 2};
+    return {std::max(a.c.qk, a.c.vd) <= 64 && 2 * cols > wide && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= 2 * cus ? 2 : 1, 1};
 }
 
 }  // namespace
 
-int rows_workgroup_columns(const RowsArgs &a, int cus) { return kRWaves * 32 * column_blocks(a, cus); }
+int rows_workgroup_columns(const RowsArgs &a, int cus) {
+    const RowsShape x = rows_shape(a, cus);
+    return kRWaves / x.ks * 32 * x.cb;
+}
 
 hipError_t launch_attend_rows(const RowsArgs &args, int cus, hipStream_t s) {
     RowsArgs a = args;
@@ -468,19 +487,32 @@ hipError_t launch_attend_rows(const RowsArgs &args, int cus, hipStream_t s) {
     if (((reinterpret_cast<uintptr_t>(a.out) | (a.out_stream * size) | (a.out_row * size)) & 7) == 0) a.aligned |= 2;
     hipError_t e;
     if (rows_16(a)) {
-        const int cb = column_blocks(a, cus);
+        const RowsShape x = rows_shape(a, cus);
         if (a.type == 1)
-            e = a.c.type == 1 ? launch_16_width<1, 1>(a, cb, s) : a.c.type == 3 ? launch_16_width<1, 3>(a, cb, s) : launch_16_width<1, 4>(a, cb, s);
+            e = a.c.type == 1 ? launch_16_width<1, 1>(a, x, s) : a.c.type == 4 ? launch_16_width<1, 4>(a, x, s) : launch_16_width<1, 3>(a, x, s);
         else
-            e = a.c.type == 2 ? launch_16_width<2, 2>(a, cb, s) : a.c.type == 3 ? launch_16_width<2, 3>(a, cb, s) : launch_16_width<2, 4>(a, cb, s);
+            e = a.c.type == 2 ? launch_16_width<2, 2>(a, x, s) : a.c.type == 4 ? launch_16_width<2, 4>(a, x, s) : launch_16_width<2, 3>(a, x, s);
     } else {
         e = launch_attend_rows_f32(a, s);
     }
     if (e != hipSuccess || !a.part) return e;
-    const int blocks = (a.c.vd + 127) / 128;
-    const long long grid = static_cast<long long>(a.batch) * a.t * a.heads * blocks;
-    hipLaunchKernelGGL(rows_join_kernel, dim3(static_cast<unsigned>(grid)), dim3(64), 0, s, a, blocks);
-    return hipGetLastError();
+    SplitArgs p;  // what the join reads
+    std::memset(&p, 0, sizeof p);
+    p.c = a.c;
+    p.q_len = a.rows;
+    p.pos = a.pos;
+    p.nk_max = a.nk_max;
+    p.t = a.t;
+    p.heads = a.heads;
+    p.batch = a.batch;
+    p.splits = a.splits;
+    p.out = a.out;
+    p.out_stream = a.out_stream;
+    p.out_row = a.out_row;
+    p.type = a.type;
+    p.part = a.part;
+    p.part_ml = a.part_ml;
+    return launch_attend_join(p, s);
 }
 
 }  // namespace cqhip
