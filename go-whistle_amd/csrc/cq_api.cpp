@@ -2925,8 +2925,8 @@ int nd_verify_drafts_dev(int32_t *accepted, int32_t *tokens, float *lp, const vo
                 return fail(CQ_ERR_MISUSE, "needle: verified tokens onto their inputs");
     }
     VerifyArgs a{accepted, tokens, lp, target, draft, target_stream, target_row, draft_stream, draft_row, type, batch, t, n,
-                 drafts, drafted, u, u_next, temperature > 0.0 ? 1.0 / temperature : 0.0, 1, n, nullptr};
-    const size_t bytes = verify_parts(a, device_info().cus);
+                 drafts, drafted, u, u_next, temperature > 0.0 ? 1.0 / temperature : 0.0, 1, n, 1, nullptr};
+    const size_t bytes = verify_parts(a);
     if ((2.0 * t + 1) * batch * a.splits > static_cast<double>(grid_limit(1024)))
         return fail(CQ_ERR_UNSUPPORTED, "needle: %d x %d drafts of %d tokens", batch, t, n);
     WsScope ws;

@@ -621,10 +621,11 @@ struct VerifyArgs {
     const float *u, *u_next;
     double inv_temp;  // 0: greedy
     int splits, chunk;
+    int choose_parts;  // of the sampled row
     double *part;
 };
-// Sets splits and chunk; the bytes of part.
-size_t verify_parts(VerifyArgs &a, int cus);
+// Sets the parts; the bytes of `part`.
+size_t verify_parts(VerifyArgs &a);
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 
 // nd_logprobs_dev: `splits` parts of `chunk` logits (a multiple of 8) a row; the parts' results

@@ -90,10 +90,9 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, unsigned
     const int z = h >= a.heads[0];
     if (z) h -= a.heads[0];
     const int b = static_cast<int>(bi / a.t), i = static_cast<int>(bi - static_cast<unsigned>(b) * a.t);
-    if (a.rows) {
-        const int n = a.rows[b];
-        if (n > a.t || i >= n) return;
-    }
+    const int n = a.rows ? a.rows[b] : a.t;  // both asked for before either is looked at
+    const long long p = a.cos_t ? static_cast<long long>(a.pos[b]) + i : 0;
+    if (n > a.t || i >= n) return;
     const int half = a.width / 2, d = V * (threadIdx.x & (LANES - 1));
     const bool live = d < half;
     float x[2][V];
@@ -147,7 +146,6 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, unsigned
     }
     if (!live) return;
     if (a.cos_t) {
-        const long long p = static_cast<long long>(a.pos[b]) + i;
         if (p >= 0 && p < a.positions) {
             const float *c = a.cos_t + p * half + d, *s = a.sin_t + p * half + d;
 #pragma unroll

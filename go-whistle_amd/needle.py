@@ -508,40 +508,57 @@ def qk_norm_rope_dev(q_out, k_out, q, k, q_gain=None, k_gain=None, rope=None, po
     some = q if q is not None else k
     if some is None or (q is None) != (q_out is None) or (k is None) != (k_out is None):
         raise CQPanic("needle: norms without heads or without an output for them")
-    if some.dim() != 4:
+    shape = some.shape
+    if len(shape) != 4:
         raise CQPanic("needle: norms of [streams, rows, heads, width]")
-    B, t, _, width = some.shape
+    B, t, heads, width = shape
     code, dtype, dev = _type(some, "heads"), some.dtype, _index(some, "heads")
-    heads, strides = [0, 0], [0] * 8
-    for z, (x, y, what) in enumerate(((q, q_out, "queries"), (k, k_out, "keys"))):
-        if x is None:
-            continue
-        n = heads[z] = x.shape[2] if x.dim() == 4 else 0
-        _want(x, what, (B, t, n, width), dtype, dev, False)
-        _want(y, f"normed {what}", (B, t, n, width), dtype, dev, False)
-        xs, ys = x.stride(), y.stride()
-        if xs[3] != 1 or ys[3] != 1 or (n > 1 and (xs[2] != width or ys[2] != width)):
-            raise CQPanic(f"needle: {what} whose heads are not side by side")
-        strides[2 * z], strides[2 * z + 1], strides[4 + 2 * z], strides[5 + 2 * z] = xs[0], xs[1], ys[0], ys[1]
-    for gain, what in ((q_gain, "query gains"), (k_gain, "key gains")):
-        if gain is not None:
-            _want(gain, what, (width,), _f32, dev)
-    cos, sin, positions = None, None, 0
+    kv_heads = 0
+    if q is None:
+        heads, qs, qo = 0, (0, 0), (0, 0)
+    else:
+        if q_out.shape != shape or q_out.dtype is not dtype or q_out.get_device() != dev:
+            _want(q_out, "normed queries", shape, dtype, dev, False)
+        qs, qo = q.stride(), q_out.stride()
+        if qs[3] != 1 or qo[3] != 1 or (heads > 1 and (qs[2] != width or qo[2] != width)):
+            raise CQPanic("needle: queries whose heads are not side by side")
+    if k is None:
+        ks = ko = (0, 0)
+    else:
+        kv_heads = k.shape[2] if k.dim() == 4 else 0
+        shape = (B, t, kv_heads, width)
+        if k.shape != shape or k.dtype is not dtype or k.get_device() != dev:
+            _want(k, "keys", shape, dtype, dev, False)
+        if k_out.shape != shape or k_out.dtype is not dtype or k_out.get_device() != dev:
+            _want(k_out, "normed keys", shape, dtype, dev, False)
+        ks, ko = k.stride(), k_out.stride()
+        if ks[3] != 1 or ko[3] != 1 or (kv_heads > 1 and (ks[2] != width or ko[2] != width)):
+            raise CQPanic("needle: keys whose heads are not side by side")
+    qg = kg = cos = sin = at = None
+    if q_gain is not None:
+        _want(q_gain, "query gains", (width,), _f32, dev)
+        qg = q_gain.data_ptr()
+    if k_gain is not None:
+        _want(k_gain, "key gains", (width,), _f32, dev)
+        kg = k_gain.data_ptr()
+    positions = 0
     if rope is not None:
         cos, sin = rope
         positions = cos.shape[0] if cos.dim() == 2 else 0
-        _want(cos, "cosines", (positions, width // 2), _f32, dev)
-        _want(sin, "sines", (positions, width // 2), _f32, dev)
+        shape = (positions, width // 2)
+        _want(cos, "cosines", shape, _f32, dev)
+        _want(sin, "sines", shape, _f32, dev)
         if pos is None:
             raise CQPanic("needle: RoPE without positions")
         _want(pos, "positions", (B,), _i32, dev)
+        cos, sin, at = cos.data_ptr(), sin.data_ptr(), pos.data_ptr()
     if rows is not None:
         _want(rows, "row counts", (B,), _i32, dev)
-    if max(B, t, *heads, width, positions) > _INT:
-        _sizes("norms", B, t, *heads, width, positions)
-    _call(lib().nd_qk_norm_rope_dev, dev, _ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), code, _heads_layout(*strides), B, t,
-          heads[0], heads[1], width, _ptr(q_gain), _ptr(k_gain), _ptr(cos), _ptr(sin), positions,
-          _ptr(pos) if rope is not None else None, _ptr(rows))
+    if B > _INT or t > _INT or heads > _INT or kv_heads > _INT or width > _INT or positions > _INT:
+        _sizes("norms", B, t, heads, kv_heads, width, positions)
+    _call(lib().nd_qk_norm_rope_dev, dev, _ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), code,
+          _heads_layout(qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1]), B, t, heads, kv_heads, width, qg, kg, cos, sin,
+          positions, at, _ptr(rows))
 
 
 def verify_drafts_dev(accepted, tokens, target, drafts, draft=None, u=None, u_next=None, drafted=None, temperature=1.0,

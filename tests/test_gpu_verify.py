@@ -121,6 +121,20 @@ def test_greedy_takes_the_first_of_equals():
     assert a.tolist() == [2, 1] and tok.tolist() == [[4321, 4090, 0], [0, 0, -1]]
 
 
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("n", [40, 20000])
+def test_many_drafts(temperature, n):
+    # more than a workgroup keeps the statistics of, nearly all of them kept
+    import torch
+
+    x, y, d, u, nxt = inputs(8, "float32", 2, 150, n, near=1e-3)
+    d = x[:, :150].argmax(-1).int()
+    d[1, 100] = (d[1, 100] + 1) % n
+    u = u * 0.5
+    a, _ = verify(x, d, y, u, nxt, None, temperature)
+    assert a.max() > 64
+
+
 def test_far_logits():
     # differences past float64's exponents, and a temperature that makes them so
     import torch
