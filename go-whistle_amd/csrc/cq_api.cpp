@@ -2446,12 +2446,11 @@ int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream,
     if (!out || !q || !pos) return fail(CQ_ERR_MISUSE, "needle: attention with a nil operand");
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % value_size(type))
         return fail(CQ_ERR_MISUSE, "needle: queries or outputs that are not aligned to their type");
-    a.q_row = q_row || q_stream ? q_row : static_cast<long long>(heads) * c->qk;
-    a.q_stream = q_row || q_stream ? q_stream : a.q_row * t;
-    const bool dense = !out_row && !out_stream;
+    a.q_row = q_row;
+    a.q_stream = q_stream;
     const long long width = static_cast<long long>(heads) * c->vd;
-    a.out_row = dense ? width : out_row;
-    a.out_stream = dense ? width * t : out_stream;
+    a.out_row = out_row;
+    a.out_stream = out_stream;
     // Of rows[b] rows the host knows only that they are rows.
     if (rows ? !rows_apart(width, batch, a.out_stream, 1, 0) || !rows_apart(width, t, a.out_row, 1, 0)
              : !rows_apart(width, batch, a.out_stream, t, a.out_row))

@@ -114,6 +114,11 @@ __device__ __forceinline__ void repair_columns(const RowsArgs &a, const RowsPlac
         const int col = col0 + c, row = col / a.group, head = p.h * a.group + col % a.group, at = p.pos + row;
         const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(row) * a.q_row +
                              static_cast<long long>(head) * a.c.qk;
+        bool nan = false;  // of the query: the outputs are NaN as they stand
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < a.c.qk) nan |= isnan(load_any(a.q, a.type, qo + lane + 64 * e));
+        if (__any(nan)) continue;
         float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int i = p.i0; i < p.i1; ++i)
             for (int j0 = tile_key<KEYS>(p, i), j1 = j0 + KEYS; j0 < j1; j0 += 64) {

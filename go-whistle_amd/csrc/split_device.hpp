@@ -285,13 +285,19 @@ __device__ __forceinline__ bool sees_row(const SplitArgs &a, int p, int j) {
 // weight 0, and 0 times an infinite or NaN value is NaN, as are parts of a weight
 // times an infinity: columns that come out as NaN are computed here, which
 // skips what they do not see. Rare, so plain. Returns value d = lane + 64 e in o[e].
+// false, and nothing, of a query that holds a NaN, whose outputs are NaN as they stand.
 template <int TYPE>
-__device__ __forceinline__ void repair_column(const SplitArgs &a, const Place &p, int row, int head, float &m, float &l,
+__device__ __forceinline__ bool repair_column(const SplitArgs &a, const Place &p, int row, int head, float &m, float &l,
                                               float (&o)[4]) {
     const int lane = threadIdx.x & 63, at = a.pos[p.b] + row;
     const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(row) * a.q_row +
                          static_cast<long long>(head) * a.c.qk;
     const unsigned char *kp = a.c.k + static_cast<long long>(p.h) * a.k_head, *vp = a.c.v + static_cast<long long>(p.h) * a.v_head;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.c.qk) nan |= isnan(load_value(a.q, a.type, qo + lane + 64 * e));
+    if (__any(nan)) return false;
     m = -INFINITY;
     l = o[0] = o[1] = o[2] = o[3] = 0.0f;
     auto value = [&](const unsigned char *r, int d) {
@@ -344,6 +350,7 @@ __device__ __forceinline__ void repair_column(const SplitArgs &a, const Place &p
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) l += xor_lane(l, s);
+    return true;
 }
 
 // Joins the wavefronts' columns (o, ml filled, outputs relative to each
@@ -402,7 +409,7 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
             int row, head;
             column_of(a, p, col0 + n, row, head);
             float m, l, o[4];
-            repair_column<TYPE>(a, p, row, head, m, l, o);
+            if (!repair_column<TYPE>(a, p, row, head, m, l, o)) continue;
             const float inv = a.part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             const long long pi = part_at(a, p, row, head);
 #pragma unroll

@@ -271,7 +271,7 @@ __device__ Decision decide(const VerifyArgs &a, int b, bool write) {
         const double x = known ? logit<TYPE>(a.target, b * a.target_stream + i * a.target_row + d) : 0.0f;
         const double y = known && a.draft ? logit<TYPE>(a.draft, b * a.draft_stream + i * a.draft_row + d) : 0.0f;
         const RowStat p = row_stat(a, b, i, lanes, at);
-        const RowStat q = a.draft ? row_stat(a, b, a.t + 1 + min(i, a.t - 1), lanes, at) : RowStat{0.0, 1.0, 0};
+        const RowStat q = a.draft && n > 0 ? row_stat(a, b, a.t + 1 + min(i, n - 1), lanes, at) : RowStat{0.0, 1.0, 0};
         bool ok = known && p.s > 0.0 && p.s < INFINITY;  // p.s: no NaN
         if (it == 0.0) {
             ok = ok && p.first == d;
@@ -297,7 +297,7 @@ __device__ Decision decide(const VerifyArgs &a, int b, bool write) {
         c.q = stats[1][c.a];
     } else {
         c.p = row_stat(a, b, c.a, lanes, at);
-        c.q = a.draft ? row_stat(a, b, a.t + 1 + min(c.a, a.t - 1), lanes, at) : RowStat{0.0, 1.0, 0};
+        c.q = a.draft && n > 0 ? row_stat(a, b, a.t + 1 + min(c.a, n - 1), lanes, at) : RowStat{0.0, 1.0, 0};
     }
     if (write && a.lp)
         for (int i = tid; i < min(c.a, kKeep); i += kCThreads) a.lp[static_cast<long long>(b) * (a.t + 1) + i] = lps[i];

@@ -582,7 +582,7 @@ int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long 
  * nk_max), and rows past the count leave their outputs as they were. q and out
  * hold values of `type` (ND_F32, ND_F16, ND_BF16): row i of stream b is
  * heads*qk values at element b*q_stream + i*q_row (heads*vd at b*out_stream +
- * i*out_row; a stream and row stride of 0: dense [batch][t][heads][width]).
+ * i*out_row).
  * Query head h reads key head h / (heads/kv_heads). A page outside the pool
  * reads page 0. Cache rows that no row attends may hold anything. The written
  * output rows share no element, and none with q.

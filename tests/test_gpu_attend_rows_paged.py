@@ -103,6 +103,38 @@ def test_strided_and_unaligned(io, name):
         check_rows(c, name, out, before, q, [3, 80], None, c.cap, 0, 0, 8.0, 5)
 
 
+@pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float32", "float16"), ("float16", "e4m3")])
+@pytest.mark.parametrize("t", [1, 3, 40])
+def test_one_query_for_all(io, name, t):
+    # a query of one stream, of one row, or of one of both, expanded: strides of 0
+    import torch
+
+    c = make_cache(gen(t), name, 3, 8, 16, 2, 64, 64)
+    for shape in ((1, t), (3, 1), (1, 1)):
+        q = torch.randn(*shape, 4, 64, generator=gen(2), device="cuda").to(getattr(torch, io)).expand(3, t, 4, 64)
+        out, want = torch.zeros(3, t, 4, 64, device="cuda", dtype=q.dtype), torch.zeros(3, t, 4, 64, device="cuda", dtype=q.dtype)
+        c.attend_rows_dev(out, q, i32([0, 30, 60]), 8.0)
+        c.attend_rows_dev(want, q.contiguous(), i32([0, 30, 60]), 8.0)
+        assert torch.equal(out, want) and out.count_nonzero() > 0
+
+
+def test_queries_that_are_not_numbers():
+    # NaN rows are NaN, and the others within the bounds of what they are without them
+    import torch
+
+    for io, name, t in (("bfloat16", "bfloat16", 200), ("float32", "float16", 6), ("float16", "e4m3", 100), ("float32", "float32", 600)):
+        c = make_cache(gen(t), name, 2, 60, 16, 2, 64, 64)
+        q = torch.randn(2, t, 4, 64, generator=gen(3), device="cuda").to(getattr(torch, io))
+        out, bad = torch.zeros_like(q), torch.zeros_like(q)
+        c.attend_rows_dev(out, q, i32([0, 90]), 8.0)
+        some = q.clone()
+        some[0, 3, 1, 7], some[1, t - 1, 0] = math.nan, math.nan
+        c.attend_rows_dev(bad, some, i32([0, 90]), 8.0)
+        assert bad[0, 3, 1].isnan().all() and bad[1, t - 1, 0].isnan().all()
+        bad[0, 3, 1], bad[1, t - 1, 0] = out[0, 3, 1], out[1, t - 1, 0]
+        check_rows(c, name, bad, torch.zeros_like(q), q, [0, 90], None, c.cap, 0, 0, 8.0, 30)
+
+
 def poison(c, b, row, what, values=True, keys=True):
     R = c.k.shape[1]
     pg = int(c.pages[b, row // R])

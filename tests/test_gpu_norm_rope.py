@@ -119,3 +119,17 @@ def test_values_at_the_ends_of_the_types():
         needle.qk_norm_rope_dev(out, None, x, None, gain)
         assert (out[0, 0] == 0).all() and ((out[0, 1].float() - 1).abs() <= 2 * half_ulp(dt)).all()
         assert out[0, 2].isnan().all() and out[0, 3].isfinite().all()
+
+
+def test_one_row_for_all():
+    # expanded inputs: strides of 0
+    import torch
+
+    g = gen(9)
+    gain, (cos, sin) = torch.rand(64, generator=g, device="cuda"), tables(g, 40, 64)
+    for shape in ((1, 5), (3, 1), (1, 1)):
+        x = torch.randn(*shape, 2, 64, generator=g, device="cuda").expand(3, 5, 2, 64)
+        out, want = torch.zeros(3, 5, 2, 64, device="cuda"), torch.zeros(3, 5, 2, 64, device="cuda")
+        needle.qk_norm_rope_dev(out, None, x, None, gain, None, (cos, sin), i32([0, 7, 30]))
+        needle.qk_norm_rope_dev(want, None, x.contiguous(), None, gain, None, (cos, sin), i32([0, 7, 30]))
+        assert torch.equal(out, want) and out.count_nonzero() > 0

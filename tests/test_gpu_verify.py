@@ -75,6 +75,14 @@ def test_strided_logits(io):
         verify(wide[..., off:off + 1000], d, drow[..., off:off + 1000].transpose(0, 1), u, nxt, None, 1.0)
 
 
+def test_one_row_for_all():
+    # expanded logits: strides of 0
+    x, y, d, u, nxt = inputs(9, "float32", 4, 3, 1500)
+    verify(x[:1].expand(4, 4, 1500), d, y[:1].expand(4, 3, 1500), u, nxt, None, 1.0)
+    verify(x[:, :1].expand(4, 4, 1500), d, y[:, :1].expand(4, 3, 1500), u, nxt, None, 1.0)
+    verify(x[:1, :1].expand(4, 4, 1500), d, None, u, nxt, [3, 0, 1, 2], 1.0)
+
+
 def test_random_numbers_at_the_ends():
     import torch
 

@@ -24,8 +24,8 @@ def read(c=None, k=P, v=P, ks=400, kr=128, vs=400, vr=128, typ=0, batch=2, t=3, 
     check(lib().kv_read_paged_dev(c or cache(), k, ks, kr, v, vs, vr, typ, batch, t, rows, pos, None))
 
 
-def attend(c=None, out=P, os=0, orow=0, q=P, typ=0, batch=2, t=3, heads=4, rows=None, pos=P, nk=64, window=0, sink=0, scale=8.0):
-    check(lib().kv_attend_rows_paged_dev(c or cache(), out, os, orow, q, 0, 0, typ, batch, t, heads, rows, pos, nk, window,
+def attend(c=None, out=P, os=768, orow=256, q=P, typ=0, batch=2, t=3, heads=4, rows=None, pos=P, nk=64, window=0, sink=0, scale=8.0):
+    check(lib().kv_attend_rows_paged_dev(c or cache(), out, os, orow, q, 768, 256, typ, batch, t, heads, rows, pos, nk, window,
                                          sink, scale, None))
 
 
@@ -86,7 +86,7 @@ def test_bad_caches(call, edit, err):
     (attend, dict(sink=-1)), (attend, dict(typ=3)), (attend, dict(heads=3)), (attend, dict(heads=0)), (attend, dict(scale=0.0)),
     (attend, dict(scale=-1.0)), (attend, dict(scale=float("nan"))), (attend, dict(scale=1e-40)), (attend, dict(out=None)),
     (attend, dict(q=None)), (attend, dict(pos=None)), (attend, dict(q=P + 2)), (attend, dict(typ=2, out=P + 1)),
-    (attend, dict(os=768, orow=255)), (attend, dict(os=700, orow=256)), (attend, dict(os=255, orow=256, rows=P)),
+    (attend, dict(os=768, orow=255)), (attend, dict(os=0, orow=0)), (attend, dict(os=768, orow=0)), (attend, dict(os=700, orow=256)), (attend, dict(os=255, orow=256, rows=P)),
     (norm, dict(batch=-1)), (norm, dict(t=-1)), (norm, dict(heads=-1)), (norm, dict(kv_heads=-1)), (norm, dict(typ=3)),
     (norm, dict(positions=-1)), (norm, dict(cos=None)), (norm, dict(sin=None)), (norm, dict(pos=None)), (norm, dict(q=None)),
     (norm, dict(k=None)), (norm, dict(qo=None)), (norm, dict(ko=None)), (norm, dict(q=FAR + 2)), (norm, dict(typ=1, k=FAR + 1)),
@@ -105,7 +105,7 @@ def test_misuse(call, kw):
 @pytest.mark.parametrize("call,kw", [
     (read, dict(batch=1 << 20, t=64, kr=128, ks=1 << 20, vr=128, vs=1 << 20)), (norm, dict(width=40)), (norm, dict(width=272)),
     (norm, dict(width=0)), (norm, dict(batch=1 << 16, t=1 << 14, layout=None, q=1 << 60, k=1 << 61, qo=FAR, ko=1 << 59)),
-    (attend, dict(batch=1 << 16, t=1 << 16)), (verify, dict(n=(1 << 30) + 1)), (verify, dict(t=(1 << 20) + 1)),
+    (attend, dict(batch=1 << 16, t=1 << 16, os=1 << 24)), (verify, dict(n=(1 << 30) + 1)), (verify, dict(t=(1 << 20) + 1)),
     (verify, dict(batch=1 << 24, n=1 << 20, tok=1 << 50, lp=1 << 51, drafts=1 << 52, u=1 << 53, nxt=1 << 54)),
 ])
 def test_unsupported(call, kw):
