@@ -2573,15 +2573,19 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream) {
             1, std::min<long long>({8LL * cus / (lists * a.waves), nk / (64LL * a.waves), 64})));
     }
     if (!many && a.pos && a.t > 1 && 2 * lists >= cus) {
-        // Rows of many lists, whose streams differ in length: smaller workgroups
-        // and more parts (5 rows of 32 streams of up to 8000 e4m3 keys, 32 heads of
-        // 128 over 8, 256 lists: 100 us with four wavefronts and three parts, 108
-        // with eight and one, 105 with two and six).
+        // Rows of many lists: smaller workgroups, and parts until the CUs hold no
+        // more wavefronts, eight of a CU's 12 with two tiles of columns or wide 16-bit
+        // heads; but where the streams' counts are given, and so their lists
+        // differ, half a round more, the long ones first (5 rows of 32 streams of
+        // e4m3 keys, 32 heads of 128 over 8, 256 lists: two, three and four parts 105,
+        // 95 and 98 us of up to 8000 keys, 80, 95 and 92 of 4000 each).
         a.waves = std::min(a.waves, 4);
-        const int fit = a.tile > 16 || std::max(a.c.qk, a.c.vd) > 64 && a.c.type < 3 ? 8 : 12;  // wavefronts a CU holds
+        const bool heavy = a.tile > 16 || (std::max(a.c.qk, a.c.vd) > 64 && a.c.type < 3);
+        const int fit = heavy && !a.q_len ? 8 : 12;
         a.splits = static_cast<int>(
             std::max<long long>(1, std::min<long long>({1LL * fit * cus / (lists * a.waves), nk / (64LL * a.waves), 64})));
     }
+    a.by_length = !many && a.pos && a.q_len && a.batch > 1 && a.batch <= 64 && lists * a.splits * a.waves > 8LL * cus;
     const int qsize = value_size(a.type);
     a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stream * qsize) |
                 static_cast<uintptr_t>(a.q_row * qsize)) & (4 * qsize - 1)) == 0;

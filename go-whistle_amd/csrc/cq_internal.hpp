@@ -545,7 +545,7 @@ struct SplitArgs {
     int group;                               // heads a key head
     int splits;                              // parts of a list, at most 64
     int tile, waves;                         // columns and wavefronts of a workgroup (attend_split)
-    int by_length;                           // streams of long memories first (cross_attend)
+    int by_length;                           // streams of long memories first (cross_attend), of long lists (causal rows)
     const void *q;
     void *out;
     long long q_stream, q_row, out_stream, out_row;  // elements

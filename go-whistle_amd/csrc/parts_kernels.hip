@@ -14,6 +14,7 @@
 #include "split_device.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cqhip {
 namespace {
@@ -86,6 +87,9 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
     constexpr int kTile = 16 * kSub;
     constexpr int kColumns = kCols * TILES;
     constexpr bool kParts16 = TYPE != 0;      // the second product in 16 bits
+    // A tile's values are asked for a tile ahead too, where the registers of two
+    // wavefronts a SIMD hold them (codes, two tiles of columns).
+    constexpr bool kAhead = kScaled<TYPE> && TILES == 2;
     // How far logits may pass the maximum before sums and outputs are scaled to
     // a new one: by 2^8, but not in float16, whose lift leaves no room.
     constexpr float kLag = TYPE == 1 ? 0.0f : 8.0f;
@@ -105,49 +109,72 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
         col_pos[t] = CAUSAL ? a.pos[p.b] + (col_ok[t] ? col[t] : p.cols - 1) / p.group : 0;
     }
 
+    // Row of the lane's key of a tile (its first kTile lanes; keys past the part's last read that one's row).
+    // Rows are looked up two tiles ahead, keys loaded one ahead, scales too; the
+    // first ones' page table entries are asked for before the queries.
+    auto row_of = [&](int j) { return array_row(a, p, min(j + (lane & (kTile - 1)), p.j1 - 1)); };
+    const int step = waves * kTile;
+    int j = p.j0 + wave * kTile, rows = 0, rows_next = 0;
+    if (j < p.j1) {
+        rows = row_of(j);
+        rows_next = row_of(j + step);
+    }
+
     // The query's pieces: in float32 with 1/scale and log2(e) folded in, or in
-    // 16-bit parts of eight.
+    // 16-bit parts of eight. All of them are asked for before any is looked at.
     constexpr int kEights = PARTS ? kPer / 8 : 1;
     float qv[TILES][PARTS ? 1 : kPieces * kPer];
     uint32_t qp[TILES][PARTS ? PARTS : 1][kPieces][kEights][4];
+    {
+        float x[TILES][kPieces][kPer];
+        auto load_all = [&](auto vec) {
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const long long qo = query_at(a, p, col_ok[t] ? col[t] : 0);
+            for (int t = 0; t < TILES; ++t) {
+                const long long qo = query_at(a, p, col_ok[t] ? col[t] : 0);
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            const int d0 = (4 * k + c) * kPer;
-            float x[kPer];
-            if (col_ok[t] && d0 < a.c.qk) {
-                load_query<kPer>(x, a, qo + d0, PARTS ? 1.0f : a.scale_log2);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
+                for (int k = 0; k < kPieces; ++k) {
+                    const int d0 = (4 * k + c) * kPer;
+                    load_query_values<kPer, decltype(vec)::value>(x[t][k], a, qo + (d0 < a.c.qk ? d0 : 0));
+                }
             }
-            if constexpr (PARTS == 0) {
+        };
+        if (a.q_vec)
+            load_all(std::true_type{});
+        else
+            load_all(std::false_type{});
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) qv[t][k * kPer + e] = x[e];
-            } else if constexpr (TYPE == 1) {  // a float16 query
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                for (int e = 0; e < kPer; e += 2)
-                    qp[t][0][k][e / 8][e / 2 % 4] =
-                        __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e])) |
-                        static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e + 1]))) << 16;
-            } else {
+            for (int k = 0; k < kPieces; ++k) {
+                const bool ok = col_ok[t] && (4 * k + c) * kPer < a.c.qk;
+                float (&y)[kPer] = x[t][k];
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) x[e] = __builtin_canonicalizef(x[e]);  // a NaN's mark in the upper half
+                for (int e = 0; e < kPer; ++e) y[e] = ok ? y[e] : 0.0f;
+                if constexpr (PARTS == 0) {
 #pragma unroll
-                for (int z = 0; z < PARTS; ++z)
+                    for (int e = 0; e < kPer; ++e) qv[t][k * kPer + e] = y[e] * a.scale_log2;
+                } else if constexpr (TYPE == 1) {  // a float16 query
 #pragma unroll
-                    for (int e = 0; e < kPer; e += 2) {
-                        qp[t][z][k][e / 8][e / 2 % 4] = upper_pair(x[e], x[e + 1]);
+                    for (int e = 0; e < kPer; e += 2)
+                        qp[t][0][k][e / 8][e / 2 % 4] =
+                            __builtin_bit_cast(uint16_t, static_cast<_Float16>(y[e])) |
+                            static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(y[e + 1]))) << 16;
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {  // what the part leaves: nothing of an infinity
-                            const float part = __uint_as_float(__float_as_uint(x[e + i]) & 0xffff0000u);
-                            x[e + i] = fabsf(part) < INFINITY ? x[e + i] - part : 0.0f;
+                    for (int e = 0; e < kPer; ++e) y[e] = __builtin_canonicalizef(y[e]);  // a NaN's mark in the upper half
+#pragma unroll
+                    for (int z = 0; z < PARTS; ++z)
+#pragma unroll
+                        for (int e = 0; e < kPer; e += 2) {
+                            qp[t][z][k][e / 8][e / 2 % 4] = upper_pair(y[e], y[e + 1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {  // what the part leaves: nothing of an infinity
+                                const float part = __uint_as_float(__float_as_uint(y[e + i]) & 0xffff0000u);
+                                y[e + i] = fabsf(part) < INFINITY ? y[e + i] - part : 0.0f;
+                            }
                         }
-                    }
+                }
             }
-        }
     }
 
     f32x4 o[TILES][kVals];
@@ -163,8 +190,6 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
     const unsigned char *kp = a.c.k + static_cast<long long>(p.h) * a.k_head, *vp = a.c.v + static_cast<long long>(p.h) * a.v_head;
     const int v_piece = r * kVals < a.c.vd ? r * (kVals * kSize) : 0;  // past the width: outputs that nothing reads
 
-    // Row of the lane's key of a tile (its first kTile lanes; keys past the part's last read that one's row).
-    auto row_of = [&](int j) { return array_row(a, p, min(j + (lane & (kTile - 1)), p.j1 - 1)); };
     auto load_keys = [&](uint32_t (&kw)[kSub][kPieces][4], int rows) {
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
@@ -198,20 +223,27 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
 
     float *lg = CAUSAL ? nullptr : a.logits;
     if (lg) lg += ((static_cast<long long>(p.b) * a.c.kv_heads + p.h) * p.group + (col_ok[0] ? col[0] : 0)) * a.nk_max;
-    const int step = waves * kTile;
-    int j = p.j0 + wave * kTile;
     if (j < p.j1) {
-        // Rows are looked up two tiles ahead, keys loaded one ahead, scales too.
-        int rows = row_of(j);
         uint32_t kw[kSub][kPieces][4];
         float scales[2] = {1.0f, 1.0f};
         load_keys(kw, rows);
         load_scales(scales, rows);
-        int rows_next = j + step < p.j1 ? row_of(j + step) : rows;
+        uint32_t va[kAhead ? kSub : 1][4][kVWords];
+        if constexpr (kAhead) load_values(va, rows);
         for (; j < p.j1; j += step) {
             const int jn = j + step;
             uint32_t vw[kSub][4][kVWords];
-            load_values(vw, rows);
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < kVWords; ++k) vw[s][i][k] = va[s][i][k];
+                if (jn < p.j1) load_values(va, rows_next);
+            } else {
+                load_values(vw, rows);
+            }
             int rows_after = rows_next;
             if (jn + step < p.j1) rows_after = row_of(jn + step);
 
@@ -291,6 +323,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
             }
             // past the last key values of 0, not that key's: a weight of 0 times an infinity
             if (!kFinite<TYPE> && j + kTile > p.j1) {
+                asm volatile("" ::: "memory");  // a branch: as selects it is paid by every tile
 #pragma unroll
                 for (int s = 0; s < kSub; ++s)
 #pragma unroll
@@ -323,12 +356,13 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
                         sc[t][s][i] = x;
                     }
                 if (!all) {
+                    asm volatile("" ::: "memory");
 #pragma unroll
                     for (int s = 0; s < kSub; ++s)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int jj = j + 16 * s + 4 * c + i;
-                            const bool seen = jj < p.j1 && (!CAUSAL || sees_row(a, col_pos[t], p.kl.row(jj)));
+                            const bool seen = (jj < p.j1) & (!CAUSAL || sees_row(a, col_pos[t], p.kl.row(jj)));
                             sc[t][s][i] = seen ? sc[t][s][i] : -INFINITY;
                         }
                 }
