@@ -49,13 +49,14 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w, int pair) {
     return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);
 }
 
+constexpr float kRowsFar = 0x1p20f;  // from a maximum of it on, logits are rounded before it is subtracted, as it was
+
 // QT: the queries' type (1 float16, 2 bfloat16); CT: the cache's (QT itself, 3
 // int8, 4 e4m3); D: widths up to D; CB: 32-column blocks a wavefront; FULL:
 // both widths are D (else steps past a width are skipped by branches, which
 // keep the compiler from interleaving the products with the softmax).
-constexpr float kRowsFar = 0x1p20f;  // from a maximum of it on, logits are rounded before it is subtracted, as it was
-// KS: 1, or 2 where few columns would leave wavefronts idle: wavefronts 0 and 1
-// take the first 32 keys of a tile, 2 and 3 the others, joined at the end.
+// KS: 1, or 2 where few columns would leave wavefronts or CUs idle: wavefronts 0 and
+// 1 take the first 32 keys of a tile, 2 and 3 the others, joined at the end.
 template <int QT, int CT, int D, int CB, int KS, bool FULL>
 __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_kernel(RowsArgs a, int col_tiles) {
     constexpr bool kCodes = CT >= 3;
@@ -464,11 +465,15 @@ hipError_t launch_16_width(const RowsArgs &a, RowsShape x, hipStream_t s) {
 bool rows_16(const RowsArgs &a) { return a.type != 0 && (a.c.type == a.type || a.c.type >= 3); }
 
 // 64 columns a wavefront for heads of up to 64 once they still give every CU a
-// workgroup: half the LDS reads an operation. The keys in halves where 64 columns are all.
+// workgroup: half the LDS reads an operation. The keys in halves where 64
+// columns are all or workgroups of 128 do not give every CU two (a prompt of 448 rows,
+// 8 heads of 64: 14.3 us whole, 11.0 in halves; 2 of 500 rows behind 2500 keys, 16
+// heads of 128 over 4: 69 and 60; 4 of 1000, 512 such workgroups: 56 and 59).
 RowsShape rows_shape(const RowsArgs &a, int cus) {
     if (!rows_16(a)) return {1, 1};
     const long long cols = static_cast<long long>(a.t) * a.group, wide = kRWaves * 64;
-    if (cols <= kRWaves / 2 * 32) return {1, 2};
+    const long long blocks = (cols + kRWaves * 32 - 1) / (kRWaves * 32) * a.batch * a.c.kv_heads;
+    if (cols <= kRWaves / 2 * 32 || blocks < 2LL * cus) return {1, 2};
     return {std::max(a.c.qk, a.c.vd) <= 64 && 2 * cols > wide && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= 2 * cus ? 2 : 1, 1};
 }
 
