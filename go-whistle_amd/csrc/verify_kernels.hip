@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a) {
         double *r = const_cast<double *>(record(a, b, row, part));
         r[0] = m;
         r[1] = ((ws[0] + ws[1]) + ws[2]) + ws[3];
-        r[2] = j0 + first;
+        r[2] = static_cast<double>(j0) + min(first, a.n);  // a.n: no logit is a number, or none was looked for
     }
 }
 

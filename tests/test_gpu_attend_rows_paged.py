@@ -81,8 +81,37 @@ def test_few_rows_over_long_caches(io, name, t):
                                      ("float32", "float32")])
 @pytest.mark.parametrize("H,Hk,w", [(8, 8, 64), (8, 8, 48), (4, 2, 128), (4, 4, 96)])
 def test_many_streams(io, name, H, Hk, w):
-    # enough columns for 64 a wavefront, full and narrower heads
+    # many short lists, full and narrower heads
     run(H, io, name, H, Hk, w, w, 16, [(b * 37) % 200 for b in range(48)], 150, rows=[150 - b % 9 * 16 for b in range(48)], sample=1)
+
+
+@pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float16", "float16"), ("float16", "i8p"), ("bfloat16", "e4m3")])
+@pytest.mark.parametrize("H,Hk,w,t", [(8, 8, 64, 150), (8, 8, 48, 150), (16, 8, 128, 100), (8, 8, 112, 130), (8, 8, 256, 100),
+                                      (8, 8, 240, 70)])
+def test_workgroups_of_whole_tiles(io, name, H, Hk, w, t):
+    # so many lists that no workgroup takes a tile's keys in halves, and that narrow heads take 64 columns a wavefront
+    pos = [(b * 37) % 200 for b in range(64)]
+    run(t, io, name, H, Hk, w, w, 16, pos, t, sample=1)
+    run(w, io, name, H, Hk, w, w, 8, pos, t, rows=[t - b % 5 * 16 for b in range(64)], window=70, sink=5, sample=1)
+
+
+@pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float16", "float16"), ("bfloat16", "e4m3")])
+@pytest.mark.parametrize("Hk,w", [(8, 64), (8, 128), (8, 240)])
+def test_whole_tiles_with_values_that_are_not_finite(io, name, Hk, w):
+    # the value of row pos[b] is seen by the first 40 rows alone
+    import torch
+
+    g, t, window, B = gen(w), 150, 40, 64
+    pos = [(b * 37) % 200 for b in range(B)]
+    c = make_cache(g, name, B, -(-(max(pos) + t) // 16), 16, Hk, w, w)
+    for b in range(B):
+        poison(c, b, pos[b], math.nan, keys=False)
+    q = torch.randn(B, t, Hk, w, generator=g, device="cuda").to(getattr(torch, io))
+    out = torch.zeros_like(q)
+    c.attend_rows_dev(out, q, i32(pos), math.sqrt(w), window=window)
+    assert out[:, :window].isnan().all() and not out[:, window:].isnan().any()
+    rest = out[:, window:]
+    check_rows(c, name, rest, rest, q[:, window:], [p + window for p in pos], None, c.cap, window, 0, math.sqrt(w), 1, 3)
 
 
 @pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float32", "float16"), ("float16", "e4m3")])
