@@ -8,8 +8,12 @@ namespace cqhip {
 namespace {
 
 // 32 columns a wavefront on v_mfma_f32_32x32x2_f32, the products of
-// cross_attend_f32_kernel.
-template <int D, bool FULL>
+// cross_attend_f32_kernel. FULL: both widths are D. Else the tiles and queries are 0
+// past a width, and with SKIP no products are made there: branches that keep the
+// compiler from interleaving, taken where they leave out a quarter of wide heads or
+// more (16 prompts of 448 rows, 8 heads over 4 of 144: 278 us, 355 without; of 240: 460
+// and 370; of 80 116 and 111; 8 heads of 16 79 and 71, of 48 162 and 74).
+template <int D, bool FULL, bool SKIP>
 __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f32_kernel(RowsArgs a, int col_tiles) {
     constexpr int kKeys = D == 64 ? 64 : 32;   // keys a tile
     constexpr int kBytes = kKeys * D * 4;
@@ -109,14 +113,14 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
             for (int e = 0; e < 16; ++e) s[e] = 0.0f;
             const unsigned char *kr = kt + (32 * kb + n) * D * 4;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-                if (FULL || 8 * c < a.c.qk) {
-                    const float4 ka = *reinterpret_cast<const float4 *>(kr + ((2 * c + half) ^ (n & 15)) * 16);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.x, q[4 * c], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.y, q[4 * c + 1], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.z, q[4 * c + 2], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.w, q[4 * c + 3], s, 0, 0, 0);
-                }
+            for (int c = 0; c < D / 8; ++c) {
+                if (SKIP && 8 * c >= a.c.qk) break;
+                const float4 ka = *reinterpret_cast<const float4 *>(kr + ((2 * c + half) ^ (n & 15)) * 16);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.x, q[4 * c], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.y, q[4 * c + 1], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.z, q[4 * c + 2], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x2f32(ka.w, q[4 * c + 3], s, 0, 0, 0);
+            }
             if (!all_see(a, first, last, j0, j0 + 31)) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = sees(a, at, j0 + 8 * (e >> 2) + 4 * half + (e & 3)) ? s[e] : -INFINITY;
@@ -143,11 +147,11 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
             for (int e = 0; e < 16; ++e) {
                 const int row = 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
 #pragma unroll
-                for (int v = 0; v < D / 32; ++v)
-                    if (FULL || 32 * v < a.c.vd) {
-                        const float va = *reinterpret_cast<const float *>(vt + row * D * 4 + (((32 * v + n) * 4) ^ (half << 7)));
-                        o[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(va, s[e], o[v], 0, 0, 0);
-                    }
+                for (int v = 0; v < D / 32; ++v) {
+                    if (SKIP && 32 * v >= a.c.vd) break;
+                    const float va = *reinterpret_cast<const float *>(vt + row * D * 4 + (((32 * v + n) * 4) ^ (half << 7)));
+                    o[v] = __builtin_amdgcn_mfma_f32_32x32x2f32(va, s[e], o[v], 0, 0, 0);
+                }
             }
         }
         if (more) store(tile_key<kKeys>(p, i + 1), buf ^ 1);
@@ -185,10 +189,12 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
 
 template <int D>
 hipError_t launch_f32(const RowsArgs &a, hipStream_t s) {
-    static std::atomic<unsigned long long> full{0}, part{0};
+    static std::atomic<unsigned long long> full{0}, part{0}, skip{0};
     constexpr int lds = 4 * (D == 64 ? 64 : 32) * D * 4;
-    return a.c.qk == D && a.c.vd == D ? launch_with(&rows_attend_f32_kernel<D, true>, a, kRWaves * 32, lds, full, s)
-                                      : launch_with(&rows_attend_f32_kernel<D, false>, a, kRWaves * 32, lds, part, s);
+    if (a.c.qk == D && a.c.vd == D) return launch_with(&rows_attend_f32_kernel<D, true, false>, a, kRWaves * 32, lds, full, s);
+    if constexpr (D == 256)
+        if (4 * std::max(a.c.qk, a.c.vd) <= 3 * D) return launch_with(&rows_attend_f32_kernel<D, false, true>, a, kRWaves * 32, lds, skip, s);
+    return launch_with(&rows_attend_f32_kernel<D, false, false>, a, kRWaves * 32, lds, part, s);
 }
 
 }  // namespace

@@ -2,7 +2,7 @@
 // with a window and first rows that stay visible (kv_attend_rows_paged_dev).
 //
 // Per (stream, key head) the query columns are the rows times the group's
-// heads, 32 or 64 a wavefront. Tiles of 64 keys (32 for wide float32 heads)
+// heads, 32 a wavefront. Tiles of 64 keys (32 for wide float32 heads)
 // pass through LDS, two buffers, shared by the workgroup's four wavefronts;
 // both products run on 32x32 matrix instructions with the columns last, so a
 // lane keeps one column's maximum, sum and outputs (the lane orders of
@@ -52,12 +52,15 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w, int pair) {
 constexpr float kRowsFar = 0x1p20f;  // from a maximum of it on, logits are rounded before it is subtracted, as it was
 
 // QT: the queries' type (1 float16, 2 bfloat16); CT: the cache's (QT itself, 3
-// int8, 4 e4m3); D: widths up to D; CB: 32-column blocks a wavefront; FULL:
-// both widths are D (else steps past a width are skipped by branches, which
-// keep the compiler from interleaving the products with the softmax).
+// int8, 4 e4m3); D: widths up to D; FULL: both widths are D, else the tiles and
+// queries are 0 past a width and take part like others (branches around
+// those products keep the compiler from interleaving them with the softmax: 64 prompts
+// of 448 rows, 8 heads of 48 over 2, 96 us against 44; 32 of 80, 58 and 44).
+// 64 columns a wavefront, at half the LDS reads a product, lost too: 64 prompts of up to 448
+// rows, 8 heads of 64, 48 us against 36; 8 of 2000 rows, 16 heads over 4, 144 and 136.
 // KS: 1, or 2 where few columns would leave wavefronts or CUs idle: wavefronts 0 and
 // 1 take the first 32 keys of a tile, 2 and 3 the others, joined at the end.
-template <int QT, int CT, int D, int CB, int KS, bool FULL>
+template <int QT, int CT, int D, int KS, bool FULL>
 __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_kernel(RowsArgs a, int col_tiles) {
     constexpr bool kCodes = CT >= 3;
     constexpr int VT = kCodes ? 2 : QT;          // the values' type in LDS
@@ -70,18 +73,16 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, half = lane >> 5;
-    constexpr int kWgCols = kRWaves / KS * 32 * CB;
+    constexpr int kWgCols = kRWaves / KS * 32;
     constexpr int kBlocks = 2 / KS;              // blocks of 32 keys of a tile a wavefront takes
     const RowsPlace p = rows_place<kRTile>(a, col_tiles, kWgCols);
     if (!p.ok) return;
     const int col_wave = wave % (kRWaves / KS), block0 = wave / (kRWaves / KS);
-    const int col0 = p.ct * kWgCols + col_wave * 32 * CB;
+    const int col0 = p.ct * kWgCols + col_wave * 32;
     const bool live = col0 < p.cols;
     // the wavefront's rows' positions, its columns' own
-    const int first = p.pos + min(col0, p.cols - 1) / a.group, last = p.pos + (min(col0 + 32 * CB, p.cols) - 1) / a.group;
-    int at[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) at[cb] = p.pos + min(col0 + 32 * cb + n, p.cols - 1) / a.group;
+    const int first = p.pos + min(col0, p.cols - 1) / a.group, last = p.pos + (min(col0 + 32, p.cols) - 1) / a.group;
+    const int at = p.pos + min(col0 + n, p.cols - 1) / a.group;
 
     const unsigned char *kp = a.c.k + static_cast<long long>(p.h) * a.k_head;
     const unsigned char *vp = a.c.v + static_cast<long long>(p.h) * a.v_head;
@@ -156,45 +157,37 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
         __syncthreads();
     }
 
-    // The queries: lane (n, half) holds coordinates 16 s + 8 half + 0..7 of its columns.
-    s16x8 q[CB][D / 16];
+    // The queries: lane (n, half) holds coordinates 16 s + 8 half + 0..7 of its column.
+    s16x8 q[D / 16];
+    const int qcol = min(col0 + n, p.cols - 1);
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q) + static_cast<long long>(p.b) * a.q_stream +
+                         static_cast<long long>(qcol / a.group) * a.q_row +
+                         static_cast<long long>(p.h * a.group + qcol % a.group) * a.c.qk;
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const int col = min(col0 + 32 * cb + n, p.cols - 1);
-        const uint16_t *qp = static_cast<const uint16_t *>(a.q) + static_cast<long long>(p.b) * a.q_stream +
-                             static_cast<long long>(col / a.group) * a.q_row +
-                             static_cast<long long>(p.h * a.group + col % a.group) * a.c.qk;
+    for (int s = 0; s < D / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (FULL || 16 * s < a.c.qk) {
+            if (a.aligned & 1) {
+                x = *reinterpret_cast<const s16x8 *>(qp + d);
+            } else {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            const int d = 16 * s + 8 * half;
-            s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (FULL || 16 * s < a.c.qk) {
-                if (a.aligned & 1) {
-                    x = *reinterpret_cast<const s16x8 *>(qp + d);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = static_cast<short>(qp[d + e]);
-                }
+                for (int e = 0; e < 8; ++e) x[e] = static_cast<short>(qp[d + e]);
             }
-            q[cb][s] = x;
         }
+        q[s] = x;
     }
 
-    f32x16 o[CB][D / 32];
-    float m[CB], l[CB];
+    f32x16 o[D / 32];
     // LDS addresses: the keys' row n of a block, the values' row (lane % 16) / 4 and piece of a transposing read.
     const int kaddr = n * D * 2, kswz = k_swizzle<D>(n);
     const int ti = lane & 15, trow = 4 * half + (ti >> 2);
     const int vaddr = trow * D * 2 + 8 * (ti & 1), vpiece = 2 * ((lane >> 4) & 1) + ((ti & 3) >> 1), vswz = v_swizzle<D>(trow);
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        m[cb] = -INFINITY;
-        l[cb] = 0.0f;
+    for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-        for (int v = 0; v < D / 32; ++v)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[cb][v][i] = 0.0f;
-    }
+        for (int i = 0; i < 16; ++i) o[v][i] = 0.0f;
 
     // Rows are looked up two tiles ahead, tiles loaded one ahead.
     int rows = 0;
@@ -227,22 +220,17 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
         const int jw = j + 32 * block0;  // the wavefront's keys of the tile
         if (live && !none_sees(a, first, last, jw, jw + 32 * kBlocks - 1)) {
             const unsigned char *kt = smem + buf * 2 * kBytes + block0 * 32 * D * 2, *vt = kt + kBytes;
-            f32x16 s[CB][kBlocks];
+            f32x16 s[kBlocks];
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
+            for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
-                for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[cb][kb][e] = 0.0f;
+                for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
-                if (FULL || 16 * ks < a.c.qk) {
 #pragma unroll
-                    for (int kb = 0; kb < kBlocks; ++kb) {
-                        const s16x8 ka = *reinterpret_cast<const s16x8 *>(kt + kb * 32 * D * 2 + kaddr + ((2 * ks + half) ^ kswz) * 16);
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][kb] = mfma16<QT>(ka, q[cb][ks], s[cb][kb]);
-                    }
+                for (int kb = 0; kb < kBlocks; ++kb) {
+                    const s16x8 ka = *reinterpret_cast<const s16x8 *>(kt + kb * 32 * D * 2 + kaddr + ((2 * ks + half) ^ kswz) * 16);
+                    s[kb] = mfma16<QT>(ka, q[ks], s[kb]);
                 }
             if constexpr (kCodes) {
                 const float *ks = scales + 2 * buf * kRTile + 32 * block0 + 4 * half;
@@ -251,13 +239,10 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const float4 x = *reinterpret_cast<const float4 *>(ks + 32 * kb + 8 * g);
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) {
-                            s[cb][kb][4 * g] *= x.x;
-                            s[cb][kb][4 * g + 1] *= x.y;
-                            s[cb][kb][4 * g + 2] *= x.z;
-                            s[cb][kb][4 * g + 3] *= x.w;
-                        }
+                        s[kb][4 * g] *= x.x;
+                        s[kb][4 * g + 1] *= x.y;
+                        s[kb][4 * g + 2] *= x.z;
+                        s[kb][4 * g + 3] *= x.w;
                     }
             }
             if (!all_see(a, first, last, jw, jw + 32 * kBlocks - 1)) {
@@ -266,81 +251,69 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int key = jw + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) s[cb][kb][e] = sees(a, at[cb], key) ? s[cb][kb][e] : -INFINITY;
+                        s[kb][e] = sees(a, at, key) ? s[kb][e] : -INFINITY;
                     }
             }
-            u32x4 w[CB][2 * kBlocks], rest[CB][2 * kBlocks];
+            u32x4 w[2 * kBlocks], rest[2 * kBlocks];
+            float mt = s[0][0];
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                float mt = s[cb][0][0];
+            for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[0][e]);
+            if constexpr (kBlocks == 2) {
 #pragma unroll
-                for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[cb][0][e]);
-                if constexpr (kBlocks == 2) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[cb][1][e]);
-                }
-                mt = halves_max(mt) * a.scale_log2;
-                float scale = a.scale_log2;
-                if (__any(mt > m[cb] + 8.0f || fabsf(m[cb]) >= kRowsFar)) {
-                    const float mn = fmaxf(m[cb], mt);
-                    const float f = m[cb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
-                    m[cb] = mn;
-                    l[cb] *= f;
-#pragma unroll
-                    for (int v = 0; v < D / 32; ++v)
-                        if (FULL || 32 * v < a.c.vd) o[cb][v] *= f;
-                    const bool far = fabsf(mn) >= kRowsFar;
-                    if (__any(far)) {
-                        const float one = far ? scale : 1.0f;
-#pragma unroll
-                        for (int kb = 0; kb < kBlocks; ++kb) s[cb][kb] *= one;
-                        scale = far ? 1.0f : scale;
-                    }
-                }
-                const float mu = m[cb] == -INFINITY ? 0.0f : m[cb] - kLift<VT>;
-                const float *vs = scales + (2 * buf + 1) * kRTile + 32 * block0 + 4 * half;
-#pragma unroll
-                for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][e], scale, -mu));
-                        float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][e + 1], scale, -mu));
-                        l[cb] += x;
-                        l[cb] += y;
-                        if constexpr (kCodes) {
-                            const float2 f = *reinterpret_cast<const float2 *>(vs + 32 * kb + 8 * (e >> 2) + (e & 3));
-                            x *= f.x;
-                            y *= f.y;
-                        }
-                        const uint32_t parts = first_parts<VT>(x, y);
-                        w[cb][2 * kb + (e >> 3)][(e & 7) >> 1] = parts;
-                        rest[cb][2 * kb + (e >> 3)][(e & 7) >> 1] = second_parts<VT>(x, y, parts);
-                    }
+                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[1][e]);
             }
+            mt = halves_max(mt) * a.scale_log2;
+            float scale = a.scale_log2;
+            if (__any(mt > m + 8.0f || fabsf(m) >= kRowsFar)) {
+                const float mn = fmaxf(m, mt);
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v) o[v] *= f;
+                const bool far = fabsf(mn) >= kRowsFar;
+                if (__any(far)) {
+                    const float one = far ? scale : 1.0f;
+#pragma unroll
+                    for (int kb = 0; kb < kBlocks; ++kb) s[kb] *= one;
+                    scale = far ? 1.0f : scale;
+                }
+            }
+            const float mu = m == -INFINITY ? 0.0f : m - kLift<VT>;
+            const float *vs = scales + (2 * buf + 1) * kRTile + 32 * block0 + 4 * half;
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    float x = __builtin_amdgcn_exp2f(fmaf(s[kb][e], scale, -mu));
+                    float y = __builtin_amdgcn_exp2f(fmaf(s[kb][e + 1], scale, -mu));
+                    l += x;
+                    l += y;
+                    if constexpr (kCodes) {
+                        const float2 f = *reinterpret_cast<const float2 *>(vs + 32 * kb + 8 * (e >> 2) + (e & 3));
+                        x *= f.x;
+                        y *= f.y;
+                    }
+                    const uint32_t parts = first_parts<VT>(x, y);
+                    w[2 * kb + (e >> 3)][(e & 7) >> 1] = parts;
+                    rest[2 * kb + (e >> 3)][(e & 7) >> 1] = second_parts<VT>(x, y, parts);
+                }
             // all first parts of 16 keys, then all second ones: no product waits for the one before it
 #pragma unroll
             for (int st = 0; st < 2 * kBlocks; ++st) {
                 s16x8 va[D / 32];
 #pragma unroll
-                for (int v = 0; v < D / 32; ++v)
-                    if (FULL || 32 * v < a.c.vd) {
-                        const unsigned char *src = vt + 16 * st * D * 2 + vaddr + ((4 * v + vpiece) ^ vswz) * 16;
-                        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)src);
-                        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4 *)(src + 8 * D * 2));
-                        va[v] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb)
-                            o[cb][v] = mfma16<VT>(va[v], __builtin_bit_cast(s16x8, w[cb][st]), o[cb][v]);
-                    }
+                for (int v = 0; v < D / 32; ++v) {
+                    const unsigned char *src = vt + 16 * st * D * 2 + vaddr + ((4 * v + vpiece) ^ vswz) * 16;
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)src);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *)(src + 8 * D * 2));
+                    va[v] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[v] = mfma16<VT>(va[v], __builtin_bit_cast(s16x8, w[st]), o[v]);
+                }
 #pragma unroll
                 for (int v = 0; v < D / 32; ++v)
-                    if (FULL || 32 * v < a.c.vd) {
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb)
-                            o[cb][v] = mfma16<VT>(va[v], __builtin_bit_cast(s16x8, rest[cb][st]), o[cb][v]);
-                    }
+                    o[v] = mfma16<VT>(va[v], __builtin_bit_cast(s16x8, rest[st]), o[v]);
             }
         }
         if constexpr (kCodes)
@@ -349,140 +322,118 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
     if constexpr (KS == 2) {
         // the other half's outputs, maximum and sum, from LDS: registers side by side
         constexpr int kRegs = D / 2 + 2;
-        float *join = reinterpret_cast<float *>(smem) + col_wave * CB * kRegs * 64 + lane;
+        float *join = reinterpret_cast<float *>(smem) + col_wave * kRegs * 64 + lane;
         __syncthreads();  // the tiles' readers are done
         if (block0 == 1) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
+            for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-                for (int v = 0; v < D / 32; ++v)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) join[(cb * kRegs + 16 * v + e) * 64] = o[cb][v][e];
-                join[(cb * kRegs + D / 2) * 64] = m[cb];
-                join[(cb * kRegs + D / 2 + 1) * 64] = l[cb];
-            }
+                for (int e = 0; e < 16; ++e) join[(16 * v + e) * 64] = o[v][e];
+            join[D / 2 * 64] = m;
+            join[(D / 2 + 1) * 64] = l;
         }
         __syncthreads();
         if (block0 == 1) return;
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            const float m1 = join[(cb * kRegs + D / 2) * 64], mn = fmaxf(m[cb], m1), mu = mn == -INFINITY ? 0.0f : mn;
-            const float f0 = __builtin_amdgcn_exp2f(m[cb] - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
-            m[cb] = mn;
-            l[cb] = l[cb] * f0 + join[(cb * kRegs + D / 2 + 1) * 64] * f1;
-#pragma unroll
-            for (int v = 0; v < D / 32; ++v)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[cb][v][e] = o[cb][v][e] * f0 + join[(cb * kRegs + 16 * v + e) * 64] * f1;
-        }
-    }
-    if (!live) return;
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const float sum = halves_sum(l[cb]);
-        const int col = col0 + 32 * cb + n;
-        bool nan = false;
+        const float m1 = join[D / 2 * 64], mn = fmaxf(m, m1), mu = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+        m = mn;
+        l = l * f0 + join[(D / 2 + 1) * 64] * f1;
 #pragma unroll
         for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) nan |= o[cb][v][e] != o[cb][v][e];
-        if (col < p.cols) {
-            const int head = p.h * a.group + col % a.group, row = col / a.group;
-            if (a.part) {
-                const long long pi = ((static_cast<long long>(p.b) * a.t + row) * a.heads + head) * a.splits + p.sp;
-                float *dst = a.part + pi * a.c.vd;
+            for (int e = 0; e < 16; ++e) o[v][e] = o[v][e] * f0 + join[(16 * v + e) * 64] * f1;
+    }
+    if (!live) return;
+    const int col = col0 + n;
+    const float sum = halves_sum(l);
+    bool nan = false;
 #pragma unroll
-                for (int v = 0; v < D / 32; ++v)
+    for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int d = 32 * v + 8 * g + 4 * half;
-                        if (FULL || d < a.c.vd)
-                            *reinterpret_cast<float4 *>(dst + d) = make_float4(o[cb][v][4 * g], o[cb][v][4 * g + 1],
-                                                                               o[cb][v][4 * g + 2], o[cb][v][4 * g + 3]);
-                    }
-                if (half == 0) {
-                    a.part_ml[2 * pi] = m[cb] - kLift<VT>;
-                    a.part_ml[2 * pi + 1] = sum;
+        for (int e = 0; e < 16; ++e) nan |= o[v][e] != o[v][e];
+    if (col < p.cols) {
+        const int head = p.h * a.group + col % a.group, row = col / a.group;
+        if (a.part) {
+            const long long pi = ((static_cast<long long>(p.b) * a.t + row) * a.heads + head) * a.splits + p.sp;
+            float *dst = a.part + pi * a.c.vd;
+#pragma unroll
+            for (int v = 0; v < D / 32; ++v)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * v + 8 * g + 4 * half;
+                    if (FULL || d < a.c.vd)
+                        *reinterpret_cast<float4 *>(dst + d) = make_float4(o[v][4 * g], o[v][4 * g + 1],
+                                                                           o[v][4 * g + 2], o[v][4 * g + 3]);
                 }
-            } else {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                uint16_t *dst = static_cast<uint16_t *>(a.out) + static_cast<long long>(p.b) * a.out_stream +
-                                static_cast<long long>(row) * a.out_row + static_cast<long long>(head) * a.c.vd;
+            if (half == 0) {
+                a.part_ml[2 * pi] = m - kLift<VT>;
+                a.part_ml[2 * pi + 1] = sum;
+            }
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint16_t *dst = static_cast<uint16_t *>(a.out) + static_cast<long long>(p.b) * a.out_stream +
+                            static_cast<long long>(row) * a.out_row + static_cast<long long>(head) * a.c.vd;
 #pragma unroll
-                for (int v = 0; v < D / 32; ++v)
+            for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int d = 32 * v + 8 * g + 4 * half;
-                        if (FULL || d < a.c.vd) {
-                            s16x4 x;
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * v + 8 * g + 4 * half;
+                    if (FULL || d < a.c.vd) {
+                        s16x4 x;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] = round16<QT>(o[cb][v][4 * g + e] * inv);
-                            if (a.aligned & 2) {
-                                *reinterpret_cast<s16x4 *>(dst + d) = x;
-                            } else {
+                        for (int e = 0; e < 4; ++e) x[e] = round16<QT>(o[v][4 * g + e] * inv);
+                        if (a.aligned & 2) {
+                            *reinterpret_cast<s16x4 *>(dst + d) = x;
+                        } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) dst[d + e] = static_cast<uint16_t>(x[e]);
-                            }
+                            for (int e = 0; e < 4; ++e) dst[d + e] = static_cast<uint16_t>(x[e]);
                         }
                     }
-            }
+                }
         }
-        const unsigned long long bad = __ballot(nan && col < p.cols);
-        if (bad) repair_columns<kRTile>(a, p, col0 + 32 * cb, static_cast<unsigned>(bad) | static_cast<unsigned>(bad >> 32));
     }
+    const unsigned long long bad = __ballot(nan && col < p.cols);
+    if (bad) repair_columns<kRTile>(a, p, col0, static_cast<unsigned>(bad) | static_cast<unsigned>(bad >> 32));
 }
 
-template <int QT, int CT, int D, int CB, int KS, bool FULL>
+template <int QT, int CT, int D, int KS, bool FULL>
 hipError_t launch_16(const RowsArgs &a, hipStream_t s) {
     static std::atomic<unsigned long long> attr{0};
     constexpr int lds = 4 * kRTile * D * 2 + (CT >= 3 ? 4 * kRTile * 4 : 0);
-    static_assert(KS == 1 || kRWaves / KS * CB * (D / 2 + 2) * 64 * 4 <= lds, "the join's registers past the tiles");
-    return launch_with(&rows_attend_kernel<QT, CT, D, CB, KS, FULL>, a, kRWaves / KS * 32 * CB, lds, attr, s);
+    static_assert(KS == 1 || kRWaves / KS * (D / 2 + 2) * 64 * 4 <= lds, "the join's registers past the tiles");
+    return launch_with(&rows_attend_kernel<QT, CT, D, KS, FULL>, a, kRWaves / KS * 32, lds, attr, s);
 }
 
-template <int QT, int CT, int D, int CB, int KS>
+template <int QT, int CT, int D, int KS>
 hipError_t launch_16_full(const RowsArgs &a, hipStream_t s) {
-    return a.c.qk == D && a.c.vd == D ? launch_16<QT, CT, D, CB, KS, true>(a, s) : launch_16<QT, CT, D, CB, KS, false>(a, s);
+    return a.c.qk == D && a.c.vd == D ? launch_16<QT, CT, D, KS, true>(a, s) : launch_16<QT, CT, D, KS, false>(a, s);
 }
-
-// What the columns of a launch ask for: 32-column blocks a wavefront, halves of the keys.
-struct RowsShape {
-    int cb, ks;
-};
 
 template <int QT, int CT>
-hipError_t launch_16_width(const RowsArgs &a, RowsShape x, hipStream_t s) {
+hipError_t launch_16_width(const RowsArgs &a, int ks, hipStream_t s) {
     const int w = std::max(a.c.qk, a.c.vd);
-    if (w <= 64)
-        return x.ks == 2   ? launch_16_full<QT, CT, 64, 1, 2>(a, s)
-               : x.cb == 2 ? launch_16_full<QT, CT, 64, 2, 1>(a, s)
-                           : launch_16_full<QT, CT, 64, 1, 1>(a, s);
-    if (w <= 128) return x.ks == 2 ? launch_16_full<QT, CT, 128, 1, 2>(a, s) : launch_16_full<QT, CT, 128, 1, 1>(a, s);
-    return x.ks == 2 ? launch_16_full<QT, CT, 256, 1, 2>(a, s) : launch_16_full<QT, CT, 256, 1, 1>(a, s);
+    if (w <= 64) return ks == 2 ? launch_16_full<QT, CT, 64, 2>(a, s) : launch_16_full<QT, CT, 64, 1>(a, s);
+    if (w <= 128) return ks == 2 ? launch_16_full<QT, CT, 128, 2>(a, s) : launch_16_full<QT, CT, 128, 1>(a, s);
+    return ks == 2 ? launch_16_full<QT, CT, 256, 2>(a, s) : launch_16_full<QT, CT, 256, 1>(a, s);
 }
 
 // 16-bit products: queries of 16 bits over a cache of their type or of codes.
 bool rows_16(const RowsArgs &a) { return a.type != 0 && (a.c.type == a.type || a.c.type >= 3); }
 
-// 64 columns a wavefront for heads of up to 64 once they still give every CU a
-// workgroup: half the LDS reads an operation. The keys in halves where 64
+// In how many parts a workgroup's wavefronts take a tile's keys: in halves where 64
 // columns are all or workgroups of 128 do not give every CU two (a prompt of 448 rows,
 // 8 heads of 64: 14.3 us whole, 11.0 in halves; 2 of 500 rows behind 2500 keys, 16
 // heads of 128 over 4: 69 and 60; 4 of 1000, 512 such workgroups: 56 and 59).
-RowsShape rows_shape(const RowsArgs &a, int cus) {
-    if (!rows_16(a)) return {1, 1};
-    const long long cols = static_cast<long long>(a.t) * a.group, wide = kRWaves * 64;
+int rows_key_parts(const RowsArgs &a, int cus) {
+    if (!rows_16(a)) return 1;
+    const long long cols = static_cast<long long>(a.t) * a.group;
     const long long blocks = (cols + kRWaves * 32 - 1) / (kRWaves * 32) * a.batch * a.c.kv_heads;
-    if (cols <= kRWaves / 2 * 32 || blocks < 2LL * cus) return {1, 2};
-    return {std::max(a.c.qk, a.c.vd) <= 64 && 2 * cols > wide && (cols + wide - 1) / wide * a.batch * a.c.kv_heads >= 2 * cus ? 2 : 1, 1};
+    return cols <= kRWaves / 2 * 32 || blocks < 2LL * cus ? 2 : 1;
 }
 
 }  // namespace
 
-int rows_workgroup_columns(const RowsArgs &a, int cus) {
-    const RowsShape x = rows_shape(a, cus);
-    return kRWaves / x.ks * 32 * x.cb;
-}
+int rows_workgroup_columns(const RowsArgs &a, int cus) { return kRWaves / rows_key_parts(a, cus) * 32; }
 
 hipError_t launch_attend_rows(const RowsArgs &args, int cus, hipStream_t s) {
     RowsArgs a = args;
@@ -492,11 +443,11 @@ hipError_t launch_attend_rows(const RowsArgs &args, int cus, hipStream_t s) {
     if (((reinterpret_cast<uintptr_t>(a.out) | (a.out_stream * size) | (a.out_row * size)) & 7) == 0) a.aligned |= 2;
     hipError_t e;
     if (rows_16(a)) {
-        const RowsShape x = rows_shape(a, cus);
+        const int ks = rows_key_parts(a, cus);
         if (a.type == 1)
-            e = a.c.type == 1 ? launch_16_width<1, 1>(a, x, s) : a.c.type == 4 ? launch_16_width<1, 4>(a, x, s) : launch_16_width<1, 3>(a, x, s);
+            e = a.c.type == 1 ? launch_16_width<1, 1>(a, ks, s) : a.c.type == 4 ? launch_16_width<1, 4>(a, ks, s) : launch_16_width<1, 3>(a, ks, s);
         else
-            e = a.c.type == 2 ? launch_16_width<2, 2>(a, x, s) : a.c.type == 4 ? launch_16_width<2, 4>(a, x, s) : launch_16_width<2, 3>(a, x, s);
+            e = a.c.type == 2 ? launch_16_width<2, 2>(a, ks, s) : a.c.type == 4 ? launch_16_width<2, 4>(a, ks, s) : launch_16_width<2, 3>(a, ks, s);
     } else {
         e = launch_attend_rows_f32(a, s);
     }
