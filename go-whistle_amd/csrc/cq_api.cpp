@@ -2507,7 +2507,7 @@ int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream,
     // Two workgroups a CU, where a part keeps 256 keys (1024 where the parts of
     // many columns have to be written and joined).
     a.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({2LL * cus / lists, keys / (tiles == 1 ? 256 : 1024), 64})));
-    if (static_cast<double>(lists + 8 * tiles) * a.splits > static_cast<double>(grid_limit(256)))
+    if (static_cast<double>(lists + 8 * tiles) * a.splits + 8.0 * batch > static_cast<double>(grid_limit(256)))
         return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads", batch, t, heads);
     WsScope ws;
     if (a.splits > 1) {

@@ -19,15 +19,30 @@ struct RowsPlace {
     int b, h, ct, sp, cols, pos, end, lo, ns, i0, i1;
     bool ok;
 };
+// Streams of unequal counts, of 1, 2, 4 or 8 key heads: a key head of all streams on
+// 8 / kv_heads XCDs, whose L2s it shares with no other, its tiles of columns in turns, each turn of
+// the streams one place on. Against lists spread over all XCDs, or whole ones
+// on one where there are 64 or more (us a call): 8 prompts of up to 2000 rows, 16 heads of 128 over
+// 4, 226 and 239; 6 of 1000, 8 heads of 64, 21 and 25; 64 of 448, 29 and 34; 32 of
+// 448, 8 heads of 128 over 2, 27 and 32; without the turns 98 became 130. One head of 100
+// equal streams, ten tiles each: 36 and 31.
+__host__ __device__ inline bool rows_by_head(const RowsArgs &a) {
+    return a.rows && 8 % a.c.kv_heads == 0 && (a.c.kv_heads > 1 || a.batch < kXcdUnits);
+}
 template <int KEYS>
 __device__ __forceinline__ RowsPlace rows_place(const RowsArgs &a, int col_tiles, int wg_cols) {
     RowsPlace p;
     p.ok = false;
-    // A (stream, key head) on one XCD; but streams of unequal counts, where there
-    // are few, over all of them: tile by tile, each turn of the units one place on.
+    // A (stream, key head) on one XCD; but streams of unequal counts by heads, or, where
+    // there are few, over all of them: tile by tile, each turn of the units one place on.
     const int units = a.batch * a.c.kv_heads;
     XcdPlace x;
-    if (a.rows && units < kXcdUnits) {
+    if (rows_by_head(a)) {
+        const int each = 8 / a.c.kv_heads, xcd = blockIdx.x & 7, slot = static_cast<int>(blockIdx.x) >> 3, turn = slot / a.batch;
+        x.within = turn * each + xcd / a.c.kv_heads;
+        x.unit = (slot - turn * a.batch + turn) % a.batch * a.c.kv_heads + xcd % a.c.kv_heads;
+        if (x.within >= col_tiles * a.splits) return p;
+    } else if (a.rows && units < kXcdUnits) {
         x.within = static_cast<int>(blockIdx.x) / units;
         x.unit = (static_cast<int>(blockIdx.x) - x.within * units + x.within) % units;
     } else {
@@ -187,7 +202,9 @@ hipError_t launch_with(F *fn, const RowsArgs &a, int wg_cols, int lds, std::atom
     if (lds > 64 * 1024)
         if (hipError_t e = lds_limit_once(reinterpret_cast<const void *>(fn), lds, attr)) return e;
     const int cols = a.t * a.group, col_tiles = (cols + wg_cols - 1) / wg_cols;
-    const long long grid = xcd_grid(static_cast<long long>(a.batch) * a.c.kv_heads, static_cast<long long>(col_tiles) * a.splits);
+    const long long per = static_cast<long long>(col_tiles) * a.splits, each = 8 / std::min(8, a.c.kv_heads);
+    const long long grid = rows_by_head(a) ? (per + each - 1) / each * 8 * a.batch
+                                           : xcd_grid(static_cast<long long>(a.batch) * a.c.kv_heads, per);
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * kRWaves), lds, s, a, col_tiles);
     return hipGetLastError();
 }

@@ -21,7 +21,7 @@
 // times their scale) on 32x32x2 products, all of it in float32.
 //
 // What bounds 8 ragged prompts of up to 2000 rows, 16 heads of 128 over 4 in
-// bfloat16 (216 to 232 us, some 600 TFLOP/s): the softmax on the vector units, 45% of all
+// bfloat16 (220 to 226 us, some 600 TFLOP/s): the softmax on the vector units, 45% of all
 // cycles, beside the products, 42%, with little overlap. 4 of up to 1000 rows over
 // int8 pages with a window of 1024, 16 heads of 64 over 4: 47 to 52 us, half of the CUs' cycles idle.
 //

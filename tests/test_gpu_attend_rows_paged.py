@@ -114,6 +114,15 @@ def test_whole_tiles_with_values_that_are_not_finite(io, name, Hk, w):
     check_rows(c, name, rest, rest, q[:, window:], [p + window for p in pos], None, c.cap, window, 0, math.sqrt(w), 1, 3)
 
 
+@pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float16", "i8p"), ("float32", "float32")])
+@pytest.mark.parametrize("B,Hk", [(1, 1), (5, 1), (70, 1), (3, 2), (5, 3), (5, 4), (2, 8), (3, 16), (40, 4)])
+def test_ragged_streams_of_any_number_of_heads(io, name, B, Hk):
+    # every tile of every stream has its workgroup, in whichever order they go over the chip
+    pos = [(b * 53) % 150 for b in range(B)]
+    for group, t in ((1, 170), (3, 75)):
+        run(B + Hk, io, name, group * Hk, Hk, 64, 64, 16, pos, t, rows=[t] + [(t * b * 7) % (t + 1) for b in range(1, B)], sample=3)
+
+
 @pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float32", "float16"), ("float16", "e4m3")])
 def test_strided_and_unaligned(io, name):
     import torch
