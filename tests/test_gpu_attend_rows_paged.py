@@ -89,7 +89,7 @@ def test_many_streams(io, name, H, Hk, w):
 @pytest.mark.parametrize("H,Hk,w,t", [(8, 8, 64, 150), (8, 8, 48, 150), (16, 8, 128, 100), (8, 8, 112, 130), (8, 8, 256, 100),
                                       (8, 8, 240, 70)])
 def test_workgroups_of_whole_tiles(io, name, H, Hk, w, t):
-    # so many lists that no workgroup takes a tile's keys in halves, and that narrow heads take 64 columns a wavefront
+    # so many lists that no workgroup takes a tile's keys in halves
     pos = [(b * 37) % 200 for b in range(64)]
     run(t, io, name, H, Hk, w, w, 16, pos, t, sample=1)
     run(w, io, name, H, Hk, w, w, 8, pos, t, rows=[t - b % 5 * 16 for b in range(64)], window=70, sink=5, sample=1)
