@@ -2327,6 +2327,77 @@ static bool rows_apart(long long width, long long n0, long long s0, long long n1
     return true;
 }
 
+// Whether some sum of multiples k * stride, k in [lo, hi] for each of n strides
+// (positive, the largest first), is in [from, to]. Of a stride only the multiples
+// that the smaller ones can still bring there are tried: one or two where
+// rows lie between others; past `steps` of them the answer is yes.
+struct Multiples {
+    __int128 stride, lo, hi;
+};
+static bool sum_reaches(const Multiples *m, int n, __int128 from, __int128 to, int &steps) {
+    if (n == 0) return from <= 0 && to >= 0;
+    __int128 least = 0, most = 0;  // what the others add
+    for (int i = 1; i < n; ++i) {
+        least += m[i].stride * m[i].lo;
+        most += m[i].stride * m[i].hi;
+    }
+    const auto below = [&](__int128 x) { return x / m->stride - (x % m->stride < 0); };  // x / stride rounded down
+    const __int128 first = std::max(m->lo, -below(most - from)), last = std::min(m->hi, below(to - least));
+    if (n == 1) return first <= last;
+    for (__int128 k = first; k <= last; ++k)
+        if (--steps < 0 || sum_reaches(m + 1, n - 1, from - k * m->stride, to - k * m->stride, steps)) return true;
+    return false;
+}
+
+// Rows of `width` elements of an array, batch x t of them.
+struct RowsOf {
+    const void *at;
+    long long width, stream, row;
+};
+// Whether rows of two arrays share an element. Exact, but that strides of four
+// kinds which take more than a million steps to tell apart count as shared.
+static bool rows_meet(const RowsOf &x, const RowsOf &y, int batch, int t, int size) {
+    const __int128 d = static_cast<long long>(reinterpret_cast<uintptr_t>(y.at) - reinterpret_cast<uintptr_t>(x.at)) / size;
+    {  // most arrays lie behind each other
+        const __int128 xs = static_cast<__int128>(batch - 1) * x.stream, xr = static_cast<__int128>(t - 1) * x.row;
+        const __int128 ys = static_cast<__int128>(batch - 1) * y.stream, yr = static_cast<__int128>(t - 1) * y.row, z = 0;
+        if (d + std::min(ys, z) + std::min(yr, z) >= std::max(xs, z) + std::max(xr, z) + x.width ||
+            d + std::max(ys, z) + std::max(yr, z) + y.width <= std::min(xs, z) + std::min(xr, z))
+            return false;
+    }
+    Multiples m[4];
+    int n = 0;
+    const auto add = [&](__int128 stride, __int128 lo, __int128 hi) {
+        if (stride < 0) {
+            stride = -stride;
+            std::swap(lo, hi);
+            lo = -lo, hi = -hi;
+        }
+        if (stride != 0 && (lo != 0 || hi != 0)) m[n++] = {stride, lo, hi};
+    };
+    // y's row less x's: where both have a stride, its multiples are one number's
+    const auto both = [&](__int128 xs, __int128 ys, __int128 most) {
+        if (xs == ys) {
+            add(ys, -most, most);
+        } else {
+            add(ys, 0, most);
+            add(xs, -most, 0);
+        }
+    };
+    both(x.stream, y.stream, batch - 1);
+    both(x.row, y.row, t - 1);
+    std::sort(m, m + n, [](const Multiples &p, const Multiples &q) { return p.stride > q.stride; });
+    int steps = 1 << 20;
+    return sum_reaches(m, n, 1 - y.width - d, x.width - 1 - d, steps);
+}
+// The same of rows[b] rows written at x. Where only the counts keep x's own
+// streams apart, the rows of one stream, and the streams' first ones.
+static bool rows_meet(const RowsOf &x, const RowsOf &y, int batch, int t, const int32_t *rows, int size) {
+    return rows && !rows_apart(x.width, batch, x.stream, t, x.row)
+               ? rows_meet(x, y, batch, 1, size) || rows_meet(x, y, 1, t, size)
+               : rows_meet(x, y, batch, t, size);
+}
+
 static int value_size(int type) { return type == ND_F32 ? 4 : type == ND_F16 || type == ND_BF16 ? 2 : 1; }
 
 int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, long long k_row, const void *v,
@@ -2812,28 +2883,6 @@ int nd_logprobs_dev(float *lp, float *ent, int32_t *top_idx, float *top_lp, cons
     return CQ_OK;
 }
 
-// Whether two arrays of rows of nx and ny values, batch x t of them, share an
-// element, as far as the host can tell apart arrays that lie inside each
-// other's reach: rows at the same strides that fit between each other.
-static bool rows_meet(const void *x, long long nx, long long xs, long long xr, const void *y, long long ny, long long ys,
-                      long long yr, int batch, int t, int size) {
-    const auto reach = [&](const void *p, long long n, long long s, long long r, __int128 &lo, __int128 &hi) {
-        const __int128 a = static_cast<__int128>(batch - 1) * s, b = static_cast<__int128>(t - 1) * r;
-        lo = reinterpret_cast<uintptr_t>(p) + size * (std::min<__int128>(a, 0) + std::min<__int128>(b, 0));
-        hi = reinterpret_cast<uintptr_t>(p) + size * (std::max<__int128>(a, 0) + std::max<__int128>(b, 0) + n);
-    };
-    __int128 x0, x1, y0, y1;
-    reach(x, nx, xs, xr, x0, x1);
-    reach(y, ny, ys, yr, y0, y1);
-    if (x1 <= y0 || y1 <= x0) return false;
-    // multiples of one stride: apart if they are modulo it
-    const long long r = t > 1 ? xr : xs;
-    if ((t > 1 && xr != yr) || (batch > 1 && xs != ys) || r <= 0 || (t > 1 && batch > 1 && xs % r != 0)) return true;
-    const __int128 d = static_cast<__int128>(reinterpret_cast<uintptr_t>(y)) - static_cast<__int128>(reinterpret_cast<uintptr_t>(x));
-    const __int128 m = (d % (r * size) + r * size) % (r * size);
-    return m < static_cast<__int128>(nx) * size || m + static_cast<__int128>(ny) * size > static_cast<__int128>(r) * size;
-}
-
 int nd_qk_norm_rope_dev(void *q_out, void *k_out, const void *q, const void *k, int type, const nd_heads_layout *layout,
                         int batch, int t, int heads, int kv_heads, int width, const float *q_gain, const float *k_gain,
                         const float *cos_t, const float *sin_t, int positions, const int32_t *pos, const int32_t *rows,
@@ -2878,8 +2927,9 @@ int nd_qk_norm_rope_dev(void *q_out, void *k_out, const void *q, const void *k, 
             if (!a.heads[o]) continue;
             const bool in_place = o == z && a.x[o] == a.y[z] && (t == 1 || a.x_row[o] == a.y_row[z]) &&
                                   (batch == 1 || a.x_stream[o] == a.y_stream[z]);
-            if ((!in_place && rows_meet(a.y[z], w[z], a.y_stream[z], a.y_row[z], a.x[o], w[o], a.x_stream[o], a.x_row[o], batch, t, size)) ||
-                (o > z && rows_meet(a.y[z], w[z], a.y_stream[z], a.y_row[z], a.y[o], w[o], a.y_stream[o], a.y_row[o], batch, t, size)))
+            const RowsOf out{a.y[z], w[z], a.y_stream[z], a.y_row[z]};
+            if ((!in_place && rows_meet(out, {a.x[o], w[o], a.x_stream[o], a.x_row[o]}, batch, t, rows, size)) ||
+                (o > z && rows_meet(out, {a.y[o], w[o], a.y_stream[o], a.y_row[o]}, batch, t, rows, size)))
                 return fail(CQ_ERR_MISUSE, "needle: normed heads onto a part of others");
         }
     }

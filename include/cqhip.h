@@ -658,7 +658,9 @@ typedef struct nd_heads_layout {
  * Rope.apply's but for the order of the float64 squares' sum; 16-bit types
  * compute in float32. The outputs may be the inputs in place (same pointer and
  * strides); else they share no element with an input. Written rows share none.
- * heads or kv_heads may be 0. width is a multiple of 16 up to 256. layout null:
+ * Rows may lie between each other in any order (where q, k and outputs do so at
+ * different strides and more than a million steps do not tell their rows
+ * apart, the call is refused). heads or kv_heads may be 0. width is a multiple of 16 up to 256. layout null:
  * dense [batch][t][heads][width]. */
 int nd_qk_norm_rope_dev(void *q_out, void *k_out, const void *q, const void *k, int type, const nd_heads_layout *layout,
                         int batch, int t, int heads, int kv_heads, int width, const float *q_gain, const float *k_gain,
