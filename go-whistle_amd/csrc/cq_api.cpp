@@ -2532,6 +2532,10 @@ int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream,
         2.0 * batch * t * heads > static_cast<double>(grid_limit(64)))
         return fail(CQ_ERR_UNSUPPORTED, "needle: attention of %d streams of %d rows of %d heads over %d keys", batch, t, heads,
                     nk_max);
+    // (queries are read again after outputs are written: of a column that is computed again)
+    if (rows_meet({out, width, out_stream, out_row}, {q, static_cast<long long>(heads) * c->qk, q_stream, q_row}, batch, t, rows,
+                  value_size(type)))
+        return fail(CQ_ERR_MISUSE, "needle: attention onto its queries");
     const int size = value_size(c->type), cus = device_info().cus;
     a.k_head = static_cast<long long>(c->qk) * size;
     a.v_head = static_cast<long long>(c->vd) * size;

@@ -586,7 +586,7 @@ int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long 
  * i*out_row).
  * Query head h reads key head h / (heads/kv_heads). A page outside the pool
  * reads page 0. Cache rows that no row attends may hold anything. The written
- * output rows share no element, and none with q.
+ * output rows share no element, and none with q (refused where the host sees it).
  * 16-bit queries over caches of their type, and over codes, take 16-bit
  * products: the operands as they are (codes exactly), the softmax weights in
  * two parts (22 bits with float16 caches, 16 else). Everything else is

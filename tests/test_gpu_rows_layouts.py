@@ -41,3 +41,24 @@ def test_packed_products_of_any_order_in_place(io, pad, order, counts):
         heads(x, 0, 4).zero_()
         heads(x, 256, 2).zero_()
     assert torch.equal(room, old)
+
+
+@pytest.mark.parametrize("io,name", [("bfloat16", "bfloat16"), ("float32", "float16"), ("float16", "e4m3")])
+@pytest.mark.parametrize("t", [1, 5, 70])
+@pytest.mark.parametrize("counts", [False, True])
+def test_attention_beside_its_queries(io, name, t, counts):
+    # queries and outputs side by side in rows of streams, and one after the other
+    import torch
+
+    from page8_ref import check_rows, make_cache
+
+    B, g, dt = 3, gen(t), getattr(torch, io)
+    c = make_cache(g, name, B, 10, 16, 2, 64, 64)
+    room = torch.randn(t, B, 512 + 40, generator=g, device="cuda").to(dt)
+    q, out = (room[..., x:x + 256].unflatten(-1, (4, 64)).transpose(0, 1) for x in (0, 264))
+    rows, pos = [t, 0, t - 1] if counts else None, [3, 80, 31]
+    before, rest, asked = out.clone(), room.clone(), q.clone()
+    c.attend_rows_dev(out, q, i32(pos), 8.0, rows=i32(rows) if counts else None)
+    check_rows(c, name, out, before, asked, pos, rows, c.cap, 0, 0, 8.0, 5)
+    room[..., 264:520] = rest[..., 264:520]
+    assert torch.equal(room, rest)

@@ -112,3 +112,22 @@ def test_large_layouts_are_settled():
     for s, r in ((6144, batch * 6144), (t * 6144 + 64, 6144), (6144, batch * 6144 + 64)):
         y = HeadsLayout(s, r, s, r, s, r, s, r)
         assert norm(y, batch, t, BASE, BASE + 2048, BASE, BASE + 2048, heads=16, kv_heads=4, width=128) is None
+
+
+def attend(batch, t, out, q, os, orow, qs, qrow, typ=0, rows=None, heads=4, qk=16, vd=16):
+    c = KvPaged(P, P, None, None, P, 1, 2, qk, vd, 4, 16, 8)
+    size = 2 if typ else 4
+    check(lib().kv_attend_rows_paged_dev(ctypes.byref(c), out * size, os, orow, q * size, qs, qrow, typ, batch, t, heads, rows, P, 64,
+                                         0, 0, 4.0, None))
+
+
+@pytest.mark.parametrize("batch,t", [(1, 1), (3, 1), (1, 5), (3, 5)])
+@pytest.mark.parametrize("typ", [0, 1])
+def test_attention_onto_its_queries(batch, t, typ):
+    # outputs of 64 in rows of 144, the queries at every place that shares an element with them
+    for rows in (None, P):
+        for qrow, qs in ((144, t * 144), (144, t * 144 + 8), (batch * 144, 144), (64, t * 64), (0, 0), (200, 77)):
+            for off in (0, 1, 63, -63, 64, 100, t * 64 - 1):
+                if share(batch, t, (BASE, 64, t * 144, 144), (BASE + off, 64, qs, qrow)):
+                    with pytest.raises(CQPanic, match="onto its queries"):
+                        attend(batch, t, BASE, BASE + off, t * 144, 144, qs, qrow, typ=typ, rows=rows)
