@@ -2459,6 +2459,8 @@ int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long 
                         widths[z], rs[z], streams[z]);
     if (static_cast<double>(batch) * t * c->kv_heads > (0xffffffffLL - 255) / 128)
         return fail(CQ_ERR_UNSUPPORTED, "needle: a read of %d x %d rows of %d heads", batch, t, c->kv_heads);
+    if (rows_meet({k, widths[0], k_stream, k_row}, {v, widths[1], v_stream, v_row}, batch, t, rows, value_size(type)))
+        return fail(CQ_ERR_MISUSE, "needle: keys and values read to one place");
     a.y[0] = k;
     a.y[1] = v;
     a.stream[0] = k_stream;

@@ -570,7 +570,7 @@ int kv_evict_paged_dev(const kv_paged *c, const int32_t *dst_pages, int dst_stri
  * i*v_row of v, kv_heads*qk and kv_heads*vd values each. Rows that the table does
  * not hold (below 0, at or past page_stride * page_rows), and rows in pages
  * outside the pool, are left as they were in the outputs. The written rows share
- * no element, keys' with values' either. */
+ * no element, keys' with values' either (refused where the host sees it). */
 int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long k_row, void *v, long long v_stream,
                       long long v_row, int type, int batch, int t, const int32_t *rows, const int32_t *pos,
                       void *stream);

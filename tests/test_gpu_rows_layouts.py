@@ -1,6 +1,7 @@
 """needle.qk_norm_rope_dev on rows whose streams lie between each other, and on
 streams padded by part of a row, against its float64 form."""
 
+import numpy as np
 import pytest
 
 from go_whistle_amd import needle
@@ -62,3 +63,25 @@ def test_attention_beside_its_queries(io, name, t, counts):
     check_rows(c, name, out, before, asked, pos, rows, c.cap, 0, 0, 8.0, 5)
     room[..., 264:520] = rest[..., 264:520]
     assert torch.equal(room, rest)
+
+
+@pytest.mark.parametrize("name", ["float16", "i8", "e4m3"])
+@pytest.mark.parametrize("counts", [False, True])
+def test_keys_and_values_read_beside_each_other(name, counts):
+    import torch
+
+    from page8_ref import cache_rows, make_cache
+    from serve_ref import host
+
+    B, t, g = 3, 20, gen(4)
+    c = make_cache(g, name, B, 5, 8, 2, 48, 64)
+    room = torch.full((t, B, 2 * (48 + 64) + 3), 7.0, device="cuda")
+    k, v = room[..., :96].unflatten(-1, (2, 48)).transpose(0, 1), room[..., 97:225].unflatten(-1, (2, 64)).transpose(0, 1)
+    pos, rows = [0, 3, 17], [t, 0, 5] if counts else [t] * 3
+    c.read_dev(k, v, i32(pos), rows=i32(rows) if counts else None)
+    for b in range(B):
+        wk, wv = cache_rows(c, b, np.arange(pos[b], pos[b] + rows[b]))
+        # one product of float32
+        assert (abs(host(k[b, :rows[b]]) - wk) <= 2.0 ** -24 * abs(wk)).all() and (abs(host(v[b, :rows[b]]) - wv) <= 2.0 ** -24 * abs(wv)).all()
+        assert (k[b, rows[b]:] == 7).all() and (v[b, rows[b]:] == 7).all()
+    assert (room[..., 96:97] == 7).all() and (room[..., 225:] == 7).all()

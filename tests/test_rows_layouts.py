@@ -131,3 +131,17 @@ def test_attention_onto_its_queries(batch, t, typ):
                 if share(batch, t, (BASE, 64, t * 144, 144), (BASE + off, 64, qs, qrow)):
                     with pytest.raises(CQPanic, match="onto its queries"):
                         attend(batch, t, BASE, BASE + off, t * 144, 144, qs, qrow, typ=typ, rows=rows)
+
+
+@pytest.mark.parametrize("batch,t", [(1, 1), (3, 1), (1, 5), (3, 5)])
+@pytest.mark.parametrize("typ", [0, 1])
+def test_keys_and_values_read_to_one_place(batch, t, typ):
+    # key rows of 2 x 16 and value rows of 2 x 32 values, each apart from its own
+    c, size = KvPaged(P, P, None, None, P, 1, 2, 16, 32, 4, 16, 8), 2 if typ else 4
+    for rows in (None, P):
+        for vrow, vs in ((144, t * 144), (144, t * 144 + 8), (batch * 144, 144), (64, t * 64), (200, 77 + t * 200)):
+            for off in (0, 1, 31, -63, 32, 100, t * 64 - 1):
+                if share(batch, t, (BASE, 32, t * 144, 144), (BASE + off, 64, vs, vrow)):
+                    with pytest.raises(CQPanic, match="to one place"):
+                        check(lib().kv_read_paged_dev(ctypes.byref(c), BASE * size, t * 144, 144, (BASE + off) * size, vs, vrow, typ,
+                                                      batch, t, rows, P, None))
