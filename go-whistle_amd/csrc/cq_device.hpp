@@ -9,6 +9,12 @@
 
 namespace cqhip {
 
+// Attention keeps a maximum that logits may pass by 2^8 before sums are scaled to
+// a new one, so a weight may be 2^8, and the sums of weights times values, of up to
+// 64 parts, may pass float32's range though the mean of the values does not.
+// From this on such sums are taken again with weights up to 1.
+constexpr float kMostSum = 0x1p120f;
+
 // A launch of `units` groups of `per` workgroups, the workgroups of a group on
 // one XCD, whose L2 they share. Ids go round the 8 XCDs: from kXcdUnits groups
 // on, group u is XCD u % 8's (neighbours in the list, which may be alike in

@@ -463,7 +463,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_parts_kernel(Spli
                         TYPE == 1 ? o[t][e][i] * (1.0f / kPartLift) : o[t][e][i];
         }
     }
-    finish<kColumns, D, CAUSAL ? TYPE : -1>(a, p, jt);
+    finish<kColumns, D, TYPE>(a, p, jt);
 }
 
 template <int TYPE, int D, int PARTS, int TILES, bool CAUSAL>

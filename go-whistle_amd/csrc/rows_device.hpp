@@ -117,8 +117,8 @@ __device__ __forceinline__ float cache_value(const unsigned char *row, int type,
 }
 
 // Columns c of `mask` (first column col0) again, key by key, by one wavefront:
-// lane j of 64 keys has its logit, then lane d its values. Rare (a NaN among
-// the outputs), so plain.
+// lane j of 64 keys has its logit, then lane d its values. The largest weight is
+// 1. Rare (a NaN or a sum past kMostSum among the outputs), so plain.
 template <int KEYS>
 __device__ __forceinline__ void repair_columns(const RowsArgs &a, const RowsPlace &p, int col0, unsigned mask) {
     const int lane = threadIdx.x & 63;

@@ -159,11 +159,11 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
     if (!live) return;
     const float sum = halves_sum(l);
     const int col = col0 + n;
-    bool nan = false;
+    bool again = false;
 #pragma unroll
     for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) nan |= o[v][e] != o[v][e];
+        for (int e = 0; e < 16; ++e) again |= !(fabsf(o[v][e]) < kMostSum);
     if (col < p.cols) {
         const int head = p.h * a.group + col % a.group, row = col / a.group;
         const long long pi = ((static_cast<long long>(p.b) * a.t + row) * a.heads + head) * a.splits + p.sp;
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_f3
             a.part_ml[2 * pi + 1] = sum;
         }
     }
-    const unsigned long long bad = __ballot(nan && col < p.cols);
+    const unsigned long long bad = __ballot(again && col < p.cols);
     if (bad) repair_columns<kKeys>(a, p, col0, static_cast<unsigned>(bad) | static_cast<unsigned>(bad >> 32));
 }
 

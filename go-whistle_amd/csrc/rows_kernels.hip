@@ -14,7 +14,7 @@
 // rows_attend_kernel, 16-bit queries over caches of their type or of 8 bits:
 // 32x32x16 products. Caches of the queries' type go straight into LDS; codes
 // pass through registers, widened exactly (keys to the queries' type, values to
-// bfloat16, whose range holds a weight times any scale): a key's scale meets
+// bfloat16, whose range holds a weight of 1 times any scale): a key's scale meets
 // its logit, a value's scale its weight. Weights take part as the sum of two
 // parts of the values' type (22 bits in float16, 16 in bfloat16).
 // rows_attend_f32_kernel, everything else: values widened to float32 (codes
@@ -26,9 +26,10 @@
 // int8 pages with a window of 1024, 16 heads of 64 over 4: 47 to 52 us, half of the CUs' cycles idle.
 //
 // A masked key has the weight 0, but 0 times an infinite or NaN value is NaN,
-// and so is a second part times an infinity: a wavefront that finds a NaN
-// among its outputs computes those columns again key by key (repair_columns),
-// which skips masked keys. Keys behind the workgroup's last are cleared.
+// and so is a second part times an infinity: a wavefront that finds a NaN, or a
+// sum that its parts' may bring past float32's range (kMostSum), among its
+// outputs computes those columns again key by key (repair_columns), which skips
+// masked keys. Keys behind the workgroup's last are cleared.
 #include "rows_device.hpp"
 
 #include <algorithm>
@@ -351,11 +352,11 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
     if (!live) return;
     const int col = col0 + n;
     const float sum = halves_sum(l);
-    bool nan = false;
+    bool again = false;
 #pragma unroll
     for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) nan |= o[v][e] != o[v][e];
+        for (int e = 0; e < 16; ++e) again |= !(fabsf(o[v][e]) < kMostSum);
     if (col < p.cols) {
         const int head = p.h * a.group + col % a.group, row = col / a.group;
         if (a.part) {
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(64 * kRWaves, D == 256 ? 1 : 2) void rows_attend_ke
                 }
         }
     }
-    const unsigned long long bad = __ballot(nan && col < p.cols);
+    const unsigned long long bad = __ballot(again && col < p.cols);
     if (bad) repair_columns<kRTile>(a, p, col0, static_cast<unsigned>(bad) | static_cast<unsigned>(bad >> 32));
 }
 

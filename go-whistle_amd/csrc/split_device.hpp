@@ -308,16 +308,17 @@ __device__ __forceinline__ bool sees_row(const SplitArgs &a, int p, int j) {
     return (j <= p) & ((a.window == 0) | (j > p - a.window) | (j < a.sink));  // no branches
 }
 
-// A causal column again, key by key, by one wavefront: lane j of 64 keys has
-// its logit, then lane d its values. A key that the column does not see has the
-// weight 0, and 0 times an infinite or NaN value is NaN, as are parts of a weight
-// times an infinity: columns that come out as NaN are computed here, which
-// skips what they do not see. Rare, so plain. Returns value d = lane + 64 e in o[e].
+// A column again, key by key, by one wavefront: lane j of 64 keys has its logit,
+// then lane d its values. A key that a causal column does not see has the weight 0,
+// and 0 times an infinite or NaN value is NaN, as are parts of a weight times an
+// infinity; and sums past kMostSum may have weights of 2^8: columns that come out
+// so are computed here, which skips what they do not see, with weights up to 1. Rare, so
+// plain. Returns value d = lane + 64 e in o[e].
 // false, and nothing, of a query that holds a NaN, whose outputs are NaN as they stand.
 template <int TYPE>
 __device__ __forceinline__ bool repair_column(const SplitArgs &a, const Place &p, int row, int head, float &m, float &l,
                                               float (&o)[4]) {
-    const int lane = threadIdx.x & 63, at = a.pos[p.b] + row;
+    const int lane = threadIdx.x & 63, at = a.pos ? a.pos[p.b] + row : 0;
     const long long qo = static_cast<long long>(p.b) * a.q_stream + static_cast<long long>(row) * a.q_row +
                          static_cast<long long>(head) * a.c.qk;
     const unsigned char *kp = a.c.k + static_cast<long long>(p.h) * a.k_head, *vp = a.c.v + static_cast<long long>(p.h) * a.v_head;
@@ -340,7 +341,7 @@ __device__ __forceinline__ bool repair_column(const SplitArgs &a, const Place &p
     };
     for (int j0 = p.j0; j0 < p.j1; j0 += 64) {
         const int j = j0 + lane;
-        const bool seen = j < p.j1 && sees_row(a, at, p.kl.row(j));
+        const bool seen = j < p.j1 && (!a.pos || sees_row(a, at, p.kl.row(j)));
         float x = -INFINITY, vs = 1.0f;
         int r = 0;
         if (seen) {
@@ -413,9 +414,11 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
     for (int n = tid >> 6; n < nc; n += waves) {
         int row, head;
         column_of(a, p, col0 + n, row, head);
+        bool again = false;
         for (int d = tid & 63; d < a.c.vd; d += 64) {
             float v = 0.0f;
             for (int w = 0; w < waves; ++w) v = fmaf(jt.o[(w * COLS + n) * jt.kRow + d], jt.ml[(w * 2) * COLS + n], v);
+            again |= !(fabsf(v) < kMostSum);
             if (a.part)
                 a.part[part_at(a, p, row, head) * a.c.vd + d] = v;
             else
@@ -424,18 +427,8 @@ __device__ __forceinline__ void finish(const SplitArgs &a, const Place &p, const
                                 static_cast<long long>(head) * a.c.vd + d,
                             v * jt.stat[COLS + n]);
         }
-    }
-    if constexpr (TYPE >= 0) {
-        for (int n = tid >> 6; n < nc; n += waves) {
-            bool nan = false;
-            for (int d = tid & 63; d < a.c.vd; d += 64) {
-                float v = 0.0f;
-                for (int w = 0; w < waves; ++w) v = fmaf(jt.o[(w * COLS + n) * jt.kRow + d], jt.ml[(w * 2) * COLS + n], v);
-                nan |= v != v;
-            }
-            if (!__any(nan)) continue;
-            int row, head;
-            column_of(a, p, col0 + n, row, head);
+        if constexpr (TYPE >= 0) {
+            if (!__any(again)) continue;
             float m, l, o[4];
             if (!repair_column<TYPE>(a, p, row, head, m, l, o)) continue;
             const float inv = a.part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;

@@ -526,7 +526,8 @@ int kv_append_paged_dev(const kv_paged *c, const void *k, long long k_stream, lo
  * form of kv_attend_int8_paged_dev (AttendInt8Spans with a float query,
  * internal/needle/int8.go:208-300) for caches of any type and length. Logits
  * are q.k / scale (scale > 0); the softmax, its sums and the products' sums
- * are float32.
+ * are float32: weights of at most 1 times the values, of all keys, whose sum has
+ * to be in float32's range (half of it where the work is split).
  * q and out hold values of `type`: batch streams of heads*qk (heads*vd),
  * q_stride (out_stride, at least heads*vd) elements apart (0: dense). Query head h reads key
  * head h / (heads/kv_heads). spans are [batch][4] as kv_attend_int8_dev
@@ -590,7 +591,8 @@ int kv_read_paged_dev(const kv_paged *c, void *k, long long k_stream, long long 
  * 16-bit queries over caches of their type, and over codes, take 16-bit
  * products: the operands as they are (codes exactly), the softmax weights in
  * two parts (22 bits with float16 caches, 16 else). Everything else is
- * float32; sums and softmax are float32 throughout. */
+ * float32; sums and softmax are float32 throughout, and as
+ * kv_attend_paged_dev's past the range of values. */
 int kv_attend_rows_paged_dev(const kv_paged *c, void *out, long long out_stream, long long out_row, const void *q,
                              long long q_stream, long long q_row, int type, int batch, int t, int heads,
                              const int32_t *rows, const int32_t *pos, int nk_max, int window, int sink, float scale,
