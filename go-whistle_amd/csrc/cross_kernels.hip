@@ -71,6 +71,7 @@ __device__ __forceinline__ int longest_first(const SplitArgs &a, int place, int 
 // below 2^20. From there on, where it could leave float16 (from 2^28) or
 // float32 (2^31), s scale is rounded first, as m is.
 constexpr float kFar = 0x1p20f;
+constexpr float kDown = 0x1p-8f;  // one over the largest weight, where the maximum lags
 constexpr int kXFlags = 4 * kXWaves;  // bytes behind the tiles: an int a wavefront
 template <int TYPE, int D, int CB, bool FULL>
 __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_kernel(SplitArgs a, int col_tiles, int aligned) {
@@ -166,9 +167,10 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
     const int ti = lane & 15, trow = 4 * half + (ti >> 2);
     const int vaddr = trow * D * 2 + 8 * (ti & 1), vpiece = 2 * ((lane >> 4) & 1) + ((ti & 3) >> 1), vswz = v_swizzle<D>(trow);
 
-    // finite: the second parts, which may be 0 or below it, meet no infinite value.
+    // finite: the second parts, which may be 0 or below it, meet no infinite value,
+    // and weights of bfloat16 memories are up to 1: 2^-8 of what they were, exactly.
     auto attend = [&](auto finite_values) {
-        constexpr bool finite = decltype(finite_values)::value;
+        constexpr bool finite = decltype(finite_values)::value, down = finite && TYPE == 2;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             m[cb] = -INFINITY;
@@ -245,8 +247,12 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], scale, -mu));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i + 1], scale, -mu));
+                        float x = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i], scale, -mu));
+                        float y = __builtin_amdgcn_exp2f(fmaf(s[cb][kb][i + 1], scale, -mu));
+                        if constexpr (down) {
+                            x *= kDown;
+                            y *= kDown;
+                        }
                         l[cb] += x;
                         l[cb] += y;
                         const uint32_t parts = first_parts<TYPE>(x, y);
@@ -283,20 +289,22 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
     };
     attend(std::false_type{});
     // A NaN: an infinite value may be behind it, which the first parts alone
-    // make infinite. All over again for the workgroup, whose wavefronts share the tiles.
-    bool nan = false;
+    // make infinite; or a sum past kMostSum, of weights of up to 2^8.
+    // All over again for the workgroup, whose wavefronts share the tiles.
+    bool again = false;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int v = 0; v < D / 32; ++v)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) nan |= o[cb][v][i] != o[cb][v][i];
-    const bool wave_nan = live && __any(nan);
+            for (int i = 0; i < 16; ++i) again |= !(fabsf(o[cb][v][i]) < kMostSum);
+    const bool wave_again = live && __any(again);
     int *flags = reinterpret_cast<int *>(smem + 4 * kBytes);
-    if (lane == 0) flags[wave] = wave_nan;
+    if (lane == 0) flags[wave] = wave_again;
     __syncthreads();  // also: the tiles' readers are done
     const int4 any = *reinterpret_cast<const int4 *>(flags);
-    if (any.x | any.y | any.z | any.w) attend(std::true_type{});
+    const bool twice = any.x | any.y | any.z | any.w;
+    if (twice) attend(std::true_type{});
     if (!live) return;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
@@ -317,7 +325,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
                             make_float4(o[cb][v][4 * g], o[cb][v][4 * g + 1], o[cb][v][4 * g + 2], o[cb][v][4 * g + 3]);
                 }
             if (half == 0) {
-                a.part_ml[2 * pi] = m[cb] - kLift<TYPE>;
+                a.part_ml[2 * pi] = m[cb] - (TYPE == 2 && twice ? -8.0f : kLift<TYPE>);
                 a.part_ml[2 * pi + 1] = sum;
             }
         } else {
@@ -350,7 +358,8 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_k
 // coordinates in four instructions (element e of the halves' pieces in the
 // e-th); O = V^T P takes S's register i as it lies (the half f's key is 8 (i /
 // 4) + 4 f + i % 4) against one value of that key a lane. Tiles of 64 keys (32
-// past heads of 64) through LDS as above; the weights stay float32. The value
+// past heads of 64) through LDS as above; the weights stay float32, and meet the
+// values as 2^-8 of what they are, so that sums of large values stay in range. The value
 // reads of the two halves, four rows apart, meet in no bank: rows with bit 2
 // set keep their 128-byte halves exchanged.
 template <int D, bool FULL>
@@ -493,6 +502,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
             for (int i = 0; i < 16; ++i) {
                 s[i] = __builtin_amdgcn_exp2f(s[i] - mu);
                 l += s[i];
+                s[i] *= kDown;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -515,7 +525,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
     float *dst = a.part ? a.part + pi * a.c.vd
                         : static_cast<float *>(a.out) + static_cast<long long>(b) * a.out_stream +
                               static_cast<long long>(row) * a.out_row + static_cast<long long>(head) * a.c.vd;
-    const float f = a.part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float f = a.part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / (sum * kDown);
 #pragma unroll
     for (int v = 0; v < D / 32; ++v)
 #pragma unroll
@@ -528,7 +538,7 @@ __global__ __launch_bounds__(64 * kXWaves, D == 256 ? 1 : 2) void cross_attend_f
         }
     if (a.part && half == 0) {
         a.part_ml[2 * pi] = m;
-        a.part_ml[2 * pi + 1] = sum;
+        a.part_ml[2 * pi + 1] = sum * kDown;
     }
 }
 

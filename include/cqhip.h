@@ -621,7 +621,8 @@ typedef struct nd_cross_layout {
  * 256; k, v and their strides (of dimensions past 1) are multiples of 16 bytes.
  * ND_F32 products are float32; with 16-bit types the products take them as they
  * are, and the softmax weights are float32 or, for many rows, two parts of the
- * type (16 bits in bfloat16, 22 in float16); sums and softmax are float32. */
+ * type (16 bits in bfloat16, 22 in float16); sums and softmax are float32, and as
+ * kv_attend_paged_dev's past the range of values. */
 int nd_cross_attend_dev(void *out, const void *q, const void *k, const void *v, int type,
                         const nd_cross_layout *layout, int batch, int t, int heads, int kv_heads, int qk, int vd,
                         int memories, int frames, const int32_t *q_len, const int32_t *k_len, const int32_t *index,

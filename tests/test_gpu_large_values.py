@@ -33,7 +33,9 @@ def large_cache(g, name, streams, n, R, Hk, qk, vd):
     k = torch.zeros(streams * per, R, Hk, qk, device="cuda")
     k[..., :16] = (lg / 256).view(-1, R, 1, 1)
     v = BIG * (0.5 + 0.5 * torch.rand(streams * per, R, Hk, vd, generator=g, device="cuda"))
-    v *= torch.where(torch.rand(vd, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    sign = torch.where(torch.rand(v.shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    v[..., :vd // 2] *= sign[0, 0, 0, :vd // 2]  # of one sign for all keys, and of either
+    v[..., vd // 2:] *= sign[..., vd // 2:]
     table = torch.randperm(streams * per, generator=g, device="cuda")
     back = torch.empty_like(table)
     back[table] = torch.arange(len(table), device="cuda")
