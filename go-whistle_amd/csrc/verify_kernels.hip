@@ -108,7 +108,9 @@ __device__ __forceinline__ const double *record(const VerifyArgs &a, int b, int 
     return a.part + ((static_cast<long long>(b) * stream_rows(a) + row) * a.splits + part) * kVRecord;
 }
 
-// The second launch's parts: their sums of weights, and how many of a stream have theirs.
+// The second launch's parts: their sums of weights (kNoSum until they are there; a
+// sum is 0 or more, or NaN), and how many of a stream have theirs.
+constexpr double kNoSum = -1.0;
 __device__ __forceinline__ double *weight_sums(const VerifyArgs &a, int b, int part) {
     return a.part + static_cast<long long>(a.batch) * stream_rows(a) * a.splits * kVRecord +
            (static_cast<long long>(b) * a.choose_parts + part) * 2;
@@ -128,7 +130,10 @@ __global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a) {
     const int n = drafted_of(a, b);
     const bool target = row <= a.t;
     if (target ? row > n : row - a.t - 1 >= n) return;
-    if (row == 0 && part == 0 && tid == 0) *finished(a, b) = 0;
+    if (row == 0 && part == 0 && a.inv_temp != 0.0) {
+        if (tid == 0) *finished(a, b) = 0;
+        for (int i = tid; i < 2 * a.choose_parts; i += kVThreads) weight_sums(a, b, 0)[i] = kNoSum;
+    }
     const char *base = static_cast<const char *>(target ? a.target : a.draft) +
                        (TYPE == 0 ? 4 : 2) * (target ? b * a.target_stream + row * a.target_row
                                                      : b * a.draft_stream + (row - a.t - 1) * a.draft_row);
@@ -414,18 +419,21 @@ __global__ __launch_bounds__(kCThreads) void verify_choose_kernel(VerifyArgs a) 
         wave_sums(part_weights());
         double total[2];
         for (int k = 0; k < 2; ++k) total[k] = lanes_sum(lane < kCWaves ? waves[k][lane] : 0.0);
+        // Another part's sum. Its workgroup has counted itself, so the sum is on its way,
+        // whether it or the count was seen first.
         auto part_sum = [&](int i, int k) {
-            return __hip_atomic_load(weight_sums(a, b, i) + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            double x;
+            do {
+                x = __hip_atomic_load(weight_sums(a, b, i) + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            } while (x == kNoSum);
+            return x;
         };
         if (a.choose_parts > 1) {
             // The sums pass by the XCDs' own L2s, on either side, so that none of them
             // has to be written back or emptied for a few values (fences of that kind
-            // cost 64 streams 15 us); they are in memory before they are counted.
-            if (tid < 2) {
-                __hip_atomic_store(weight_sums(a, b, part) + tid, total[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            __syncthreads();
+            // cost 64 streams 15 us). Nothing orders them and the count: a sum that is not
+            // there yet says so.
+            if (tid < 2) __hip_atomic_store(weight_sums(a, b, part) + tid, total[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (tid == 0)
                 last_one = __hip_atomic_fetch_add(finished(a, b), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.choose_parts - 1;
             __syncthreads();
