@@ -512,7 +512,12 @@ typedef struct kv_paged {
  * have those rows' codes rounded anew, from their float32 values, under the new
  * one. A page that the appended rows begin, and every page behind, takes its
  * scale from them alone; rows behind the last appended one stand for nothing. Codes
- * are the nearest (ties to the even one) to float32(x / scale). The scale goes
+ * are the nearest (ties to the even one) to float32(x / scale). So a row is off
+ * by up to half a step for each scale that its page has had since (int8: half
+ * of each scale; e4m3: 2^-4 of the value, at least 2^-10 of the scale): once for
+ * a page appended whole, up to page_rows times for one that grows token by token while
+ * its rows do, and the errors may add up. Rows that are appended over (refused
+ * drafts) leave the scale of a begun page where they raised it. The scale goes
  * by the finite values: infinities are held as the largest code of their sign,
  * NaN as 0 (int8) or NaN (e4m3); a page of zeros has the scale 0. Streams of one
  * call that append into one page race, also in different rows of it: a shared
