@@ -200,6 +200,7 @@ hipError_t launch_f32(const RowsArgs &a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_attend_rows_f32(const RowsArgs &a, hipStream_t s) {
+    if (a.c.type != 0) return hipErrorInvalidValue;  // the split form has them
     const int w = std::max(a.c.qk, a.c.vd);
     return w <= 64 ? launch_f32<64>(a, s) : w <= 128 ? launch_f32<128>(a, s) : launch_f32<256>(a, s);
 }

@@ -17,8 +17,9 @@
 // bfloat16, whose range holds a weight of 1 times any scale): a key's scale meets
 // its logit, a value's scale its weight. Weights take part as the sum of two
 // parts of the values' type (22 bits in float16, 16 in bfloat16).
-// rows_attend_f32_kernel, everything else: values widened to float32 (codes
-// times their scale) on 32x32x2 products, all of it in float32.
+// rows_attend_f32_kernel, queries of any type over float32 caches: 32x32x2
+// products, all of it in float32. The other pairs of types take the split form
+// (parts_kernels.hip) at any number of columns.
 //
 // What bounds 8 ragged prompts of up to 2000 rows, 16 heads of 128 over 4 in
 // bfloat16 (220 to 226 us, some 600 TFLOP/s): the softmax on the vector units, 45% of all
