@@ -220,8 +220,9 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_lanes_kernel(Spli
     finish<COLS, D>(a, p, jt);
 }
 
-// TYPE: the cache's type; D: widths up to D (64, 128, 256); PARTS: 16-bit
-// parts of a query value (0: the products of the logits in float32).
+// TYPE: the cache's type (codes with a scale a page, 4 and 5, are attend_parts_kernel's);
+// D: widths up to D (64, 128, 256); PARTS: 16-bit parts of a query value (0: the
+// products of the logits in float32).
 template <int TYPE, int D, int PARTS>
 __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(SplitArgs a, int col_tiles) {
     constexpr int kSize = kValueSize<TYPE>;
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
 #pragma unroll
                         for (int k = 0; k < kVWords; ++k) vw[s][i][k] = 0;
                     }
-                    if constexpr (kScaled<TYPE>) {
+                    if constexpr (TYPE == 3) {
                         ksc[s][i] = a.c.ks[scale_at(a, row, p.h)];
                         vsc[s][i] = a.c.vs[scale_at(a, row, p.h)];
                     }
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                             uint32_t ka[4];
 #pragma unroll
                             for (int z = 0; z < 4; ++z)
-                                ka[z] = kScaled<TYPE> ? upper_pair(piece_value<TYPE>(kw[s][k], 8 * e + 2 * z),
+                                ka[z] = TYPE == 3 ? upper_pair(piece_value<TYPE>(kw[s][k], 8 * e + 2 * z),
                                                                piece_value<TYPE>(kw[s][k], 8 * e + 2 * z + 1))
                                                   : kw[s][k][z];
 #pragma unroll
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                         }
             }
             // An infinite key times a part of 0 is NaN: such logits again, in float32.
-            if constexpr (PARTS == 3 && !kScaled<TYPE>) {
+            if constexpr (PARTS == 3 && TYPE != 3) {
                 bool nan = false;
 #pragma unroll
                 for (int s = 0; s < kSub; ++s)
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                     const int jj = j + 16 * s + 4 * c + i;
                     float x = sc[s][i];
                     if constexpr (PARTS > 0) x *= a.scale_log2;
-                    if constexpr (kScaled<TYPE>) x *= ksc[s][i];
+                    if constexpr (TYPE == 3) x *= ksc[s][i];
                     if (jj >= p.j1) {
                         x = -INFINITY;
                     } else if (a.acc_out && col_ok) {
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(D <= 128 ? 512 : 256) void attend_split_kernel(Spli
                 for (int i = 0; i < 4; ++i) {
                     float w = __builtin_amdgcn_exp2f(sc[s][i] - mu);
                     l += w;
-                    if constexpr (kScaled<TYPE>) w = j + 16 * s + 4 * c + i >= p.j1 ? 0.0f : w * vsc[s][i];
+                    if constexpr (TYPE == 3) w = j + 16 * s + 4 * c + i >= p.j1 ? 0.0f : w * vsc[s][i];
 #pragma unroll
                     for (int e = 0; e < kVals; ++e)
                         o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece_value<TYPE>(vw[s][i], e), w, o[e], 0, 0, 0);
