@@ -2485,7 +2485,10 @@ static int run_split_attend(SplitArgs &a, hipStream_t stream);
 // - float32 queries over 16-bit caches and codes, and 16-bit queries over the other
 //   16-bit type: the split form, whose products are 16-bit parts where the tiles
 //   would be float32's (8 streams, 8 heads of 64 over 2, 2000 bfloat16 keys: 512
-//   columns 44 against 68, 2048 112 against 207).
+//   columns 44 against 68, 2048 112 against 207). Over float16 caches, whose range does not
+//   hold a float32 or bfloat16 query's parts, the logits' products are float32's there too: 16,
+//   64, 256, 512 and 2048 columns of the last of those keys 18, 25, 36, 53 and 135 us,
+//   over bfloat16 ones 15, 21, 30, 41 and 88; 8 prompts of 2000 rows of 8 heads 407 and 252.
 // - float32 caches: the tiles once they give two blocks of 32 columns a CU (16
 //   streams, 8 heads of 64, 500 keys: 512 columns 207 against 154; 4 streams, 16
 //   heads of 128 over 4, 3000 keys: 1024 columns 287 against 263, 512 167 against 207).

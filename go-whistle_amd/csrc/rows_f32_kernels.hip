@@ -1,5 +1,11 @@
 // gfx950 causal attention of many rows over paged float32 caches
 // (rows_kernels.hip describes the tiles, the masks and the columns computed again).
+//
+// What bounds it: 16 prompts of 448 rows, 8 heads of 64, 64 to 73 us (21.5 at the rate
+// of a large float32 product): one round of workgroups, of which the first rows' walk 128
+// keys and the last rows' all; matrix units busy 34% of all cycles, CUs 71%. 8 prompts of 2000
+// rows 355 us (214), 63% and 86%. Heads past 128 leave one workgroup a CU, whose four
+// wavefronts wait half of their cycles: 16 prompts, 8 heads of 240 over 4, 300 to 370 us (81).
 #include "rows_device.hpp"
 
 #include <algorithm>

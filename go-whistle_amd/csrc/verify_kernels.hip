@@ -16,7 +16,7 @@
 // greedy, T = 0, needs one workgroup a stream). Some ten waits for memory and
 // exchanges bound it where there are few streams, and the float64 units, as an
 // exponential is some 25 of their operations: 4 drafts of one stream of 8199 tokens
-// 4.8 and 14 us (18.6 with 4096 tokens a workgroup of 1024 threads), 8 of 64 streams of 16,384 17
+// 4.8 and 14.4 us (18.6 with 4096 tokens a workgroup of 1024 threads), 8 of 64 streams of 16,384 17
 // and 22 (29 with 16 tokens a thread). The last step as a launch of its own: 13 us beside 8.
 #include "cq_internal.hpp"
 #include "cq_device.hpp"
@@ -35,7 +35,8 @@ constexpr int kCHold = 4;                      // logits a thread there
 constexpr int kCChunk = kCThreads * kCHold;    // logits of its parts
 constexpr int kVRecord = 3;                    // doubles of a part: maximum, sum, index of the first largest
 
-// exp(x) for x <= 0: 2^k times the series of exp(r) to r^11, |r| <= ln(2) / 2, off by 6e-15; 0 below -708.
+// exp(x) for x <= 0: 2^k times Taylor's series of exp(r) to r^11, r = x - k ln(2) with ln(2) in two
+// parts (Cody and Waite), |r| <= ln(2) / 2, off by 6e-15; 0 below -708.
 __device__ __forceinline__ double exp_down(double x) {
     const double k = rint(x * 1.44269504088896338700e+00);
     double r = fma(-k, 6.93147180369123816490e-01, x);
